@@ -16,6 +16,13 @@
  *         bytes when kv_dtype == SLO_KV_FP8_E4M3FN
  *   scale [num_blocks, block_size, num_kv_heads]            fp32 (FP8 only)
  *   slot  = block_table[pos / block_size] * block_size + pos % block_size
+ * A 4-bit pool (kv_dtype == SLO_KV_FP4_E2M1) stores its pages head by head:
+ *   K/V   [num_blocks, num_kv_heads, block_size, head_dim / 2]   two E2M1 codes
+ *         a byte, the even channel in the low half
+ *   scale [num_blocks, num_kv_heads, block_size, head_dim / 32]  E8M0 bytes, one
+ *         per 32 channels: value = code * 2^(scale - 127)
+ * Accumulated attention weights lie head by head as well, whatever the pool's
+ * format: scores [num_blocks, num_kv_heads, block_size] fp32.
  */
 #ifndef SLO_ATTN_H_
 #define SLO_ATTN_H_
@@ -38,7 +45,7 @@ enum {
   SLO_ERR_STATE = 5        /* a workspace word that must be zero between launches is not */
 };
 
-enum { SLO_KV_BF16 = 0, SLO_KV_FP8_E4M3FN = 1 };
+enum { SLO_KV_BF16 = 0, SLO_KV_FP8_E4M3FN = 1, SLO_KV_FP4_E2M1 = 2 };
 
 enum { SLO_PHASE_DECODE = 1, SLO_PHASE_PREFILL = 2, SLO_PHASE_ALL = 3 };
 /* Or-ed into phases: the rows of new_k / new_v may lie any multiple of 8
@@ -299,6 +306,108 @@ int slo_attention_workspace_check(const void* workspace, size_t workspace_bytes,
  */
 #define SLO_NOALLOC_SCRATCH_BYTES (64u << 20)
 int slo_paged_attention_noalloc(const slo_paged_attention_args* args, slo_stream_t stream);
+
+/*
+ * slo_store_kvcache into a 4-bit pool.  Per (token, kv head, 32 channels) the
+ * scale is the smallest power of two, at least scale_floor (itself a power of
+ * two from 2^-100 to 2^125) and at most 2^125, at which the largest magnitude
+ * is below 7; the code is x / scale rounded to the nearest E2M1 value (0, 0.5,
+ * 1, 1.5, 2, 3, 4, 6), ties to the even code, saturating at 6.  The sign is
+ * kept; infinities and NaN count as the largest finite bf16 of their sign.
+ * Slots outside [0, num_blocks * block_size) are skipped.
+ */
+int slo_store_kvcache_fp4(const void* key, int64_t key_row_stride, const void* value,
+                          int64_t value_row_stride, const int32_t* slot_mapping, int32_t num_tokens,
+                          int32_t num_kv_heads, int32_t head_dim, void* k_cache, void* v_cache,
+                          void* k_scale, void* v_scale, int32_t num_blocks, int32_t block_size,
+                          float scale_floor, slo_stream_t stream);
+
+/*
+ * Reads cached tokens back: row i of k_out / v_out (bf16 [num_tokens,
+ * num_kv_heads, head_dim], contiguous) is the token at slot_mapping[i], as
+ * stored (bf16), code * scale rounded to bf16 (E4M3FN) or the value exactly
+ * (4 bits); zeros for a slot outside the pool.  k_scale / v_scale: fp32 or
+ * E8M0 bytes, as the format has them.
+ */
+int slo_load_kvcache(const void* k_cache, const void* v_cache, const void* k_scale,
+                     const void* v_scale, int32_t kv_dtype, int32_t num_blocks, int32_t block_size,
+                     const int32_t* slot_mapping, int32_t num_tokens, int32_t num_kv_heads,
+                     int32_t head_dim, void* k_out, void* v_out, slo_stream_t stream);
+
+/*
+ * slo_paged_attention over a 4-bit pool: the same arguments (k_scale / v_scale
+ * point to E8M0 bytes, kv_dtype is SLO_KV_FP4_E2M1) and the same rows, masks
+ * and outputs; a row without keys gives zeros.  Prefill rows are read through
+ * prefill_tables (without tables they read no pool: slo_paged_attention takes
+ * them); store_slot_mapping must be NULL and softmax_scale not zero.  The
+ * workspace (16-byte aligned, slo_paged_attention_fp4_workspace_bytes of the
+ * same arguments; it need not be cleared and holds nothing between calls) may
+ * not be used by two calls that overlap.
+ */
+int slo_paged_attention_fp4_workspace_bytes(const slo_paged_attention_args* args, size_t* bytes);
+int slo_paged_attention_fp4(const slo_paged_attention_args* args, slo_stream_t stream);
+
+/*
+ * Adds the attention weights of a step's queries to the scores of the cached
+ * keys they look at: for every row and key j of it,
+ *   w = sum over the row's queries i that see j and the heads h of the kv
+ *       head's group of softmax_j(softmax_scale * q[i, h] . k[j])
+ *   scores[slot(j), kv head] = w            j one of the row's own new tokens
+ *                              += w         j older
+ * (the new tokens are the last of the row's keys: decode_lens[b] - 1, or the
+ * last Lq), so a slot that is taken into use again starts from its own weight.
+ * Rows, masks and K as in slo_paged_attention; V, out and the new_k / new_v
+ * fields are not read.  K comes from a bf16, E4M3FN or 4-bit pool; prefill
+ * rows need prefill_tables.  Rows that share an old page both count (fp32
+ * atomic adds: there the order of the additions may vary).  Workspace as for
+ * slo_paged_attention_fp4.
+ */
+int slo_accumulate_attention_workspace_bytes(const slo_paged_attention_args* args, size_t* bytes);
+int slo_accumulate_attention(const slo_paged_attention_args* args, float* scores, slo_stream_t stream);
+
+/*
+ * Arguments of slo_evict_kv.  The pool's arrays hold num_layers layers one
+ * after another (one layer: num_layers 1).
+ */
+typedef struct slo_evict_kv_args {
+  void* k_cache;
+  void* v_cache;
+  void* k_scale;      /* NULL for bf16 */
+  void* v_scale;
+  float* scores;      /* [num_layers, num_blocks, num_kv_heads, block_size] */
+  int32_t kv_dtype;
+  int32_t num_layers;
+  int32_t num_blocks;
+  int32_t block_size;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t num_rows;
+  const int32_t* lens;    /* [num_rows] cached tokens */
+  const int32_t* tables;  /* [num_rows, >= table_width], -1 padded */
+  int32_t table_stride;
+  int32_t table_width;
+  int32_t budget;         /* tokens a row keeps, > 0 */
+  int32_t recent;         /* of them, the newest ones kept whatever their weight */
+  int32_t* new_lens;      /* [num_rows]: min(len, budget) */
+  int32_t* kept;          /* [num_layers, num_rows, num_kv_heads, budget]: positions, -1 past the row */
+} slo_evict_kv_args;
+
+/*
+ * Evicts cached tokens by accumulated weight.  A row of at most `budget`
+ * tokens stays as it is.  A longer one keeps, in every layer and for every kv
+ * head by itself, its newest `recent` tokens and the budget - recent heaviest
+ * of the others (ties: the lowest position; NaN weighs less than any number);
+ * they are moved, in position order, with their scales and scores, to the
+ * row's first `budget` places, and the scores of its other places up to its
+ * length become zero.  The kept positions are written to `kept`.  The pages
+ * past the budget can then be freed.  Two rows may not share a page, or a row
+ * hold one twice.  Tokens in no page of the pool weigh nothing and do not
+ * move.
+ */
+int slo_evict_kv(const slo_evict_kv_args* args, slo_stream_t stream);
+
+/* Size of slo_evict_kv_args, for binding checks. */
+size_t slo_evict_kv_args_size(void);
 
 /* Description of the last error on the calling thread ("" if none). */
 const char* slo_last_error(void);

@@ -29,3 +29,5 @@ int check_launch(const char* what) {
 extern "C" const char* slo_last_error(void) { return g_last_error; }
 
 extern "C" size_t slo_paged_attention_args_size(void) { return sizeof(slo_paged_attention_args); }
+
+extern "C" size_t slo_evict_kv_args_size(void) { return sizeof(slo_evict_kv_args); }

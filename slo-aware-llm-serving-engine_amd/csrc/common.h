@@ -24,7 +24,7 @@ typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
 
 // KV element formats accepted by the C-ABI.
-enum KvDtype : int { KV_BF16 = 0, KV_FP8_E4M3FN = 1 };
+enum KvDtype : int { KV_BF16 = 0, KV_FP8_E4M3FN = 1, KV_FP4_E2M1 = 2 };
 
 constexpr float kFp8Max = 448.0f;
 constexpr float kLog2e = 1.4426950408889634f;

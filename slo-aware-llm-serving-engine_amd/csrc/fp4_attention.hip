@@ -1,0 +1,566 @@
+// Ragged paged attention over a 4-bit KV pool (gfx950).
+//
+// out[i, h] = sum_j softmax_j(scale q[i, h] . k[j]) v[j] over the keys j that
+// query i sees, with K and V read from 4-bit pages (fp4.h).  One pass over the
+// keys with a running maximum and sum per (query, head):
+//
+//   S^T = K q^T      A = K (rows: 16 tokens), B = q (columns: 16 queries or heads)
+//   O^T += V^T P^T   A = V^T (rows: 16 channels), B = P (columns: the same 16)
+//
+// Transposed products keep a column's statistics in the lanes that hold its
+// scores and its outputs, and the 8 probabilities that a lane has of two
+// 16-token tiles (tokens 4 kg + i and 16 + 4 kg + i, kg = lane / 16) are, as
+// they lie, the operand of the second product for that order of its 32 tokens.
+// Codes become bf16 operands by v_cvt_scalef32_pk_bf16_fp4, exactly, scale
+// included: two channels of a token per instruction.  For K that is the
+// operand's order (lane: one token, the 32 channels of one scale, 16 bytes);
+// for V (lane: 8 tokens, 8 channels, 4 bytes each) two v_perm_b32 per two pairs
+// turn channel pairs into token pairs.  Probabilities are rounded to bf16 and
+// their sum is taken of the rounded values (one more row of the second
+// product, of ones), so a weight's rounding cancels where one key dominates.
+// Sums, maxima and outputs are fp32 until the one rounding at the end.
+#include "capi_internal.h"
+#include "fp4.h"
+#include <type_traits>
+
+namespace slo {
+namespace {
+
+constexpr int HD4 = 128;        // head_dim
+constexpr int KT = 32;          // tokens per step of a wavefront
+constexpr int RECORD = HD4 + 4;  // floats of a partial result: outputs, maximum, sum, 2 unused
+constexpr float kNone = -1e30f;  // running maximum before the first key
+
+struct Fp4Params {
+  const uint16_t* q;
+  int64_t q_stride;
+  uint16_t* out;
+  int64_t out_stride;
+  int num_q_rows;
+  const uint8_t *kc, *vc, *ks, *vs;
+  int num_blocks, block_size;
+  const int32_t* lens;  // decode rows: key counts; null for prefill rows
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  const int32_t* tables;
+  int table_stride, table_width;
+  int first_row;  // query row of the phase's first query
+  int hq, hkv, group;
+  float scale_log2;  // |softmax scale| * log2(e)
+  uint32_t q_sign;   // 0x80008000 where the scale is negative
+  float* partial;    // [query rows of the phase, hq, splits] records when splits > 1
+  int splits, chunk;
+};
+
+struct Row {
+  int64_t q0;  // first query row
+  int lq, lk, prefix;
+};
+
+__device__ __forceinline__ Row row_of(const Fp4Params& p, int r) {
+  Row g;
+  const int cap = p.table_width * p.block_size;
+  if (p.lens) {
+    g.q0 = p.first_row + r;
+    g.lq = 1;
+    g.lk = min(max(p.lens[r], 0), cap);
+    g.prefix = g.lk - 1;
+  } else {
+    const int start = p.cu_q[r], k = p.cu_k[r + 1] - p.cu_k[r];
+    g.q0 = (int64_t)p.first_row + start;
+    g.lq = p.cu_q[r + 1] - start;
+    g.prefix = k - g.lq;
+    g.lk = min(k, cap);
+    if (start < 0 || g.q0 + g.lq > p.num_q_rows) g.lq = 0;
+  }
+  return g;
+}
+
+// One step's cache lines in registers.
+struct Tile {
+  u32x4 k[2], vs[2];
+  uint32_t v[8], ks[2];
+};
+
+__device__ __forceinline__ void load_tile(Tile& t, const Fp4Params& p, int64_t row, int lane) {
+  const int c = lane & 15, kg = lane >> 4;
+  const uint8_t* k = p.kc + row * 64 + c * 64 + kg * 16;
+  const uint8_t* v = p.vc + row * 64 + kg * 256 + c * 4;
+  const uint8_t* ks = p.ks + row * 4 + c * 4 + kg;
+  const uint8_t* vs = p.vs + row * 4 + kg * 16;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    t.k[h] = *reinterpret_cast<const u32x4*>(k + h * 1024);
+    t.ks[h] = ks[h * 64];
+    t.vs[h] = *reinterpret_cast<const u32x4*>(vs + h * 64);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t.v[4 * h + i] = *reinterpret_cast<const uint32_t*>(v + h * 1024 + i * 64);
+  }
+}
+
+template <int NT>
+struct Acc {
+  f32x4 o[NT][8], l[NT];
+  float m[NT];
+};
+
+__device__ __forceinline__ float column_max(float x) {  // over the four lanes of a column
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+template <int NT, bool MASK>
+__device__ __forceinline__ void step(const Tile& t, const bf16x8 (&q)[NT][4], Acc<NT>& a, float c, int kv0,
+                                     const int (&limit)[NT], int kend, int lane) {
+  const int kg = lane >> 4;
+  f32x4 s[NT][2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const float sc = e8m0(t.ks[h]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bf16x8 k = as_bf16x8(e2m1_decode8(t.k[h][i], sc));
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[n][h] = mfma16(k, q[n][i], i ? s[n][h] : f32x4{0, 0, 0, 0});
+    }
+  }
+  bf16x8 pr[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    if (MASK) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (kv0 + 16 * h + 4 * kg + i >= limit[n]) s[n][h][i] = -INFINITY;
+    }
+    float top = fmaxf(s[n][0][0], s[n][0][1]);
+#pragma unroll
+    for (int i = 2; i < 8; ++i) top = fmaxf(top, s[n][i >> 2][i & 3]);
+    // The reference only moves where a score passes it by 2^8: probabilities
+    // up to 256 round like those below 1, and the outputs' rescale is rare.
+    if (__any(top * c > a.m[n] + 8.0f)) {
+      const float m = fmaxf(a.m[n], column_max(top) * c);
+      const float w = __builtin_amdgcn_exp2f(a.m[n] - m);
+      a.m[n] = m;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) a.o[n][e] *= w;
+      a.l[n] *= w;
+    }
+    u32x4 b;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      b[i] = pack_bf16x2(__builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i >> 1][2 * (i & 1)], c, -a.m[n])),
+                         __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i >> 1][2 * (i & 1) + 1], c, -a.m[n])));
+    pr[n] = as_bf16x8(b);
+  }
+  float vs[8];
+  const int byte = 8 * ((lane & 15) >> 2);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    uint32_t code = (t.vs[j >> 2][j & 3] >> byte) & 0xffu;
+    // A token past the row's keys may be anything in the pages: its weight is
+    // zero, and its scale must not make that a NaN.
+    if (MASK) code = kv0 + 16 * (j >> 2) + 4 * kg + (j & 3) < kend ? code : 0u;
+    vs[j] = e8m0(code);
+  }
+  auto pair = [&](auto sel) {
+    constexpr int B = decltype(sel)::value;
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = e2m1_pair<B>(t.v[j], vs[j]);
+    u32x4 lo, hi;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      lo[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x05040100u);
+      hi[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x07060302u);
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      a.o[n][2 * B] = mfma16(as_bf16x8(lo), pr[n], a.o[n][2 * B]);
+      a.o[n][2 * B + 1] = mfma16(as_bf16x8(hi), pr[n], a.o[n][2 * B + 1]);
+    }
+  };
+  const bf16x8 ones = as_bf16x8(u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
+#pragma unroll
+  for (int n = 0; n < NT; ++n) a.l[n] = mfma16(ones, pr[n], a.l[n]);
+  pair(std::integral_constant<int, 0>{});
+  pair(std::integral_constant<int, 1>{});
+  pair(std::integral_constant<int, 2>{});
+  pair(std::integral_constant<int, 3>{});
+}
+
+// Walks a row's tokens in steps of `stride` through its table; pages that are
+// not in the pool count as unseen keys.
+struct Walk {
+  const int32_t* table;
+  int page, off, block_size, num_blocks, hkv, head;
+  __device__ __forceinline__ void advance(int by) {
+    off += by;
+    while (off >= block_size) {
+      off -= block_size;
+      ++page;
+    }
+  }
+  __device__ __forceinline__ int64_t row(bool& ok) const {
+    const int b = table[page];
+    ok = b >= 0 && b < num_blocks;
+    return ((int64_t)(ok ? b : 0) * hkv + head) * block_size + off;
+  }
+};
+
+// Runs a wavefront's columns over tokens begin, begin + stride, ... < end.
+template <int NT>
+__device__ __forceinline__ void attend(const Fp4Params& p, int r, int head, const bf16x8 (&q)[NT][4], Acc<NT>& a, int begin,
+                                       int end, int stride, int full, const int (&limit)[NT], int kend, int lane) {
+  if (begin >= end) return;
+  Walk w{p.tables + (int64_t)r * p.table_stride, begin / p.block_size, 0, p.block_size, p.num_blocks, p.hkv, head};
+  w.off = begin - w.page * p.block_size;
+  Tile t[2];
+  bool ok[2];
+  int64_t row = w.row(ok[0]);
+  load_tile(t[0], p, row, lane);
+  for (int kv0 = begin; kv0 < end; kv0 += 2 * stride) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int at = kv0 + u * stride;
+      if (at >= end) break;
+      if (at + stride < end) {
+        w.advance(stride);
+        row = w.row(ok[u ^ 1]);
+        load_tile(t[u ^ 1], p, row, lane);
+      }
+      if (!ok[u]) continue;
+      if (at + KT <= full)
+        step<NT, false>(t[u], q, a, p.scale_log2, at, limit, kend, lane);
+      else
+        step<NT, true>(t[u], q, a, p.scale_log2, at, limit, kend, lane);
+    }
+  }
+}
+
+__device__ __forceinline__ bf16x8 load_q(const Fp4Params& p, int64_t row, int h, int channel, bool live) {
+  u32x4 x = {0, 0, 0, 0};
+  if (live) x = *reinterpret_cast<const u32x4*>(p.q + row * p.q_stride + h * HD4 + channel);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] ^= p.q_sign;
+  return as_bf16x8(x);
+}
+
+template <int NT>
+__device__ __forceinline__ void clear(Acc<NT>& a) {
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) a.o[n][e] = f32x4{0, 0, 0, 0};
+    a.l[n] = f32x4{0, 0, 0, 0};
+    a.m[n] = kNone;
+  }
+}
+
+// Decode rows: a workgroup takes one chunk of one (row, kv head), its four
+// wavefronts every fourth 32-token step, all heads of the group as columns.
+// The wavefronts' results meet in LDS.
+__global__ void __launch_bounds__(256, 2)
+fp4_decode_kernel(Fp4Params p) {
+  __shared__ float so[4][16][HD4];
+  __shared__ float sm[4][16], sl[4][16];
+  const int head = blockIdx.x, split = blockIdx.y, r = blockIdx.z;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Row g = row_of(p, r);
+  const int k0 = split * p.chunk, k1 = min(k0 + p.chunk, g.lk);
+  if (split && k0 >= g.lk) return;
+  const int col = lane & 15, kg = lane >> 4;
+  bf16x8 q[1][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) q[0][i] = load_q(p, g.q0, head * p.group + col, 32 * kg + 8 * i, col < p.group);
+  Acc<1> a;
+  clear(a);
+  const int limit[1] = {g.lk};
+  attend<1>(p, r, head, q, a, k0 + wave * KT, k1, 4 * KT, g.lk, limit, g.lk, lane);
+  if (col < p.group) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; e += 4)
+        *reinterpret_cast<f32x4*>(&so[wave][col][32 * kg + 8 * i + e]) =
+            f32x4{a.o[0][e][i], a.o[0][e + 1][i], a.o[0][e + 2][i], a.o[0][e + 3][i]};
+    if (kg == 0) {
+      sm[wave][col] = a.m[0];
+      sl[wave][col] = a.l[0][0];
+    }
+  }
+  __syncthreads();
+  for (int x = threadIdx.x; x < p.group * (HD4 / 4); x += 256) {
+    const int h = x >> 5, d = (x & 31) * 4;
+    float m = sm[0][h];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) m = fmaxf(m, sm[w][h]);
+    f32x4 o = {0, 0, 0, 0};
+    float l = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = __builtin_amdgcn_exp2f(sm[w][h] - m);
+      o += *reinterpret_cast<const f32x4*>(&so[w][h][d]) * f;
+      l += sl[w][h] * f;
+    }
+    if (p.splits == 1) {
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      *reinterpret_cast<u32x2*>(p.out + g.q0 * p.out_stride + (head * p.group + h) * HD4 + d) =
+          u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
+    } else {
+      float* rec = p.partial + (((int64_t)r * p.hq + head * p.group + h) * p.splits + split) * RECORD;
+      *reinterpret_cast<f32x4*>(rec + d) = o;
+      if (d == 0) {
+        rec[HD4] = m;
+        rec[HD4 + 1] = l;
+      }
+    }
+  }
+}
+
+// Prefill rows: a wavefront takes 16 NT columns, (query, head of the group)
+// pairs of consecutive queries of one row, over its keys (or one chunk of
+// them), the latest queries first; the four wavefronts of a workgroup take
+// neighbouring columns and so read the same tokens from L1.
+template <int NT>
+__global__ void __launch_bounds__(256, 1)
+fp4_prefill_kernel(Fp4Params p, int tiles) {
+  const int head = blockIdx.x, r = blockIdx.z;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int split = blockIdx.y % p.splits;
+  const int tile = (tiles - 1 - (int)(blockIdx.y / p.splits)) * 4 + wave;
+  const int per = 16 * NT / p.group;  // queries of a wavefront
+  const Row g = row_of(p, r);
+  const int t0 = tile * per, t1 = min(t0 + per, g.lq);
+  if (t0 >= g.lq) return;
+  const int kend = min(max(g.prefix + t1, 0), g.lk);
+  const int k0 = split * p.chunk, k1 = p.splits == 1 ? kend : min(k0 + p.chunk, kend);
+  if (split && k0 >= kend) return;
+  const int col = lane & 15, kg = lane >> 4;
+  bf16x8 q[NT][4];
+  int limit[NT], tok[NT], h[NT];
+  bool live[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int x = 16 * n + col;
+    tok[n] = t0 + x / p.group;
+    h[n] = head * p.group + x % p.group;
+    live[n] = x < per * p.group && tok[n] < t1;
+    limit[n] = live[n] ? min(g.prefix + tok[n] + 1, g.lk) : 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[n][i] = load_q(p, g.q0 + tok[n], h[n], 32 * kg + 8 * i, live[n]);
+  }
+  Acc<NT> a;
+  clear(a);
+  attend<NT>(p, r, head, q, a, k0, k1, KT, min(g.prefix + t0 + 1, g.lk), limit, kend, lane);
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    if (!live[n]) continue;
+    if (p.splits == 1) {
+      const float inv = a.l[n][0] == 0.0f ? 0.0f : 1.0f / a.l[n][0];
+      uint16_t* out = p.out + (g.q0 + tok[n]) * p.out_stride + h[n] * HD4 + 32 * kg;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<u32x4*>(out + 8 * i) =
+            u32x4{pack_bf16x2(a.o[n][0][i] * inv, a.o[n][1][i] * inv), pack_bf16x2(a.o[n][2][i] * inv, a.o[n][3][i] * inv),
+                  pack_bf16x2(a.o[n][4][i] * inv, a.o[n][5][i] * inv), pack_bf16x2(a.o[n][6][i] * inv, a.o[n][7][i] * inv)};
+    } else {
+      float* rec = p.partial + (((g.q0 - p.first_row + tok[n]) * p.hq + h[n]) * p.splits + split) * RECORD;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; e += 4)
+          *reinterpret_cast<f32x4*>(rec + 32 * kg + 8 * i + e) =
+              f32x4{a.o[n][e][i], a.o[n][e + 1][i], a.o[n][e + 2][i], a.o[n][e + 3][i]};
+      if (kg == 0) {
+        rec[HD4] = a.m[n];
+        rec[HD4 + 1] = a.l[n][0];
+      }
+    }
+  }
+}
+
+// Joins the partial results of the phase's chunks, in chunk order: one
+// wavefront per (query, head), two channels a lane.
+__global__ void __launch_bounds__(256)
+fp4_join_kernel(Fp4Params p) {
+  const int lane = threadIdx.x & 63;
+  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int r = blockIdx.y;
+  const Row g = row_of(p, r);
+  const int i = (int)(unit / p.hq), h = (int)(unit % p.hq);
+  if (i >= g.lq) return;
+  const int kend = min(max(g.prefix + i + 1, 0), g.lk);
+  const int n = min(max(1, (kend + p.chunk - 1) / p.chunk), p.splits);
+  const float* rec = p.partial + ((g.q0 - p.first_row + i) * p.hq + h) * (int64_t)p.splits * RECORD;
+  float m = kNone;
+  for (int s = lane; s < n; s += 64) m = fmaxf(m, rec[(int64_t)s * RECORD + HD4]);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) m = wave_max_xor(m, d);
+  float x = 0, y = 0, l = 0;
+  for (int s = 0; s < n; ++s) {
+    const float* e = rec + (int64_t)s * RECORD;
+    const float w = __builtin_amdgcn_exp2f(e[HD4] - m);
+    x += e[2 * lane] * w;
+    y += e[2 * lane + 1] * w;
+    l += e[HD4 + 1] * w;
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  *reinterpret_cast<uint32_t*>(p.out + (g.q0 + i) * p.out_stride + h * HD4 + 2 * lane) = pack_bf16x2(x * inv, y * inv);
+}
+
+constexpr int kPrefillNT = 2;
+
+// Workgroups that fill the GPU (256 CUs) about four times over: chunks of a
+// long row are split off until a launch has that many.
+int splits_of(int64_t groups, int64_t capacity, int least, int most_groups, int& chunk) {
+  int64_t want = (most_groups + groups - 1) / groups;
+  int64_t c = (capacity + want - 1) / (want < 1 ? 1 : want);
+  c = (c + 127) / 128 * 128;
+  if (c < least) c = least;
+  if (c > (1 << 30)) c = 1 << 30;
+  chunk = (int)c;
+  const int64_t n = (capacity + c - 1) / c;
+  return n < 1 ? 1 : (int)n;
+}
+
+struct Plan {
+  bool dwork;
+  int dsplits, dchunk, psplits, pchunk, ptiles;
+  size_t dbytes, pbytes;
+};
+
+Plan plan_of(const slo_paged_attention_args* a) {
+  Plan n = {false, 1, 1 << 30, 1, 1 << 30, 0, 0, 0};
+  if (a->num_decode > 0 && (a->phases & SLO_PHASE_DECODE)) {
+    n.dwork = true;
+    n.dsplits = splits_of((int64_t)a->num_decode * a->num_kv_heads, (int64_t)a->decode_table_width * a->block_size, 256, 2048,
+                          n.dchunk);
+    if (n.dsplits > 1) n.dbytes = (size_t)a->num_decode * a->num_heads * n.dsplits * RECORD * 4;
+  }
+  if (a->num_prefill > 0 && (a->phases & SLO_PHASE_PREFILL) && a->max_q > 0) {
+    const int per = 16 * kPrefillNT / (a->num_heads / a->num_kv_heads);
+    n.ptiles = ((a->max_q + per - 1) / per + 3) / 4;
+    const int64_t cap = (int64_t)a->prefill_table_width * a->block_size;
+    n.psplits = splits_of((int64_t)a->num_prefill * a->num_kv_heads * n.ptiles, cap < a->max_k ? cap : a->max_k, 512, 512,
+                          n.pchunk);
+    if (n.psplits > 1) n.pbytes = (size_t)(a->num_q_rows - a->num_decode) * a->num_heads * n.psplits * RECORD * 4;
+  }
+  return n;
+}
+
+int check_args(const slo_paged_attention_args* a) {
+  if (!a) return fail(SLO_ERR_INVALID, "paged_attention_fp4: null args");
+  if (a->head_dim != HD4) return fail(SLO_ERR_UNSUPPORTED, "paged_attention_fp4: head_dim must be 128");
+  if (a->num_heads <= 0 || a->num_kv_heads <= 0 || a->num_heads % a->num_kv_heads)
+    return fail(SLO_ERR_INVALID, "paged_attention_fp4: num_heads must be a multiple of num_kv_heads");
+  if (a->num_heads / a->num_kv_heads > 16)
+    return fail(SLO_ERR_UNSUPPORTED, "paged_attention_fp4: at most 16 query heads per kv head");
+  if (a->kv_dtype != KV_FP4_E2M1) return fail(SLO_ERR_INVALID, "paged_attention_fp4: kv_dtype must be SLO_KV_FP4_E2M1");
+  if (a->num_q_rows < 0 || a->num_decode < 0 || a->num_prefill < 0 || a->num_decode > a->num_q_rows)
+    return fail(SLO_ERR_INVALID, "paged_attention_fp4: bad row counts");
+  if (!(a->softmax_scale != 0.0f) || a->softmax_scale - a->softmax_scale != 0.0f)
+    return fail(SLO_ERR_INVALID, "paged_attention_fp4: softmax_scale must be finite and not zero");
+  if (a->store_slot_mapping) return fail(SLO_ERR_INVALID, "paged_attention_fp4: store the new rows first");
+  if (a->num_decode > 65535 || a->num_prefill > 65535)
+    return fail(SLO_ERR_UNSUPPORTED, "paged_attention_fp4: more than 65535 rows");
+  const bool dec = a->num_decode > 0 && (a->phases & SLO_PHASE_DECODE);
+  const bool pre = a->num_prefill > 0 && (a->phases & SLO_PHASE_PREFILL);
+  if (!dec && !pre) return SLO_OK;
+  if (!a->q || !a->out) return fail(SLO_ERR_INVALID, "paged_attention_fp4: null pointer");
+  if ((a->q_row_stride % 8) || (a->out_row_stride % 8) || a->q_row_stride < a->num_heads * HD4 ||
+      a->out_row_stride < a->num_heads * HD4 || (reinterpret_cast<uintptr_t>(a->q) % 16) ||
+      (reinterpret_cast<uintptr_t>(a->out) % 16))
+    return fail(SLO_ERR_INVALID, "paged_attention_fp4: q and out rows must be 16-byte aligned");
+  if (!a->k_cache || !a->v_cache || !a->k_scale || !a->v_scale || a->num_blocks <= 0)
+    return fail(SLO_ERR_INVALID, "paged_attention_fp4: no KV pool or no scales");
+  if ((reinterpret_cast<uintptr_t>(a->k_cache) % 16) || (reinterpret_cast<uintptr_t>(a->v_cache) % 16) ||
+      (reinterpret_cast<uintptr_t>(a->k_scale) % 16) || (reinterpret_cast<uintptr_t>(a->v_scale) % 16))
+    return fail(SLO_ERR_INVALID, "paged_attention_fp4: pools and scales must be 16-byte aligned");
+  if (a->block_size <= 0 || a->block_size % 64)
+    return fail(SLO_ERR_UNSUPPORTED, "paged_attention_fp4: block_size must be a multiple of 64");
+  if (dec && (!a->decode_lens || !a->decode_tables || a->decode_table_width <= 0))
+    return fail(SLO_ERR_INVALID, "paged_attention_fp4: missing decode metadata");
+  if (pre && (!a->prefill_cu_q || !a->prefill_cu_k || !a->prefill_tables || a->prefill_table_width <= 0))
+    return fail(SLO_ERR_INVALID, "paged_attention_fp4: missing prefill metadata");
+  if ((dec && (int64_t)a->decode_table_width * a->block_size > (1 << 30)) ||
+      (pre && (int64_t)a->prefill_table_width * a->block_size > (1 << 30)))
+    return fail(SLO_ERR_UNSUPPORTED, "paged_attention_fp4: tables span more than 2^30 tokens");
+  return SLO_OK;
+}
+
+}  // namespace
+}  // namespace slo
+
+using namespace slo;
+
+extern "C" int slo_paged_attention_fp4_workspace_bytes(const slo_paged_attention_args* a, size_t* bytes) {
+  if (!bytes) return fail(SLO_ERR_INVALID, "paged_attention_fp4: null pointer");
+  const int rc = check_args(a);
+  if (rc) return rc;
+  const Plan n = plan_of(a);
+  *bytes = n.dbytes + n.pbytes;
+  return SLO_OK;
+}
+
+extern "C" int slo_paged_attention_fp4(const slo_paged_attention_args* a, slo_stream_t stream) {
+  const int rc = check_args(a);
+  if (rc) return rc;
+  const Plan n = plan_of(a);
+  if (n.dbytes + n.pbytes > 0 && (!a->workspace || a->workspace_bytes < n.dbytes + n.pbytes ||
+                                  reinterpret_cast<uintptr_t>(a->workspace) % 16))
+    return fail(SLO_ERR_WORKSPACE, "paged_attention_fp4: workspace smaller than slo_paged_attention_fp4_workspace_bytes");
+  if (!n.dwork && !n.ptiles) return SLO_OK;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  Fp4Params p = {};
+  p.q = static_cast<const uint16_t*>(a->q);
+  p.q_stride = a->q_row_stride;
+  p.out = static_cast<uint16_t*>(a->out);
+  p.out_stride = a->out_row_stride;
+  p.num_q_rows = a->num_q_rows;
+  p.kc = static_cast<const uint8_t*>(a->k_cache);
+  p.vc = static_cast<const uint8_t*>(a->v_cache);
+  p.ks = reinterpret_cast<const uint8_t*>(a->k_scale);
+  p.vs = reinterpret_cast<const uint8_t*>(a->v_scale);
+  p.num_blocks = a->num_blocks;
+  p.block_size = a->block_size;
+  p.hq = a->num_heads;
+  p.hkv = a->num_kv_heads;
+  p.group = a->num_heads / a->num_kv_heads;
+  p.scale_log2 = (a->softmax_scale < 0 ? -a->softmax_scale : a->softmax_scale) * kLog2e;
+  p.q_sign = a->softmax_scale < 0 ? 0x80008000u : 0u;
+  if (n.dwork) {
+    p.lens = a->decode_lens;
+    p.tables = a->decode_tables;
+    p.table_stride = a->decode_table_stride;
+    p.table_width = a->decode_table_width;
+    p.first_row = 0;
+    p.splits = n.dsplits;
+    p.chunk = n.dchunk;
+    p.partial = static_cast<float*>(a->workspace);
+    hipLaunchKernelGGL(fp4_decode_kernel, dim3(p.hkv, p.splits, a->num_decode), dim3(256), 0, s, p);
+    if (p.splits > 1)
+      hipLaunchKernelGGL(fp4_join_kernel, dim3((p.hq + 3) / 4, a->num_decode), dim3(256), 0, s, p);
+  }
+  if (n.ptiles) {
+    p.lens = nullptr;
+    p.cu_q = a->prefill_cu_q;
+    p.cu_k = a->prefill_cu_k;
+    p.tables = a->prefill_tables;
+    p.table_stride = a->prefill_table_stride;
+    p.table_width = a->prefill_table_width;
+    p.first_row = a->num_decode;
+    p.splits = n.psplits;
+    p.chunk = n.pchunk;
+    p.partial = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + n.dbytes);
+    hipLaunchKernelGGL(fp4_prefill_kernel<kPrefillNT>, dim3(p.hkv, n.ptiles * p.splits, a->num_prefill), dim3(256), 0, s, p,
+                       n.ptiles);
+    if (p.splits > 1)
+      hipLaunchKernelGGL(fp4_join_kernel, dim3((unsigned)(((int64_t)a->max_q * p.hq + 3) / 4), a->num_prefill), dim3(256), 0, s,
+                         p);
+  }
+  return check_launch("paged_attention_fp4");
+}

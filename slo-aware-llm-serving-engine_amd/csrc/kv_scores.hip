@@ -1,0 +1,513 @@
+// Accumulated attention weights of cached tokens (gfx950).
+//
+// scores[slot of key j, kv head] += sum over the step's queries i and the
+// heads h of the kv head's group of softmax_j(scale q[i, h] . k[j]); the keys
+// that the step itself adds start from that sum.  K comes from a bf16, E4M3FN
+// or 4-bit pool; V is not read.
+//
+// S^T = K q^T by v_mfma_f32_16x16x32_bf16 (rows: 16 tokens, columns: 16 (query,
+// head) pairs), so a lane has 4 tokens of one column.  A weight needs its row's
+// maximum and sum first, so each phase takes two passes:
+//
+//  * decode rows (one query): the first pass writes the logits (fp32) and each
+//    chunk's maximum and sum, the second turns them into weights.  The logits
+//    are 4 bytes per (head, token), a sixteenth to a quarter of K itself, so K
+//    is read once.
+//  * prefill rows: the first pass finds every (query, head)'s log2-sum; the
+//    second computes S^T again, 32 keys of a wavefront against all queries,
+//    and sums the weights over the queries in registers (writing the scores of
+//    a 1,000-query chunk would take more than the two products).
+//
+// A key's sum over queries is taken in one order, whatever the grid.  Old keys
+// get it by fp32 atomic adds, so rows that share a page (a cached prefix) both
+// count; only for such a page does the order of its rows' additions vary.
+#include "capi_internal.h"
+#include "fp4.h"
+
+namespace slo {
+namespace {
+
+constexpr int HDS = 128;
+constexpr float kNone = -1e30f;
+
+struct ScoreParams {
+  const uint16_t* q;
+  int64_t q_stride;
+  int num_q_rows;
+  const uint8_t* kc;
+  const void* ks;
+  int num_blocks, block_size;
+  const int32_t* lens;
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  const int32_t* tables;
+  int table_stride, table_width;
+  int first_row;
+  int hq, hkv, group;
+  float scale_log2;
+  uint32_t q_sign;
+  float* scores;   // [num_blocks, hkv, block_size]
+  float* logits;   // decode: [rows, hq, capacity], log2 units
+  float2* partial;  // decode: [rows, hq, splits] (maximum, sum)
+  float* lse;      // prefill: [queries, hq], log2 units
+  int splits, chunk, capacity;
+};
+
+struct Row {
+  int64_t q0;
+  int lq, lk, prefix;
+};
+
+__device__ __forceinline__ Row row_of(const ScoreParams& p, int r) {
+  Row g;
+  const int cap = p.table_width * p.block_size;
+  if (p.lens) {
+    g.q0 = p.first_row + r;
+    g.lq = 1;
+    g.lk = min(max(p.lens[r], 0), cap);
+    g.prefix = g.lk - 1;
+  } else {
+    const int start = p.cu_q[r], k = p.cu_k[r + 1] - p.cu_k[r];
+    g.q0 = (int64_t)p.first_row + start;
+    g.lq = p.cu_q[r + 1] - start;
+    g.prefix = k - g.lq;
+    g.lk = min(k, cap);
+    if (start < 0 || g.q0 + g.lq > p.num_q_rows) g.lq = 0;
+  }
+  return g;
+}
+
+// Channels of a lane's k-group kg in product i, by how the format's rows load
+// in 16-byte pieces: the sum over channels is the same in any order.
+template <int KV>
+__device__ __forceinline__ int channel_of(int i, int kg) {
+  return KV == KV_BF16 ? 32 * i + 8 * kg : KV == KV_FP8_E4M3FN ? 64 * (i >> 1) + 16 * kg + 8 * (i & 1) : 32 * kg + 8 * i;
+}
+
+template <int KV>
+__device__ __forceinline__ bf16x8 load_q(const ScoreParams& p, int64_t row, int h, int i, int kg, bool live) {
+  u32x4 x = {0, 0, 0, 0};
+  if (live) x = *reinterpret_cast<const u32x4*>(p.q + row * p.q_stride + h * HDS + channel_of<KV>(i, kg));
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x[j] ^= p.q_sign;
+  return as_bf16x8(x);
+}
+
+// 16 tokens' keys of one kv head as they lie in the pool.
+template <int KV>
+struct Keys {
+  static constexpr int N = KV == KV_BF16 ? 4 : KV == KV_FP8_E4M3FN ? 2 : 1;
+  u32x4 w[N];
+  float scale[KV == KV_FP8_E4M3FN ? 4 : 1];
+  uint32_t code;
+
+  // `block` page, token `off` of it
+  __device__ __forceinline__ void load(const ScoreParams& p, int block, int off, int head, int lane) {
+    const int col = lane & 15, kg = lane >> 4;
+    if (KV == KV_FP4_E2M1) {
+      const int64_t row = ((int64_t)block * p.hkv + head) * p.block_size + off + col;
+      w[0] = *reinterpret_cast<const u32x4*>(p.kc + row * 64 + kg * 16);
+      code = static_cast<const uint8_t*>(p.ks)[row * 4 + kg];
+    } else {
+      const int64_t slot = (int64_t)block * p.block_size + off;
+      const int rb = KV == KV_BF16 ? 256 : 128;
+      const uint8_t* at = p.kc + ((slot + col) * p.hkv + head) * rb + kg * 16;
+#pragma unroll
+      for (int i = 0; i < N; ++i) w[i] = *reinterpret_cast<const u32x4*>(at + i * 64);
+      if (KV == KV_FP8_E4M3FN) {
+        const float* s = static_cast<const float*>(p.ks) + (slot + 4 * kg) * p.hkv + head;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) scale[i & (sizeof(scale) / 4 - 1)] = s[(int64_t)i * p.hkv];
+      }
+    }
+  }
+  __device__ __forceinline__ bf16x8 operand(int i) const {
+    if (KV == KV_BF16) return as_bf16x8(w[i & (N - 1)]);
+    if (KV == KV_FP8_E4M3FN) {
+      const u32x4& x = w[(i >> 1) & (N - 1)];
+      const u32x2 a = fp8x4_to_bf16x4(x[2 * (i & 1)]), b = fp8x4_to_bf16x4(x[2 * (i & 1) + 1]);
+      return as_bf16x8(u32x4{a.x, a.y, b.x, b.y});
+    }
+    return as_bf16x8(e2m1_decode8(w[0][i], e8m0(code)));
+  }
+  // token 4 kg + i's factor of the products
+  __device__ __forceinline__ float factor(int i) const { return KV == KV_FP8_E4M3FN ? scale[i & (sizeof(scale) / 4 - 1)] : 1.0f; }
+};
+
+__device__ __forceinline__ int page_of(const ScoreParams& p, int r, int token, int& off) {
+  const int page = token / p.block_size;
+  off = token - page * p.block_size;
+  const int b = p.tables[(int64_t)r * p.table_stride + page];
+  return b >= 0 && b < p.num_blocks ? b : -1;
+}
+
+// (m, l) with the maximum m and the sum l of 2^(x - m); absorbs another pair.
+__device__ __forceinline__ void absorb(float& m, float& l, float m2, float l2) {
+  const float top = fmaxf(m, m2);
+  l = l * __builtin_amdgcn_exp2f(m - top) + l2 * __builtin_amdgcn_exp2f(m2 - top);
+  m = top;
+}
+
+// Decode rows, first pass: one chunk of one (row, kv head) per workgroup, its
+// four wavefronts every fourth 16-token tile.
+template <int KV>
+__global__ void __launch_bounds__(256)
+score_logits_kernel(ScoreParams p) {
+  __shared__ float sm[4][64], sl[4][64];
+  const int head = blockIdx.x, split = blockIdx.y, r = blockIdx.z;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, kg = lane >> 4;
+  const Row g = row_of(p, r);
+  const int k0 = split * p.chunk, k1 = min(k0 + p.chunk, g.lk);
+  if (k0 >= g.lk) return;
+  bf16x8 q[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) q[i] = load_q<KV>(p, g.q0, head * p.group + col, i, kg, col < p.group);
+  float* logits = p.logits + ((int64_t)r * p.hq + head * p.group + col) * p.capacity;
+  float m = kNone, l = 0.0f;
+  for (int at = k0 + 16 * wave; at < k1; at += 64) {
+    int off;
+    const int block = page_of(p, r, at, off);
+    f32x4 s = {0, 0, 0, 0};
+    if (block >= 0) {
+      Keys<KV> k;
+      k.load(p, block, off, head, lane);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s = mfma16(k.operand(i), q[i], s);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[i] *= k.factor(i) * p.scale_log2;
+    }
+    float top = kNone;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (block < 0 || at + 4 * kg + i >= g.lk) s[i] = -INFINITY;
+      top = fmaxf(top, s[i]);
+    }
+    if (col < p.group) *reinterpret_cast<f32x4*>(logits + at + 4 * kg) = s;
+    float sum = 0.0f;
+    const float n = fmaxf(m, top);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum += __builtin_amdgcn_exp2f(s[i] - n);
+    l = l * __builtin_amdgcn_exp2f(m - n) + sum;
+    m = n;
+  }
+  sm[wave][lane] = m;
+  sl[wave][lane] = l;
+  __syncthreads();
+  if (threadIdx.x < p.group) {
+    m = kNone, l = 0.0f;
+    for (int w = 0; w < 4; ++w)
+      for (int k = 0; k < 4; ++k) absorb(m, l, sm[w][16 * k + threadIdx.x], sl[w][16 * k + threadIdx.x]);
+    p.partial[((int64_t)r * p.hq + head * p.group + threadIdx.x) * p.splits + split] = float2{m, l};
+  }
+}
+
+__device__ __forceinline__ void add_score(const ScoreParams& p, const Row& g, int block, int off, int head, int token, float w) {
+  float* s = p.scores + ((int64_t)block * p.hkv + head) * p.block_size + off;
+  if (token >= g.prefix)
+    *s = w;
+  else
+    unsafeAtomicAdd(s, w);
+}
+
+// Decode rows, second pass: one lane per token.
+__global__ void __launch_bounds__(256)
+score_decode_kernel(ScoreParams p) {
+  __shared__ float lse[16];
+  const int head = blockIdx.x, r = blockIdx.z;
+  const Row g = row_of(p, r);
+  const int token = blockIdx.y * 256 + threadIdx.x;
+  if ((int)blockIdx.y * 256 >= g.lk) return;
+  if (threadIdx.x < p.group) {
+    const int n = (g.lk + p.chunk - 1) / p.chunk;
+    const float2* e = p.partial + ((int64_t)r * p.hq + head * p.group + threadIdx.x) * p.splits;
+    float m = kNone, l = 0.0f;
+    for (int s = 0; s < n; ++s) absorb(m, l, e[s].x, e[s].y);
+    lse[threadIdx.x] = m + __builtin_amdgcn_logf(l);
+  }
+  __syncthreads();
+  if (token >= g.lk) return;
+  int off;
+  const int block = page_of(p, r, token, off);
+  if (block < 0) return;
+  const float* x = p.logits + ((int64_t)r * p.hq + head * p.group) * p.capacity + token;
+  float w = 0.0f;
+  for (int h = 0; h < p.group; ++h) w += __builtin_amdgcn_exp2f(x[(int64_t)h * p.capacity] - lse[h]);
+  add_score(p, g, block, off, head, token, w);
+}
+
+// Prefill rows, first pass: 16 NT (query, head) columns of one row per
+// workgroup, its four wavefronts every fourth 16-token tile of their keys.
+template <int KV, int NT>
+__global__ void __launch_bounds__(256)
+score_lse_kernel(ScoreParams p, int tiles) {
+  __shared__ float sm[NT][4][64], sl[NT][4][64];
+  const int head = blockIdx.x, r = blockIdx.z;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, kg = lane >> 4;
+  const int per = 16 * NT / p.group;
+  const Row g = row_of(p, r);
+  const int t0 = (tiles - 1 - (int)blockIdx.y) * per, t1 = min(t0 + per, g.lq);
+  if (t0 >= g.lq) return;
+  const int kend = min(max(g.prefix + t1, 0), g.lk);
+  bf16x8 q[NT][4];
+  int limit[NT];
+  float m[NT], l[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int x = 16 * n + col, tok = t0 + x / p.group;
+    const bool live = x < per * p.group && tok < t1;
+    limit[n] = live ? min(g.prefix + tok + 1, g.lk) : 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[n][i] = load_q<KV>(p, g.q0 + tok, head * p.group + x % p.group, i, kg, live);
+    m[n] = kNone;
+    l[n] = 0.0f;
+  }
+  const int full = min(g.prefix + t0 + 1, g.lk);
+  for (int at = 16 * wave; at < kend; at += 64) {
+    int off;
+    const int block = page_of(p, r, at, off);
+    if (block < 0) continue;
+    Keys<KV> k;
+    k.load(p, block, off, head, lane);
+    f32x4 s[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) s[n] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bf16x8 a = k.operand(i);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[n] = mfma16(a, q[n][i], s[n]);
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[n][i] *= k.factor(i) * p.scale_log2;
+        if (at + 16 > full && at + 4 * kg + i >= limit[n]) s[n][i] = -INFINITY;
+      }
+      const float top = fmaxf(fmaxf(m[n], fmaxf(s[n][0], s[n][1])), fmaxf(s[n][2], s[n][3]));
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum += __builtin_amdgcn_exp2f(s[n][i] - top);
+      l[n] = l[n] * __builtin_amdgcn_exp2f(m[n] - top) + sum;
+      m[n] = top;
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    sm[n][wave][lane] = m[n];
+    sl[n][wave][lane] = l[n];
+  }
+  __syncthreads();
+  const int x = threadIdx.x, tok = t0 + x / p.group;
+  if (x < per * p.group && tok < t1) {
+    float mm = kNone, ll = 0.0f;
+    for (int w = 0; w < 4; ++w)
+      for (int k = 0; k < 4; ++k) absorb(mm, ll, sm[x >> 4][w][16 * k + (x & 15)], sl[x >> 4][w][16 * k + (x & 15)]);
+    p.lse[(g.q0 - p.first_row + tok) * p.hq + head * p.group + x % p.group] = mm + __builtin_amdgcn_logf(ll);
+  }
+}
+
+// Prefill rows, second pass: 32 keys of one (row, kv head) per wavefront
+// against every column that sees one of them.
+template <int KV>
+__global__ void __launch_bounds__(256)
+score_prefill_kernel(ScoreParams p) {
+  const int head = blockIdx.x, r = blockIdx.z;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, kg = lane >> 4;
+  const Row g = row_of(p, r);
+  const int at = (blockIdx.y * 4 + wave) * 32;
+  if (at >= g.lk || g.lq <= 0) return;
+  int off;
+  const int block = page_of(p, r, at, off);
+  if (block < 0) return;
+  bf16x8 a[2][4];
+  float factor[2][4];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    Keys<KV> k;
+    k.load(p, block, off + 16 * h, head, lane);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[h][i] = k.operand(i);
+      factor[h][i] = k.factor(i) * p.scale_log2;
+    }
+  }
+  f32x4 w[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+  const int columns = g.lq * p.group;
+  for (int x0 = max(at - g.prefix, 0) * p.group; x0 < columns; x0 += 16) {
+    const int x = x0 + col, tok = x / p.group, hh = head * p.group + x % p.group;
+    const bool live = x < columns;
+    const float lse = live ? p.lse[(g.q0 - p.first_row + tok) * p.hq + hh] : INFINITY;
+    f32x4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bf16x8 q = load_q<KV>(p, g.q0 + tok, hh, i, kg, live);
+      s[0] = mfma16(a[0][i], q, s[0]);
+      s[1] = mfma16(a[1][i], q, s[1]);
+    }
+    const int limit = live ? min(g.prefix + tok + 1, g.lk) : 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][i], factor[h][i], -lse));
+        w[h][i] += at + 16 * h + 4 * kg + i < limit ? e : 0.0f;
+      }
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float e = w[h][i];
+#pragma unroll
+      for (int d = 1; d < 16; d <<= 1) e += __shfl_xor(e, d, 64);
+      const int token = at + 16 * h + 4 * kg + i;
+      if (col == 0 && token < g.lk) add_score(p, g, block, off + 16 * h + 4 * kg + i, head, token, e);
+    }
+}
+
+constexpr int kLseNT = 4;
+
+struct Plan {
+  int splits, chunk, tiles;
+  size_t logits, partial, lse;
+};
+
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+Plan plan_of(const slo_paged_attention_args* a) {
+  Plan n = {1, 1 << 30, 0, 0, 0, 0};
+  if (a->num_decode > 0 && (a->phases & SLO_PHASE_DECODE)) {
+    const int64_t cap = (int64_t)a->decode_table_width * a->block_size, groups = (int64_t)a->num_decode * a->num_kv_heads;
+    const int64_t want = (2048 + groups - 1) / groups;
+    int64_t c = ((cap + want - 1) / want + 127) / 128 * 128;
+    if (c < 256) c = 256;
+    n.chunk = (int)c;
+    n.splits = (int)((cap + c - 1) / c);
+    n.logits = up256((size_t)a->num_decode * a->num_heads * cap * 4);
+    n.partial = up256((size_t)a->num_decode * a->num_heads * n.splits * 8);
+  }
+  if (a->num_prefill > 0 && (a->phases & SLO_PHASE_PREFILL) && a->max_q > 0) {
+    const int per = 16 * kLseNT / (a->num_heads / a->num_kv_heads);
+    n.tiles = (a->max_q + per - 1) / per;
+    n.lse = up256((size_t)(a->num_q_rows - a->num_decode) * a->num_heads * 4);
+  }
+  return n;
+}
+
+int check_args(const slo_paged_attention_args* a) {
+  if (!a) return fail(SLO_ERR_INVALID, "accumulate_attention: null args");
+  if (a->head_dim != HDS) return fail(SLO_ERR_UNSUPPORTED, "accumulate_attention: head_dim must be 128");
+  if (a->num_heads <= 0 || a->num_kv_heads <= 0 || a->num_heads % a->num_kv_heads)
+    return fail(SLO_ERR_INVALID, "accumulate_attention: num_heads must be a multiple of num_kv_heads");
+  if (a->num_heads / a->num_kv_heads > 16)
+    return fail(SLO_ERR_UNSUPPORTED, "accumulate_attention: at most 16 query heads per kv head");
+  if (a->kv_dtype < KV_BF16 || a->kv_dtype > KV_FP4_E2M1) return fail(SLO_ERR_INVALID, "accumulate_attention: bad kv_dtype");
+  if (a->num_q_rows < 0 || a->num_decode < 0 || a->num_prefill < 0 || a->num_decode > a->num_q_rows)
+    return fail(SLO_ERR_INVALID, "accumulate_attention: bad row counts");
+  if (!(a->softmax_scale != 0.0f) || a->softmax_scale - a->softmax_scale != 0.0f)
+    return fail(SLO_ERR_INVALID, "accumulate_attention: softmax_scale must be finite and not zero");
+  if (a->num_decode > 65535 || a->num_prefill > 65535)
+    return fail(SLO_ERR_UNSUPPORTED, "accumulate_attention: more than 65535 rows");
+  const bool dec = a->num_decode > 0 && (a->phases & SLO_PHASE_DECODE);
+  const bool pre = a->num_prefill > 0 && (a->phases & SLO_PHASE_PREFILL);
+  if (!dec && !pre) return SLO_OK;
+  if (!a->q) return fail(SLO_ERR_INVALID, "accumulate_attention: null pointer");
+  if ((a->q_row_stride % 8) || a->q_row_stride < a->num_heads * HDS || (reinterpret_cast<uintptr_t>(a->q) % 16))
+    return fail(SLO_ERR_INVALID, "accumulate_attention: q rows must be 16-byte aligned");
+  if (!a->k_cache || a->num_blocks <= 0) return fail(SLO_ERR_INVALID, "accumulate_attention: no KV pool");
+  if (a->kv_dtype != KV_BF16 && !a->k_scale) return fail(SLO_ERR_INVALID, "accumulate_attention: a quantised pool needs k_scale");
+  if (reinterpret_cast<uintptr_t>(a->k_cache) % 16)
+    return fail(SLO_ERR_INVALID, "accumulate_attention: the pool must be 16-byte aligned");
+  if (a->block_size <= 0 || a->block_size % 64)
+    return fail(SLO_ERR_UNSUPPORTED, "accumulate_attention: block_size must be a multiple of 64");
+  if (dec && (!a->decode_lens || !a->decode_tables || a->decode_table_width <= 0))
+    return fail(SLO_ERR_INVALID, "accumulate_attention: missing decode metadata");
+  if (pre && (!a->prefill_cu_q || !a->prefill_cu_k || !a->prefill_tables || a->prefill_table_width <= 0))
+    return fail(SLO_ERR_INVALID, "accumulate_attention: missing prefill metadata");
+  if ((dec && (int64_t)a->decode_table_width * a->block_size > (1 << 24)) ||
+      (pre && (int64_t)a->prefill_table_width * a->block_size > (1 << 24)))
+    return fail(SLO_ERR_UNSUPPORTED, "accumulate_attention: tables span more than 2^24 tokens");
+  return SLO_OK;
+}
+
+template <int KV>
+void launch(const ScoreParams& d, const ScoreParams& f, const slo_paged_attention_args* a, const Plan& n, hipStream_t s) {
+  if (n.logits) {
+    hipLaunchKernelGGL(score_logits_kernel<KV>, dim3(d.hkv, d.splits, a->num_decode), dim3(256), 0, s, d);
+    hipLaunchKernelGGL(score_decode_kernel, dim3(d.hkv, (d.capacity + 255) / 256, a->num_decode), dim3(256), 0, s, d);
+  }
+  if (n.tiles) {
+    hipLaunchKernelGGL((score_lse_kernel<KV, kLseNT>), dim3(f.hkv, n.tiles, a->num_prefill), dim3(256), 0, s, f, n.tiles);
+    const int cap = f.table_width * f.block_size;
+    hipLaunchKernelGGL(score_prefill_kernel<KV>, dim3(f.hkv, (cap + 127) / 128, a->num_prefill), dim3(256), 0, s, f);
+  }
+}
+
+}  // namespace
+}  // namespace slo
+
+using namespace slo;
+
+extern "C" int slo_accumulate_attention_workspace_bytes(const slo_paged_attention_args* a, size_t* bytes) {
+  if (!bytes) return fail(SLO_ERR_INVALID, "accumulate_attention: null pointer");
+  const int rc = check_args(a);
+  if (rc) return rc;
+  const Plan n = plan_of(a);
+  *bytes = n.logits + n.partial + n.lse;
+  return SLO_OK;
+}
+
+extern "C" int slo_accumulate_attention(const slo_paged_attention_args* a, float* scores, slo_stream_t stream) {
+  const int rc = check_args(a);
+  if (rc) return rc;
+  const Plan n = plan_of(a);
+  const size_t need = n.logits + n.partial + n.lse;
+  if (!need) return SLO_OK;
+  if (!scores) return fail(SLO_ERR_INVALID, "accumulate_attention: null pointer");
+  if (!a->workspace || a->workspace_bytes < need || reinterpret_cast<uintptr_t>(a->workspace) % 16)
+    return fail(SLO_ERR_WORKSPACE, "accumulate_attention: workspace smaller than slo_accumulate_attention_workspace_bytes");
+  ScoreParams p = {};
+  p.q = static_cast<const uint16_t*>(a->q);
+  p.q_stride = a->q_row_stride;
+  p.num_q_rows = a->num_q_rows;
+  p.kc = static_cast<const uint8_t*>(a->k_cache);
+  p.ks = a->k_scale;
+  p.num_blocks = a->num_blocks;
+  p.block_size = a->block_size;
+  p.hq = a->num_heads;
+  p.hkv = a->num_kv_heads;
+  p.group = a->num_heads / a->num_kv_heads;
+  p.scale_log2 = (a->softmax_scale < 0 ? -a->softmax_scale : a->softmax_scale) * kLog2e;
+  p.q_sign = a->softmax_scale < 0 ? 0x80008000u : 0u;
+  p.scores = scores;
+  char* ws = static_cast<char*>(a->workspace);
+  ScoreParams d = p, f = p;
+  d.lens = a->decode_lens;
+  d.tables = a->decode_tables;
+  d.table_stride = a->decode_table_stride;
+  d.table_width = a->decode_table_width;
+  d.splits = n.splits;
+  d.chunk = n.chunk;
+  d.capacity = a->decode_table_width * a->block_size;
+  d.logits = reinterpret_cast<float*>(ws);
+  d.partial = reinterpret_cast<float2*>(ws + n.logits);
+  f.cu_q = a->prefill_cu_q;
+  f.cu_k = a->prefill_cu_k;
+  f.tables = a->prefill_tables;
+  f.table_stride = a->prefill_table_stride;
+  f.table_width = a->prefill_table_width;
+  f.first_row = a->num_decode;
+  f.lse = reinterpret_cast<float*>(ws + n.logits + n.partial);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (a->kv_dtype == KV_BF16)
+    launch<KV_BF16>(d, f, a, n, s);
+  else if (a->kv_dtype == KV_FP8_E4M3FN)
+    launch<KV_FP8_E4M3FN>(d, f, a, n, s);
+  else
+    launch<KV_FP4_E2M1>(d, f, a, n, s);
+  return check_launch("accumulate_attention");
+}

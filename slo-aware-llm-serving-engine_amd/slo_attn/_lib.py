@@ -16,6 +16,7 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
 SLO_OK = 0
 KV_BF16 = 0
 KV_FP8_E4M3FN = 1
+KV_FP4_E2M1 = 2
 PHASE_DECODE = 1
 PHASE_PREFILL = 2
 PHASE_ALL = 3
@@ -23,6 +24,7 @@ NEW_ROWS_STRIDED = 256  # or-ed into phases: strided new K/V rows (decode rows o
 FP8_SCALE_FLOOR = 2.0 ** -64
 NOALLOC_SCRATCH_BYTES = 64 << 20
 FP8_MAX = 448.0
+FP4_GROUP = 32  # channels per scale of a 4-bit pool
 
 _c_int32 = ctypes.c_int32
 _c_int64 = ctypes.c_int64
@@ -62,6 +64,20 @@ class PagedAttentionArgs(ctypes.Structure):
     ]
 
 
+class EvictKvArgs(ctypes.Structure):
+    """Mirror of ``slo_evict_kv_args`` (include/slo_attn.h)."""
+
+    _fields_ = [
+        ("k_cache", _c_void_p), ("v_cache", _c_void_p), ("k_scale", _c_void_p), ("v_scale", _c_void_p),
+        ("scores", _c_void_p),
+        ("kv_dtype", _c_int32), ("num_layers", _c_int32), ("num_blocks", _c_int32), ("block_size", _c_int32),
+        ("num_kv_heads", _c_int32), ("head_dim", _c_int32), ("num_rows", _c_int32),
+        ("lens", _c_void_p), ("tables", _c_void_p), ("table_stride", _c_int32), ("table_width", _c_int32),
+        ("budget", _c_int32), ("recent", _c_int32),
+        ("new_lens", _c_void_p), ("kept", _c_void_p),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -74,6 +90,14 @@ EXPORTS = (
     "slo_paged_attention",
     "slo_paged_attention_noalloc",
     "slo_attention_workspace_check",
+    "slo_store_kvcache_fp4",
+    "slo_load_kvcache",
+    "slo_paged_attention_fp4_workspace_bytes",
+    "slo_paged_attention_fp4",
+    "slo_accumulate_attention_workspace_bytes",
+    "slo_accumulate_attention",
+    "slo_evict_kv",
+    "slo_evict_kv_args_size",
     "slo_last_error",
     "slo_paged_attention_args_size",
 )
@@ -118,12 +142,33 @@ def load() -> ctypes.CDLL:
         lib.slo_paged_attention_noalloc.argtypes = [ctypes.POINTER(PagedAttentionArgs), _c_void_p]
         lib.slo_attention_workspace_check.restype = ctypes.c_int
         lib.slo_attention_workspace_check.argtypes = [_c_void_p, ctypes.c_size_t, _c_void_p, _c_void_p]
+        lib.slo_store_kvcache_fp4.restype = ctypes.c_int
+        lib.slo_store_kvcache_fp4.argtypes = [
+            _c_void_p, _c_int64, _c_void_p, _c_int64, _c_void_p, _c_int32, _c_int32, _c_int32, _c_void_p, _c_void_p,
+            _c_void_p, _c_void_p, _c_int32, _c_int32, ctypes.c_float, _c_void_p]
+        lib.slo_load_kvcache.restype = ctypes.c_int
+        lib.slo_load_kvcache.argtypes = [
+            _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int32, _c_int32, _c_int32, _c_void_p, _c_int32, _c_int32,
+            _c_int32, _c_void_p, _c_void_p, _c_void_p]
+        for name in ("slo_paged_attention_fp4_workspace_bytes", "slo_accumulate_attention_workspace_bytes"):
+            getattr(lib, name).restype = ctypes.c_int
+            getattr(lib, name).argtypes = [ctypes.POINTER(PagedAttentionArgs), ctypes.POINTER(ctypes.c_size_t)]
+        lib.slo_paged_attention_fp4.restype = ctypes.c_int
+        lib.slo_paged_attention_fp4.argtypes = [ctypes.POINTER(PagedAttentionArgs), _c_void_p]
+        lib.slo_accumulate_attention.restype = ctypes.c_int
+        lib.slo_accumulate_attention.argtypes = [ctypes.POINTER(PagedAttentionArgs), _c_void_p, _c_void_p]
+        lib.slo_evict_kv.restype = ctypes.c_int
+        lib.slo_evict_kv.argtypes = [ctypes.POINTER(EvictKvArgs), _c_void_p]
+        lib.slo_evict_kv_args_size.restype = ctypes.c_size_t
+        lib.slo_evict_kv_args_size.argtypes = []
         lib.slo_last_error.restype = ctypes.c_char_p
         lib.slo_last_error.argtypes = []
         lib.slo_paged_attention_args_size.restype = ctypes.c_size_t
         lib.slo_paged_attention_args_size.argtypes = []
         if lib.slo_paged_attention_args_size() != ctypes.sizeof(PagedAttentionArgs):
             raise RuntimeError("slo_paged_attention_args layout mismatch between header and binding")
+        if lib.slo_evict_kv_args_size() != ctypes.sizeof(EvictKvArgs):
+            raise RuntimeError("slo_evict_kv_args layout mismatch between header and binding")
         _lib = lib
         return lib
 

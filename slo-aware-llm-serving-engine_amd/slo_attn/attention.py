@@ -12,7 +12,12 @@ Mirrors nanovllm/layers/attention.py:33-79: same constructor, attributes
 
 Optional ``k_scale`` / ``v_scale`` attributes (fp32
 ``[num_blocks, block_size, num_kv_heads]``) select the E4M3FN pool when the
-runner assigns uint8 / float8_e4m3fn ``k_cache`` / ``v_cache`` views.
+runner assigns uint8 / float8_e4m3fn ``k_cache`` / ``v_cache`` views; with
+float4_e2m1fn_x2 views they are the E8M0 scales of a 4-bit pool (``KVPool``
+allocates either).  An optional ``kv_scores`` attribute (fp32 ``[num_blocks,
+num_kv_heads, block_size]``) has every step add its attention weights to the
+scores of the cached tokens (``accumulate_attention``); all rows then need
+block tables.
 ``forward(q, k, v, kv_stored=True)`` skips the KV write, for callers whose
 ``qk_norm_rope_store`` already wrote this step's K/V into the pool.
 """
@@ -24,7 +29,7 @@ from torch import nn
 from . import _lib
 from .context import get_context
 from .mixed_attention import forward_mixed
-from .ops import check_store, foldable, folds_alone, paged_attention, store_kvcache
+from .ops import accumulate_attention, check_store, foldable, folds_alone, is_fp4, paged_attention, store_kvcache
 
 __all__ = ["Attention", "store_kvcache"]
 
@@ -43,6 +48,7 @@ class Attention(nn.Module):
         self.num_kv_heads = num_kv_heads
         self.k_cache = self.v_cache = torch.tensor([])
         self.k_scale = self.v_scale = None
+        self.kv_scores = None
 
     def _scales(self):
         return () if self.k_scale is None else (self.k_scale, self.v_scale)
@@ -51,8 +57,15 @@ class Attention(nn.Module):
         context = get_context()
         k_cache, v_cache = self.k_cache, self.v_cache
         if context.mixed is not None:
-            return forward_mixed(q, k, v, k_cache, v_cache, context, self.scale,
-                                 _stored if kv_stored else store_kvcache, self.k_scale, self.v_scale)
+            o = forward_mixed(q, k, v, k_cache, v_cache, context, self.scale,
+                              _stored if kv_stored else store_kvcache, self.k_scale, self.v_scale)
+            if self.kv_scores is not None:
+                meta = context.mixed
+                self._weigh(q, num_decode=meta.num_decode, decode_lens=meta.decode_lens, decode_tables=meta.decode_tables,
+                            num_prefill=meta.prefill_cu_q.numel() - 1 if meta.num_prefill_tokens else 0,
+                            prefill_cu_q=meta.prefill_cu_q, prefill_cu_k=meta.prefill_cu_k, max_q=meta.max_q,
+                            max_k=meta.max_k, prefill_tables=meta.prefill_tables)
+            return o
         have_cache = bool(k_cache.numel() and v_cache.numel())
         # The pool is written inside the attention launch (same result, one
         # launch less) in decode steps, also from views of the QKV projection
@@ -65,7 +78,7 @@ class Attention(nn.Module):
         # contiguous bf16 rows only; otherwise the store kernel runs first.
         paged = context.is_prefill and context.block_tables is not None
         fold = have_cache and not kv_stored and (
-            (self.k_scale is None and foldable(k, v))
+            (self.k_scale is None and not is_fp4(k_cache) and foldable(k, v))
             or (not paged and folds_alone(q, k, v, k_cache, self.k_scale)))
         if fold:
             check_store(k, v, k_cache, v_cache, context.slot_mapping, *self._scales())
@@ -75,7 +88,7 @@ class Attention(nn.Module):
         if context.is_prefill:
             rows = context.cu_seqlens_q.numel() - 1
             pool = paged or fold
-            return paged_attention(
+            o = paged_attention(
                 q, k_cache if pool else None, v_cache if pool else None, self.scale,
                 num_kv_heads=self.num_kv_heads, k_scale=self.k_scale if pool else None,
                 v_scale=self.v_scale if pool else None, num_prefill=rows,
@@ -83,9 +96,20 @@ class Attention(nn.Module):
                 max_q=context.max_seqlen_q, max_k=context.max_seqlen_k,
                 prefill_tables=context.block_tables, k=None if paged else k, v=None if paged else v,
                 phases=_lib.PHASE_ALL if paged else _lib.PHASE_ALL | _lib.NEW_ROWS_STRIDED, **store)
+            if self.kv_scores is not None and have_cache:
+                self._weigh(q, num_prefill=rows, prefill_cu_q=context.cu_seqlens_q, prefill_cu_k=context.cu_seqlens_k,
+                            max_q=context.max_seqlen_q, max_k=context.max_seqlen_k, prefill_tables=context.block_tables)
+            return o
         o = paged_attention(
             q, k_cache, v_cache, self.scale, num_kv_heads=self.num_kv_heads,
             k_scale=self.k_scale, v_scale=self.v_scale, num_decode=q.shape[0],
             decode_lens=context.context_lens, decode_tables=context.block_tables,
             phases=_lib.PHASE_ALL | _lib.NEW_ROWS_STRIDED, **store)
+        if self.kv_scores is not None:
+            self._weigh(q, num_decode=q.shape[0], decode_lens=context.context_lens, decode_tables=context.block_tables)
         return o.unsqueeze(1)
+
+    def _weigh(self, q, **rows):
+        """The step's attention weights into ``kv_scores``."""
+        accumulate_attention(q, self.k_cache, self.kv_scores, self.scale, num_kv_heads=self.num_kv_heads,
+                             k_scale=self.k_scale, **rows)

@@ -14,7 +14,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .ops import check_store, foldable, folds_alone, paged_attention, store_kvcache
+from .ops import check_store, foldable, folds_alone, is_fp4, paged_attention, store_kvcache
 
 
 @dataclass
@@ -36,7 +36,8 @@ def forward_mixed(q, k, v, k_cache, v_cache, context, scale, store_fn,
     """Write all new K/V first, then attend: decode rows first, prefill after.
 
     Same arguments as the reference (mixed_attention.py:29).  ``k_scale`` /
-    ``v_scale`` are the fp32 scale pools of an E4M3FN cache.  ``phases``
+    ``v_scale`` are the fp32 scale pools of an E4M3FN cache or the E8M0 ones of
+    a 4-bit cache.  ``phases``
     restricts the launch to decode or prefill rows (the split mode that mirrors
     the reference's per-phase calls); rows of the other phase are left
     untouched in the returned tensor.
@@ -57,7 +58,8 @@ def forward_mixed(q, k, v, k_cache, v_cache, context, scale, store_fn,
     # tokens' tiles in every item (24 decode rows and two chunks, one after a
     # 1,024-token prefix: 108 against 72 us).  Any other store_fn runs first.
     alone = not meta.num_prefill_tokens or (not meta.num_decode and not meta.prefill_has_history)
-    fold = (store_fn is store_kvcache and phases == _lib.PHASE_ALL
+    # A 4-bit pool keeps the store kernel: its launches read pages only.
+    fold = (store_fn is store_kvcache and phases == _lib.PHASE_ALL and not is_fp4(k_cache)
             and ((foldable(k, v)
                   and (k_scale is None or (q.shape[1] <= 8 * k.shape[1] and not meta.num_prefill_tokens)))
                  or (alone and folds_alone(q, k, v, k_cache, k_scale))))

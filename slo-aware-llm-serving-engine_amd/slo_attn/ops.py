@@ -15,6 +15,8 @@ import torch
 
 from . import _lib
 
+_FP4_DTYPE = getattr(torch, "float4_e2m1fn_x2", None)
+_E8M0_DTYPES = (torch.uint8,) + ((torch.float8_e8m0fnu,) if hasattr(torch, "float8_e8m0fnu") else ())
 _FP8_DTYPES = (torch.uint8,) + ((torch.float8_e4m3fn,) if hasattr(torch, "float8_e4m3fn") else ())
 
 
@@ -23,7 +25,56 @@ def kv_dtype_code(cache: torch.Tensor) -> int:
         return _lib.KV_BF16
     if cache.dtype in _FP8_DTYPES:
         return _lib.KV_FP8_E4M3FN
-    raise TypeError(f"KV cache dtype {cache.dtype} is not bf16 or E4M3FN bytes")
+    if cache.dtype == _FP4_DTYPE:
+        return _lib.KV_FP4_E2M1
+    raise TypeError(f"KV cache dtype {cache.dtype} is not bf16, E4M3FN bytes or float4_e2m1fn_x2")
+
+
+def is_fp4(cache: torch.Tensor | None) -> bool:
+    """Whether a pool view is a 4-bit one (``torch.float4_e2m1fn_x2``: two E2M1 codes a byte)."""
+    return cache is not None and _FP4_DTYPE is not None and cache.dtype == _FP4_DTYPE
+
+
+def _pool_geometry(k_cache, k_scale, v_cache=None, v_scale=None, head_dim=None, want_v=True):
+    """Checks a layer's pool views and returns ``(code, blocks, block_size, kv_heads, head_dim)``.
+
+    bf16 and E4M3FN pools are ``[blocks, block_size, kv_heads, head_dim]`` with
+    fp32 scales ``[blocks, block_size, kv_heads]`` (E4M3FN); 4-bit pools
+    ``[blocks, kv_heads, block_size, head_dim / 2]`` with E8M0 scales
+    ``[blocks, kv_heads, block_size, head_dim / 32]``.
+    """
+    code = kv_dtype_code(k_cache)
+    caches, scales = ((k_cache, v_cache), (k_scale, v_scale)) if want_v else ((k_cache,), (k_scale,))
+    for c in caches:
+        if kv_dtype_code(c) != code:
+            raise TypeError("k_cache and v_cache formats differ")
+        if c.dim() != 4 or c.shape != k_cache.shape or not c.is_contiguous():
+            raise ValueError("KV pool views must be contiguous, 4-dimensional and of one shape")
+    if code == _lib.KV_FP4_E2M1:
+        blocks, heads, block, d = k_cache.shape
+        d *= 2
+        shape, dtypes = (blocks, heads, block, d // _lib.FP4_GROUP), _E8M0_DTYPES
+    else:
+        blocks, block, heads, d = k_cache.shape
+        shape, dtypes = (blocks, block, heads), (torch.float32,)
+    if head_dim is not None and d != head_dim:
+        raise ValueError(f"KV pool holds head_dim {d}, not {head_dim}")
+    if code != _lib.KV_BF16:
+        for sc in scales:
+            if sc is None:
+                raise ValueError("a quantised pool needs its scales")
+            if sc.dtype not in dtypes or tuple(sc.shape) != shape or not sc.is_contiguous():
+                kind = "E8M0" if code == _lib.KV_FP4_E2M1 else "fp32"
+                raise ValueError(f"scale pools must be contiguous {kind} {list(shape)}")
+    return code, blocks, block, heads, d
+
+
+def _check_scores(kv_scores, blocks, heads, block, layers=()):
+    if kv_scores.dtype != torch.float32:
+        raise TypeError("kv_scores must be fp32")
+    if tuple(kv_scores.shape) != (*layers, blocks, heads, block) or \
+            not kv_scores.is_contiguous():
+        raise ValueError("kv_scores must be contiguous fp32 [num_blocks, num_kv_heads, block_size]")
 
 
 def _require_gpu(*tensors) -> torch.device:
@@ -62,6 +113,8 @@ def check_store(key, value, k_cache, v_cache, slot_mapping, k_scale=None, v_scal
     formats); returns ``(device, kv_dtype code)``."""
     N, num_heads, head_dim = key.shape
     D = num_heads * head_dim
+    if is_fp4(k_cache):
+        return _check_store_fp4(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale)
     # Same stride contract as the reference store (attention.py:36-39).
     assert key.stride(-1) == 1 and value.stride(-1) == 1
     assert key.stride(1) == head_dim and value.stride(1) == head_dim
@@ -84,6 +137,23 @@ def check_store(key, value, k_cache, v_cache, slot_mapping, k_scale=None, v_scal
         for s in (k_scale, v_scale):
             if s.dtype != torch.float32 or not s.is_contiguous() or s.numel() != num_slots * num_heads:
                 raise ValueError("scale pools must be contiguous fp32 [num_blocks, block_size, num_kv_heads]")
+    _int32(slot_mapping, "slot_mapping")
+    return device, code
+
+
+def _check_store_fp4(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale):
+    N, num_heads, head_dim = key.shape
+    assert key.stride(-1) == 1 and value.stride(-1) == 1
+    assert key.stride(1) == head_dim and value.stride(1) == head_dim
+    assert slot_mapping.numel() == N
+    device = _require_gpu(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale)
+    if key.dtype != torch.bfloat16 or value.dtype != torch.bfloat16:
+        raise TypeError("key/value must be bf16")
+    if value.shape != key.shape:
+        raise ValueError("key/value shapes differ")
+    code, _, _, heads, _ = _pool_geometry(k_cache, k_scale, v_cache, v_scale, head_dim)
+    if heads != num_heads:
+        raise ValueError("KV pool must be [num_blocks, num_kv_heads, block_size, head_dim / 2]")
     _int32(slot_mapping, "slot_mapping")
     return device, code
 
@@ -115,9 +185,9 @@ def folds_alone(q: torch.Tensor, key: torch.Tensor, value: torch.Tensor, k_cache
     carries the KV write of ``key``/``value``: ``foldable_strided`` rows, one
     per query row, into a 4-dimensional pool view; with an E4M3FN pool at most
     8 query heads per kv head.  Everything else (keys of a whole cold row
-    beside the queries of its last tokens, a pool view of merged heads) keeps
-    the store kernel's own launch, which takes it."""
-    return (key.dim() == 3 and key.shape[0] == q.shape[0] and k_cache.dim() == 4 and foldable_strided(key, value)
+    beside the queries of its last tokens, a pool view of merged heads, a 4-bit
+    pool) keeps the store kernel's own launch, which takes it."""
+    return (not is_fp4(k_cache) and key.dim() == 3 and key.shape[0] == q.shape[0] and k_cache.dim() == 4 and foldable_strided(key, value)
             and (k_scale is None or q.shape[1] <= 8 * key.shape[1]))
 
 
@@ -131,16 +201,49 @@ def store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
     strided (a view of the fused QKV output).  ``k_cache``/``v_cache``:
     ``[num_blocks, block_size, num_kv_heads, head_dim]``; for E4M3FN caches
     (uint8 or float8_e4m3fn) ``k_scale``/``v_scale`` are the fp32
-    ``[num_blocks, block_size, num_kv_heads]`` scale pools.
+    ``[num_blocks, block_size, num_kv_heads]`` scale pools.  4-bit caches
+    (float4_e2m1fn_x2) are ``[num_blocks, num_kv_heads, block_size,
+    head_dim / 2]`` with E8M0 scales ``[num_blocks, num_kv_heads, block_size,
+    head_dim / 32]`` (uint8 or float8_e8m0fnu), one per 32 channels;
+    ``scale_floor`` is then a power of two.
     """
     device, code = check_store(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale)
     N, num_heads, head_dim = key.shape
+    if code == _lib.KV_FP4_E2M1:
+        _lib.check(_lib.load().slo_store_kvcache_fp4(
+            _ptr(key), key.stride(0), _ptr(value), value.stride(0), _ptr(slot_mapping), N, num_heads, head_dim,
+            _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), k_cache.shape[0], k_cache.shape[2],
+            float(scale_floor), _stream(device)), "slo_store_kvcache_fp4")
+        return
     num_slots = k_cache.shape[0] * k_cache.shape[1]
     lib = _lib.load()
     _lib.check(lib.slo_store_kvcache(
         _ptr(key), key.stride(0), _ptr(value), value.stride(0), _ptr(slot_mapping), N, num_heads,
         head_dim, code, _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), num_slots,
         float(scale_floor), _stream(device)), "slo_store_kvcache")
+
+
+def load_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: torch.Tensor,
+                 k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None):
+    """Cached tokens read back: ``(k, v)``, bf16 ``[N, num_kv_heads, head_dim]`` rows of the tokens at
+    ``slot_mapping`` (int32), the inverse of ``store_kvcache``.
+
+    For moving tokens to a pool of another format or to the host.  bf16 rows
+    come back as stored, 4-bit values exactly, E4M3FN values as code * scale
+    rounded to bf16; a slot outside the pool gives zeros.
+    """
+    device = _require_gpu(k_cache, v_cache, slot_mapping, k_scale, v_scale)
+    code, blocks, block, heads, head_dim = _pool_geometry(k_cache, k_scale, v_cache, v_scale)
+    _int32(slot_mapping, "slot_mapping")
+    if slot_mapping.dim() != 1:
+        raise ValueError("slot_mapping must be a 1-dimensional int32 tensor")
+    N = slot_mapping.numel()
+    k = torch.empty((N, heads, head_dim), dtype=torch.bfloat16, device=device)
+    v = torch.empty_like(k)
+    _lib.check(_lib.load().slo_load_kvcache(
+        _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), code, blocks, block, _ptr(slot_mapping), N, heads,
+        head_dim, _ptr(k), _ptr(v), _stream(device)), "slo_load_kvcache")
+    return k, v
 
 
 # ------------------------------------------- fused q/k norm + RoPE + KV write
@@ -169,8 +272,9 @@ def qk_norm_rope_store(qkv: torch.Tensor, positions: torch.Tensor, q_norm_weight
     ``qkv``: ``[N, (num_heads + 2*num_kv_heads) * head_dim]`` bf16 (the fused
     projection output; rows may be strided).  Returns ``(q, k, v)``: q and k
     normalised and rotated (new contiguous bf16 tensors), v a view of ``qkv``.
-    The pool receives the rotated k and v at ``slot_mapping`` (bf16 or
-    E4M3FN with ``k_scale``/``v_scale``), as ``store_kvcache`` writes them.
+    The pool receives the rotated k and v at ``slot_mapping`` (bf16, or
+    E4M3FN or 4 bits with ``k_scale``/``v_scale``), as ``store_kvcache`` writes
+    them; into a 4-bit pool they go in a second launch.
     """
     if qkv.dim() != 2 or qkv.stride(-1) != 1:
         raise ValueError("qkv must be a [tokens, width] tensor with contiguous rows")
@@ -195,9 +299,14 @@ def qk_norm_rope_store(qkv: torch.Tensor, positions: torch.Tensor, q_norm_weight
         raise TypeError("k_cache and v_cache formats differ")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError("KV pool views must be contiguous")
-    if k_cache.shape[-2:] != (num_kv_heads, head_dim) or v_cache.shape != k_cache.shape:
+    fp4 = code == _lib.KV_FP4_E2M1
+    if fp4:
+        if _pool_geometry(k_cache, k_scale, v_cache, v_scale, head_dim)[3] != num_kv_heads:
+            raise ValueError("KV pool must be [num_blocks, num_kv_heads, block_size, head_dim / 2]")
+    elif k_cache.shape[-2:] != (num_kv_heads, head_dim) or v_cache.shape != k_cache.shape:
         raise ValueError("KV pool must be [num_blocks, block_size, num_kv_heads, head_dim]")
-    num_slots = k_cache.shape[0] * k_cache.shape[1]
+    # A pool of no slots: the fused kernel writes q and k only.
+    num_slots = 0 if fp4 else k_cache.shape[0] * k_cache.shape[1]
     if code == _lib.KV_FP8_E4M3FN:
         if k_scale is None or v_scale is None:
             raise ValueError("an E4M3FN pool needs k_scale and v_scale")
@@ -212,9 +321,11 @@ def qk_norm_rope_store(qkv: torch.Tensor, positions: torch.Tensor, q_norm_weight
     _lib.check(_lib.load().slo_qk_norm_rope_store(
         _ptr(qkv), qkv.stride(0), _ptr(positions), N, num_heads, num_kv_heads, head_dim, _ptr(q_norm_weight),
         _ptr(k_norm_weight), float(eps), _ptr(cos_sin), cos_sin.shape[0], _ptr(q), _ptr(k), _ptr(slot_mapping),
-        code, _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), num_slots, float(scale_floor),
-        _stream(device)), "slo_qk_norm_rope_store")
+        _lib.KV_BF16 if fp4 else code, _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), num_slots,
+        float(scale_floor), _stream(device)), "slo_qk_norm_rope_store")
     v = qkv[:, (num_heads + num_kv_heads) * head_dim:].view(N, num_kv_heads, head_dim)
+    if fp4:
+        store_kvcache(k, v, k_cache, v_cache, slot_mapping, k_scale, v_scale, scale_floor)
     return q, k, v
 
 
@@ -320,6 +431,147 @@ def reserve_workspace(device, max_decode_rows: int, max_decode_len: int, num_hea
 
 
 # ---------------------------------------------------------------- attention
+def _pool_args(args, k_cache, k_scale, v_cache, v_scale, num_kv_heads, head_dim, want_v=True):
+    code, blocks, block, heads, _ = _pool_geometry(k_cache, k_scale, v_cache, v_scale, head_dim, want_v)
+    if heads != num_kv_heads:
+        raise ValueError(f"KV pool holds {heads} kv heads, not {num_kv_heads}")
+    args.kv_dtype, args.num_blocks, args.block_size = code, blocks, block
+    args.k_cache, args.k_scale = _ptr(k_cache), _ptr(k_scale)
+    args.v_cache, args.v_scale = _ptr(v_cache), _ptr(v_scale)
+
+
+def _row_args(args, T, num_decode, decode_lens, decode_tables, num_prefill, cu_q, cu_k, max_q, max_k, tables, phases):
+    """Fills in the rows of the asked phases, all read through block tables."""
+    args.num_decode, args.phases = num_decode, phases
+    if not 0 <= num_decode <= T:
+        raise ValueError("num_decode must be from 0 to the number of query rows")
+    if num_decode and phases & _lib.PHASE_DECODE:
+        _int32(decode_lens, "decode_lens")
+        _int32(decode_tables, "decode_tables")
+        if decode_tables.dim() != 2 or decode_tables.stride(1) != 1:
+            raise ValueError("decode_tables must be a row-major [rows, width] int32 tensor")
+        if decode_lens.numel() < num_decode or decode_tables.shape[0] < num_decode:
+            raise ValueError("decode metadata has fewer rows than num_decode")
+        args.decode_lens, args.decode_tables = _ptr(decode_lens), _ptr(decode_tables)
+        args.decode_table_stride, args.decode_table_width = decode_tables.stride(0), decode_tables.shape[1]
+    if num_prefill and phases & _lib.PHASE_PREFILL:
+        _int32(cu_q, "cu_seqlens_q")
+        _int32(cu_k, "cu_seqlens_k")
+        _int32(tables, "block_tables")
+        if cu_q.numel() < num_prefill + 1 or cu_k.numel() < num_prefill + 1:
+            raise ValueError("cu_seqlens shorter than num_prefill + 1")
+        if tables.dim() != 2 or tables.stride(1) != 1 or tables.shape[0] < num_prefill:
+            raise ValueError("block_tables must be a row-major [rows, width] int32 tensor")
+        args.num_prefill, args.prefill_cu_q, args.prefill_cu_k = num_prefill, _ptr(cu_q), _ptr(cu_k)
+        args.max_q, args.max_k = int(max_q), int(max_k)
+        args.prefill_tables = _ptr(tables)
+        args.prefill_table_stride, args.prefill_table_width = tables.stride(0), tables.shape[1]
+
+
+def _own_workspace(args, size_of, what, device):
+    """A workspace of the call's own, from torch's allocator: calls on several streams, and graphs captured apart,
+    do not share it.  It need not be cleared.  Returned to keep it alive until the launch is enqueued."""
+    need = ctypes.c_size_t(0)
+    _lib.check(size_of(ctypes.byref(args), ctypes.byref(need)), what)
+    if need.value:
+        ws = torch.empty(need.value, dtype=torch.uint8, device=device)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), need.value
+        return ws
+    return None
+
+
+def accumulate_attention(q: torch.Tensor, k_cache: torch.Tensor, kv_scores: torch.Tensor, softmax_scale: float, *,
+                         num_kv_heads: int, k_scale: torch.Tensor | None = None, num_decode: int = 0,
+                         decode_lens: torch.Tensor | None = None, decode_tables: torch.Tensor | None = None,
+                         num_prefill: int = 0, prefill_cu_q: torch.Tensor | None = None,
+                         prefill_cu_k: torch.Tensor | None = None, max_q: int = 0, max_k: int = 0,
+                         prefill_tables: torch.Tensor | None = None, phases: int = _lib.PHASE_ALL) -> None:
+    """Adds the attention weights of a step's queries to their keys' scores.
+
+    The rows are ``paged_attention``'s, over a bf16, E4M3FN or 4-bit pool, all
+    read through block tables.  ``kv_scores`` (fp32 ``[num_blocks,
+    num_kv_heads, block_size]``) gains, for every cached key of a row, the sum
+    over the row's queries and over the query heads of the kv head of their
+    softmax weights; the row's new tokens (the last one of a decode row, the
+    last ``cu_q[r+1] - cu_q[r]`` of a prefill row) start from that sum, whatever
+    their slots held.  A cached prefix that was never weighed has to be zero
+    (``KVPool.reset_blocks``).  Rows of one call may share old pages: each adds
+    its weights, in an order that is not fixed.  ``evict_kv`` reads the scores.
+    """
+    if q.dim() != 3:
+        raise ValueError("q must be [tokens, num_heads, head_dim]")
+    T, num_heads, head_dim = q.shape
+    device = _require_gpu(q, k_cache, kv_scores, k_scale, decode_lens, decode_tables, prefill_cu_q, prefill_cu_k,
+                          prefill_tables)
+    if q.dtype != torch.bfloat16:
+        raise TypeError("q must be bf16")
+    if q.stride(-1) != 1 or q.stride(1) != head_dim:
+        raise ValueError("q rows must hold contiguous heads")
+    phases &= _lib.PHASE_ALL
+    if num_prefill and phases & _lib.PHASE_PREFILL and prefill_tables is None:
+        raise ValueError("accumulate_attention reads prefill rows through block tables")
+    args = _lib.PagedAttentionArgs()
+    args.q, args.q_row_stride, args.num_q_rows = _ptr(q), q.stride(0), T
+    _pool_args(args, k_cache, k_scale, None, None, num_kv_heads, head_dim, want_v=False)
+    _check_scores(kv_scores, args.num_blocks, num_kv_heads, args.block_size)
+    _row_args(args, T, num_decode, decode_lens, decode_tables, num_prefill, prefill_cu_q, prefill_cu_k, max_q, max_k,
+              prefill_tables, phases)
+    args.num_heads, args.num_kv_heads, args.head_dim = num_heads, num_kv_heads, head_dim
+    args.softmax_scale = float(softmax_scale)
+    ws = _own_workspace(args, _lib.load().slo_accumulate_attention_workspace_bytes, "slo_accumulate_attention", device)
+    _lib.check(_lib.load().slo_accumulate_attention(ctypes.byref(args), _ptr(kv_scores), _stream(device)),
+               "slo_accumulate_attention")
+    del ws
+
+
+def evict_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, kv_scores: torch.Tensor, lens: torch.Tensor,
+             tables: torch.Tensor, budget: int, recent: int, k_scale: torch.Tensor | None = None,
+             v_scale: torch.Tensor | None = None):
+    """Cuts rows of more than ``budget`` cached tokens back to it; returns ``(new_lens, kept)``.
+
+    Such a row keeps, for every kv head by itself, its newest ``recent`` tokens
+    and the ``budget - recent`` others with the largest ``kv_scores`` (ties: the
+    lowest position; NaN below every number).  They are moved, in position
+    order, with their scales and scores, to the row's first ``budget`` places,
+    so the row is from then on one of ``budget`` tokens whose further pages can
+    be freed; the scores of the places given up become zero.  Rotated keys keep
+    their positions: new tokens go to the next free place of the row but are
+    rotated by their own position in the text.
+
+    ``lens`` int32 ``[rows]`` and ``tables`` int32 ``[rows, width]`` describe the
+    rows; no two may share a page.  With a leading layer dimension on the pools,
+    the scales and the scores (``pool.kv[0]`` of every layer), all layers are cut
+    by one call, each by its own scores.  ``new_lens`` is int32 ``[rows]``,
+    ``kept`` the kept positions, int32 ``[(layers,) rows, num_kv_heads, budget]``,
+    -1 past a row that is shorter.
+    """
+    device = _require_gpu(k_cache, v_cache, kv_scores, lens, tables, k_scale, v_scale)
+    layered = k_cache.dim() == 5
+    if layered and (v_cache.shape != k_cache.shape or kv_scores.shape[:1] != k_cache.shape[:1]
+                    or any(s is not None and s.shape[:1] != k_cache.shape[:1] for s in (k_scale, v_scale))
+                    or any(t is not None and not t.is_contiguous() for t in (k_cache, v_cache, kv_scores, k_scale, v_scale))):
+        raise ValueError("pools, scales and scores of several layers must be contiguous, with one leading layer dimension")
+    layers = k_cache.shape[0] if layered else 1
+    one = [t if t is None or not layered else t[0] for t in (k_cache, k_scale, v_cache, v_scale)]
+    code, blocks, block, heads, head_dim = _pool_geometry(*one)
+    _check_scores(kv_scores, blocks, heads, block, (layers,) if layered else ())
+    _int32(lens, "lens")
+    _int32(tables, "tables")
+    if lens.dim() != 1 or tables.dim() != 2 or tables.stride(1) != 1 or tables.shape[0] != lens.numel():
+        raise ValueError("lens must be [rows] and tables a row-major [rows, width] int32 tensor")
+    rows, budget, recent = lens.numel(), int(budget), int(recent)
+    if budget <= 0 or not 0 <= recent <= budget:
+        raise ValueError("budget must be positive and recent from 0 to budget")
+    new_lens = torch.empty(rows, dtype=torch.int32, device=device)
+    kept = torch.empty((*((layers,) if layered else ()), rows, heads, budget), dtype=torch.int32, device=device)
+    args = _lib.EvictKvArgs(
+        _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(kv_scores), code, layers, blocks, block, heads,
+        head_dim, rows, _ptr(lens), _ptr(tables), tables.stride(0), tables.shape[1], budget, recent, _ptr(new_lens),
+        _ptr(kept))
+    _lib.check(_lib.load().slo_evict_kv(ctypes.byref(args), _stream(device)), "slo_evict_kv")
+    return new_lens, kept
+
+
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor | None, v_cache: torch.Tensor | None,
                     softmax_scale: float, *, num_kv_heads: int,
                     k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
@@ -350,6 +602,12 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor | None, v_cache: torc
     store (``store_scale_floor``), the new tokens are read as its codes and
     scales, and at most 8 query heads may share a kv head.
 
+    A 4-bit pool (``store_kvcache``) is read by kernels of its own, one launch
+    for the decode rows and one for the prefill rows (and one that joins the
+    parts of long rows); ``store_slot_mapping`` then stores first.  Prefill rows
+    without tables read no pool and run as with any other.  ``noalloc`` is
+    refused.
+
     ``noalloc=True`` launches through ``slo_paged_attention_noalloc``, which
     uses the library's static per-GPU scratch instead of this module's
     workspace (pass ``out`` as well and nothing is allocated).
@@ -371,6 +629,31 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor | None, v_cache: torc
     args.q, args.q_row_stride = q.data_ptr(), q.stride(0)
     args.out, args.out_row_stride = out.data_ptr(), out.stride(0)
     args.num_q_rows = T
+    if is_fp4(k_cache):
+        if out.dtype != torch.bfloat16:
+            raise TypeError("out must be bf16")
+        if noalloc:
+            raise ValueError("noalloc launches take bf16 and E4M3FN pools")
+        if store_slot_mapping is not None:
+            store_kvcache(new_k, new_v, k_cache, v_cache, store_slot_mapping, k_scale, v_scale, store_scale_floor)
+        phases &= _lib.PHASE_ALL
+        if num_prefill and prefill_tables is None and phases & _lib.PHASE_PREFILL:
+            paged_attention(q, None, None, softmax_scale, num_kv_heads=num_kv_heads, num_decode=num_decode,
+                            decode_lens=decode_lens, decode_tables=decode_tables, num_prefill=num_prefill,
+                            prefill_cu_q=prefill_cu_q, prefill_cu_k=prefill_cu_k, max_q=max_q, max_k=max_k, k=k, v=v,
+                            phases=_lib.PHASE_PREFILL, out=out)
+            phases &= ~_lib.PHASE_PREFILL
+        if not phases:
+            return out
+        _pool_args(args, k_cache, k_scale, v_cache, v_scale, num_kv_heads, head_dim)
+        _row_args(args, T, num_decode, decode_lens, decode_tables, num_prefill, prefill_cu_q, prefill_cu_k, max_q, max_k,
+                  prefill_tables, phases)
+        args.num_heads, args.num_kv_heads, args.head_dim = num_heads, num_kv_heads, head_dim
+        args.softmax_scale = float(softmax_scale)
+        ws = _own_workspace(args, _lib.load().slo_paged_attention_fp4_workspace_bytes, "slo_paged_attention_fp4", device)
+        _lib.check(_lib.load().slo_paged_attention_fp4(ctypes.byref(args), _stream(device)), "slo_paged_attention_fp4")
+        del ws
+        return out
     code = _lib.KV_BF16
     if k_cache is not None and k_cache.numel():
         code = kv_dtype_code(k_cache)

@@ -83,18 +83,17 @@ struct Tile {
 };
 
 __device__ __forceinline__ void load_tile(Tile& t, const Fp4Params& p, int64_t row, int lane) {
-  const int c = lane & 15, kg = lane >> 4;
-  const uint8_t* k = p.kc + row * 64 + c * 64 + kg * 16;
-  const uint8_t* v = p.vc + row * 64 + kg * 256 + c * 4;
-  const uint8_t* ks = p.ks + row * 4 + c * 4 + kg;
-  const uint8_t* vs = p.vs + row * 4 + kg * 16;
+  // `row` is the wavefront's: scalar bases, and 32-bit offsets of the lane.
+  const uint32_t c = lane & 15, kg = lane >> 4;
+  const uint8_t *k = p.kc + row * 64, *v = p.vc + row * 64, *ks = p.ks + row * 4, *vs = p.vs + row * 4;
+  const uint32_t ko = c * 64 + kg * 16, vo = kg * 256 + c * 4, kso = c * 4 + kg, vso = kg * 16;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    t.k[h] = *reinterpret_cast<const u32x4*>(k + h * 1024);
-    t.ks[h] = ks[h * 64];
-    t.vs[h] = *reinterpret_cast<const u32x4*>(vs + h * 64);
+    t.k[h] = *reinterpret_cast<const u32x4*>(k + (ko + h * 1024));
+    t.ks[h] = ks[kso + h * 64];
+    t.vs[h] = *reinterpret_cast<const u32x4*>(vs + (vso + h * 64));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) t.v[4 * h + i] = *reinterpret_cast<const uint32_t*>(v + h * 1024 + i * 64);
+    for (int i = 0; i < 4; ++i) t.v[4 * h + i] = *reinterpret_cast<const uint32_t*>(v + (vo + h * 1024 + i * 64));
   }
 }
 
@@ -111,8 +110,27 @@ __device__ __forceinline__ float column_max(float x) {  // over the four lanes o
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-template <int NT, bool MASK>
-__device__ __forceinline__ void step(const Tile& t, const bf16x8 (&q)[NT][4], Acc<NT>& a, float c, int kv0,
+// The reference of column n's weights follows a new maximum only where a score
+// passes it by 2^8: weights up to 256 round like those below 1, and the
+// rescaling of the outputs is rare.
+template <int NT>
+__device__ __forceinline__ void move_reference(Acc<NT>& a, int n, float top) {
+  if (__any(top > a.m[n] + 8.0f)) {
+    const float m = fmaxf(a.m[n], column_max(top));
+    const float w = __builtin_amdgcn_exp2f(a.m[n] - m);
+    a.m[n] = m;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) a.o[n][e] *= w;
+    a.l[n] *= w;
+  }
+}
+
+__device__ __forceinline__ bf16x8 ones() {
+  return as_bf16x8(u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
+}
+
+template <int NT>
+__device__ __forceinline__ void step(const Tile& t, bool masked, const bf16x8 (&q)[NT][4], Acc<NT>& a, float c, int kv0,
                                      const int (&limit)[NT], int kend, int lane) {
   const int kg = lane >> 4;
   f32x4 s[NT][2];
@@ -129,7 +147,7 @@ __device__ __forceinline__ void step(const Tile& t, const bf16x8 (&q)[NT][4], Ac
   bf16x8 pr[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    if (MASK) {
+    if (masked) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -139,16 +157,7 @@ __device__ __forceinline__ void step(const Tile& t, const bf16x8 (&q)[NT][4], Ac
     float top = fmaxf(s[n][0][0], s[n][0][1]);
 #pragma unroll
     for (int i = 2; i < 8; ++i) top = fmaxf(top, s[n][i >> 2][i & 3]);
-    // The reference only moves where a score passes it by 2^8: probabilities
-    // up to 256 round like those below 1, and the outputs' rescale is rare.
-    if (__any(top * c > a.m[n] + 8.0f)) {
-      const float m = fmaxf(a.m[n], column_max(top) * c);
-      const float w = __builtin_amdgcn_exp2f(a.m[n] - m);
-      a.m[n] = m;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) a.o[n][e] *= w;
-      a.l[n] *= w;
-    }
+    move_reference(a, n, top * c);
     u32x4 b;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -156,15 +165,22 @@ __device__ __forceinline__ void step(const Tile& t, const bf16x8 (&q)[NT][4], Ac
                          __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i >> 1][2 * (i & 1) + 1], c, -a.m[n])));
     pr[n] = as_bf16x8(b);
   }
+  // The lane's scale byte of each token, rotated to the exponent's place: the
+  // conversion reads nothing but the exponent of its scale (all mantissas and
+  // both signs give the same bits, checked on gfx950).
   float vs[8];
-  const int byte = 8 * ((lane & 15) >> 2);
+  const int turn = (9 + 8 * ((lane & 15) >> 2)) & 31;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    uint32_t code = (t.vs[j >> 2][j & 3] >> byte) & 0xffu;
-    // A token past the row's keys may be anything in the pages: its weight is
-    // zero, and its scale must not make that a NaN.
-    if (MASK) code = kv0 + 16 * (j >> 2) + 4 * kg + (j & 3) < kend ? code : 0u;
-    vs[j] = e8m0(code);
+    const uint32_t x = t.vs[j >> 2][j & 3];
+    vs[j] = __uint_as_float(__builtin_amdgcn_alignbit(x, x, turn));
+  }
+  // A token past the row's keys may be anything in the pages: its weight is
+  // zero, and its scale must not make that a NaN.
+  if (masked) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (kv0 + 16 * (j >> 2) + 4 * kg + (j & 3) >= kend) vs[j] = 0.0f;
   }
   auto pair = [&](auto sel) {
     constexpr int B = decltype(sel)::value;
@@ -183,9 +199,8 @@ __device__ __forceinline__ void step(const Tile& t, const bf16x8 (&q)[NT][4], Ac
       a.o[n][2 * B + 1] = mfma16(as_bf16x8(hi), pr[n], a.o[n][2 * B + 1]);
     }
   };
-  const bf16x8 ones = as_bf16x8(u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
 #pragma unroll
-  for (int n = 0; n < NT; ++n) a.l[n] = mfma16(ones, pr[n], a.l[n]);
+  for (int n = 0; n < NT; ++n) a.l[n] = mfma16(ones(), pr[n], a.l[n]);
   pair(std::integral_constant<int, 0>{});
   pair(std::integral_constant<int, 1>{});
   pair(std::integral_constant<int, 2>{});
@@ -218,26 +233,21 @@ __device__ __forceinline__ void attend(const Fp4Params& p, int r, int head, cons
   if (begin >= end) return;
   Walk w{p.tables + (int64_t)r * p.table_stride, begin / p.block_size, 0, p.block_size, p.num_blocks, p.hkv, head};
   w.off = begin - w.page * p.block_size;
-  Tile t[2];
-  bool ok[2];
-  int64_t row = w.row(ok[0]);
-  load_tile(t[0], p, row, lane);
-  for (int kv0 = begin; kv0 < end; kv0 += 2 * stride) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int at = kv0 + u * stride;
-      if (at >= end) break;
-      if (at + stride < end) {
-        w.advance(stride);
-        row = w.row(ok[u ^ 1]);
-        load_tile(t[u ^ 1], p, row, lane);
-      }
-      if (!ok[u]) continue;
-      if (at + KT <= full)
-        step<NT, false>(t[u], q, a, p.scale_log2, at, limit, kend, lane);
-      else
-        step<NT, true>(t[u], q, a, p.scale_log2, at, limit, kend, lane);
+  Tile t;
+  bool ok;
+  int64_t row = w.row(ok);
+  load_tile(t, p, row, lane);
+  for (int at = begin; at < end; at += stride) {
+    Tile n;
+    bool next_ok = false;
+    if (at + stride < end) {
+      w.advance(stride);
+      row = w.row(next_ok);
+      load_tile(n, p, row, lane);
     }
+    if (ok) step<NT>(t, at + KT > full, q, a, p.scale_log2, at, limit, kend, lane);
+    t = n;
+    ok = next_ok;
   }
 }
 
@@ -263,7 +273,7 @@ __device__ __forceinline__ void clear(Acc<NT>& a) {
 // Decode rows: a workgroup takes one chunk of one (row, kv head), its four
 // wavefronts every fourth 32-token step, all heads of the group as columns.
 // The wavefronts' results meet in LDS.
-__global__ void __launch_bounds__(256, 2)
+__global__ void __launch_bounds__(256, 3)
 fp4_decode_kernel(Fp4Params p) {
   __shared__ float so[4][16][HD4];
   __shared__ float sm[4][16], sl[4][16];
@@ -321,54 +331,194 @@ fp4_decode_kernel(Fp4Params p) {
   }
 }
 
-// Prefill rows: a wavefront takes 16 NT columns, (query, head of the group)
-// pairs of consecutive queries of one row, over its keys (or one chunk of
-// them), the latest queries first; the four wavefronts of a workgroup take
-// neighbouring columns and so read the same tokens from L1.
+// One 64-token step of a workgroup as bf16 operands in LDS, in the order in
+// which lanes read them (16 bytes a lane, no bank twice): K's four operands of
+// each 16 tokens, V's eight of each 32 tokens.
+struct Stage {
+  u32x4 k[4][4][64], v[2][8][64];
+};
+
+// A wavefront's quarter of a step: 16 tokens of K, and four channels of every
+// lane's eight of 32 tokens of V.
+struct Quarter {
+  u32x4 k, vs[2];
+  uint32_t ks;
+  uint16_t v[8];
+};
+
+__device__ __forceinline__ void load_quarter(Quarter& t, const Fp4Params& p, int64_t row, int wave, int lane) {
+  const uint32_t c = lane & 15, kg = lane >> 4;
+  const uint8_t *k = p.kc + (row + 16 * wave) * 64, *ks = p.ks + (row + 16 * wave) * 4;
+  const int64_t vrow = row + 32 * (wave >> 1);
+  const uint8_t *v = p.vc + vrow * 64 + 2 * (wave & 1), *vs = p.vs + vrow * 4;
+  const uint32_t ko = c * 64 + kg * 16, kso = c * 4 + kg, vo = kg * 256 + c * 4, vso = kg * 16;
+  t.k = *reinterpret_cast<const u32x4*>(k + ko);
+  t.ks = ks[kso];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    t.vs[h] = *reinterpret_cast<const u32x4*>(vs + (vso + h * 64));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t.v[4 * h + i] = *reinterpret_cast<const uint16_t*>(v + (vo + h * 1024 + i * 64));
+  }
+}
+
+// `left`: tokens of the step that belong to the row; V's scales past them are
+// cleared (see step).
+__device__ __forceinline__ void stage(Stage& s, const Quarter& t, int left, int wave, int lane) {
+  const int c = lane & 15, kg = lane >> 4;
+  const float sc = e8m0(t.ks);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s.k[wave][i][lane] = e2m1_decode8(t.k[i], sc);
+  float vs[8];
+  const int turn = (9 + 8 * (c >> 2)) & 31;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t x = t.vs[j >> 2][j & 3];
+    vs[j] = __uint_as_float(__builtin_amdgcn_alignbit(x, x, turn));
+  }
+  if (left < 64) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (32 * (wave >> 1) + 16 * (j >> 2) + 4 * kg + (j & 3) >= left) vs[j] = 0.0f;
+  }
+  u32x4 o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t a0 = e2m1_pair<0>(t.v[2 * i], vs[2 * i]), b0 = e2m1_pair<0>(t.v[2 * i + 1], vs[2 * i + 1]);
+    const uint32_t a1 = e2m1_pair<1>(t.v[2 * i], vs[2 * i]), b1 = e2m1_pair<1>(t.v[2 * i + 1], vs[2 * i + 1]);
+    o[0][i] = __builtin_amdgcn_perm(b0, a0, 0x05040100u);
+    o[1][i] = __builtin_amdgcn_perm(b0, a0, 0x07060302u);
+    o[2][i] = __builtin_amdgcn_perm(b1, a1, 0x05040100u);
+    o[3][i] = __builtin_amdgcn_perm(b1, a1, 0x07060302u);
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) s.v[wave >> 1][4 * (wave & 1) + e][lane] = o[e];
+}
+
+// 64 tokens of a wavefront's columns against the staged operands.
 template <int NT>
-__global__ void __launch_bounds__(256, 1)
+__device__ __forceinline__ void staged_step(const Stage& st, bool masked, const bf16x8 (&q)[NT][4], Acc<NT>& a, float c, int kv0,
+                                            const int (&limit)[NT], int lane) {
+  const int kg = lane >> 4;
+  f32x4 s[NT][4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bf16x8 k = as_bf16x8(st.k[t][i][lane]);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[n][t] = mfma16(k, q[n][i], i ? s[n][t] : f32x4{0, 0, 0, 0});
+    }
+  }
+  bf16x8 pr[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    if (masked) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (kv0 + 16 * t + 4 * kg + i >= limit[n]) s[n][t][i] = -INFINITY;
+    }
+    float top = fmaxf(s[n][0][0], s[n][0][1]);
+#pragma unroll
+    for (int i = 2; i < 16; ++i) top = fmaxf(top, s[n][i >> 2][i & 3]);
+    move_reference(a, n, top * c);
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      u32x4 b;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x4& x = s[n][2 * g + (i >> 1)];
+        b[i] = pack_bf16x2(__builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * (i & 1)], c, -a.m[n])),
+                           __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * (i & 1) + 1], c, -a.m[n])));
+      }
+      pr[n][g] = as_bf16x8(b);
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) a.l[n] = mfma16(ones(), pr[n][g], a.l[n]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const bf16x8 v = as_bf16x8(st.v[g][e][lane]);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) a.o[n][e] = mfma16(v, pr[n][g], a.o[n][e]);
+    }
+  }
+}
+
+// Prefill rows: a workgroup takes 64 NT columns, (query, head of the group)
+// pairs of consecutive queries of one row, over its keys (or one chunk of
+// them), the latest queries first.  Its four wavefronts turn each 64-token
+// step's codes into operands together, each a quarter, one step ahead of the
+// products, and each runs 16 NT columns over them.
+template <int NT>
+__global__ void __launch_bounds__(256, 2)
 fp4_prefill_kernel(Fp4Params p, int tiles) {
+  __shared__ Stage st[2];
   const int head = blockIdx.x, r = blockIdx.z;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int split = blockIdx.y % p.splits;
-  const int tile = (tiles - 1 - (int)(blockIdx.y / p.splits)) * 4 + wave;
   const int per = 16 * NT / p.group;  // queries of a wavefront
   const Row g = row_of(p, r);
-  const int t0 = tile * per, t1 = min(t0 + per, g.lq);
-  if (t0 >= g.lq) return;
-  const int kend = min(max(g.prefix + t1, 0), g.lk);
-  const int k0 = split * p.chunk, k1 = p.splits == 1 ? kend : min(k0 + p.chunk, kend);
-  if (split && k0 >= kend) return;
+  const int w0 = (tiles - 1 - (int)(blockIdx.y / p.splits)) * 4 * per;  // the workgroup's first query
+  if (w0 >= g.lq) return;
+  const int all = min(max(g.prefix + min(w0 + 4 * per, g.lq), 0), g.lk);  // keys that one of its queries sees
+  const int k0 = split * p.chunk, k1 = p.splits == 1 ? all : min(k0 + p.chunk, all);
+  if (split && k0 >= all) return;
+  const int t0 = w0 + wave * per, t1 = min(t0 + per, g.lq);
+  const int kend = t0 < g.lq ? min(max(g.prefix + t1, 0), g.lk) : 0;  // that one of the wavefront's sees
+  const int full = min(g.prefix + t0 + 1, g.lk);                      // that all of them see
   const int col = lane & 15, kg = lane >> 4;
   bf16x8 q[NT][4];
-  int limit[NT], tok[NT], h[NT];
-  bool live[NT];
+  int limit[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const int x = 16 * n + col;
-    tok[n] = t0 + x / p.group;
-    h[n] = head * p.group + x % p.group;
-    live[n] = x < per * p.group && tok[n] < t1;
-    limit[n] = live[n] ? min(g.prefix + tok[n] + 1, g.lk) : 0;
+    const int x = 16 * n + col, tok = t0 + x / p.group;
+    const bool live = x < per * p.group && tok < t1;
+    limit[n] = live ? min(g.prefix + tok + 1, g.lk) : 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) q[n][i] = load_q(p, g.q0 + tok[n], h[n], 32 * kg + 8 * i, live[n]);
+    for (int i = 0; i < 4; ++i) q[n][i] = load_q(p, g.q0 + tok, head * p.group + x % p.group, 32 * kg + 8 * i, live);
   }
   Acc<NT> a;
   clear(a);
-  attend<NT>(p, r, head, q, a, k0, k1, KT, min(g.prefix + t0 + 1, g.lk), limit, kend, lane);
+  if (k0 < k1) {
+    Walk w{p.tables + (int64_t)r * p.table_stride, k0 / p.block_size, 0, p.block_size, p.num_blocks, p.hkv, head};
+    w.off = k0 - w.page * p.block_size;
+    Quarter t;
+    bool ok, next_ok = false;
+    load_quarter(t, p, w.row(ok), wave, lane);
+    for (int at = k0, b = 0; at < k1; at += 64, b ^= 1) {
+      stage(st[b], t, all - at, wave, lane);
+      if (at + 64 < k1) {
+        w.advance(64);
+        load_quarter(t, p, w.row(next_ok), wave, lane);
+      }
+      // Two buffers: a wavefront comes to write this one again only past the
+      // next step's barrier, when every wavefront has left it.
+      __syncthreads();
+      if (ok && at < kend) staged_step<NT>(st[b], at + 64 > full, q, a, p.scale_log2, at, limit, lane);
+      ok = next_ok;
+    }
+  }
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    if (!live[n]) continue;
+    int x = 16 * n + col;
+    asm("" : "+v"(x));  // found again here, so that the loop need not hold it in registers
+    const int tok = t0 + x / p.group, h = head * p.group + x % p.group;
+    if (x >= per * p.group || tok >= t1) continue;
     if (p.splits == 1) {
       const float inv = a.l[n][0] == 0.0f ? 0.0f : 1.0f / a.l[n][0];
-      uint16_t* out = p.out + (g.q0 + tok[n]) * p.out_stride + h[n] * HD4 + 32 * kg;
+      uint16_t* out = p.out + (g.q0 + tok) * p.out_stride + h * HD4 + 32 * kg;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         *reinterpret_cast<u32x4*>(out + 8 * i) =
             u32x4{pack_bf16x2(a.o[n][0][i] * inv, a.o[n][1][i] * inv), pack_bf16x2(a.o[n][2][i] * inv, a.o[n][3][i] * inv),
                   pack_bf16x2(a.o[n][4][i] * inv, a.o[n][5][i] * inv), pack_bf16x2(a.o[n][6][i] * inv, a.o[n][7][i] * inv)};
     } else {
-      float* rec = p.partial + (((g.q0 - p.first_row + tok[n]) * p.hq + h[n]) * p.splits + split) * RECORD;
+      float* rec = p.partial + (((g.q0 - p.first_row + tok) * p.hq + h) * p.splits + split) * RECORD;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -383,45 +533,70 @@ fp4_prefill_kernel(Fp4Params p, int tiles) {
   }
 }
 
-// Joins the partial results of the phase's chunks, in chunk order: one
-// wavefront per (query, head), two channels a lane.
-__global__ void __launch_bounds__(256)
+// Joins the partial results of the phase's chunks: a workgroup of W half
+// wavefronts per (query, head), four channels a lane.  Half wavefront i takes
+// chunks i, i + W, ... and the W sums meet in LDS in that order.
+template <int W>
+__global__ void __launch_bounds__(32 * W < 256 ? 256 : 32 * W)
 fp4_join_kernel(Fp4Params p) {
-  const int lane = threadIdx.x & 63;
-  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  constexpr int UNITS = 32 * W < 256 ? 8 / W : 1;  // (query, head) pairs of a workgroup
+  __shared__ f32x4 so[UNITS][W][32];
+  __shared__ float sl[UNITS][W];
+  const int lane = threadIdx.x & 31, i = (threadIdx.x >> 5) % W, u = (threadIdx.x >> 5) / W;
   const int r = blockIdx.y;
   const Row g = row_of(p, r);
-  const int i = (int)(unit / p.hq), h = (int)(unit % p.hq);
-  if (i >= g.lq) return;
-  const int kend = min(max(g.prefix + i + 1, 0), g.lk);
-  const int n = min(max(1, (kend + p.chunk - 1) / p.chunk), p.splits);
-  const float* rec = p.partial + ((g.q0 - p.first_row + i) * p.hq + h) * (int64_t)p.splits * RECORD;
+  const int unit = (int)blockIdx.x * UNITS + u, query = unit / p.hq, h = unit - query * p.hq;
+  const bool live = query < g.lq;
+  const int kend = min(max(g.prefix + query + 1, 0), g.lk);
+  const int n = live ? min(max(1, (kend + p.chunk - 1) / p.chunk), p.splits) : 0;
+  const float* rec = p.partial + ((g.q0 - p.first_row + (live ? query : 0)) * p.hq + h) * (int64_t)p.splits * RECORD;
   float m = kNone;
-  for (int s = lane; s < n; s += 64) m = fmaxf(m, rec[(int64_t)s * RECORD + HD4]);
+  for (int s = lane; s < n; s += 32) m = fmaxf(m, rec[(int64_t)s * RECORD + HD4]);
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) m = wave_max_xor(m, d);
-  float x = 0, y = 0, l = 0;
-  for (int s = 0; s < n; ++s) {
+  for (int d = 1; d < 32; d <<= 1) m = wave_max_xor(m, d);
+  f32x4 o = {0, 0, 0, 0};
+  float l = 0;
+#pragma unroll 4
+  for (int s = i; s < n; s += W) {
     const float* e = rec + (int64_t)s * RECORD;
     const float w = __builtin_amdgcn_exp2f(e[HD4] - m);
-    x += e[2 * lane] * w;
-    y += e[2 * lane + 1] * w;
+    o += *reinterpret_cast<const f32x4*>(e + 4 * lane) * w;
     l += e[HD4 + 1] * w;
   }
+  if (W > 1) {
+    so[u][i][lane] = o;
+    if (lane == 0) sl[u][i] = l;
+    __syncthreads();
+    if (i) return;
+#pragma unroll
+    for (int k = 1; k < W; ++k) {
+      o += so[u][k][lane];
+      l += sl[u][k];
+    }
+  }
+  if (!live) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  *reinterpret_cast<uint32_t*>(p.out + (g.q0 + i) * p.out_stride + h * HD4 + 2 * lane) = pack_bf16x2(x * inv, y * inv);
+  *reinterpret_cast<u32x2*>(p.out + (g.q0 + query) * p.out_stride + h * HD4 + 4 * lane) =
+      u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
+}
+
+void launch_join(const Fp4Params& p, int64_t units, int rows, hipStream_t s) {
+  // Many chunks: 8 half wavefronts share them.
+  if (p.splits > 8)
+    hipLaunchKernelGGL(fp4_join_kernel<8>, dim3((unsigned)units, rows), dim3(256), 0, s, p);
+  else
+    hipLaunchKernelGGL(fp4_join_kernel<1>, dim3((unsigned)((units + 7) / 8), rows), dim3(256), 0, s, p);
 }
 
 constexpr int kPrefillNT = 2;
+constexpr int kDecodeTarget = 1024, kPrefillTarget = 640;
 
-// Workgroups that fill the GPU (256 CUs) about four times over: chunks of a
-// long row are split off until a launch has that many.
-int splits_of(int64_t groups, int64_t capacity, int least, int most_groups, int& chunk) {
-  int64_t want = (most_groups + groups - 1) / groups;
-  int64_t c = (capacity + want - 1) / (want < 1 ? 1 : want);
-  c = (c + 127) / 128 * 128;
+// Chunks of `capacity` keys for a launch of so many workgroups per chunk:
+// enough for `target` workgroups, at least `least` keys each.
+int splits_of(int64_t groups, int64_t capacity, int least, int target, int& chunk) {
+  const int64_t want = groups > 0 ? (target + groups - 1) / groups : 1;
+  int64_t c = ((capacity + want - 1) / want + 127) / 128 * 128;
   if (c < least) c = least;
-  if (c > (1 << 30)) c = 1 << 30;
   chunk = (int)c;
   const int64_t n = (capacity + c - 1) / c;
   return n < 1 ? 1 : (int)n;
@@ -437,7 +612,7 @@ Plan plan_of(const slo_paged_attention_args* a) {
   Plan n = {false, 1, 1 << 30, 1, 1 << 30, 0, 0, 0};
   if (a->num_decode > 0 && (a->phases & SLO_PHASE_DECODE)) {
     n.dwork = true;
-    n.dsplits = splits_of((int64_t)a->num_decode * a->num_kv_heads, (int64_t)a->decode_table_width * a->block_size, 256, 2048,
+    n.dsplits = splits_of((int64_t)a->num_decode * a->num_kv_heads, (int64_t)a->decode_table_width * a->block_size, 256, kDecodeTarget,
                           n.dchunk);
     if (n.dsplits > 1) n.dbytes = (size_t)a->num_decode * a->num_heads * n.dsplits * RECORD * 4;
   }
@@ -445,8 +620,9 @@ Plan plan_of(const slo_paged_attention_args* a) {
     const int per = 16 * kPrefillNT / (a->num_heads / a->num_kv_heads);
     n.ptiles = ((a->max_q + per - 1) / per + 3) / 4;
     const int64_t cap = (int64_t)a->prefill_table_width * a->block_size;
-    n.psplits = splits_of((int64_t)a->num_prefill * a->num_kv_heads * n.ptiles, cap < a->max_k ? cap : a->max_k, 512, 512,
-                          n.pchunk);
+    // The rows' queries together, not every row's maximum, make the workgroups.
+    const int64_t tiles = (a->num_q_rows - a->num_decode) / (4 * per) + a->num_prefill;
+    n.psplits = splits_of(tiles * a->num_kv_heads, cap < a->max_k ? cap : a->max_k, 512, kPrefillTarget, n.pchunk);
     if (n.psplits > 1) n.pbytes = (size_t)(a->num_q_rows - a->num_decode) * a->num_heads * n.psplits * RECORD * 4;
   }
   return n;
@@ -543,7 +719,7 @@ extern "C" int slo_paged_attention_fp4(const slo_paged_attention_args* a, slo_st
     p.partial = static_cast<float*>(a->workspace);
     hipLaunchKernelGGL(fp4_decode_kernel, dim3(p.hkv, p.splits, a->num_decode), dim3(256), 0, s, p);
     if (p.splits > 1)
-      hipLaunchKernelGGL(fp4_join_kernel, dim3((p.hq + 3) / 4, a->num_decode), dim3(256), 0, s, p);
+      launch_join(p, p.hq, a->num_decode, s);
   }
   if (n.ptiles) {
     p.lens = nullptr;
@@ -559,8 +735,7 @@ extern "C" int slo_paged_attention_fp4(const slo_paged_attention_args* a, slo_st
     hipLaunchKernelGGL(fp4_prefill_kernel<kPrefillNT>, dim3(p.hkv, n.ptiles * p.splits, a->num_prefill), dim3(256), 0, s, p,
                        n.ptiles);
     if (p.splits > 1)
-      hipLaunchKernelGGL(fp4_join_kernel, dim3((unsigned)(((int64_t)a->max_q * p.hq + 3) / 4), a->num_prefill), dim3(256), 0, s,
-                         p);
+      launch_join(p, (int64_t)a->max_q * p.hq, a->num_prefill, s);
   }
   return check_launch("paged_attention_fp4");
 }

@@ -21,6 +21,7 @@
 // Sums, maxima and outputs are fp32 until the one rounding at the end.
 #include "capi_internal.h"
 #include "fp4.h"
+#include "tile_io.h"
 #include <type_traits>
 
 namespace slo {
@@ -48,8 +49,9 @@ struct Fp4Params {
   int hq, hkv, group;
   float scale_log2;  // |softmax scale| * log2(e)
   uint32_t q_sign;   // 0x80008000 where the scale is negative
-  float* partial;    // [query rows of the phase, hq, splits] records when splits > 1
-  int splits, chunk;
+  float* partial;    // prefill rows: [queries, hq, splits] records when splits > 1; decode rows: [chunks, hq]
+  int splits, chunk;  // prefill rows
+  int rows, budget;   // decode rows: about so many chunks over all rows
 };
 
 struct Row {
@@ -76,24 +78,101 @@ __device__ __forceinline__ Row row_of(const Fp4Params& p, int r) {
   return g;
 }
 
-// One step's cache lines in registers.
+// The chunks of the decode rows, found on the GPU from the rows' lengths (a
+// captured launch knows no more of them than its tables' width): chunks of one
+// length over all rows, in units of 128 tokens, such that there are about
+// `budget`; a row's own are equal.  Every wavefront works it out for itself, 64
+// rows at a time.
+struct Chunk {
+  int row, index, count;  // the row's chunk `index` of `count`
+  int first;              // number of the row's first chunk
+  int k0, k1;
+};
+
+__device__ __forceinline__ int units_of(const Fp4Params& p, int r) {
+  const int cap = p.table_width * p.block_size;
+  return r < p.rows ? (min(max(p.lens[r], 0), cap) + 127) >> 7 : 0;
+}
+
+// Inclusive sum over the wavefront by DPP: within rows of 16 lanes, then the
+// rows' last lanes onto the rows behind them.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr 1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast 15
+  return x + __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast 31
+}
+
+__device__ __forceinline__ int chunk_units(const Fp4Params& p, int lane) {
+  int total = 0;  // at most 65,535 rows of 2^15 units
+  for (int r = lane; r < p.rows; r += 64) total += units_of(p, r);
+  total = __builtin_amdgcn_readlane(wave_scan(total), 63);
+  return max((total + p.budget - 1) / p.budget, 2);
+}
+
+// Chunk number i (by_row: the first one of row i); false past the last.
+__device__ __forceinline__ bool find_chunk(const Fp4Params& p, int i, bool by_row, int lane, Chunk& c) {
+  const int per = chunk_units(p, lane);
+  int before = 0;
+  for (int base = 0; base < p.rows; base += 64) {
+    const int u = units_of(p, base + lane), n = base + lane < p.rows ? max(1, (u + per - 1) / per) : 0;
+    const int upto = wave_scan(n);
+    const uint64_t past = __ballot(by_row ? base + lane >= i : before + upto > i);
+    const int at = past ? __builtin_ctzll(past) : 64;
+    if (at < 64 && base + at < p.rows) {
+      c.row = base + at;
+      c.count = __builtin_amdgcn_readlane(n, at);
+      c.first = before + __builtin_amdgcn_readlane(upto, at) - c.count;
+      c.index = by_row ? 0 : i - c.first;
+      const int mine = (__builtin_amdgcn_readlane(u, at) + c.count - 1) / c.count * 128;
+      c.k0 = c.index * mine;
+      c.k1 = c.k0 + mine;
+      return true;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  return false;
+}
+
+// A decode wavefront's steps arrive in LDS by DMA, kDepth in flight.  Codes
+// land as their lanes fetch them, so the lanes fetch in an order that lets both
+// operands be read without a bank conflict: of K, 16-byte part p of token t
+// lies at part p ^ (t / 4 mod 4) of its place; of V, token t lies at place
+// t ^ (t / 4 mod 4).  Both stay within the 256 bytes of four tokens, so a
+// fetch still takes whole lines.
+struct Step {
+  uint8_t k[2048], v[2048], ks[128], vs[128];
+};
+constexpr int kDepth = 2, kStepLoads = 5;
+
+__device__ __forceinline__ void fetch(const Fp4Params& p, int64_t row, uint32_t to, int lane) {
+  const uint32_t t = lane >> 2, x = (lane >> 4) & 3;
+  const uint32_t ko = t * 64 + ((lane & 3) ^ x) * 16, vo = (t ^ x) * 64 + (lane & 3) * 16;
+  const uint8_t *k = p.kc + row * 64, *v = p.vc + row * 64;
+  dma16_nt_at(k, ko, to);
+  dma16_nt_at(k, ko + 1024, to + 1024);
+  dma16_nt_at(v, vo, to + 2048);
+  dma16_nt_at(v, vo + 1024, to + 3072);
+  dma4((lane < 32 ? p.ks : p.vs) + row * 4 + (lane & 31) * 4, to + 4096);
+}
+
 struct Tile {
   u32x4 k[2], vs[2];
   uint32_t v[8], ks[2];
 };
 
-__device__ __forceinline__ void load_tile(Tile& t, const Fp4Params& p, int64_t row, int lane) {
-  // `row` is the wavefront's: scalar bases, and 32-bit offsets of the lane.
-  const uint32_t c = lane & 15, kg = lane >> 4;
-  const uint8_t *k = p.kc + row * 64, *v = p.vc + row * 64, *ks = p.ks + row * 4, *vs = p.vs + row * 4;
-  const uint32_t ko = c * 64 + kg * 16, vo = kg * 256 + c * 4, kso = c * 4 + kg, vso = kg * 16;
+__device__ __forceinline__ void read_step(Tile& t, const Step& s, int lane) {
+  const int c = lane & 15, kg = lane >> 4;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    t.k[h] = *reinterpret_cast<const u32x4*>(k + (ko + h * 1024));
-    t.ks[h] = ks[kso + h * 64];
-    t.vs[h] = *reinterpret_cast<const u32x4*>(vs + (vso + h * 64));
+    t.k[h] = *reinterpret_cast<const u32x4*>(s.k + h * 1024 + c * 64 + (kg ^ (c >> 2)) * 16);
+    t.ks[h] = s.ks[h * 64 + c * 4 + kg];
+    t.vs[h] = *reinterpret_cast<const u32x4*>(s.vs + h * 64 + kg * 16);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) t.v[4 * h + i] = *reinterpret_cast<const uint32_t*>(v + (vo + h * 1024 + i * 64));
+    for (int i = 0; i < 4; ++i)
+      t.v[4 * h + i] = *reinterpret_cast<const uint32_t*>(s.v + h * 1024 + kg * 256 + (i ^ kg) * 64 + c * 4);
   }
 }
 
@@ -210,7 +289,7 @@ __device__ __forceinline__ void step(const Tile& t, bool masked, const bf16x8 (&
 // Walks a row's tokens in steps of `stride` through its table; pages that are
 // not in the pool count as unseen keys.
 struct Walk {
-  const int32_t* table;
+  const __attribute__((address_space(4))) int32_t* table;  // read by scalar loads
   int page, off, block_size, num_blocks, hkv, head;
   __device__ __forceinline__ void advance(int by) {
     off += by;
@@ -226,29 +305,8 @@ struct Walk {
   }
 };
 
-// Runs a wavefront's columns over tokens begin, begin + stride, ... < end.
-template <int NT>
-__device__ __forceinline__ void attend(const Fp4Params& p, int r, int head, const bf16x8 (&q)[NT][4], Acc<NT>& a, int begin,
-                                       int end, int stride, int full, const int (&limit)[NT], int kend, int lane) {
-  if (begin >= end) return;
-  Walk w{p.tables + (int64_t)r * p.table_stride, begin / p.block_size, 0, p.block_size, p.num_blocks, p.hkv, head};
-  w.off = begin - w.page * p.block_size;
-  Tile t;
-  bool ok;
-  int64_t row = w.row(ok);
-  load_tile(t, p, row, lane);
-  for (int at = begin; at < end; at += stride) {
-    Tile n;
-    bool next_ok = false;
-    if (at + stride < end) {
-      w.advance(stride);
-      row = w.row(next_ok);
-      load_tile(n, p, row, lane);
-    }
-    if (ok) step<NT>(t, at + KT > full, q, a, p.scale_log2, at, limit, kend, lane);
-    t = n;
-    ok = next_ok;
-  }
+__device__ __forceinline__ const __attribute__((address_space(4))) int32_t* row_table(const Fp4Params& p, int r) {
+  return (const __attribute__((address_space(4))) int32_t*)(uintptr_t)(p.tables + (int64_t)r * p.table_stride);
 }
 
 __device__ __forceinline__ bf16x8 load_q(const Fp4Params& p, int64_t row, int h, int channel, bool live) {
@@ -272,16 +330,23 @@ __device__ __forceinline__ void clear(Acc<NT>& a) {
 
 // Decode rows: a workgroup takes one chunk of one (row, kv head), its four
 // wavefronts every fourth 32-token step, all heads of the group as columns.
-// The wavefronts' results meet in LDS.
-__global__ void __launch_bounds__(256, 3)
+// Each wavefront fetches its own steps, so the loop has no barrier; the
+// wavefronts' results meet in LDS.
+template <int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, 4)
 fp4_decode_kernel(Fp4Params p) {
-  __shared__ float so[4][16][HD4];
-  __shared__ float sm[4][16], sl[4][16];
-  const int head = blockIdx.x, split = blockIdx.y, r = blockIdx.z;
+  __shared__ union {
+    Step steps[kDepth];
+    float o[16][HD4];
+  } ring[WAVES];
+  __shared__ float sm[WAVES][16], sl[WAVES][16];
+  const int head = blockIdx.x;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Chunk chunk;
+  if (!find_chunk(p, blockIdx.y, false, lane, chunk)) return;
+  const int r = chunk.row;
   const Row g = row_of(p, r);
-  const int k0 = split * p.chunk, k1 = min(k0 + p.chunk, g.lk);
-  if (split && k0 >= g.lk) return;
+  const int k0 = chunk.k0, k1 = min(chunk.k1, g.lk);
   const int col = lane & 15, kg = lane >> 4;
   bf16x8 q[1][4];
 #pragma unroll
@@ -289,13 +354,55 @@ fp4_decode_kernel(Fp4Params p) {
   Acc<1> a;
   clear(a);
   const int limit[1] = {g.lk};
-  attend<1>(p, r, head, q, a, k0 + wave * KT, k1, 4 * KT, g.lk, limit, g.lk, lane);
+  const int begin = k0 + wave * KT, steps = (k1 - begin + WAVES * KT - 1) / (WAVES * KT);
+  if (steps > 0) {
+    Walk w{row_table(p, r), begin / p.block_size, 0, p.block_size, p.num_blocks, p.hkv, head};
+    w.off = begin - w.page * p.block_size;
+    const uint32_t lds = lds_addr(&ring[wave]);
+    uint32_t ok = 0;  // bit i: the step that lies i steps ahead reads a page of the pool
+    int sent = 0, to = 0;
+    auto send = [&] {
+      bool in;
+      const int64_t row = w.row(in);
+      ok |= (uint32_t)in << (kDepth - 1);
+      fetch(p, row, lds + to * (uint32_t)sizeof(Step), lane);
+      to = to == kDepth - 1 ? 0 : to + 1;
+      if (++sent < steps) w.advance(WAVES * KT);
+    };
+    for (int i = 0; i < kDepth - 1; ++i) {
+      ok >>= 1;
+      if (sent < steps) send();
+    }
+    int from = 0;
+    for (int i = 0; i < steps; ++i) {
+      // Bit 0 is now step i's.  The place that the next fetch fills was read in
+      // the last iteration; its reads have returned.
+      ok >>= 1;
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+      if (sent < steps) send();
+      const int ahead = sent - 1 - i;
+      asm volatile("" ::: "memory");
+      if (ahead >= 2)
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * kStepLoads));
+      else if (ahead == 1)
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(kStepLoads));
+      else
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+      asm volatile("" ::: "memory");
+      Tile t;
+      read_step(t, ring[wave].steps[from], lane);
+      from = from == kDepth - 1 ? 0 : from + 1;
+      const int at = begin + WAVES * KT * i;
+      if (ok & 1) step<1>(t, at + KT > g.lk, q, a, p.scale_log2, at, limit, g.lk, lane);
+    }
+  }
+  auto& so = ring;
   if (col < p.group) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int e = 0; e < 8; e += 4)
-        *reinterpret_cast<f32x4*>(&so[wave][col][32 * kg + 8 * i + e]) =
+        *reinterpret_cast<f32x4*>(&so[wave].o[col][32 * kg + 8 * i + e]) =
             f32x4{a.o[0][e][i], a.o[0][e + 1][i], a.o[0][e + 2][i], a.o[0][e + 3][i]};
     if (kg == 0) {
       sm[wave][col] = a.m[0];
@@ -303,25 +410,25 @@ fp4_decode_kernel(Fp4Params p) {
     }
   }
   __syncthreads();
-  for (int x = threadIdx.x; x < p.group * (HD4 / 4); x += 256) {
+  for (int x = threadIdx.x; x < p.group * (HD4 / 4); x += 64 * WAVES) {
     const int h = x >> 5, d = (x & 31) * 4;
     float m = sm[0][h];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) m = fmaxf(m, sm[w][h]);
+    for (int w = 1; w < WAVES; ++w) m = fmaxf(m, sm[w][h]);
     f32x4 o = {0, 0, 0, 0};
     float l = 0;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
       const float f = __builtin_amdgcn_exp2f(sm[w][h] - m);
-      o += *reinterpret_cast<const f32x4*>(&so[w][h][d]) * f;
+      o += *reinterpret_cast<const f32x4*>(&so[w].o[h][d]) * f;
       l += sl[w][h] * f;
     }
-    if (p.splits == 1) {
+    if (chunk.count == 1) {
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       *reinterpret_cast<u32x2*>(p.out + g.q0 * p.out_stride + (head * p.group + h) * HD4 + d) =
           u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
     } else {
-      float* rec = p.partial + (((int64_t)r * p.hq + head * p.group + h) * p.splits + split) * RECORD;
+      float* rec = p.partial + ((int64_t)blockIdx.y * p.hq + head * p.group + h) * RECORD;
       *reinterpret_cast<f32x4*>(rec + d) = o;
       if (d == 0) {
         rec[HD4] = m;
@@ -485,7 +592,7 @@ fp4_prefill_kernel(Fp4Params p, int tiles) {
   Acc<NT> a;
   clear(a);
   if (k0 < k1) {
-    Walk w{p.tables + (int64_t)r * p.table_stride, k0 / p.block_size, 0, p.block_size, p.num_blocks, p.hkv, head};
+    Walk w{row_table(p, r), k0 / p.block_size, 0, p.block_size, p.num_blocks, p.hkv, head};
     w.off = k0 - w.page * p.block_size;
     Quarter t;
     bool ok, next_ok = false;
@@ -546,19 +653,31 @@ fp4_join_kernel(Fp4Params p) {
   const int r = blockIdx.y;
   const Row g = row_of(p, r);
   const int unit = (int)blockIdx.x * UNITS + u, query = unit / p.hq, h = unit - query * p.hq;
-  const bool live = query < g.lq;
-  const int kend = min(max(g.prefix + query + 1, 0), g.lk);
-  const int n = live ? min(max(1, (kend + p.chunk - 1) / p.chunk), p.splits) : 0;
-  const float* rec = p.partial + ((g.q0 - p.first_row + (live ? query : 0)) * p.hq + h) * (int64_t)p.splits * RECORD;
+  bool live = query < g.lq;
+  int n = 0;
+  const float* rec = p.partial;
+  int64_t stride = RECORD;
+  if (p.lens) {
+    Chunk c;
+    find_chunk(p, r, true, threadIdx.x & 63, c);
+    if (c.count == 1) return;  // written by its only chunk
+    n = live ? c.count : 0;
+    rec += ((int64_t)c.first * p.hq + h) * RECORD;
+    stride = (int64_t)p.hq * RECORD;
+  } else if (live) {
+    const int kend = min(max(g.prefix + query + 1, 0), g.lk);
+    n = min(max(1, (kend + p.chunk - 1) / p.chunk), p.splits);
+    rec += ((g.q0 - p.first_row + query) * p.hq + h) * (int64_t)p.splits * RECORD;
+  }
   float m = kNone;
-  for (int s = lane; s < n; s += 32) m = fmaxf(m, rec[(int64_t)s * RECORD + HD4]);
+  for (int s = lane; s < n; s += 32) m = fmaxf(m, rec[s * stride + HD4]);
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) m = wave_max_xor(m, d);
   f32x4 o = {0, 0, 0, 0};
   float l = 0;
 #pragma unroll 4
   for (int s = i; s < n; s += W) {
-    const float* e = rec + (int64_t)s * RECORD;
+    const float* e = rec + s * stride;
     const float w = __builtin_amdgcn_exp2f(e[HD4] - m);
     o += *reinterpret_cast<const f32x4*>(e + 4 * lane) * w;
     l += e[HD4 + 1] * w;
@@ -580,16 +699,16 @@ fp4_join_kernel(Fp4Params p) {
       u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
 }
 
-void launch_join(const Fp4Params& p, int64_t units, int rows, hipStream_t s) {
-  // Many chunks: 8 half wavefronts share them.
-  if (p.splits > 8)
-    hipLaunchKernelGGL(fp4_join_kernel<8>, dim3((unsigned)units, rows), dim3(256), 0, s, p);
-  else
-    hipLaunchKernelGGL(fp4_join_kernel<1>, dim3((unsigned)((units + 7) / 8), rows), dim3(256), 0, s, p);
-}
-
 constexpr int kPrefillNT = 2;
-constexpr int kDecodeTarget = 1024, kPrefillTarget = 640;
+constexpr int kPrefillTarget = 1024;
+// Chunks of all decode rows and heads together: one for each of the four
+// workgroups that a CU holds.  64 rows of 512-4,096 tokens, 8 kv heads: 36.6 us
+// and 5.1 us to join them, 38.1 + 6.6 with twice as many, 42.1 + 6.8 with four
+// times; three rows of 20,000-60,000 30.2 + 4.2, 32.1 + 5.8, 35.9 + 7.2.
+constexpr int kDecodeChunks = 1024;
+// Rows of at most this many tokens are not cut, and eight wavefronts take each:
+// one row of 1,000 6.7 us, 5.4 + 4.4 us as two chunks and their join.
+constexpr int kWholeRow = 1024;
 
 // Chunks of `capacity` keys for a launch of so many workgroups per chunk:
 // enough for `target` workgroups, at least `least` keys each.
@@ -603,18 +722,18 @@ int splits_of(int64_t groups, int64_t capacity, int least, int target, int& chun
 }
 
 struct Plan {
-  bool dwork;
-  int dsplits, dchunk, psplits, pchunk, ptiles;
+  bool dwork, joined;
+  int budget, psplits, pchunk, ptiles;
   size_t dbytes, pbytes;
 };
 
 Plan plan_of(const slo_paged_attention_args* a) {
-  Plan n = {false, 1, 1 << 30, 1, 1 << 30, 0, 0, 0};
+  Plan n = {false, false, 0, 1, 1 << 30, 0, 0, 0};
   if (a->num_decode > 0 && (a->phases & SLO_PHASE_DECODE)) {
     n.dwork = true;
-    n.dsplits = splits_of((int64_t)a->num_decode * a->num_kv_heads, (int64_t)a->decode_table_width * a->block_size, 256, kDecodeTarget,
-                          n.dchunk);
-    if (n.dsplits > 1) n.dbytes = (size_t)a->num_decode * a->num_heads * n.dsplits * RECORD * 4;
+    n.joined = (int64_t)a->decode_table_width * a->block_size > kWholeRow;
+    n.budget = n.joined ? (kDecodeChunks + a->num_kv_heads - 1) / a->num_kv_heads : 0;
+    if (n.joined) n.dbytes = (size_t)(n.budget + a->num_decode) * a->num_heads * RECORD * 4;
   }
   if (a->num_prefill > 0 && (a->phases & SLO_PHASE_PREFILL) && a->max_q > 0) {
     const int per = 16 * kPrefillNT / (a->num_heads / a->num_kv_heads);
@@ -662,9 +781,9 @@ int check_args(const slo_paged_attention_args* a) {
     return fail(SLO_ERR_INVALID, "paged_attention_fp4: missing decode metadata");
   if (pre && (!a->prefill_cu_q || !a->prefill_cu_k || !a->prefill_tables || a->prefill_table_width <= 0))
     return fail(SLO_ERR_INVALID, "paged_attention_fp4: missing prefill metadata");
-  if ((dec && (int64_t)a->decode_table_width * a->block_size > (1 << 30)) ||
-      (pre && (int64_t)a->prefill_table_width * a->block_size > (1 << 30)))
-    return fail(SLO_ERR_UNSUPPORTED, "paged_attention_fp4: tables span more than 2^30 tokens");
+  if ((dec && (int64_t)a->decode_table_width * a->block_size > (1 << 22)) ||
+      (pre && (int64_t)a->prefill_table_width * a->block_size > (1 << 22)))
+    return fail(SLO_ERR_UNSUPPORTED, "paged_attention_fp4: tables span more than 2^22 tokens");
   return SLO_OK;
 }
 
@@ -714,12 +833,15 @@ extern "C" int slo_paged_attention_fp4(const slo_paged_attention_args* a, slo_st
     p.table_stride = a->decode_table_stride;
     p.table_width = a->decode_table_width;
     p.first_row = 0;
-    p.splits = n.dsplits;
-    p.chunk = n.dchunk;
+    p.rows = a->num_decode;
+    p.budget = n.joined ? n.budget : 1;
     p.partial = static_cast<float*>(a->workspace);
-    hipLaunchKernelGGL(fp4_decode_kernel, dim3(p.hkv, p.splits, a->num_decode), dim3(256), 0, s, p);
-    if (p.splits > 1)
-      launch_join(p, p.hq, a->num_decode, s);
+    if (n.joined) {
+      hipLaunchKernelGGL(fp4_decode_kernel<4>, dim3(p.hkv, n.budget + p.rows), dim3(256), 0, s, p);
+      hipLaunchKernelGGL(fp4_join_kernel<8>, dim3(p.hq, p.rows), dim3(256), 0, s, p);
+    } else {
+      hipLaunchKernelGGL(fp4_decode_kernel<8>, dim3(p.hkv, p.rows), dim3(512), 0, s, p);
+    }
   }
   if (n.ptiles) {
     p.lens = nullptr;
@@ -735,7 +857,8 @@ extern "C" int slo_paged_attention_fp4(const slo_paged_attention_args* a, slo_st
     hipLaunchKernelGGL(fp4_prefill_kernel<kPrefillNT>, dim3(p.hkv, n.ptiles * p.splits, a->num_prefill), dim3(256), 0, s, p,
                        n.ptiles);
     if (p.splits > 1)
-      launch_join(p, (int64_t)a->max_q * p.hq, a->num_prefill, s);
+      hipLaunchKernelGGL(fp4_join_kernel<1>, dim3((unsigned)(((int64_t)a->max_q * p.hq + 7) / 8), a->num_prefill), dim3(256),
+                         0, s, p);
   }
   return check_launch("paged_attention_fp4");
 }

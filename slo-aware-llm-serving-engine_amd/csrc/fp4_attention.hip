@@ -32,6 +32,17 @@ constexpr int KT = 32;          // tokens per step of a wavefront
 constexpr int RECORD = HD4 + 4;  // floats of a partial result: outputs, maximum, sum, 2 unused
 constexpr float kNone = -1e30f;  // running maximum before the first key
 
+// What a prefill workgroup leaves for the join: the two tiles that it may have
+// shared with its neighbours, the first and the last of its share, as they lie
+// in the registers of its lanes (16 NT columns of a wavefront; four channels
+// a piece), and where the last one's other parts are.
+constexpr int kPrefillNT = 2;
+struct Part {
+  f32x4 o[2][4 * kPrefillNT][8][64];
+  float m[2][64 * kPrefillNT], l[2][64 * kPrefillNT];
+  int32_t row, tile, count, unused;  // count > 0: the last tile goes on in the next count - 1 shares
+};
+
 struct Fp4Params {
   const uint16_t* q;
   int64_t q_stride;
@@ -49,9 +60,11 @@ struct Fp4Params {
   int hq, hkv, group;
   float scale_log2;  // |softmax scale| * log2(e)
   uint32_t q_sign;   // 0x80008000 where the scale is negative
-  float* partial;    // prefill rows: [queries, hq, splits] records when splits > 1; decode rows: [chunks, hq]
-  int splits, chunk;  // prefill rows
-  int rows, budget;   // decode rows: about so many chunks over all rows
+  int rows;
+  int budget;      // decode rows: about so many chunks over all rows
+  float* partial;  // decode rows: [chunks, hq] records
+  int shares;      // prefill rows: workgroups per kv head
+  Part* parts;     // prefill rows: [shares, hkv]
 };
 
 struct Row {
@@ -445,28 +458,21 @@ struct Stage {
   u32x4 k[4][4][64], v[2][8][64];
 };
 
-// A wavefront's quarter of a step: 16 tokens of K, and four channels of every
-// lane's eight of 32 tokens of V.
+// A wavefront's quarter of a step: 16 tokens of K, and of V.
 struct Quarter {
-  u32x4 k, vs[2];
-  uint32_t ks;
-  uint16_t v[8];
+  u32x4 k, vs;
+  uint32_t ks, v[4];
 };
 
 __device__ __forceinline__ void load_quarter(Quarter& t, const Fp4Params& p, int64_t row, int wave, int lane) {
   const uint32_t c = lane & 15, kg = lane >> 4;
-  const uint8_t *k = p.kc + (row + 16 * wave) * 64, *ks = p.ks + (row + 16 * wave) * 4;
-  const int64_t vrow = row + 32 * (wave >> 1);
-  const uint8_t *v = p.vc + vrow * 64 + 2 * (wave & 1), *vs = p.vs + vrow * 4;
-  const uint32_t ko = c * 64 + kg * 16, kso = c * 4 + kg, vo = kg * 256 + c * 4, vso = kg * 16;
-  t.k = *reinterpret_cast<const u32x4*>(k + ko);
-  t.ks = ks[kso];
+  row += 16 * wave;
+  const uint8_t *k = p.kc + row * 64, *v = p.vc + row * 64, *ks = p.ks + row * 4, *vs = p.vs + row * 4;
+  t.k = *reinterpret_cast<const u32x4*>(k + (c * 64 + kg * 16));
+  t.ks = ks[c * 4 + kg];
+  t.vs = *reinterpret_cast<const u32x4*>(vs + kg * 16);
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    t.vs[h] = *reinterpret_cast<const u32x4*>(vs + (vso + h * 64));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) t.v[4 * h + i] = *reinterpret_cast<const uint16_t*>(v + (vo + h * 1024 + i * 64));
-  }
+  for (int i = 0; i < 4; ++i) t.v[i] = *reinterpret_cast<const uint32_t*>(v + (kg * 256 + c * 4 + i * 64));
 }
 
 // `left`: tokens of the step that belong to the row; V's scales past them are
@@ -476,46 +482,52 @@ __device__ __forceinline__ void stage(Stage& s, const Quarter& t, int left, int 
   const float sc = e8m0(t.ks);
 #pragma unroll
   for (int i = 0; i < 4; ++i) s.k[wave][i][lane] = e2m1_decode8(t.k[i], sc);
-  float vs[8];
+  float vs[4];
   const int turn = (9 + 8 * (c >> 2)) & 31;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t x = t.vs[j >> 2][j & 3];
-    vs[j] = __uint_as_float(__builtin_amdgcn_alignbit(x, x, turn));
-  }
+  for (int i = 0; i < 4; ++i) vs[i] = __uint_as_float(__builtin_amdgcn_alignbit(t.vs[i], t.vs[i], turn));
   if (left < 64) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (32 * (wave >> 1) + 16 * (j >> 2) + 4 * kg + (j & 3) >= left) vs[j] = 0.0f;
+    for (int i = 0; i < 4; ++i)
+      if (16 * wave + 4 * kg + i >= left) vs[i] = 0.0f;
   }
-  u32x4 o[4];
+  // Tokens 4 kg + i of the wavefront's 16: half of a lane's 32-token operands.
+  auto pair = [&](auto sel) {
+    constexpr int B = decltype(sel)::value;
+    uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t a0 = e2m1_pair<0>(t.v[2 * i], vs[2 * i]), b0 = e2m1_pair<0>(t.v[2 * i + 1], vs[2 * i + 1]);
-    const uint32_t a1 = e2m1_pair<1>(t.v[2 * i], vs[2 * i]), b1 = e2m1_pair<1>(t.v[2 * i + 1], vs[2 * i + 1]);
-    o[0][i] = __builtin_amdgcn_perm(b0, a0, 0x05040100u);
-    o[1][i] = __builtin_amdgcn_perm(b0, a0, 0x07060302u);
-    o[2][i] = __builtin_amdgcn_perm(b1, a1, 0x05040100u);
-    o[3][i] = __builtin_amdgcn_perm(b1, a1, 0x07060302u);
-  }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) s.v[wave >> 1][4 * (wave & 1) + e][lane] = o[e];
+    for (int i = 0; i < 4; ++i) w[i] = e2m1_pair<B>(t.v[i], vs[i]);
+    u32x2* lo = reinterpret_cast<u32x2*>(&s.v[wave >> 1][2 * B][lane]) + (wave & 1);
+    u32x2* hi = reinterpret_cast<u32x2*>(&s.v[wave >> 1][2 * B + 1][lane]) + (wave & 1);
+    *lo = u32x2{__builtin_amdgcn_perm(w[1], w[0], 0x05040100u), __builtin_amdgcn_perm(w[3], w[2], 0x05040100u)};
+    *hi = u32x2{__builtin_amdgcn_perm(w[1], w[0], 0x07060302u), __builtin_amdgcn_perm(w[3], w[2], 0x07060302u)};
+  };
+  pair(std::integral_constant<int, 0>{});
+  pair(std::integral_constant<int, 1>{});
+  pair(std::integral_constant<int, 2>{});
+  pair(std::integral_constant<int, 3>{});
 }
 
-// 64 tokens of a wavefront's columns against the staged operands.
+// 64 tokens of a wavefront's columns against the staged operands, read four
+// ahead of the products.
 template <int NT>
 __device__ __forceinline__ void staged_step(const Stage& st, bool masked, const bf16x8 (&q)[NT][4], Acc<NT>& a, float c, int kv0,
                                             const int (&limit)[NT], int lane) {
   const int kg = lane >> 4;
   f32x4 s[NT][4];
+  bf16x8 x[2][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[0][i] = as_bf16x8(st.k[0][i][lane]);
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const bf16x8 k = as_bf16x8(st.k[t][i][lane]);
+    for (int i = 0; i < 4; ++i) x[(t + 1) & 1][i] = as_bf16x8(t < 3 ? st.k[t + 1][i][lane] : st.v[0][i][lane]);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) s[n][t] = mfma16(k, q[n][i], i ? s[n][t] : f32x4{0, 0, 0, 0});
-    }
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[n][t] = mfma16(x[t & 1][i], q[n][i], i ? s[n][t] : f32x4{0, 0, 0, 0});
+    __builtin_amdgcn_sched_barrier(0);
   }
   bf16x8 pr[NT][2];
 #pragma unroll
@@ -536,50 +548,134 @@ __device__ __forceinline__ void staged_step(const Stage& st, bool masked, const 
       u32x4 b;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const f32x4& x = s[n][2 * g + (i >> 1)];
-        b[i] = pack_bf16x2(__builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * (i & 1)], c, -a.m[n])),
-                           __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * (i & 1) + 1], c, -a.m[n])));
+        const f32x4& e = s[n][2 * g + (i >> 1)];
+        b[i] = pack_bf16x2(__builtin_amdgcn_exp2f(__builtin_fmaf(e[2 * (i & 1)], c, -a.m[n])),
+                           __builtin_amdgcn_exp2f(__builtin_fmaf(e[2 * (i & 1) + 1], c, -a.m[n])));
       }
       pr[n][g] = as_bf16x8(b);
     }
   }
 #pragma unroll
-  for (int g = 0; g < 2; ++g) {
+  for (int j = 0; j < 4; ++j) {  // V's operands, four at a time
+    const int g = j >> 1;
+    if (j < 3) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) a.l[n] = mfma16(ones(), pr[n][g], a.l[n]);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const bf16x8 v = as_bf16x8(st.v[g][e][lane]);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) a.o[n][e] = mfma16(v, pr[n][g], a.o[n][e]);
+      for (int i = 0; i < 4; ++i) x[(j + 1) & 1][i] = as_bf16x8(st.v[(j + 1) >> 1][4 * ((j + 1) & 1) + i][lane]);
     }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) a.o[n][4 * (j & 1) + i] = mfma16(x[j & 1][i], pr[n][g], a.o[n][4 * (j & 1) + i]);
+    if (j & 1) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) a.l[n] = mfma16(ones(), pr[n][g], a.l[n]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
 
-// Prefill rows: a workgroup takes 64 NT columns, (query, head of the group)
-// pairs of consecutive queries of one row, over its keys (or one chunk of
-// them), the latest queries first.  Its four wavefronts turn each 64-token
-// step's codes into operands together, each a quarter, one step ahead of the
-// products, and each runs 16 NT columns over them.
-template <int NT>
-__global__ void __launch_bounds__(256, 2)
-fp4_prefill_kernel(Fp4Params p, int tiles) {
-  __shared__ Stage st[2];
-  const int head = blockIdx.x, r = blockIdx.z;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int split = blockIdx.y % p.splits;
-  const int per = 16 * NT / p.group;  // queries of a wavefront
+// Prefill rows.  A tile is 64 NT columns, (query, head of the group) pairs of
+// consecutive queries of one row, and has as many 64-token steps as its last
+// query sees.  All tiles' steps, in row order, are cut into equal shares, one
+// for each workgroup of a kv head: causal tiles differ in length, a row may be
+// long and its queries few, and the lengths are known on the GPU only.  A tile
+// that lies in one share is written out; the parts of one that is cut meet in
+// fp4_join_prefill_kernel.
+__device__ __forceinline__ int tiles_of(const Fp4Params& p, int per, int r) {
   const Row g = row_of(p, r);
-  const int w0 = (tiles - 1 - (int)(blockIdx.y / p.splits)) * 4 * per;  // the workgroup's first query
-  if (w0 >= g.lq) return;
-  const int all = min(max(g.prefix + min(w0 + 4 * per, g.lq), 0), g.lk);  // keys that one of its queries sees
-  const int k0 = split * p.chunk, k1 = p.splits == 1 ? all : min(k0 + p.chunk, all);
-  if (split && k0 >= all) return;
+  return g.lq > 0 ? (g.lq + per - 1) / per : 0;
+}
+
+__device__ __forceinline__ int steps_of(const Row& g, int per, int t) {
+  return (max(min(g.prefix + min((t + 1) * per, g.lq), g.lk), 1) + 63) >> 6;
+}
+
+// Sum over a 256-thread workgroup, before this thread and in all.
+__device__ __forceinline__ int group_scan(int x, int* sums, int& total) {
+  const int wave = threadIdx.x >> 6;
+  const int upto = wave_scan(x);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) sums[wave] = upto;
+  __syncthreads();
+  total = sums[0] + sums[1] + sums[2] + sums[3];
+  int before = upto - x;
+  for (int w = 0; w < wave; ++w) before += sums[w];
+  return before;
+}
+
+constexpr int kMaxPrefillRows = 1024;
+constexpr int kLeastSteps = 4;  // of a share
+
+struct Plan256 {
+  int first[kMaxPrefillRows + 1];  // number of each row's first tile
+  int sums[4];
+  int row, tile, skip;  // where the share begins
+  int each;             // steps of a share
+};
+
+// The number of the tiles' row, tile `i` of all.
+__device__ __forceinline__ int row_of_tile(const Plan256& s, int rows, int i) {
+  int lo = 0, hi = rows;  // first[lo] <= i < first[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (s.first[mid] <= i) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+// Finds this workgroup's share; returns its number of steps.
+__device__ __forceinline__ int find_share(const Fp4Params& p, int per, int share, Plan256& s) {
+  const int tid = threadIdx.x;
+  int tiles = 0;
+  for (int base = 0; base < p.rows; base += 256) {
+    int all;
+    const int n = base + tid < p.rows ? tiles_of(p, per, base + tid) : 0;
+    const int before = group_scan(n, s.sums, all);
+    if (base + tid < p.rows) s.first[base + tid] = tiles + before;
+    tiles += all;
+  }
+  if (tid == 0) s.first[p.rows] = tiles;
+  __syncthreads();
+  auto steps = [&](int i) {
+    if (i >= tiles) return 0;
+    const int r = row_of_tile(s, p.rows, i);
+    return steps_of(row_of(p, r), per, i - s.first[r]);
+  };
+  int mine = 0, total, ignored;
+  for (int i = tid; i < tiles; i += 256) mine += steps(i);
+  group_scan(mine, s.sums, total);
+  const int each = max((total + p.shares - 1) / p.shares, kLeastSteps);
+  if (tid == 0) s.each = each;
+  const int begin = share * each;
+  if (begin >= total) return 0;
+  int before = 0;
+  for (int base = 0; base < tiles; base += 256) {
+    const int n = steps(base + tid);
+    const int at = before + group_scan(n, s.sums, ignored);
+    if (at <= begin && begin < at + n) {
+      const int r = row_of_tile(s, p.rows, base + tid);
+      s.row = r;
+      s.tile = base + tid - s.first[r];
+      s.skip = begin - at;
+    }
+    before += ignored;
+    if (before > begin) break;
+  }
+  __syncthreads();
+  return min(each, total - begin);
+}
+
+// Steps [from, to) of one tile for this wavefront's columns.
+template <int NT>
+__device__ __forceinline__ void run_tile(const Fp4Params& p, const Row& g, int r, int head, int w0, int from, int to,
+                                         Stage (&st)[2], int& buf, bf16x8 (&q)[NT][4], Acc<NT>& a, int wave, int lane) {
+  const int per = 16 * NT / p.group;
   const int t0 = w0 + wave * per, t1 = min(t0 + per, g.lq);
-  const int kend = t0 < g.lq ? min(max(g.prefix + t1, 0), g.lk) : 0;  // that one of the wavefront's sees
-  const int full = min(g.prefix + t0 + 1, g.lk);                      // that all of them see
+  const int all = min(max(g.prefix + min(w0 + 4 * per, g.lq), 0), g.lk);  // keys that one of the tile's queries sees
+  const int kend = t0 < g.lq ? min(max(g.prefix + t1, 0), g.lk) : 0;      // that one of the wavefront's sees
+  const int full = min(g.prefix + t0 + 1, g.lk);                          // that all of them see
   const int col = lane & 15, kg = lane >> 4;
-  bf16x8 q[NT][4];
   int limit[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -589,118 +685,183 @@ fp4_prefill_kernel(Fp4Params p, int tiles) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) q[n][i] = load_q(p, g.q0 + tok, head * p.group + x % p.group, 32 * kg + 8 * i, live);
   }
-  Acc<NT> a;
   clear(a);
-  if (k0 < k1) {
-    Walk w{row_table(p, r), k0 / p.block_size, 0, p.block_size, p.num_blocks, p.hkv, head};
-    w.off = k0 - w.page * p.block_size;
-    Quarter t;
-    bool ok, next_ok = false;
-    load_quarter(t, p, w.row(ok), wave, lane);
-    for (int at = k0, b = 0; at < k1; at += 64, b ^= 1) {
-      stage(st[b], t, all - at, wave, lane);
-      if (at + 64 < k1) {
-        w.advance(64);
-        load_quarter(t, p, w.row(next_ok), wave, lane);
-      }
-      // Two buffers: a wavefront comes to write this one again only past the
-      // next step's barrier, when every wavefront has left it.
-      __syncthreads();
-      if (ok && at < kend) staged_step<NT>(st[b], at + 64 > full, q, a, p.scale_log2, at, limit, lane);
-      ok = next_ok;
+  const int k0 = from * 64, k1 = min(to * 64, all);
+  if (k0 >= k1) return;
+  Walk w{row_table(p, r), k0 / p.block_size, 0, p.block_size, p.num_blocks, p.hkv, head};
+  w.off = k0 - w.page * p.block_size;
+  Quarter t;
+  bool ok, next_ok = false;
+  load_quarter(t, p, w.row(ok), wave, lane);
+  for (int at = k0; at < k1; at += 64, buf ^= 1) {
+    stage(st[buf], t, all - at, wave, lane);
+    if (at + 64 < k1) {
+      w.advance(64);
+      load_quarter(t, p, w.row(next_ok), wave, lane);
     }
-  }
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    int x = 16 * n + col;
-    asm("" : "+v"(x));  // found again here, so that the loop need not hold it in registers
-    const int tok = t0 + x / p.group, h = head * p.group + x % p.group;
-    if (x >= per * p.group || tok >= t1) continue;
-    if (p.splits == 1) {
-      const float inv = a.l[n][0] == 0.0f ? 0.0f : 1.0f / a.l[n][0];
-      uint16_t* out = p.out + (g.q0 + tok) * p.out_stride + h * HD4 + 32 * kg;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<u32x4*>(out + 8 * i) =
-            u32x4{pack_bf16x2(a.o[n][0][i] * inv, a.o[n][1][i] * inv), pack_bf16x2(a.o[n][2][i] * inv, a.o[n][3][i] * inv),
-                  pack_bf16x2(a.o[n][4][i] * inv, a.o[n][5][i] * inv), pack_bf16x2(a.o[n][6][i] * inv, a.o[n][7][i] * inv)};
-    } else {
-      float* rec = p.partial + (((g.q0 - p.first_row + tok) * p.hq + h) * p.splits + split) * RECORD;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int e = 0; e < 8; e += 4)
-          *reinterpret_cast<f32x4*>(rec + 32 * kg + 8 * i + e) =
-              f32x4{a.o[n][e][i], a.o[n][e + 1][i], a.o[n][e + 2][i], a.o[n][e + 3][i]};
-      if (kg == 0) {
-        rec[HD4] = a.m[n];
-        rec[HD4 + 1] = a.l[n][0];
-      }
-    }
+    // Two buffers: a wavefront comes to write this one again only past the
+    // next step's barrier, when every wavefront has left it.  The barrier
+    // waits for LDS only: the loads of the next step stay in flight.
+    lds_sync();
+    if (ok && at < kend) staged_step<NT>(st[buf], at + 64 > full, q, a, p.scale_log2, at, limit, lane);
+    ok = next_ok;
   }
 }
 
-// Joins the partial results of the phase's chunks: a workgroup of W half
-// wavefronts per (query, head), four channels a lane.  Half wavefront i takes
-// chunks i, i + W, ... and the W sums meet in LDS in that order.
-template <int W>
-__global__ void __launch_bounds__(32 * W < 256 ? 256 : 32 * W)
-fp4_join_kernel(Fp4Params p) {
-  constexpr int UNITS = 32 * W < 256 ? 8 / W : 1;  // (query, head) pairs of a workgroup
-  __shared__ f32x4 so[UNITS][W][32];
-  __shared__ float sl[UNITS][W];
-  const int lane = threadIdx.x & 31, i = (threadIdx.x >> 5) % W, u = (threadIdx.x >> 5) / W;
-  const int r = blockIdx.y;
-  const Row g = row_of(p, r);
-  const int unit = (int)blockIdx.x * UNITS + u, query = unit / p.hq, h = unit - query * p.hq;
-  bool live = query < g.lq;
-  int n = 0;
-  const float* rec = p.partial;
-  int64_t stride = RECORD;
-  if (p.lens) {
-    Chunk c;
-    find_chunk(p, r, true, threadIdx.x & 63, c);
-    if (c.count == 1) return;  // written by its only chunk
-    n = live ? c.count : 0;
-    rec += ((int64_t)c.first * p.hq + h) * RECORD;
-    stride = (int64_t)p.hq * RECORD;
-  } else if (live) {
-    const int kend = min(max(g.prefix + query + 1, 0), g.lk);
-    n = min(max(1, (kend + p.chunk - 1) / p.chunk), p.splits);
-    rec += ((g.q0 - p.first_row + query) * p.hq + h) * (int64_t)p.splits * RECORD;
+// A workgroup's four wavefronts turn each step's codes into operands together,
+// each a quarter, one step ahead of the products, and each runs 16 NT columns
+// over them.
+template <int NT>
+__global__ void __launch_bounds__(256, 2)
+fp4_prefill_kernel(Fp4Params p) {
+  __shared__ Stage st[2];
+  __shared__ Plan256 plan;
+  const int head = blockIdx.x, share = blockIdx.y;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int per = 4 * (16 * NT / p.group);
+  Part& part = p.parts[(int64_t)share * p.hkv + head];
+  int left = find_share(p, per, share, plan);
+  int r = plan.row, tile = plan.tile, from = plan.skip, buf = 0;
+  int open_row = 0, open_tile = 0, open = 0;
+  while (left > 0) {
+    const Row g = row_of(p, r);
+    const int steps = steps_of(g, per, tile), to = min(steps, from + left);
+    bf16x8 q[NT][4];
+    Acc<NT> a;
+    run_tile<NT>(p, g, r, head, tile * per, from, to, st, buf, q, a, wave, lane);
+    int c = lane & 15;
+    asm("" : "+v"(c));  // found again here, so that the loop need not hold it in registers
+    const int kg = lane >> 4;
+    if (from == 0 && to == steps) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int x = 16 * n + c, tok = tile * per + wave * (per >> 2) + x / p.group, h = head * p.group + x % p.group;
+        if (x >= (per >> 2) * p.group || tok >= g.lq) continue;
+        const float inv = a.l[n][0] == 0.0f ? 0.0f : 1.0f / a.l[n][0];
+        uint16_t* out = p.out + (g.q0 + tok) * p.out_stride + h * HD4 + 32 * kg;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<u32x4*>(out + 8 * i) =
+              u32x4{pack_bf16x2(a.o[n][0][i] * inv, a.o[n][1][i] * inv), pack_bf16x2(a.o[n][2][i] * inv, a.o[n][3][i] * inv),
+                    pack_bf16x2(a.o[n][4][i] * inv, a.o[n][5][i] * inv), pack_bf16x2(a.o[n][6][i] * inv, a.o[n][7][i] * inv)};
+      }
+    } else {
+      // A part that does not begin its tile is its share's first.
+      const int k = from == 0;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int block = NT * wave + n;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 8; e += 4)
+            part.o[k][block][2 * i + (e >> 2)][lane] = f32x4{a.o[n][e][i], a.o[n][e + 1][i], a.o[n][e + 2][i], a.o[n][e + 3][i]};
+        if (kg == 0) {
+          part.m[k][16 * block + c] = a.m[n];
+          part.l[k][16 * block + c] = a.l[n][0];
+        }
+      }
+      if (k) {
+        open_row = r;
+        open_tile = tile;
+        open = steps - to;
+      }
+    }
+    left -= to - from;
+    from = 0;
+    if (left > 0 && ++tile >= (g.lq + per - 1) / per) {
+      tile = 0;
+      do ++r;
+      while (tiles_of(p, per, r) == 0);
+    }
   }
+  if (threadIdx.x == 0) {
+    part.row = open_row;
+    part.tile = open_tile;
+    part.count = open ? 1 + (open + plan.each - 1) / plan.each : 0;
+  }
+}
+
+// Joins the parts of the tiles that were cut, in order: one workgroup per 16
+// columns of the tile that a share leaves open.
+template <int NT>
+__global__ void __launch_bounds__(256)
+fp4_join_prefill_kernel(Fp4Params p) {
+  const int head = blockIdx.x, share = blockIdx.y, block = blockIdx.z;
+  const Part* part = p.parts + (int64_t)share * p.hkv + head;
+  const int count = part->count;
+  if (count == 0) return;
+  const Row g = row_of(p, part->row);
+  const int quarter = 16 * NT / p.group;
+  const int lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
+  const int x = 16 * (block % NT) + col, tok = (part->tile * 4 + block / NT) * quarter + x / p.group;
+  if (x >= quarter * p.group || tok >= g.lq) return;
+  const int at = 16 * block + col;
+  float m = part->m[1][at];
+  for (int s = 1; s < count; ++s) m = fmaxf(m, part[(int64_t)s * p.hkv].m[0][at]);
+  f32x4 o[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+  float l = 0;
+#pragma unroll 2
+  for (int s = 0; s < count; ++s) {
+    const Part& e = part[(int64_t)s * p.hkv];
+    const int k = s == 0;
+    const float w = __builtin_amdgcn_exp2f(e.m[k][at] - m);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) o[j] += e.o[k][block][(threadIdx.x >> 6) + 4 * j][lane] * w;
+    l += e.l[k][at] * w;
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  uint16_t* out = p.out + (g.q0 + tok) * p.out_stride + (head * p.group + x % p.group) * HD4 + 32 * kg;
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    *reinterpret_cast<u32x2*>(out + 4 * ((threadIdx.x >> 6) + 4 * j)) =
+        u32x2{pack_bf16x2(o[j][0] * inv, o[j][1] * inv), pack_bf16x2(o[j][2] * inv, o[j][3] * inv)};
+}
+
+// Joins the partial results of a decode row's chunks: a workgroup per (row,
+// head), four channels a lane.  Half wavefront i takes chunks i, i + 8, ... and
+// the eight sums meet in LDS in that order.
+__global__ void __launch_bounds__(256)
+fp4_join_decode_kernel(Fp4Params p) {
+  __shared__ f32x4 so[8][32];
+  __shared__ float sl[8];
+  const int lane = threadIdx.x & 31, i = threadIdx.x >> 5, h = blockIdx.x, r = blockIdx.y;
+  Chunk c;
+  find_chunk(p, r, true, threadIdx.x & 63, c);
+  if (c.count == 1) return;  // written by its only chunk
+  const float* rec = p.partial + ((int64_t)c.first * p.hq + h) * RECORD;
+  const int64_t stride = (int64_t)p.hq * RECORD;
   float m = kNone;
-  for (int s = lane; s < n; s += 32) m = fmaxf(m, rec[s * stride + HD4]);
+  for (int s = lane; s < c.count; s += 32) m = fmaxf(m, rec[s * stride + HD4]);
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) m = wave_max_xor(m, d);
   f32x4 o = {0, 0, 0, 0};
   float l = 0;
 #pragma unroll 4
-  for (int s = i; s < n; s += W) {
+  for (int s = i; s < c.count; s += 8) {
     const float* e = rec + s * stride;
     const float w = __builtin_amdgcn_exp2f(e[HD4] - m);
     o += *reinterpret_cast<const f32x4*>(e + 4 * lane) * w;
     l += e[HD4 + 1] * w;
   }
-  if (W > 1) {
-    so[u][i][lane] = o;
-    if (lane == 0) sl[u][i] = l;
-    __syncthreads();
-    if (i) return;
+  so[i][lane] = o;
+  if (lane == 0) sl[i] = l;
+  __syncthreads();
+  if (i) return;
 #pragma unroll
-    for (int k = 1; k < W; ++k) {
-      o += so[u][k][lane];
-      l += sl[u][k];
-    }
+  for (int k = 1; k < 8; ++k) {
+    o += so[k][lane];
+    l += sl[k];
   }
-  if (!live) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  *reinterpret_cast<u32x2*>(p.out + (g.q0 + query) * p.out_stride + h * HD4 + 4 * lane) =
+  *reinterpret_cast<u32x2*>(p.out + (int64_t)r * p.out_stride + h * HD4 + 4 * lane) =
       u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
 }
 
-constexpr int kPrefillNT = 2;
-constexpr int kPrefillTarget = 1024;
+// Two prefill workgroups fit a CU (64 KiB of LDS and 256 registers each); all
+// heads' shares together are one for each.
+constexpr int kPrefillShares = 512;
+
 // Chunks of all decode rows and heads together: one for each of the four
 // workgroups that a CU holds.  64 rows of 512-4,096 tokens, 8 kv heads: 36.6 us
 // and 5.1 us to join them, 38.1 + 6.6 with twice as many, 42.1 + 6.8 with four
@@ -710,25 +871,14 @@ constexpr int kDecodeChunks = 1024;
 // one row of 1,000 6.7 us, 5.4 + 4.4 us as two chunks and their join.
 constexpr int kWholeRow = 1024;
 
-// Chunks of `capacity` keys for a launch of so many workgroups per chunk:
-// enough for `target` workgroups, at least `least` keys each.
-int splits_of(int64_t groups, int64_t capacity, int least, int target, int& chunk) {
-  const int64_t want = groups > 0 ? (target + groups - 1) / groups : 1;
-  int64_t c = ((capacity + want - 1) / want + 127) / 128 * 128;
-  if (c < least) c = least;
-  chunk = (int)c;
-  const int64_t n = (capacity + c - 1) / c;
-  return n < 1 ? 1 : (int)n;
-}
-
 struct Plan {
   bool dwork, joined;
-  int budget, psplits, pchunk, ptiles;
+  int budget, shares;
   size_t dbytes, pbytes;
 };
 
 Plan plan_of(const slo_paged_attention_args* a) {
-  Plan n = {false, false, 0, 1, 1 << 30, 0, 0, 0};
+  Plan n = {false, false, 0, 0, 0, 0};
   if (a->num_decode > 0 && (a->phases & SLO_PHASE_DECODE)) {
     n.dwork = true;
     n.joined = (int64_t)a->decode_table_width * a->block_size > kWholeRow;
@@ -736,13 +886,13 @@ Plan plan_of(const slo_paged_attention_args* a) {
     if (n.joined) n.dbytes = (size_t)(n.budget + a->num_decode) * a->num_heads * RECORD * 4;
   }
   if (a->num_prefill > 0 && (a->phases & SLO_PHASE_PREFILL) && a->max_q > 0) {
-    const int per = 16 * kPrefillNT / (a->num_heads / a->num_kv_heads);
-    n.ptiles = ((a->max_q + per - 1) / per + 3) / 4;
-    const int64_t cap = (int64_t)a->prefill_table_width * a->block_size;
-    // The rows' queries together, not every row's maximum, make the workgroups.
-    const int64_t tiles = (a->num_q_rows - a->num_decode) / (4 * per) + a->num_prefill;
-    n.psplits = splits_of(tiles * a->num_kv_heads, cap < a->max_k ? cap : a->max_k, 512, kPrefillTarget, n.pchunk);
-    if (n.psplits > 1) n.pbytes = (size_t)(a->num_q_rows - a->num_decode) * a->num_heads * n.psplits * RECORD * 4;
+    const int per = 4 * (16 * kPrefillNT / (a->num_heads / a->num_kv_heads));
+    const int64_t cap = (int64_t)a->prefill_table_width * a->block_size, keys = cap < a->max_k ? cap : a->max_k;
+    // The rows' queries together bound the tiles; no more shares than steps / kLeastSteps.
+    const int64_t tiles = (a->num_q_rows - a->num_decode) / per + a->num_prefill, steps = tiles * ((keys + 63) / 64);
+    const int64_t most = (steps + kLeastSteps - 1) / kLeastSteps, full = (kPrefillShares + a->num_kv_heads - 1) / a->num_kv_heads;
+    n.shares = (int)(most < 1 ? 1 : most < full ? most : full);
+    n.pbytes = (size_t)n.shares * a->num_kv_heads * sizeof(Part);
   }
   return n;
 }
@@ -760,8 +910,8 @@ int check_args(const slo_paged_attention_args* a) {
   if (!(a->softmax_scale != 0.0f) || a->softmax_scale - a->softmax_scale != 0.0f)
     return fail(SLO_ERR_INVALID, "paged_attention_fp4: softmax_scale must be finite and not zero");
   if (a->store_slot_mapping) return fail(SLO_ERR_INVALID, "paged_attention_fp4: store the new rows first");
-  if (a->num_decode > 65535 || a->num_prefill > 65535)
-    return fail(SLO_ERR_UNSUPPORTED, "paged_attention_fp4: more than 65535 rows");
+  if (a->num_decode > 65535 || a->num_prefill > kMaxPrefillRows)
+    return fail(SLO_ERR_UNSUPPORTED, "paged_attention_fp4: more than 65535 decode or 1024 prefill rows");
   const bool dec = a->num_decode > 0 && (a->phases & SLO_PHASE_DECODE);
   const bool pre = a->num_prefill > 0 && (a->phases & SLO_PHASE_PREFILL);
   if (!dec && !pre) return SLO_OK;
@@ -808,7 +958,7 @@ extern "C" int slo_paged_attention_fp4(const slo_paged_attention_args* a, slo_st
   if (n.dbytes + n.pbytes > 0 && (!a->workspace || a->workspace_bytes < n.dbytes + n.pbytes ||
                                   reinterpret_cast<uintptr_t>(a->workspace) % 16))
     return fail(SLO_ERR_WORKSPACE, "paged_attention_fp4: workspace smaller than slo_paged_attention_fp4_workspace_bytes");
-  if (!n.dwork && !n.ptiles) return SLO_OK;
+  if (!n.dwork && !n.shares) return SLO_OK;
   hipStream_t s = static_cast<hipStream_t>(stream);
   Fp4Params p = {};
   p.q = static_cast<const uint16_t*>(a->q);
@@ -838,12 +988,12 @@ extern "C" int slo_paged_attention_fp4(const slo_paged_attention_args* a, slo_st
     p.partial = static_cast<float*>(a->workspace);
     if (n.joined) {
       hipLaunchKernelGGL(fp4_decode_kernel<4>, dim3(p.hkv, n.budget + p.rows), dim3(256), 0, s, p);
-      hipLaunchKernelGGL(fp4_join_kernel<8>, dim3(p.hq, p.rows), dim3(256), 0, s, p);
+      hipLaunchKernelGGL(fp4_join_decode_kernel, dim3(p.hq, p.rows), dim3(256), 0, s, p);
     } else {
       hipLaunchKernelGGL(fp4_decode_kernel<8>, dim3(p.hkv, p.rows), dim3(512), 0, s, p);
     }
   }
-  if (n.ptiles) {
+  if (n.shares) {
     p.lens = nullptr;
     p.cu_q = a->prefill_cu_q;
     p.cu_k = a->prefill_cu_k;
@@ -851,14 +1001,12 @@ extern "C" int slo_paged_attention_fp4(const slo_paged_attention_args* a, slo_st
     p.table_stride = a->prefill_table_stride;
     p.table_width = a->prefill_table_width;
     p.first_row = a->num_decode;
-    p.splits = n.psplits;
-    p.chunk = n.pchunk;
-    p.partial = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + n.dbytes);
-    hipLaunchKernelGGL(fp4_prefill_kernel<kPrefillNT>, dim3(p.hkv, n.ptiles * p.splits, a->num_prefill), dim3(256), 0, s, p,
-                       n.ptiles);
-    if (p.splits > 1)
-      hipLaunchKernelGGL(fp4_join_kernel<1>, dim3((unsigned)(((int64_t)a->max_q * p.hq + 7) / 8), a->num_prefill), dim3(256),
-                         0, s, p);
+    p.rows = a->num_prefill;
+    p.shares = n.shares;
+    p.parts = reinterpret_cast<Part*>(static_cast<char*>(a->workspace) + n.dbytes);
+    hipLaunchKernelGGL(fp4_prefill_kernel<kPrefillNT>, dim3(p.hkv, p.shares), dim3(256), 0, s, p);
+    if (p.shares > 1)
+      hipLaunchKernelGGL(fp4_join_prefill_kernel<kPrefillNT>, dim3(p.hkv, p.shares - 1, 4 * kPrefillNT), dim3(256), 0, s, p);
   }
   return check_launch("paged_attention_fp4");
 }

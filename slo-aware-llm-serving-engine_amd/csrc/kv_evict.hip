@@ -12,13 +12,14 @@
 namespace slo {
 namespace {
 
-constexpr int SELECT_NT = 1024;
+constexpr int SELECT_NT = 512, RUN = 16;
 
 struct EvictParams {
   float* scores;  // [layers, num_blocks, hkv, block_size]
   const int32_t* lens;
   const int32_t* tables;
   int table_stride, table_width, num_blocks, block_size, hkv, rows, budget, recent;
+  float inv_block;    // 1 / block_size
   int32_t* new_lens;  // [rows]
   int32_t* kept;      // [layers, rows, hkv, budget]
 };
@@ -27,10 +28,23 @@ __device__ __forceinline__ int length_of(const EvictParams& p, int r) {
   return min(max(p.lens[r], 0), p.table_width * p.block_size);
 }
 
+// token / block_size and the remainder, by the reciprocal and one correction
+// (tokens are below 2^24, so the product is off by less than one).
+__device__ __forceinline__ int block_of(const EvictParams& p, int token, int& off) {
+  int b = (int)((float)token * p.inv_block);
+  off = token - b * p.block_size;
+  if (off < 0) {
+    --b;
+    off += p.block_size;
+  } else if (off >= p.block_size) {
+    ++b;
+    off -= p.block_size;
+  }
+  return b;
+}
+
 __device__ __forceinline__ int page_at(const EvictParams& p, int r, int token, int& off) {
-  const int page = token / p.block_size;
-  off = token - page * p.block_size;
-  const int b = p.tables[(int64_t)r * p.table_stride + page];
+  const int b = p.tables[(int64_t)r * p.table_stride + block_of(p, token, off)];
   return b >= 0 && b < p.num_blocks ? b : -1;
 }
 
@@ -41,15 +55,9 @@ __device__ __forceinline__ uint32_t order_key(float w) {
   return w != w ? 0u : u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
-__device__ __forceinline__ uint32_t key_at(const EvictParams& p, const float* scores, int r, int head, int token) {
-  int off;
-  const int b = page_at(p, r, token, off);
-  return b < 0 ? 0u : order_key(scores[((int64_t)b * p.hkv + head) * p.block_size + off]);
-}
-
 // Exclusive sum over the workgroup's threads; `total` receives the whole.
 __device__ __forceinline__ int block_scan(int x, int* sums, int& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int s = x;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
@@ -60,7 +68,8 @@ __device__ __forceinline__ int block_scan(int x, int* sums, int& total) {
   if (lane == 63) sums[wave] = s;
   __syncthreads();
   int before = 0, all = 0;
-  for (int w = 0; w < waves; ++w) {
+#pragma unroll
+  for (int w = 0; w < SELECT_NT / 64; ++w) {
     before += w < wave ? sums[w] : 0;
     all += sums[w];
   }
@@ -68,14 +77,30 @@ __device__ __forceinline__ int block_scan(int x, int* sums, int& total) {
   return before + s - x;
 }
 
+// A thread's run of tokens t0 .. t0 + RUN - 1 (inside one page) as keys.
+__device__ __forceinline__ void load_run(const EvictParams& p, const float* scores, int r, int head, int t0, int end,
+                                         uint32_t (&k)[RUN]) {
+  int b = -1, off = 0;
+  if (t0 < end) b = page_at(p, r, t0, off);
+#pragma unroll
+  for (int i = 0; i < RUN; i += 4) {
+    f32x4 x = {0, 0, 0, 0};
+    if (b >= 0) x = *reinterpret_cast<const f32x4*>(scores + ((int64_t)b * p.hkv + head) * p.block_size + off + i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) k[i + j] = b < 0 ? 0u : order_key(x[j]);
+  }
+}
+
 // The choice.  The budget - recent heaviest of the first n - recent tokens are
-// those above the key T of that rank and the first few equal to it; T is found
-// by its bytes, most significant first, from a histogram of the keys that
-// share the bytes found so far.  Then one pass in position order writes the
-// kept positions.
+// those above the key T of that rank and the first few equal to it.  T is
+// found by its 11, 11 and 10 bits, most significant first, from a histogram of
+// the keys that share the bits found so far; then one sum over the threads
+// places every kept position.  A thread owns RUN consecutive tokens, so a row of
+// up to SELECT_NT * RUN tokens is read once and stays in registers; a longer
+// one is read again for each step.
 __global__ void __launch_bounds__(SELECT_NT)
 evict_select_kernel(EvictParams p) {
-  __shared__ int hist[256], sums[SELECT_NT / 64], found[2];
+  __shared__ int hist[2048], sums[SELECT_NT / 64], found[2];
   const int head = blockIdx.x, r = blockIdx.y, layer = blockIdx.z;
   const int n = length_of(p, r), tid = threadIdx.x;
   int32_t* kept = p.kept + (((int64_t)layer * p.rows + r) * p.hkv + head) * p.budget;
@@ -86,102 +111,135 @@ evict_select_kernel(EvictParams p) {
   }
   const float* scores = p.scores + (int64_t)layer * p.num_blocks * p.hkv * p.block_size;
   const int old = n - p.recent;
+  constexpr int SPAN = SELECT_NT * RUN;
+  uint32_t k[RUN];
+  load_run(p, scores, r, head, tid * RUN, old, k);
   int need = p.budget - p.recent;  // still to choose among the keys that match `prefix`
   uint32_t prefix = 0;
-  for (int shift = 24; shift >= 0 && need > 0; shift -= 8) {
-    for (int i = tid; i < 256; i += SELECT_NT) hist[i] = 0;
+#pragma unroll
+  for (int step = 0; step < 3; ++step) {
+    const int shift = step == 0 ? 21 : step == 1 ? 10 : 0, bins = step == 2 ? 1024 : 2048;
+    const uint32_t known = step == 0 ? 0u : step == 1 ? 0xffe00000u : 0xfffffc00u;
+    if (need <= 0) break;
+    for (int i = tid; i < 2048; i += SELECT_NT) hist[i] = 0;
     __syncthreads();
-    for (int t = tid; t < old; t += SELECT_NT) {
-      const uint32_t k = key_at(p, scores, r, head, t);
-      if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1);
+    for (int base = 0; base < old; base += SPAN) {
+      const int t0 = base + tid * RUN;
+      if (base) load_run(p, scores, r, head, t0, old, k);
+#pragma unroll
+      for (int i = 0; i < RUN; ++i)
+        if (t0 + i < old && ((k[i] ^ prefix) & known) == 0) atomicAdd(&hist[(k[i] >> shift) & (bins - 1)], 1);
     }
     __syncthreads();
-    // Thread b holds bin 255 - b: the keys above a bin are those before it.
-    int total;
-    const int mine = tid < 256 ? hist[255 - tid] : 0;
-    const int above = block_scan(mine, sums, total);
-    if (tid < 256 && above < need && above + mine >= need) {
-      found[0] = 255 - tid;
-      found[1] = above;
+    // Thread t adds up the bins from the top: those above its own are before it.
+    constexpr int PER = 2048 / SELECT_NT;
+    int mine = 0, bin[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      bin[i] = hist[2047 - (tid * PER + i)];  // empty above `bins`
+      mine += bin[i];
+    }
+    int total, above = block_scan(mine, sums, total);
+    if (above < need && above + mine >= need) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        if (above < need && above + bin[i] >= need) {
+          found[0] = 2047 - (tid * PER + i);
+          found[1] = above;
+        }
+        above += bin[i];
+      }
     }
     __syncthreads();
     prefix |= (uint32_t)found[0] << shift;
     need -= found[1];
+    if (old > SPAN) load_run(p, scores, r, head, tid * RUN, old, k);
     __syncthreads();
   }
-  // need: how many of the keys equal to prefix are kept (none where no old token is).
+  // `need` of the keys equal to prefix are kept, the first ones; none where no
+  // old token is kept.
   const bool any = p.budget > p.recent;
   int equal_before = 0, kept_before = 0;
-  for (int t0 = 0; t0 < n; t0 += SELECT_NT) {
-    const int t = t0 + tid;
-    bool above = false, equal = false;
-    if (t < n) {
-      if (t >= old) {
-        above = true;
-      } else if (any) {
-        const uint32_t k = key_at(p, scores, r, head, t);
-        above = k > prefix;
-        equal = k == prefix;
-      }
+  for (int base = 0; base < n; base += SPAN) {
+    const int t0 = base + tid * RUN;
+    if (base) load_run(p, scores, r, head, t0, old, k);
+    int above = 0, equal = 0;
+#pragma unroll
+    for (int i = 0; i < RUN; ++i) {
+      const int t = t0 + i;
+      above += t < n && (t >= old || (any && k[i] > prefix));
+      equal += t < old && any && k[i] == prefix;
     }
-    int equals, keeps;
-    const int e = equal_before + block_scan(equal, sums, equals);
-    const bool keep = above || (equal && e < need);
-    const int at = kept_before + block_scan(keep, sums, keeps);
-    if (keep) kept[at] = t;
-    equal_before += equals;
-    kept_before += keeps;
+    int total;
+    const int before = block_scan(above | equal << 16, sums, total);  // both are at most SPAN < 2^15
+    int eq = equal_before + (before >> 16), at = kept_before + (before & 0xffff) + min(eq, need) - min(equal_before, need);
+#pragma unroll
+    for (int i = 0; i < RUN; ++i) {
+      const int t = t0 + i;
+      const bool is = t < old && any && k[i] == prefix;
+      if ((t < n && (t >= old || (any && k[i] > prefix))) || (is && eq < need)) kept[at++] = t;
+      eq += is;
+    }
+    kept_before += (total & 0xffff) + min(equal_before + (total >> 16), need) - min(equal_before, need);
+    equal_before += total >> 16;
   }
 }
 
-// One array of the pool that moves with the tokens: `unit` bytes of a token's
-// `row` bytes per lane.
+// One array of the pool that moves with the tokens, or 64 bytes of each of its
+// rows: `unit` bytes of a lane, `units` lanes a token.
 struct Stream {
   uint8_t* base;
   int64_t layer_bytes, page_bytes;
-  int head_bytes, token_bytes, row;
+  int head_bytes, token_bytes, unit, units;
 };
+
+constexpr int kMaxStreams = 20, kDepth = 8;
 
 struct MoveParams {
   EvictParams e;
-  Stream s[5];
-  int streams;
+  Stream s[kMaxStreams];
 };
 
-// The move, in place: a workgroup takes one array of one (layer, row, kv head)
+// The move, in place: a workgroup takes one stream of one (layer, row, kv head)
 // and fills its places in ascending order.  The token that comes to place i
-// lies at i or later, so once the tiles up to some place have been read, what
-// is stored there is not read again: each tile is loaded whole, and stored
-// after a barrier.
-template <typename U, int DEPTH>
-__device__ void move_stream(const EvictParams& p, const Stream& s, int r, int head, int layer, int n) {
-  const int per = s.row / (int)sizeof(U);  // units of a token
+// lies at i or later, so once the places up to some point have been read, what
+// is stored there is not read again: a tile of 256 kDepth units is loaded whole,
+// and stored after a barrier.  A row's order leaves no more workgroups than
+// streams, so each keeps kDepth loads a lane in flight (a tile is 512 tokens of
+// 64 bytes).
+template <typename U>
+__device__ __forceinline__ void move_stream(const EvictParams& p, const Stream& s, int r, int head, int layer) {
   const int32_t* kept = p.kept + (((int64_t)layer * p.rows + r) * p.hkv + head) * p.budget;
   uint8_t* base = s.base + layer * s.layer_bytes + (int64_t)head * s.head_bytes;
-  const int units = p.budget * per;
-  for (int u0 = 0; u0 < units; u0 += 256 * DEPTH) {
-    U x[DEPTH];
-    uint8_t* to[DEPTH];
+  const int shift = s.units == 4 ? 2 : s.units == 2 ? 1 : 0;  // 1, 2 or 4 lanes a token
+  const int part = (threadIdx.x & (s.units - 1)) * (int)sizeof(U), tile = (256 >> shift) * kDepth;
+  for (int i0 = 0; i0 < p.budget; i0 += tile) {
+    int src[kDepth];
 #pragma unroll
-    for (int d = 0; d < DEPTH; ++d) {
-      const int u = u0 + 256 * d + (int)threadIdx.x;
-      to[d] = nullptr;
-      if (u >= units) continue;
-      const int i = u / per, part = (u - i * per) * (int)sizeof(U);
-      const int src = kept[i];
-      if (src == i || src < 0) continue;
+    for (int d = 0; d < kDepth; ++d) {
+      const int i = i0 + ((256 * d + (int)threadIdx.x) >> shift);
+      src[d] = i < p.budget ? kept[i] : -1;
+      if (src[d] == i) src[d] = -1;  // already there
+    }
+    U x[kDepth];
+    int64_t to[kDepth];
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d) {
+      const int i = i0 + ((256 * d + (int)threadIdx.x) >> shift);
+      to[d] = -1;
+      if (src[d] < 0) continue;
       int soff, doff;
-      const int sb = page_at(p, r, src, soff), db = page_at(p, r, i, doff);
+      const int sb = page_at(p, r, src[d], soff), db = page_at(p, r, i, doff);
       if (sb < 0 || db < 0) continue;
-      x[d] = *reinterpret_cast<const U*>(base + sb * s.page_bytes + (int64_t)soff * s.token_bytes + part);
-      to[d] = base + db * s.page_bytes + (int64_t)doff * s.token_bytes + part;
+      x[d] = *reinterpret_cast<const U*>(base + (sb * s.page_bytes + (int64_t)soff * s.token_bytes + part));
+      to[d] = db * s.page_bytes + (int64_t)doff * s.token_bytes + part;
     }
     // The barrier alone orders LDS accesses; the loads have to have come back.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
 #pragma unroll
-    for (int d = 0; d < DEPTH; ++d)
-      if (to[d]) *reinterpret_cast<U*>(to[d]) = x[d];
+    for (int d = 0; d < kDepth; ++d)
+      if (to[d] >= 0) *reinterpret_cast<U*>(base + to[d]) = x[d];
   }
 }
 
@@ -192,12 +250,12 @@ evict_move_kernel(MoveParams m) {
   const int n = length_of(p, r);
   if (n <= p.budget) return;
   const Stream& s = m.s[which];
-  if (s.row % 16 == 0) {
-    move_stream<u32x4, 4>(p, s, r, head, layer, n);
-  } else if (s.row % 4 == 0) {
-    move_stream<uint32_t, 4>(p, s, r, head, layer, n);
+  if (s.unit == 16) {
+    move_stream<u32x4>(p, s, r, head, layer);
+  } else if (s.unit == 4) {
+    move_stream<uint32_t>(p, s, r, head, layer);
   } else {
-    move_stream<uint16_t, 4>(p, s, r, head, layer, n);
+    move_stream<uint16_t>(p, s, r, head, layer);
   }
   if (which) return;
   // Stream 0 is the scores: the places given up start again from zero.
@@ -231,8 +289,9 @@ extern "C" int slo_evict_kv(const slo_evict_kv_args* a, slo_stream_t stream) {
   if (a->kv_dtype != KV_BF16 && (!a->k_scale || !a->v_scale)) return fail(SLO_ERR_INVALID, "evict_kv: a quantised pool needs its scales");
   if ((reinterpret_cast<uintptr_t>(a->k_cache) % 16) || (reinterpret_cast<uintptr_t>(a->v_cache) % 16) ||
       (reinterpret_cast<uintptr_t>(a->k_scale) % 4) || (reinterpret_cast<uintptr_t>(a->v_scale) % 4) ||
-      (reinterpret_cast<uintptr_t>(a->scores) % 4))
-    return fail(SLO_ERR_INVALID, "evict_kv: pools must be 16-byte aligned");
+      (reinterpret_cast<uintptr_t>(a->scores) % 16))
+    return fail(SLO_ERR_INVALID, "evict_kv: pools and scores must be 16-byte aligned");
+  if (a->block_size % 64) return fail(SLO_ERR_UNSUPPORTED, "evict_kv: block_size must be a multiple of 64");
   if ((int64_t)a->table_width * a->block_size > (1 << 24) || a->budget > (1 << 24))
     return fail(SLO_ERR_UNSUPPORTED, "evict_kv: more than 2^24 tokens a row");
   MoveParams m = {};
@@ -251,25 +310,30 @@ extern "C" int slo_evict_kv(const slo_evict_kv_args* a, slo_stream_t stream) {
   p.new_lens = a->new_lens;
   p.kept = a->kept;
   const bool fp4 = a->kv_dtype == KV_FP4_E2M1;
-  // Head by head pages (4-bit pools and the scores) or token by token.
-  auto stream_of = [&](void* base, int row, bool by_head) {
+  p.inv_block = 1.0f / (float)a->block_size;
+  // Rows of `row` bytes, pages head by head (4-bit pools and the scores) or
+  // token by token, in streams of up to 64 bytes of each row.
+  int streams = 0;
+  auto add = [&](void* base, int row, bool by_head) {
     const int64_t page = (int64_t)a->block_size * a->num_kv_heads * row;
-    return Stream{static_cast<uint8_t*>(base), page * a->num_blocks, page, by_head ? a->block_size * row : row,
-                  by_head ? row : a->num_kv_heads * row, row};
+    const int unit = row % 16 == 0 ? 16 : row % 4 == 0 ? 4 : 2, most = 4 * unit;
+    for (int at = 0; at < row; at += most) {
+      const int bytes = row - at < most ? row - at : most;
+      m.s[streams++] = Stream{static_cast<uint8_t*>(base) + at, page * a->num_blocks, page, by_head ? a->block_size * row : row,
+                              by_head ? row : a->num_kv_heads * row, unit, bytes / unit};
+    }
   };
   const int row = a->kv_dtype == KV_BF16 ? 2 * a->head_dim : fp4 ? a->head_dim / 2 : a->head_dim;
-  m.s[0] = stream_of(a->scores, 4, true);
-  m.s[1] = stream_of(a->k_cache, row, fp4);
-  m.s[2] = stream_of(a->v_cache, row, fp4);
-  m.streams = 3;
+  add(a->scores, 4, true);
+  add(a->k_cache, row, fp4);
+  add(a->v_cache, row, fp4);
   if (a->kv_dtype != KV_BF16) {
     const int scale = fp4 ? a->head_dim / kFp4Group : 4;
-    m.s[3] = stream_of(a->k_scale, scale, fp4);
-    m.s[4] = stream_of(a->v_scale, scale, fp4);
-    m.streams = 5;
+    add(a->k_scale, scale, fp4);
+    add(a->v_scale, scale, fp4);
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
   hipLaunchKernelGGL(evict_select_kernel, dim3(p.hkv, p.rows, a->num_layers), dim3(SELECT_NT), 0, s, p);
-  hipLaunchKernelGGL(evict_move_kernel, dim3(p.hkv * m.streams, p.rows, a->num_layers), dim3(256), 0, s, m);
+  hipLaunchKernelGGL(evict_move_kernel, dim3(p.hkv * streams, p.rows, a->num_layers), dim3(256), 0, s, m);
   return check_launch("evict_kv");
 }

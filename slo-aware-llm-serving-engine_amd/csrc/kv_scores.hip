@@ -14,7 +14,7 @@
 //    are 4 bytes per (head, token), a sixteenth to a quarter of K itself, so K
 //    is read once.
 //  * prefill rows: the first pass finds every (query, head)'s log2-sum; the
-//    second computes S^T again, 32 keys of a wavefront against all queries,
+//    second computes S^T again, 64 keys of a workgroup against all queries,
 //    and sums the weights over the queries in registers (writing the scores of
 //    a 1,000-query chunk would take more than the two products).
 //
@@ -27,6 +27,10 @@
 namespace slo {
 namespace {
 
+#ifndef LW
+#define LW 3
+#define LN 2
+#endif
 constexpr int HDS = 128;
 constexpr float kNone = -1e30f;
 
@@ -102,6 +106,7 @@ struct Keys {
   uint32_t code;
 
   // `block` page, token `off` of it
+  template <bool SCALE = true>
   __device__ __forceinline__ void load(const ScoreParams& p, int block, int off, int head, int lane) {
     const int col = lane & 15, kg = lane >> 4;
     if (KV == KV_FP4_E2M1) {
@@ -114,7 +119,7 @@ struct Keys {
       const uint8_t* at = p.kc + ((slot + col) * p.hkv + head) * rb + kg * 16;
 #pragma unroll
       for (int i = 0; i < N; ++i) w[i] = *reinterpret_cast<const u32x4*>(at + i * 64);
-      if (KV == KV_FP8_E4M3FN) {
+      if (KV == KV_FP8_E4M3FN && SCALE) {
         const float* s = static_cast<const float*>(p.ks) + (slot + 4 * kg) * p.hkv + head;
 #pragma unroll
         for (int i = 0; i < 4; ++i) scale[i & (sizeof(scale) / 4 - 1)] = s[(int64_t)i * p.hkv];
@@ -237,9 +242,13 @@ score_decode_kernel(ScoreParams p) {
 }
 
 // Prefill rows, first pass: 16 NT (query, head) columns of one row per
-// workgroup, its four wavefronts every fourth 16-token tile of their keys.
+// workgroup, its four wavefronts every fourth pair of 16-token tiles of their
+// keys, the next pair's loads ahead of the products.  A lane sums its own
+// tokens' weights against a reference of its own, which follows a new maximum
+// only where that passes it by 2^8 (sums of weights up to 256 round like those
+// below 1); the lanes meet at the end.
 template <int KV, int NT>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, LW)
 score_lse_kernel(ScoreParams p, int tiles) {
   __shared__ float sm[NT][4][64], sl[NT][4][64];
   const int head = blockIdx.x, r = blockIdx.z;
@@ -264,34 +273,59 @@ score_lse_kernel(ScoreParams p, int tiles) {
     l[n] = 0.0f;
   }
   const int full = min(g.prefix + t0 + 1, g.lk);
-  for (int at = 16 * wave; at < kend; at += 64) {
+  Keys<KV> k[2];
+  auto load = [&](int at) {
     int off;
     const int block = page_of(p, r, at, off);
-    if (block < 0) continue;
-    Keys<KV> k;
-    k.load(p, block, off, head, lane);
-    f32x4 s[NT];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) s[n] = f32x4{0, 0, 0, 0};
+    for (int h = 0; h < 2; ++h) k[h].load(p, block < 0 ? 0 : block, (block < 0 ? 0 : off) + 16 * h, head, lane);
+    return block >= 0;
+  };
+  int at = 32 * wave;
+  bool ok = at < kend && load(at);
+  for (; at < kend; at += 128) {
+    bf16x8 a[2][4];
+    float f[2][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const bf16x8 a = k.operand(i);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) s[n] = mfma16(a, q[n][i], s[n]);
-    }
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        s[n][i] *= k.factor(i) * p.scale_log2;
-        if (at + 16 > full && at + 4 * kg + i >= limit[n]) s[n][i] = -INFINITY;
+        a[h][i] = k[h].operand(i);
+        f[h][i] = k[h].factor(i) * p.scale_log2;
       }
-      const float top = fmaxf(fmaxf(m[n], fmaxf(s[n][0], s[n][1])), fmaxf(s[n][2], s[n][3]));
-      float sum = 0.0f;
+    const bool now = ok;
+    if (at + 128 < kend) ok = load(at + 128);
+    if (!now) continue;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum += __builtin_amdgcn_exp2f(s[n][i] - top);
-      l[n] = l[n] * __builtin_amdgcn_exp2f(m[n] - top) + sum;
-      m[n] = top;
+    for (int n = 0; n < NT; ++n) {
+      f32x4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[0] = mfma16(a[0][i], q[n][i], s[0]);
+        s[1] = mfma16(a[1][i], q[n][i], s[1]);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[h][i] *= f[h][i];
+      if (at + 32 > full) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (at + 16 * h + 4 * kg + i >= limit[n]) s[h][i] = -INFINITY;
+      }
+      const float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                              fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+      if (__any(top > m[n] + 8.0f)) {
+        const float to = fmaxf(m[n], top);
+        l[n] *= __builtin_amdgcn_exp2f(m[n] - to);
+        m[n] = to;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) l[n] += __builtin_amdgcn_exp2f(s[h][i] - m[n]);
     }
   }
 #pragma unroll
@@ -304,72 +338,116 @@ score_lse_kernel(ScoreParams p, int tiles) {
   if (x < per * p.group && tok < t1) {
     float mm = kNone, ll = 0.0f;
     for (int w = 0; w < 4; ++w)
-      for (int k = 0; k < 4; ++k) absorb(mm, ll, sm[x >> 4][w][16 * k + (x & 15)], sl[x >> 4][w][16 * k + (x & 15)]);
+      for (int j = 0; j < 4; ++j) absorb(mm, ll, sm[x >> 4][w][16 * j + (x & 15)], sl[x >> 4][w][16 * j + (x & 15)]);
     p.lse[(g.q0 - p.first_row + tok) * p.hq + head * p.group + x % p.group] = mm + __builtin_amdgcn_logf(ll);
   }
 }
 
-// Prefill rows, second pass: 32 keys of one (row, kv head) per wavefront
-// against every column that sees one of them.
+// Prefill rows, second pass: a workgroup takes 64 keys of one (row, kv head),
+// held as operands in every wavefront's registers, and its six wavefronts every
+// sixth 16 of the columns that see one of them.  A lane sums its 16
+// tokens' weights over its columns; lanes, then wavefronts, are added in order
+// at the end.
+constexpr int kSumWaves = 6, kSumKeys = 64;
+
 template <int KV>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(64 * kSumWaves, 3)
 score_prefill_kernel(ScoreParams p) {
+  __shared__ float sums[kSumWaves][kSumKeys];
+  __shared__ f32x4 factors[KV == KV_FP8_E4M3FN ? kSumKeys / 4 : 1];  // E4M3FN scales, in LDS to save registers
   const int head = blockIdx.x, r = blockIdx.z;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, kg = lane >> 4;
   const Row g = row_of(p, r);
-  const int at = (blockIdx.y * 4 + wave) * 32;
+  const int at = blockIdx.y * kSumKeys;
   if (at >= g.lk || g.lq <= 0) return;
   int off;
   const int block = page_of(p, r, at, off);
   if (block < 0) return;
-  bf16x8 a[2][4];
-  float factor[2][4];
+  bf16x8 a[4][4];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < 4; ++h) {
     Keys<KV> k;
-    k.load(p, block, off + 16 * h, head, lane);
+    k.template load<false>(p, block, off + 16 * h, head, lane);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      a[h][i] = k.operand(i);
-      factor[h][i] = k.factor(i) * p.scale_log2;
-    }
+    for (int i = 0; i < 4; ++i) a[h][i] = k.operand(i);
   }
-  f32x4 w[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-  const int columns = g.lq * p.group;
-  for (int x0 = max(at - g.prefix, 0) * p.group; x0 < columns; x0 += 16) {
-    const int x = x0 + col, tok = x / p.group, hh = head * p.group + x % p.group;
+  if (KV == KV_FP8_E4M3FN) {
+    if (threadIdx.x < kSumKeys)
+      reinterpret_cast<float*>(factors)[threadIdx.x] =
+          static_cast<const float*>(p.ks)[((int64_t)block * p.block_size + off + threadIdx.x) * p.hkv + head] * p.scale_log2;
+    __syncthreads();
+  }
+  float w[4][4] = {};
+  const int columns = g.lq * p.group, stride = 16 * kSumWaves;
+  // This lane's column, query and head; the next ones by addition.
+  int x = max(at - g.prefix, 0) * p.group + 16 * wave + col;
+  int tok = x / p.group, hh = x - tok * p.group;
+  const int dt = stride / p.group, dh = stride - dt * p.group;
+  bf16x8 q[4];
+  float lse;
+  auto load = [&] {
     const bool live = x < columns;
-    const float lse = live ? p.lse[(g.q0 - p.first_row + tok) * p.hq + hh] : INFINITY;
-    f32x4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const bf16x8 q = load_q<KV>(p, g.q0 + tok, hh, i, kg, live);
-      s[0] = mfma16(a[0][i], q, s[0]);
-      s[1] = mfma16(a[1][i], q, s[1]);
+    for (int i = 0; i < 4; ++i) q[i] = load_q<KV>(p, g.q0 + tok, head * p.group + hh, i, kg, live);
+    // A column past the last weighs nothing.
+    lse = live ? p.lse[(g.q0 - p.first_row + tok) * p.hq + head * p.group + hh] : INFINITY;
+  };
+  if (x - col < columns) load();
+  while (x - col < columns) {
+    asm volatile("" ::: "memory");  // the factors are read again, not held
+    f32x4 s[4] = {};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int h = 0; h < 4; ++h) s[h] = mfma16(a[h][i], q[i], s[h]);
+    const float ref = lse;
+    const int limit = min(g.prefix + tok + 1, g.lk);
+    // The next columns load while this one's weights are taken.
+    x += stride;
+    tok += dt;
+    hh += dh;
+    if (hh >= p.group) {
+      hh -= p.group;
+      ++tok;
     }
-    const int limit = live ? min(g.prefix + tok + 1, g.lk) : 0;
+    if (x - col < columns) load();
+    auto add = [&](bool masked) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 4; ++h) {
+        const f32x4 f = KV == KV_FP8_E4M3FN ? factors[4 * h + kg] : f32x4{p.scale_log2, p.scale_log2, p.scale_log2, p.scale_log2};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][i], factor[h][i], -lse));
-        w[h][i] += at + 16 * h + 4 * kg + i < limit ? e : 0.0f;
+        for (int i = 0; i < 4; ++i) {
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][i], f[i], -ref));
+          w[h][i] += masked && at + 16 * h + 4 * kg + i >= limit ? 0.0f : e;
+        }
       }
+    };
+    if (__any(limit < at + kSumKeys))
+      add(true);
+    else
+      add(false);
   }
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
+  for (int h = 0; h < 4; ++h)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float e = w[h][i];
 #pragma unroll
       for (int d = 1; d < 16; d <<= 1) e += __shfl_xor(e, d, 64);
-      const int token = at + 16 * h + 4 * kg + i;
-      if (col == 0 && token < g.lk) add_score(p, g, block, off + 16 * h + 4 * kg + i, head, token, e);
+      if (col == 0) sums[wave][16 * h + 4 * kg + i] = e;
     }
+  __syncthreads();
+  const int token = at + (int)threadIdx.x;
+  if (threadIdx.x < kSumKeys && token < g.lk) {
+    float e = 0.0f;
+#pragma unroll
+    for (int v = 0; v < kSumWaves; ++v) e += sums[v][threadIdx.x];
+    add_score(p, g, block, off + threadIdx.x, head, token, e);
+  }
 }
 
-constexpr int kLseNT = 4;
+constexpr int kLseNT = LN;
 
 struct Plan {
   int splits, chunk, tiles;
@@ -442,8 +520,10 @@ void launch(const ScoreParams& d, const ScoreParams& f, const slo_paged_attentio
   }
   if (n.tiles) {
     hipLaunchKernelGGL((score_lse_kernel<KV, kLseNT>), dim3(f.hkv, n.tiles, a->num_prefill), dim3(256), 0, s, f, n.tiles);
-    const int cap = f.table_width * f.block_size;
-    hipLaunchKernelGGL(score_prefill_kernel<KV>, dim3(f.hkv, (cap + 127) / 128, a->num_prefill), dim3(256), 0, s, f);
+    const int64_t most = (int64_t)f.table_width * f.block_size;
+    const int64_t keys = a->max_k > 0 ? ((int64_t)a->max_k + 63) / 64 * 64 : 64;
+    const int cap = (int)(most < keys ? most : keys);
+    hipLaunchKernelGGL(score_prefill_kernel<KV>, dim3(f.hkv, cap / kSumKeys, a->num_prefill), dim3(64 * kSumWaves), 0, s, f);
   }
 }
 

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 LIB_NAME = "libslo_attn.so"
@@ -62,6 +63,12 @@ class PagedAttentionArgs(ctypes.Structure):
         ("num_new_rows", _c_int32),
         ("store_scale_floor", ctypes.c_float),
     ]
+
+
+# PagedAttentionArgs as bytes: the wrappers of calls of a few microseconds build
+# it from one tuple in field order (a ctypes field takes 0.1 us to set).
+_CODES = {_c_void_p: "P", _c_int64: "q", _c_int32: "i", ctypes.c_float: "f", ctypes.c_size_t: "N"}
+pack_attention_args = struct.Struct("@" + "".join(_CODES[t] for _, t in PagedAttentionArgs._fields_) + "0P").pack
 
 
 class EvictKvArgs(ctypes.Structure):
@@ -152,11 +159,11 @@ def load() -> ctypes.CDLL:
             _c_int32, _c_void_p, _c_void_p, _c_void_p]
         for name in ("slo_paged_attention_fp4_workspace_bytes", "slo_accumulate_attention_workspace_bytes"):
             getattr(lib, name).restype = ctypes.c_int
-            getattr(lib, name).argtypes = [ctypes.POINTER(PagedAttentionArgs), ctypes.POINTER(ctypes.c_size_t)]
+            getattr(lib, name).argtypes = [ctypes.c_char_p, ctypes.POINTER(ctypes.c_size_t)]
         lib.slo_paged_attention_fp4.restype = ctypes.c_int
-        lib.slo_paged_attention_fp4.argtypes = [ctypes.POINTER(PagedAttentionArgs), _c_void_p]
+        lib.slo_paged_attention_fp4.argtypes = [ctypes.c_char_p, _c_void_p]
         lib.slo_accumulate_attention.restype = ctypes.c_int
-        lib.slo_accumulate_attention.argtypes = [ctypes.POINTER(PagedAttentionArgs), _c_void_p, _c_void_p]
+        lib.slo_accumulate_attention.argtypes = [ctypes.c_char_p, _c_void_p, _c_void_p]
         lib.slo_evict_kv.restype = ctypes.c_int
         lib.slo_evict_kv.argtypes = [ctypes.POINTER(EvictKvArgs), _c_void_p]
         lib.slo_evict_kv_args_size.restype = ctypes.c_size_t

@@ -8,6 +8,7 @@ There is no CPU path: CPU tensors are rejected.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import threading
 
@@ -16,6 +17,7 @@ import torch
 from . import _lib
 
 _FP4_DTYPE = getattr(torch, "float4_e2m1fn_x2", None)
+_FP32 = (torch.float32,)
 _E8M0_DTYPES = (torch.uint8,) + ((torch.float8_e8m0fnu,) if hasattr(torch, "float8_e8m0fnu") else ())
 _FP8_DTYPES = (torch.uint8,) + ((torch.float8_e4m3fn,) if hasattr(torch, "float8_e4m3fn") else ())
 
@@ -35,7 +37,7 @@ def is_fp4(cache: torch.Tensor | None) -> bool:
     return cache is not None and _FP4_DTYPE is not None and cache.dtype == _FP4_DTYPE
 
 
-def _pool_geometry(k_cache, k_scale, v_cache=None, v_scale=None, head_dim=None, want_v=True):
+def _pool_geometry(k_cache, k_scale, v_cache=None, v_scale=None, want_v=True):
     """Checks a layer's pool views and returns ``(code, blocks, block_size, kv_heads, head_dim)``.
 
     bf16 and E4M3FN pools are ``[blocks, block_size, kv_heads, head_dim]`` with
@@ -44,36 +46,35 @@ def _pool_geometry(k_cache, k_scale, v_cache=None, v_scale=None, head_dim=None, 
     ``[blocks, kv_heads, block_size, head_dim / 32]``.
     """
     code = kv_dtype_code(k_cache)
-    caches, scales = ((k_cache, v_cache), (k_scale, v_scale)) if want_v else ((k_cache,), (k_scale,))
-    for c in caches:
-        if kv_dtype_code(c) != code:
+    shape = k_cache.shape
+    if len(shape) != 4 or not k_cache.is_contiguous():
+        raise ValueError("KV pool views must be contiguous and 4-dimensional")
+    if want_v:
+        if kv_dtype_code(v_cache) != code:
             raise TypeError("k_cache and v_cache formats differ")
-        if c.dim() != 4 or c.shape != k_cache.shape or not c.is_contiguous():
-            raise ValueError("KV pool views must be contiguous, 4-dimensional and of one shape")
+        if v_cache.shape != shape or not v_cache.is_contiguous():
+            raise ValueError("k_cache and v_cache must be contiguous and of one shape")
     if code == _lib.KV_FP4_E2M1:
-        blocks, heads, block, d = k_cache.shape
+        blocks, heads, block, d = shape
         d *= 2
-        shape, dtypes = (blocks, heads, block, d // _lib.FP4_GROUP), _E8M0_DTYPES
+        want, dtypes = (blocks, heads, block, d // _lib.FP4_GROUP), _E8M0_DTYPES
     else:
-        blocks, block, heads, d = k_cache.shape
-        shape, dtypes = (blocks, block, heads), (torch.float32,)
-    if head_dim is not None and d != head_dim:
-        raise ValueError(f"KV pool holds head_dim {d}, not {head_dim}")
+        blocks, block, heads, d = shape
+        want, dtypes = (blocks, block, heads), _FP32
     if code != _lib.KV_BF16:
-        for sc in scales:
+        for sc in (k_scale, v_scale) if want_v else (k_scale,):
             if sc is None:
                 raise ValueError("a quantised pool needs its scales")
-            if sc.dtype not in dtypes or tuple(sc.shape) != shape or not sc.is_contiguous():
+            if sc.dtype not in dtypes or sc.shape != want or not sc.is_contiguous():
                 kind = "E8M0" if code == _lib.KV_FP4_E2M1 else "fp32"
-                raise ValueError(f"scale pools must be contiguous {kind} {list(shape)}")
+                raise ValueError(f"scale pools must be contiguous {kind} {list(want)}")
     return code, blocks, block, heads, d
 
 
 def _check_scores(kv_scores, blocks, heads, block, layers=()):
     if kv_scores.dtype != torch.float32:
         raise TypeError("kv_scores must be fp32")
-    if tuple(kv_scores.shape) != (*layers, blocks, heads, block) or \
-            not kv_scores.is_contiguous():
+    if kv_scores.shape != (*layers, blocks, heads, block) or not kv_scores.is_contiguous():
         raise ValueError("kv_scores must be contiguous fp32 [num_blocks, num_kv_heads, block_size]")
 
 
@@ -99,6 +100,32 @@ def _stream(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _one_device(first: torch.Tensor, *others) -> int:
+    """The index of the GPU that holds all tensors (None: left out)."""
+    device = first.device
+    if device.type != "cuda":
+        raise RuntimeError("slo_attn kernels need GPU tensors; there is no CPU fallback")
+    for t in others:
+        if t is not None and t.device != device:
+            if t.device.type != "cuda":
+                raise RuntimeError("slo_attn kernels need GPU tensors; there is no CPU fallback")
+            raise RuntimeError(f"tensors on different devices: {device} vs {t.device}")
+    return device.index
+
+
+def _launch(index: int, what: str, *args) -> None:
+    """Calls an entry point on the current stream of GPU ``index``, which need not be the current one."""
+    lib = _lib.load()
+    with contextlib.nullcontext() if torch.cuda.current_device() == index else torch.cuda.device(index):
+        rc = getattr(lib, what)(*args, _raw_stream(index))
+    if rc:
+        _lib.check(rc, what)
+
+
 def _int32(t: torch.Tensor, name: str) -> torch.Tensor:
     if t.dtype != torch.int32:
         raise TypeError(f"{name} must be int32, got {t.dtype}")
@@ -114,7 +141,8 @@ def check_store(key, value, k_cache, v_cache, slot_mapping, k_scale=None, v_scal
     N, num_heads, head_dim = key.shape
     D = num_heads * head_dim
     if is_fp4(k_cache):
-        return _check_store_fp4(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale)
+        index, _ = _check_store_fp4(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale)
+        return torch.device("cuda", index), _lib.KV_FP4_E2M1
     # Same stride contract as the reference store (attention.py:36-39).
     assert key.stride(-1) == 1 and value.stride(-1) == 1
     assert key.stride(1) == head_dim and value.stride(1) == head_dim
@@ -142,20 +170,22 @@ def check_store(key, value, k_cache, v_cache, slot_mapping, k_scale=None, v_scal
 
 
 def _check_store_fp4(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale):
-    N, num_heads, head_dim = key.shape
-    assert key.stride(-1) == 1 and value.stride(-1) == 1
-    assert key.stride(1) == head_dim and value.stride(1) == head_dim
+    """``check_store`` for a 4-bit pool; returns ``(device index, its geometry)``."""
+    N, num_heads, head_dim = shape = key.shape
+    ks, vs = key.stride(), value.stride()
+    assert ks[2] == 1 and vs[2] == 1
+    assert ks[1] == head_dim and vs[1] == head_dim
     assert slot_mapping.numel() == N
-    device = _require_gpu(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale)
+    index = _one_device(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale)
     if key.dtype != torch.bfloat16 or value.dtype != torch.bfloat16:
         raise TypeError("key/value must be bf16")
-    if value.shape != key.shape:
+    if value.shape != shape:
         raise ValueError("key/value shapes differ")
-    code, _, _, heads, _ = _pool_geometry(k_cache, k_scale, v_cache, v_scale, head_dim)
-    if heads != num_heads:
+    geometry = _pool_geometry(k_cache, k_scale, v_cache, v_scale)
+    if geometry[3] != num_heads or geometry[4] != head_dim:
         raise ValueError("KV pool must be [num_blocks, num_kv_heads, block_size, head_dim / 2]")
     _int32(slot_mapping, "slot_mapping")
-    return device, code
+    return index, geometry
 
 
 def foldable(key: torch.Tensor, value: torch.Tensor) -> bool:
@@ -207,14 +237,15 @@ def store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
     head_dim / 32]`` (uint8 or float8_e8m0fnu), one per 32 channels;
     ``scale_floor`` is then a power of two.
     """
+    if is_fp4(k_cache):
+        index, (_, blocks, block, _, _) = _check_store_fp4(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale)
+        N, num_heads, head_dim = key.shape
+        _launch(index, "slo_store_kvcache_fp4", key.data_ptr(), key.stride(0), value.data_ptr(), value.stride(0),
+                slot_mapping.data_ptr(), N, num_heads, head_dim, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+                v_scale.data_ptr(), blocks, block, scale_floor)
+        return
     device, code = check_store(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale)
     N, num_heads, head_dim = key.shape
-    if code == _lib.KV_FP4_E2M1:
-        _lib.check(_lib.load().slo_store_kvcache_fp4(
-            _ptr(key), key.stride(0), _ptr(value), value.stride(0), _ptr(slot_mapping), N, num_heads, head_dim,
-            _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), k_cache.shape[0], k_cache.shape[2],
-            float(scale_floor), _stream(device)), "slo_store_kvcache_fp4")
-        return
     num_slots = k_cache.shape[0] * k_cache.shape[1]
     lib = _lib.load()
     _lib.check(lib.slo_store_kvcache(
@@ -232,17 +263,15 @@ def load_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: tor
     come back as stored, 4-bit values exactly, E4M3FN values as code * scale
     rounded to bf16; a slot outside the pool gives zeros.
     """
-    device = _require_gpu(k_cache, v_cache, slot_mapping, k_scale, v_scale)
+    index = _one_device(k_cache, v_cache, slot_mapping, k_scale, v_scale)
     code, blocks, block, heads, head_dim = _pool_geometry(k_cache, k_scale, v_cache, v_scale)
-    _int32(slot_mapping, "slot_mapping")
-    if slot_mapping.dim() != 1:
-        raise ValueError("slot_mapping must be a 1-dimensional int32 tensor")
+    if slot_mapping.dtype != torch.int32 or slot_mapping.dim() != 1 or slot_mapping.stride(0) != 1:
+        raise ValueError("slot_mapping must be a contiguous 1-dimensional int32 tensor")
     N = slot_mapping.numel()
-    k = torch.empty((N, heads, head_dim), dtype=torch.bfloat16, device=device)
+    k = torch.empty((N, heads, head_dim), dtype=torch.bfloat16, device=k_cache.device)
     v = torch.empty_like(k)
-    _lib.check(_lib.load().slo_load_kvcache(
-        _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), code, blocks, block, _ptr(slot_mapping), N, heads,
-        head_dim, _ptr(k), _ptr(v), _stream(device)), "slo_load_kvcache")
+    _launch(index, "slo_load_kvcache", k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), code, blocks,
+            block, slot_mapping.data_ptr(), N, heads, head_dim, k.data_ptr(), v.data_ptr())
     return k, v
 
 
@@ -301,7 +330,7 @@ def qk_norm_rope_store(qkv: torch.Tensor, positions: torch.Tensor, q_norm_weight
         raise ValueError("KV pool views must be contiguous")
     fp4 = code == _lib.KV_FP4_E2M1
     if fp4:
-        if _pool_geometry(k_cache, k_scale, v_cache, v_scale, head_dim)[3] != num_kv_heads:
+        if _pool_geometry(k_cache, k_scale, v_cache, v_scale)[3:] != (num_kv_heads, head_dim):
             raise ValueError("KV pool must be [num_blocks, num_kv_heads, block_size, head_dim / 2]")
     elif k_cache.shape[-2:] != (num_kv_heads, head_dim) or v_cache.shape != k_cache.shape:
         raise ValueError("KV pool must be [num_blocks, block_size, num_kv_heads, head_dim]")
@@ -431,29 +460,21 @@ def reserve_workspace(device, max_decode_rows: int, max_decode_len: int, num_hea
 
 
 # ---------------------------------------------------------------- attention
-def _pool_args(args, k_cache, k_scale, v_cache, v_scale, num_kv_heads, head_dim, want_v=True):
-    code, blocks, block, heads, _ = _pool_geometry(k_cache, k_scale, v_cache, v_scale, head_dim, want_v)
-    if heads != num_kv_heads:
-        raise ValueError(f"KV pool holds {heads} kv heads, not {num_kv_heads}")
-    args.kv_dtype, args.num_blocks, args.block_size = code, blocks, block
-    args.k_cache, args.k_scale = _ptr(k_cache), _ptr(k_scale)
-    args.v_cache, args.v_scale = _ptr(v_cache), _ptr(v_scale)
-
-
-def _row_args(args, T, num_decode, decode_lens, decode_tables, num_prefill, cu_q, cu_k, max_q, max_k, tables, phases):
-    """Fills in the rows of the asked phases, all read through block tables."""
-    args.num_decode, args.phases = num_decode, phases
+def _row_args(T, num_decode, decode_lens, decode_tables, num_prefill, cu_q, cu_k, max_q, max_k, tables, phases):
+    """Checks the rows of the asked phases, all read through block tables, and returns their fields of
+    ``PagedAttentionArgs``: those of the decode rows, then those of the prefill rows."""
     if not 0 <= num_decode <= T:
         raise ValueError("num_decode must be from 0 to the number of query rows")
+    decode, prefill = (num_decode, None, None, 0, 0), (0, None, None, 0, 0, None, 0, 0)
     if num_decode and phases & _lib.PHASE_DECODE:
         _int32(decode_lens, "decode_lens")
         _int32(decode_tables, "decode_tables")
         if decode_tables.dim() != 2 or decode_tables.stride(1) != 1:
             raise ValueError("decode_tables must be a row-major [rows, width] int32 tensor")
-        if decode_lens.numel() < num_decode or decode_tables.shape[0] < num_decode:
+        rows, width = decode_tables.shape
+        if decode_lens.numel() < num_decode or rows < num_decode:
             raise ValueError("decode metadata has fewer rows than num_decode")
-        args.decode_lens, args.decode_tables = _ptr(decode_lens), _ptr(decode_tables)
-        args.decode_table_stride, args.decode_table_width = decode_tables.stride(0), decode_tables.shape[1]
+        decode = num_decode, decode_lens.data_ptr(), decode_tables.data_ptr(), decode_tables.stride(0), width
     if num_prefill and phases & _lib.PHASE_PREFILL:
         _int32(cu_q, "cu_seqlens_q")
         _int32(cu_k, "cu_seqlens_k")
@@ -462,22 +483,46 @@ def _row_args(args, T, num_decode, decode_lens, decode_tables, num_prefill, cu_q
             raise ValueError("cu_seqlens shorter than num_prefill + 1")
         if tables.dim() != 2 or tables.stride(1) != 1 or tables.shape[0] < num_prefill:
             raise ValueError("block_tables must be a row-major [rows, width] int32 tensor")
-        args.num_prefill, args.prefill_cu_q, args.prefill_cu_k = num_prefill, _ptr(cu_q), _ptr(cu_k)
-        args.max_q, args.max_k = int(max_q), int(max_k)
-        args.prefill_tables = _ptr(tables)
-        args.prefill_table_stride, args.prefill_table_width = tables.stride(0), tables.shape[1]
+        prefill = (num_prefill, cu_q.data_ptr(), cu_k.data_ptr(), int(max_q), int(max_k), tables.data_ptr(), tables.stride(0),
+                   tables.shape[1])
+    return decode, prefill
 
 
-def _own_workspace(args, size_of, what, device):
-    """A workspace of the call's own, from torch's allocator: calls on several streams, and graphs captured apart,
-    do not share it.  It need not be cleared.  Returned to keep it alive until the launch is enqueued."""
-    need = ctypes.c_size_t(0)
-    _lib.check(size_of(ctypes.byref(args), ctypes.byref(need)), what)
-    if need.value:
-        ws = torch.empty(need.value, dtype=torch.uint8, device=device)
-        args.workspace, args.workspace_bytes = ws.data_ptr(), need.value
-        return ws
-    return None
+_NO_ROWS, _NO_STORE = (None, 0, None, 0, 0), (None, None, 0, None, 0, 0, 0.0)
+
+
+def _pool_call(what, extra, index, device, q, out, k_cache, v_cache, k_scale, v_scale, geometry, rows, scale, phases):
+    """Calls ``what`` over a pool with a workspace of the call's own, from torch's allocator: calls on several streams,
+    and graphs captured apart, do not share one, and it need not be cleared."""
+    code, blocks, block, heads, head_dim = geometry
+    T, num_heads, _ = q.shape
+    decode, prefill = rows
+    fields = (q.data_ptr(), q.stride(0) if T > 1 else num_heads * head_dim, _ptr(out) or 0,
+              0 if out is None else out.stride(0) if T > 1 else num_heads * head_dim, T, k_cache.data_ptr(), _ptr(v_cache) or 0,
+              _ptr(k_scale) or 0, _ptr(v_scale) or 0, code, blocks, block, *(x or 0 for x in decode), *(x or 0 for x in prefill),
+              0, 0, 0, 0, 0, num_heads, heads, head_dim, scale)
+    args = _lib.pack_attention_args(*fields, 0, 0, phases, 0, 0, 0, 0, 0, 0, 0.0)
+    need = _workspace_need(args, what, T, num_heads, heads, code, block, phases, decode[0], decode[4], prefill[0], prefill[3],
+                           prefill[4], prefill[7])
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        args = _lib.pack_attention_args(*fields, ws.data_ptr(), need, phases, 0, 0, 0, 0, 0, 0, 0.0)
+    _launch(index, what, args, *extra)
+
+
+_sizes: dict[tuple, int] = {}  # workspace bytes by entry point and sizes
+
+
+def _workspace_need(args, *key) -> int:
+    what = key[0]
+    need = _sizes.get(key)
+    if need is None:
+        size = ctypes.c_size_t(0)
+        _lib.check(getattr(_lib.load(), what + "_workspace_bytes")(args, ctypes.byref(size)), what)
+        if len(_sizes) >= 4096:
+            _sizes.clear()
+        need = _sizes[key] = size.value
+    return need
 
 
 def accumulate_attention(q: torch.Tensor, k_cache: torch.Tensor, kv_scores: torch.Tensor, softmax_scale: float, *,
@@ -498,30 +543,32 @@ def accumulate_attention(q: torch.Tensor, k_cache: torch.Tensor, kv_scores: torc
     (``KVPool.reset_blocks``).  Rows of one call may share old pages: each adds
     its weights, in an order that is not fixed.  ``evict_kv`` reads the scores.
     """
-    if q.dim() != 3:
-        raise ValueError("q must be [tokens, num_heads, head_dim]")
-    T, num_heads, head_dim = q.shape
-    device = _require_gpu(q, k_cache, kv_scores, k_scale, decode_lens, decode_tables, prefill_cu_q, prefill_cu_k,
-                          prefill_tables)
-    if q.dtype != torch.bfloat16:
-        raise TypeError("q must be bf16")
-    if q.stride(-1) != 1 or q.stride(1) != head_dim:
-        raise ValueError("q rows must hold contiguous heads")
+    index, geometry = _check_query(q, num_kv_heads, k_cache, k_scale, None, None, False, kv_scores, decode_lens, decode_tables,
+                                   prefill_cu_q, prefill_cu_k, prefill_tables)
+    _check_scores(kv_scores, geometry[1], num_kv_heads, geometry[2])
     phases &= _lib.PHASE_ALL
     if num_prefill and phases & _lib.PHASE_PREFILL and prefill_tables is None:
         raise ValueError("accumulate_attention reads prefill rows through block tables")
-    args = _lib.PagedAttentionArgs()
-    args.q, args.q_row_stride, args.num_q_rows = _ptr(q), q.stride(0), T
-    _pool_args(args, k_cache, k_scale, None, None, num_kv_heads, head_dim, want_v=False)
-    _check_scores(kv_scores, args.num_blocks, num_kv_heads, args.block_size)
-    _row_args(args, T, num_decode, decode_lens, decode_tables, num_prefill, prefill_cu_q, prefill_cu_k, max_q, max_k,
-              prefill_tables, phases)
-    args.num_heads, args.num_kv_heads, args.head_dim = num_heads, num_kv_heads, head_dim
-    args.softmax_scale = float(softmax_scale)
-    ws = _own_workspace(args, _lib.load().slo_accumulate_attention_workspace_bytes, "slo_accumulate_attention", device)
-    _lib.check(_lib.load().slo_accumulate_attention(ctypes.byref(args), _ptr(kv_scores), _stream(device)),
-               "slo_accumulate_attention")
-    del ws
+    rows = _row_args(q.shape[0], num_decode, decode_lens, decode_tables, num_prefill, prefill_cu_q, prefill_cu_k, max_q, max_k,
+                     prefill_tables, phases)
+    _pool_call("slo_accumulate_attention", (kv_scores.data_ptr(),), index, q.device, q, None, k_cache, None, k_scale, None,
+               geometry, rows, float(softmax_scale), phases)
+
+
+def _check_query(q, num_kv_heads, k_cache, k_scale, v_cache, v_scale, want_v, *others):
+    """Checks q against a pool; returns ``(device index, the pool's geometry)``."""
+    if q.dim() != 3:
+        raise ValueError("q must be [tokens, num_heads, head_dim]")
+    index = _one_device(q, k_cache, k_scale, v_cache, v_scale, *others)
+    if q.dtype != torch.bfloat16:
+        raise TypeError("q must be bf16")
+    stride, head_dim = q.stride(), q.shape[2]
+    if stride[2] != 1 or stride[1] != head_dim:
+        raise ValueError("q rows must hold contiguous heads")
+    geometry = _pool_geometry(k_cache, k_scale, v_cache, v_scale, want_v)
+    if geometry[3] != num_kv_heads or geometry[4] != head_dim:
+        raise ValueError(f"KV pool holds {geometry[3]} kv heads of {geometry[4]}, not {num_kv_heads} of {head_dim}")
+    return index, geometry
 
 
 def evict_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, kv_scores: torch.Tensor, lens: torch.Tensor,
@@ -545,7 +592,7 @@ def evict_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, kv_scores: torch.Tens
     ``kept`` the kept positions, int32 ``[(layers,) rows, num_kv_heads, budget]``,
     -1 past a row that is shorter.
     """
-    device = _require_gpu(k_cache, v_cache, kv_scores, lens, tables, k_scale, v_scale)
+    index = _one_device(k_cache, v_cache, kv_scores, lens, tables, k_scale, v_scale)
     layered = k_cache.dim() == 5
     if layered and (v_cache.shape != k_cache.shape or kv_scores.shape[:1] != k_cache.shape[:1]
                     or any(s is not None and s.shape[:1] != k_cache.shape[:1] for s in (k_scale, v_scale))
@@ -562,13 +609,13 @@ def evict_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, kv_scores: torch.Tens
     rows, budget, recent = lens.numel(), int(budget), int(recent)
     if budget <= 0 or not 0 <= recent <= budget:
         raise ValueError("budget must be positive and recent from 0 to budget")
-    new_lens = torch.empty(rows, dtype=torch.int32, device=device)
-    kept = torch.empty((*((layers,) if layered else ()), rows, heads, budget), dtype=torch.int32, device=device)
+    new_lens = torch.empty(rows, dtype=torch.int32, device=lens.device)
+    kept = torch.empty((*((layers,) if layered else ()), rows, heads, budget), dtype=torch.int32, device=lens.device)
     args = _lib.EvictKvArgs(
         _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(kv_scores), code, layers, blocks, block, heads,
         head_dim, rows, _ptr(lens), _ptr(tables), tables.stride(0), tables.shape[1], budget, recent, _ptr(new_lens),
         _ptr(kept))
-    _lib.check(_lib.load().slo_evict_kv(ctypes.byref(args), _stream(device)), "slo_evict_kv")
+    _launch(index, "slo_evict_kv", ctypes.byref(args))
     return new_lens, kept
 
 
@@ -612,6 +659,10 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor | None, v_cache: torc
     uses the library's static per-GPU scratch instead of this module's
     workspace (pass ``out`` as well and nothing is allocated).
     """
+    if is_fp4(k_cache):
+        return _paged_attention_fp4(q, k_cache, v_cache, softmax_scale, num_kv_heads, k_scale, v_scale, num_decode, decode_lens,
+                                    decode_tables, num_prefill, prefill_cu_q, prefill_cu_k, max_q, max_k, prefill_tables, k, v,
+                                    phases, out, store_slot_mapping, new_k, new_v, noalloc, store_scale_floor)
     if q.dim() != 3:
         raise ValueError("q must be [tokens, num_heads, head_dim]")
     T, num_heads, head_dim = q.shape
@@ -629,31 +680,6 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor | None, v_cache: torc
     args.q, args.q_row_stride = q.data_ptr(), q.stride(0)
     args.out, args.out_row_stride = out.data_ptr(), out.stride(0)
     args.num_q_rows = T
-    if is_fp4(k_cache):
-        if out.dtype != torch.bfloat16:
-            raise TypeError("out must be bf16")
-        if noalloc:
-            raise ValueError("noalloc launches take bf16 and E4M3FN pools")
-        if store_slot_mapping is not None:
-            store_kvcache(new_k, new_v, k_cache, v_cache, store_slot_mapping, k_scale, v_scale, store_scale_floor)
-        phases &= _lib.PHASE_ALL
-        if num_prefill and prefill_tables is None and phases & _lib.PHASE_PREFILL:
-            paged_attention(q, None, None, softmax_scale, num_kv_heads=num_kv_heads, num_decode=num_decode,
-                            decode_lens=decode_lens, decode_tables=decode_tables, num_prefill=num_prefill,
-                            prefill_cu_q=prefill_cu_q, prefill_cu_k=prefill_cu_k, max_q=max_q, max_k=max_k, k=k, v=v,
-                            phases=_lib.PHASE_PREFILL, out=out)
-            phases &= ~_lib.PHASE_PREFILL
-        if not phases:
-            return out
-        _pool_args(args, k_cache, k_scale, v_cache, v_scale, num_kv_heads, head_dim)
-        _row_args(args, T, num_decode, decode_lens, decode_tables, num_prefill, prefill_cu_q, prefill_cu_k, max_q, max_k,
-                  prefill_tables, phases)
-        args.num_heads, args.num_kv_heads, args.head_dim = num_heads, num_kv_heads, head_dim
-        args.softmax_scale = float(softmax_scale)
-        ws = _own_workspace(args, _lib.load().slo_paged_attention_fp4_workspace_bytes, "slo_paged_attention_fp4", device)
-        _lib.check(_lib.load().slo_paged_attention_fp4(ctypes.byref(args), _stream(device)), "slo_paged_attention_fp4")
-        del ws
-        return out
     code = _lib.KV_BF16
     if k_cache is not None and k_cache.numel():
         code = kv_dtype_code(k_cache)
@@ -733,4 +759,32 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor | None, v_cache: torc
     args.workspace, args.workspace_bytes = ws.data_ptr(), ws.numel()
     _lib.check(_lib.load().slo_paged_attention(ctypes.byref(args), _stream(device)),
                "slo_paged_attention")
+    return out
+
+
+def _paged_attention_fp4(q, k_cache, v_cache, softmax_scale, num_kv_heads, k_scale, v_scale, num_decode, decode_lens,
+                         decode_tables, num_prefill, cu_q, cu_k, max_q, max_k, tables, k, v, phases, out, slot_mapping, new_k,
+                         new_v, noalloc, scale_floor):
+    """``paged_attention`` over a 4-bit pool."""
+    index, geometry = _check_query(q, num_kv_heads, k_cache, k_scale, v_cache, v_scale, True, decode_lens, decode_tables, cu_q,
+                                   cu_k, tables, k, v, out)
+    if noalloc:
+        raise ValueError("noalloc launches take bf16 and E4M3FN pools")
+    if out is None:
+        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+    elif out.dtype != torch.bfloat16:
+        raise TypeError("out must be bf16")
+    elif out.shape != q.shape or out.stride(2) != 1 or out.stride(1) != q.shape[2]:
+        raise ValueError("out must be [tokens, num_heads, head_dim] with contiguous heads")
+    if slot_mapping is not None:
+        store_kvcache(new_k, new_v, k_cache, v_cache, slot_mapping, k_scale, v_scale, scale_floor)
+    phases &= _lib.PHASE_ALL
+    if num_prefill and tables is None and phases & _lib.PHASE_PREFILL:
+        paged_attention(q, None, None, softmax_scale, num_kv_heads=num_kv_heads, num_decode=num_decode, decode_lens=decode_lens,
+                        decode_tables=decode_tables, num_prefill=num_prefill, prefill_cu_q=cu_q, prefill_cu_k=cu_k, max_q=max_q,
+                        max_k=max_k, k=k, v=v, phases=_lib.PHASE_PREFILL, out=out)
+        phases &= ~_lib.PHASE_PREFILL
+    rows = _row_args(q.shape[0], num_decode, decode_lens, decode_tables, num_prefill, cu_q, cu_k, max_q, max_k, tables, phases)
+    _pool_call("slo_paged_attention_fp4", (), index, q.device, q, out, k_cache, v_cache, k_scale, v_scale, geometry, rows,
+               float(softmax_scale), phases)
     return out

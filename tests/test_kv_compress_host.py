@@ -120,10 +120,10 @@ def attention_args(**over):
 def test_attention_refusals_without_a_gpu(over, code, word):
     lib = _lib.load()
     need = ctypes.c_size_t(0)
-    for call in (lambda a: lib.slo_paged_attention_fp4(ctypes.byref(a), None),
-                 lambda a: lib.slo_paged_attention_fp4_workspace_bytes(ctypes.byref(a), ctypes.byref(need)),
-                 lambda a: lib.slo_accumulate_attention(ctypes.byref(a), 4096, None),
-                 lambda a: lib.slo_accumulate_attention_workspace_bytes(ctypes.byref(a), ctypes.byref(need))):
+    for call in (lambda a: lib.slo_paged_attention_fp4(bytes(a), None),
+                 lambda a: lib.slo_paged_attention_fp4_workspace_bytes(bytes(a), ctypes.byref(need)),
+                 lambda a: lib.slo_accumulate_attention(bytes(a), 4096, None),
+                 lambda a: lib.slo_accumulate_attention_workspace_bytes(bytes(a), ctypes.byref(need))):
         assert call(attention_args(**over)) == code
         assert word in lib.slo_last_error().decode()
 
@@ -132,20 +132,20 @@ def test_workspace_refusals_without_a_gpu():
     lib = _lib.load()
     need = ctypes.c_size_t(0)
     a = attention_args()
-    assert lib.slo_accumulate_attention_workspace_bytes(ctypes.byref(a), ctypes.byref(need)) == 0 and need.value > 0
+    assert lib.slo_accumulate_attention_workspace_bytes(bytes(a), ctypes.byref(need)) == 0 and need.value > 0
     a.workspace, a.workspace_bytes = 4096, need.value - 1
-    assert lib.slo_accumulate_attention(ctypes.byref(a), 4096, None) == 3
+    assert lib.slo_accumulate_attention(bytes(a), 4096, None) == 3
     a.workspace, a.workspace_bytes = None, need.value
-    assert lib.slo_accumulate_attention(ctypes.byref(a), 4096, None) == 3
-    assert lib.slo_accumulate_attention(ctypes.byref(attention_args(kv_dtype=3)), 4096, None) == 1
-    assert lib.slo_paged_attention_fp4(ctypes.byref(attention_args(kv_dtype=1)), None) == 1
-    assert lib.slo_paged_attention_fp4(ctypes.byref(attention_args(store_slot_mapping=4096)), None) == 1
+    assert lib.slo_accumulate_attention(bytes(a), 4096, None) == 3
+    assert lib.slo_accumulate_attention(bytes(attention_args(kv_dtype=3)), 4096, None) == 1
+    assert lib.slo_paged_attention_fp4(bytes(attention_args(kv_dtype=1)), None) == 1
+    assert lib.slo_paged_attention_fp4(bytes(attention_args(store_slot_mapping=4096)), None) == 1
     a = attention_args(decode_table_width=4096, num_decode=1)  # one long row: split, so it needs a workspace
-    assert lib.slo_paged_attention_fp4_workspace_bytes(ctypes.byref(a), ctypes.byref(need)) == 0 and need.value > 0
-    assert lib.slo_paged_attention_fp4(ctypes.byref(a), None) == 3
+    assert lib.slo_paged_attention_fp4_workspace_bytes(bytes(a), ctypes.byref(need)) == 0 and need.value > 0
+    assert lib.slo_paged_attention_fp4(bytes(a), None) == 3
     # nothing to do
-    assert lib.slo_paged_attention_fp4(ctypes.byref(attention_args(num_decode=0)), None) == 0
-    assert lib.slo_accumulate_attention(ctypes.byref(attention_args(num_decode=0)), 4096, None) == 0
+    assert lib.slo_paged_attention_fp4(bytes(attention_args(num_decode=0)), None) == 0
+    assert lib.slo_accumulate_attention(bytes(attention_args(num_decode=0)), 4096, None) == 0
     assert lib.slo_paged_attention_fp4(None, None) == 1 and lib.slo_accumulate_attention(None, None, None) == 1
 
 
@@ -181,6 +181,18 @@ def test_evict_refusals_without_a_gpu():
         assert call(**over) == 1, over
     for over in (dict(head_dim=96), dict(num_rows=65536), dict(table_width=1 << 20)):
         assert call(**over) == 4, over
+
+
+def test_packed_arguments_are_the_struct():
+    values = {t: i for i, t in enumerate(_lib.PagedAttentionArgs._fields_, 1)}
+    a = _lib.PagedAttentionArgs()
+    for (name, _), i in values.items():
+        setattr(a, name, i)
+    packed = _lib.pack_attention_args(*range(1, len(values) + 1))
+    assert len(packed) == ctypes.sizeof(a)
+    back = _lib.PagedAttentionArgs.from_buffer_copy(packed)
+    for name, _ in _lib.PagedAttentionArgs._fields_:
+        assert getattr(back, name) == getattr(a, name), name
 
 
 def test_host_layer_refuses_cpu_tensors():

@@ -9,10 +9,11 @@
 // head) pairs), so a lane has 4 tokens of one column.  A weight needs its row's
 // maximum and sum first, so each phase takes two passes:
 //
-//  * decode rows (one query): the first pass writes the logits (fp32) and each
-//    chunk's maximum and sum, the second turns them into weights.  The logits
-//    are 4 bytes per (head, token), a sixteenth to a quarter of K itself, so K
-//    is read once.
+//  * decode rows (one query): the first pass keeps the logits (fp32), the second
+//    turns them into weights, so K is read once.  A row's logits stay in LDS if
+//    they fit; those of longer rows go through memory (4 bytes per (head,
+//    token), a sixteenth to a quarter of K itself), with each chunk's maximum
+//    and sum.
 //  * prefill rows: the first pass finds every (query, head)'s log2-sum; the
 //    second computes S^T again, 64 keys of a workgroup against all queries,
 //    and sums the weights over the queries in registers (writing the scores of
@@ -23,14 +24,11 @@
 // count; only for such a page does the order of its rows' additions vary.
 #include "capi_internal.h"
 #include "fp4.h"
+#include "tile_io.h"
 
 namespace slo {
 namespace {
 
-#ifndef LW
-#define LW 3
-#define LN 2
-#endif
 constexpr int HDS = 128;
 constexpr float kNone = -1e30f;
 
@@ -48,8 +46,7 @@ struct ScoreParams {
   int table_stride, table_width;
   int first_row;
   int hq, hkv, group;
-  float scale_log2;
-  uint32_t q_sign;
+  float scale_log2;  // softmax scale * log2(e)
   float* scores;   // [num_blocks, hkv, block_size]
   float* logits;   // decode: [rows, hq, capacity], log2 units
   float2* partial;  // decode: [rows, hq, splits] (maximum, sum)
@@ -92,8 +89,6 @@ template <int KV>
 __device__ __forceinline__ bf16x8 load_q(const ScoreParams& p, int64_t row, int h, int i, int kg, bool live) {
   u32x4 x = {0, 0, 0, 0};
   if (live) x = *reinterpret_cast<const u32x4*>(p.q + row * p.q_stride + h * HDS + channel_of<KV>(i, kg));
-#pragma unroll
-  for (int j = 0; j < 4; ++j) x[j] ^= p.q_sign;
   return as_bf16x8(x);
 }
 
@@ -153,58 +148,61 @@ __device__ __forceinline__ void absorb(float& m, float& l, float m2, float l2) {
   m = top;
 }
 
-// Decode rows, first pass: one chunk of one (row, kv head) per workgroup, its
-// four wavefronts every fourth 16-token tile.
-template <int KV>
-__global__ void __launch_bounds__(256)
-score_logits_kernel(ScoreParams p) {
-  __shared__ float sm[4][64], sl[4][64];
-  const int head = blockIdx.x, split = blockIdx.y, r = blockIdx.z;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+// Logits (log2 units) of tokens begin, begin + stride, ... < end of a decode
+// row, 16 T at a time, the next ones' loads ahead of the products; `put` takes
+// four tokens' logits of this lane's column.  Returns the lane's maximum and sum.
+template <int KV, typename Put>
+__device__ __forceinline__ float2 decode_logits(const ScoreParams& p, const Row& g, int r, int head, int begin, int end,
+                                                int stride, int lane, Put put) {
+  constexpr int T = KV == KV_FP4_E2M1 ? 4 : 2;
   const int col = lane & 15, kg = lane >> 4;
-  const Row g = row_of(p, r);
-  const int k0 = split * p.chunk, k1 = min(k0 + p.chunk, g.lk);
-  if (k0 >= g.lk) return;
+  float m = kNone, l = 0.0f;
+  if (begin >= end) return float2{m, l};
+  Keys<KV> k[T];
+  auto load = [&](Keys<KV>(&to)[T], int at) {
+    int off;
+    const int block = page_of(p, r, at, off);
+#pragma unroll
+    for (int t = 0; t < T; ++t) to[t].load(p, block < 0 ? 0 : block, (block < 0 ? 0 : off) + 16 * t, head, lane);
+    return block >= 0;
+  };
+  bool ok = load(k, begin);
   bf16x8 q[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) q[i] = load_q<KV>(p, g.q0, head * p.group + col, i, kg, col < p.group);
-  float* logits = p.logits + ((int64_t)r * p.hq + head * p.group + col) * p.capacity;
-  float m = kNone, l = 0.0f;
-  for (int at = k0 + 16 * wave; at < k1; at += 64) {
-    int off;
-    const int block = page_of(p, r, at, off);
-    f32x4 s = {0, 0, 0, 0};
-    if (block >= 0) {
-      Keys<KV> k;
-      k.load(p, block, off, head, lane);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s = mfma16(k.operand(i), q[i], s);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[i] *= k.factor(i) * p.scale_log2;
-    }
+  for (int at = begin; at < end; at += stride) {
+    Keys<KV> n[T];
+    bool next_ok = false;
+    if (at + stride < end) next_ok = load(n, at + stride);
+    f32x4 s[T];
     float top = kNone;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (block < 0 || at + 4 * kg + i >= g.lk) s[i] = -INFINITY;
-      top = fmaxf(top, s[i]);
-    }
-    if (col < p.group) *reinterpret_cast<f32x4*>(logits + at + 4 * kg) = s;
-    float sum = 0.0f;
-    const float n = fmaxf(m, top);
+    for (int t = 0; t < T; ++t) {
+      s[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum += __builtin_amdgcn_exp2f(s[i] - n);
-    l = l * __builtin_amdgcn_exp2f(m - n) + sum;
-    m = n;
+      for (int i = 0; i < 4; ++i) s[t] = mfma16(k[t].operand(i), q[i], s[t]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[t][i] *= k[t].factor(i) * p.scale_log2;
+        if (!ok || at + 16 * t + 4 * kg + i >= g.lk) s[t][i] = -INFINITY;
+        top = fmaxf(top, s[t][i]);
+      }
+      put(at + 16 * t + 4 * kg, s[t]);
+    }
+    if (__any(top > m + 8.0f)) {  // sums of weights up to 256 round like those below 1
+      const float to = fmaxf(m, top);
+      l *= __builtin_amdgcn_exp2f(m - to);
+      m = to;
+    }
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) l += __builtin_amdgcn_exp2f(s[t][i] - m);
+#pragma unroll
+    for (int t = 0; t < T; ++t) k[t] = n[t];
+    ok = next_ok;
   }
-  sm[wave][lane] = m;
-  sl[wave][lane] = l;
-  __syncthreads();
-  if (threadIdx.x < p.group) {
-    m = kNone, l = 0.0f;
-    for (int w = 0; w < 4; ++w)
-      for (int k = 0; k < 4; ++k) absorb(m, l, sm[w][16 * k + threadIdx.x], sl[w][16 * k + threadIdx.x]);
-    p.partial[((int64_t)r * p.hq + head * p.group + threadIdx.x) * p.splits + split] = float2{m, l};
-  }
+  return float2{m, l};
 }
 
 __device__ __forceinline__ void add_score(const ScoreParams& p, const Row& g, int block, int off, int head, int token, float w) {
@@ -215,30 +213,117 @@ __device__ __forceinline__ void add_score(const ScoreParams& p, const Row& g, in
     unsafeAtomicAdd(s, w);
 }
 
-// Decode rows, second pass: one lane per token.
+// (maximum, sum) of a column over its four lanes, in each of them.
+__device__ __forceinline__ float2 column_lse(float2 e) {
+  const float m = col_max(e.x);
+  return float2{m, col_sum(e.y * __builtin_amdgcn_exp2f(e.x - m))};
+}
+
+// Decode rows whose logits fit LDS: a workgroup takes a (row, kv head) whole,
+// so one launch does, and K is all that moves.
+constexpr int kRowLogits = 16384;
+
+template <int KV, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, 4)
+score_row_kernel(ScoreParams p) {
+  __shared__ float logits[kRowLogits];  // [group, capacity]
+  __shared__ float sm[WAVES][16], sl[WAVES][16], lse[16];
+  const int head = blockIdx.x, r = blockIdx.y;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15;
+  const Row g = row_of(p, r);
+  constexpr int SPAN = KV == KV_FP4_E2M1 ? 64 : 32;
+  float* mine = logits + col * p.capacity;
+  const float2 e = column_lse(decode_logits<KV>(p, g, r, head, wave * SPAN, g.lk, WAVES * SPAN, lane, [&](int at, const f32x4& s) {
+    if (col < p.group && at < p.capacity) *reinterpret_cast<f32x4*>(mine + at) = s;
+  }));
+  if (lane < 16) {
+    sm[wave][lane] = e.x;
+    sl[wave][lane] = e.y;
+  }
+  __syncthreads();
+  if (wave == 0) {  // lane: column, and a quarter of the wavefronts
+    float2 f = {kNone, 0.0f};
+#pragma unroll
+    for (int w = 0; w < WAVES; w += 4) absorb(f.x, f.y, sm[w + (lane >> 4)][col], sl[w + (lane >> 4)][col]);
+    f = column_lse(f);
+    if (lane < 16) lse[lane] = f.x + __builtin_amdgcn_logf(f.y);
+  }
+  __syncthreads();
+  for (int token = threadIdx.x; token < g.lk; token += 64 * WAVES) {
+    int off;
+    const int block = page_of(p, r, token, off);
+    if (block < 0) continue;
+    float w = 0.0f;
+    for (int h = 0; h < p.group; ++h) w += __builtin_amdgcn_exp2f(logits[h * p.capacity + token] - lse[h]);
+    add_score(p, g, block, off, head, token, w);
+  }
+}
+
+// Longer rows, first pass: one chunk of one (row, kv head) per workgroup, its
+// four wavefronts every fourth step.
+template <int KV>
+__global__ void __launch_bounds__(256, 4)
+score_logits_kernel(ScoreParams p) {
+  __shared__ float sm[4][16], sl[4][16];
+  const int head = blockIdx.x, split = blockIdx.y, r = blockIdx.z;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15;
+  const Row g = row_of(p, r);
+  const int k0 = split * p.chunk, k1 = min(k0 + p.chunk, g.lk);
+  if (k0 >= g.lk) return;
+  constexpr int SPAN = KV == KV_FP4_E2M1 ? 64 : 32;
+  float* logits = p.logits + ((int64_t)r * p.hq + head * p.group + col) * p.capacity;
+  const float2 e = column_lse(decode_logits<KV>(p, g, r, head, k0 + wave * SPAN, k1, 4 * SPAN, lane, [&](int at, const f32x4& s) {
+    if (col < p.group) *reinterpret_cast<f32x4*>(logits + at) = s;
+  }));
+  if (lane < 16) {
+    sm[wave][lane] = e.x;
+    sl[wave][lane] = e.y;
+  }
+  __syncthreads();
+  if (threadIdx.x < p.group) {
+    float m = kNone, l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) absorb(m, l, sm[w][threadIdx.x], sl[w][threadIdx.x]);
+    p.partial[((int64_t)r * p.hq + head * p.group + threadIdx.x) * p.splits + split] = float2{m, l};
+  }
+}
+
+// Second pass: four tokens a lane.
 __global__ void __launch_bounds__(256)
 score_decode_kernel(ScoreParams p) {
   __shared__ float lse[16];
   const int head = blockIdx.x, r = blockIdx.z;
   const Row g = row_of(p, r);
-  const int token = blockIdx.y * 256 + threadIdx.x;
-  if ((int)blockIdx.y * 256 >= g.lk) return;
-  if (threadIdx.x < p.group) {
-    const int n = (g.lk + p.chunk - 1) / p.chunk;
-    const float2* e = p.partial + ((int64_t)r * p.hq + head * p.group + threadIdx.x) * p.splits;
+  if ((int)blockIdx.y * 1024 >= g.lk) return;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int n = (g.lk + p.chunk - 1) / p.chunk;
+  for (int h = wave; h < p.group; h += 4) {
+    const float2* e = p.partial + ((int64_t)r * p.hq + head * p.group + h) * p.splits;
     float m = kNone, l = 0.0f;
-    for (int s = 0; s < n; ++s) absorb(m, l, e[s].x, e[s].y);
-    lse[threadIdx.x] = m + __builtin_amdgcn_logf(l);
+    for (int s = lane; s < n; s += 64) absorb(m, l, e[s].x, e[s].y);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const float m2 = __shfl_xor(m, d, 64), l2 = __shfl_xor(l, d, 64);
+      absorb(m, l, m2, l2);
+    }
+    if (lane == 0) lse[h] = m + __builtin_amdgcn_logf(l);
   }
   __syncthreads();
+  const int token = blockIdx.y * 1024 + threadIdx.x * 4;
   if (token >= g.lk) return;
   int off;
   const int block = page_of(p, r, token, off);
   if (block < 0) return;
   const float* x = p.logits + ((int64_t)r * p.hq + head * p.group) * p.capacity + token;
-  float w = 0.0f;
-  for (int h = 0; h < p.group; ++h) w += __builtin_amdgcn_exp2f(x[(int64_t)h * p.capacity] - lse[h]);
-  add_score(p, g, block, off, head, token, w);
+  f32x4 w = {0, 0, 0, 0};
+  for (int h = 0; h < p.group; ++h) {
+    const f32x4 y = *reinterpret_cast<const f32x4*>(x + (int64_t)h * p.capacity);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] += __builtin_amdgcn_exp2f(y[i] - lse[h]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (token + i < g.lk) add_score(p, g, block, off + i, head, token + i, w[i]);
 }
 
 // Prefill rows, first pass: 16 NT (query, head) columns of one row per
@@ -248,7 +333,7 @@ score_decode_kernel(ScoreParams p) {
 // only where that passes it by 2^8 (sums of weights up to 256 round like those
 // below 1); the lanes meet at the end.
 template <int KV, int NT>
-__global__ void __launch_bounds__(256, LW)
+__global__ void __launch_bounds__(256, 2)
 score_lse_kernel(ScoreParams p, int tiles) {
   __shared__ float sm[NT][4][64], sl[NT][4][64];
   const int head = blockIdx.x, r = blockIdx.z;
@@ -304,28 +389,26 @@ score_lse_kernel(ScoreParams p, int tiles) {
         s[0] = mfma16(a[0][i], q[n][i], s[0]);
         s[1] = mfma16(a[1][i], q[n][i], s[1]);
       }
+      float e[8];
+      auto weights = [&] {
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+        for (int j = 0; j < 8; ++j) {
+          e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j >> 2][j & 3], f[j >> 2][j & 3], -m[n]));
+          if (at + 32 > full && at + 16 * (j >> 2) + 4 * kg + (j & 3) >= limit[n]) e[j] = 0.0f;
+        }
+        return fmaxf(fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])), fmaxf(fmaxf(e[4], e[5]), fmaxf(e[6], e[7])));
+      };
+      // The weights themselves tell whether the reference has to move.
+      if (__any(weights() > 256.0f)) {
+        float top = m[n];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[h][i] *= f[h][i];
-      if (at + 32 > full) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (at + 16 * h + 4 * kg + i >= limit[n]) s[h][i] = -INFINITY;
+        for (int j = 0; j < 8; ++j)
+          if (at + 16 * (j >> 2) + 4 * kg + (j & 3) < limit[n]) top = fmaxf(top, s[j >> 2][j & 3] * f[j >> 2][j & 3]);
+        l[n] *= __builtin_amdgcn_exp2f(m[n] - top);
+        m[n] = top;
+        weights();
       }
-      const float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                              fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-      if (__any(top > m[n] + 8.0f)) {
-        const float to = fmaxf(m[n], top);
-        l[n] *= __builtin_amdgcn_exp2f(m[n] - to);
-        m[n] = to;
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) l[n] += __builtin_amdgcn_exp2f(s[h][i] - m[n]);
+      l[n] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
     }
   }
 #pragma unroll
@@ -348,11 +431,19 @@ score_lse_kernel(ScoreParams p, int tiles) {
 // sixth 16 of the columns that see one of them.  A lane sums its 16
 // tokens' weights over its columns; lanes, then wavefronts, are added in order
 // at the end.
-constexpr int kSumWaves = 6, kSumKeys = 64;
+constexpr int kSumWaves = 6, kSumKeys = 64, kSumDepth = 3;
+
+// 16 columns as their lanes take them: four operands of q, and the log2-sums.
+// They arrive by LDS DMA, kSumDepth in flight.
+struct Columns {
+  u32x4 q[4][64];
+  float lse[64];
+};
 
 template <int KV>
 __global__ void __launch_bounds__(64 * kSumWaves, 3)
 score_prefill_kernel(ScoreParams p) {
+  __shared__ Columns ring[kSumWaves][kSumDepth];
   __shared__ float sums[kSumWaves][kSumKeys];
   __shared__ f32x4 factors[KV == KV_FP8_E4M3FN ? kSumKeys / 4 : 1];  // E4M3FN scales, in LDS to save registers
   const int head = blockIdx.x, r = blockIdx.z;
@@ -364,6 +455,34 @@ score_prefill_kernel(ScoreParams p) {
   int off;
   const int block = page_of(p, r, at, off);
   if (block < 0) return;
+  // This wavefront's columns first + stride i; the next ones' query and head by
+  // addition.  A column past the last is read as the last and weighs nothing.
+  const int columns = g.lq * p.group, stride = 16 * kSumWaves;
+  const int first = max(at - g.prefix, 0) * p.group + 16 * wave;
+  const int count = first < columns ? (columns - first + stride - 1) / stride : 0;
+  const int dt = stride / p.group, dh = stride - dt * p.group;
+  int tok = (first + col) / p.group, hh = first + col - tok * p.group;  // of the columns that are fetched next
+  const uint32_t lds = lds_addr(&ring[wave][0]);
+  int to = 0;
+  auto fetch = [&] {
+    const bool live = tok < g.lq;
+    const int64_t row = g.q0 + (live ? tok : g.lq - 1);
+    const int h = head * p.group + (live ? hh : p.group - 1);
+    const uint16_t* q = p.q + row * p.q_stride + h * HDS;
+    const uint32_t base = lds + to * (uint32_t)sizeof(Columns);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dma16(q + channel_of<KV>(i, kg), base + 1024 * i);
+    dma4(p.lse + (row - p.first_row) * p.hq + h, base + 4096);
+    to = to == kSumDepth - 1 ? 0 : to + 1;
+    tok += dt;
+    hh += dh;
+    if (hh >= p.group) {
+      hh -= p.group;
+      ++tok;
+    }
+  };
+  int now_tok = tok, now_hh = hh, sent = 0;
+  for (; sent < kSumDepth - 1 && sent < count; ++sent) fetch();
   bf16x8 a[4][4];
 #pragma unroll
   for (int h = 0; h < 4; ++h) {
@@ -379,39 +498,39 @@ score_prefill_kernel(ScoreParams p) {
     __syncthreads();
   }
   float w[4][4] = {};
-  const int columns = g.lq * p.group, stride = 16 * kSumWaves;
-  // This lane's column, query and head; the next ones by addition.
-  int x = max(at - g.prefix, 0) * p.group + 16 * wave + col;
-  int tok = x / p.group, hh = x - tok * p.group;
-  const int dt = stride / p.group, dh = stride - dt * p.group;
-  bf16x8 q[4];
-  float lse;
-  auto load = [&] {
-    const bool live = x < columns;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) q[i] = load_q<KV>(p, g.q0 + tok, head * p.group + hh, i, kg, live);
-    // A column past the last weighs nothing.
-    lse = live ? p.lse[(g.q0 - p.first_row + tok) * p.hq + head * p.group + hh] : INFINITY;
-  };
-  if (x - col < columns) load();
-  while (x - col < columns) {
-    asm volatile("" ::: "memory");  // the factors are read again, not held
+  int from = 0;
+  for (int c = 0; c < count; ++c) {
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the place that the next fetch fills has been read
+    if (sent < count) {
+      fetch();
+      ++sent;
+    }
+    const int ahead = sent - 1 - c;
+    asm volatile("" ::: "memory");
+    if (ahead >= 2)
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm(10));
+    else if (ahead == 1)
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm(5));
+    else
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+    asm volatile("" ::: "memory");
+    const Columns& x = ring[wave][from];
+    from = from == kSumDepth - 1 ? 0 : from + 1;
     f32x4 s[4] = {};
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i) {
+      const bf16x8 q = as_bf16x8(x.q[i][lane]);
 #pragma unroll
-      for (int h = 0; h < 4; ++h) s[h] = mfma16(a[h][i], q[i], s[h]);
-    const float ref = lse;
-    const int limit = min(g.prefix + tok + 1, g.lk);
-    // The next columns load while this one's weights are taken.
-    x += stride;
-    tok += dt;
-    hh += dh;
-    if (hh >= p.group) {
-      hh -= p.group;
-      ++tok;
+      for (int h = 0; h < 4; ++h) s[h] = mfma16(a[h][i], q, s[h]);
     }
-    if (x - col < columns) load();
+    const float ref = x.lse[lane];
+    const int limit = now_tok < g.lq ? min(g.prefix + now_tok + 1, g.lk) : 0;
+    now_tok += dt;
+    now_hh += dh;
+    if (now_hh >= p.group) {
+      now_hh -= p.group;
+      ++now_tok;
+    }
     auto add = [&](bool masked) {
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
@@ -447,9 +566,10 @@ score_prefill_kernel(ScoreParams p) {
   }
 }
 
-constexpr int kLseNT = LN;
+constexpr int kLseNT = 4;
 
 struct Plan {
+  bool whole;  // decode rows in one launch
   int splits, chunk, tiles;
   size_t logits, partial, lse;
 };
@@ -457,16 +577,17 @@ struct Plan {
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 Plan plan_of(const slo_paged_attention_args* a) {
-  Plan n = {1, 1 << 30, 0, 0, 0, 0};
+  Plan n = {false, 1, 1 << 30, 0, 0, 0, 0};
   if (a->num_decode > 0 && (a->phases & SLO_PHASE_DECODE)) {
     const int64_t cap = (int64_t)a->decode_table_width * a->block_size, groups = (int64_t)a->num_decode * a->num_kv_heads;
+    n.whole = cap * (a->num_heads / a->num_kv_heads) <= kRowLogits;
     const int64_t want = (2048 + groups - 1) / groups;
     int64_t c = ((cap + want - 1) / want + 127) / 128 * 128;
     if (c < 256) c = 256;
     n.chunk = (int)c;
     n.splits = (int)((cap + c - 1) / c);
-    n.logits = up256((size_t)a->num_decode * a->num_heads * cap * 4);
-    n.partial = up256((size_t)a->num_decode * a->num_heads * n.splits * 8);
+    if (!n.whole) n.logits = up256((size_t)a->num_decode * a->num_heads * cap * 4);
+    if (!n.whole) n.partial = up256((size_t)a->num_decode * a->num_heads * n.splits * 8);
   }
   if (a->num_prefill > 0 && (a->phases & SLO_PHASE_PREFILL) && a->max_q > 0) {
     const int per = 16 * kLseNT / (a->num_heads / a->num_kv_heads);
@@ -514,9 +635,15 @@ int check_args(const slo_paged_attention_args* a) {
 
 template <int KV>
 void launch(const ScoreParams& d, const ScoreParams& f, const slo_paged_attention_args* a, const Plan& n, hipStream_t s) {
+  // Two workgroups fit a CU (64 KiB of logits): where there are few rows, each
+  // gets sixteen wavefronts instead of eight.
+  if (n.whole && a->num_decode * d.hkv <= 256)
+    hipLaunchKernelGGL((score_row_kernel<KV, 16>), dim3(d.hkv, a->num_decode), dim3(1024), 0, s, d);
+  else if (n.whole)
+    hipLaunchKernelGGL((score_row_kernel<KV, 8>), dim3(d.hkv, a->num_decode), dim3(512), 0, s, d);
   if (n.logits) {
     hipLaunchKernelGGL(score_logits_kernel<KV>, dim3(d.hkv, d.splits, a->num_decode), dim3(256), 0, s, d);
-    hipLaunchKernelGGL(score_decode_kernel, dim3(d.hkv, (d.capacity + 255) / 256, a->num_decode), dim3(256), 0, s, d);
+    hipLaunchKernelGGL(score_decode_kernel, dim3(d.hkv, (d.capacity + 1023) / 1024, a->num_decode), dim3(256), 0, s, d);
   }
   if (n.tiles) {
     hipLaunchKernelGGL((score_lse_kernel<KV, kLseNT>), dim3(f.hkv, n.tiles, a->num_prefill), dim3(256), 0, s, f, n.tiles);
@@ -546,9 +673,9 @@ extern "C" int slo_accumulate_attention(const slo_paged_attention_args* a, float
   if (rc) return rc;
   const Plan n = plan_of(a);
   const size_t need = n.logits + n.partial + n.lse;
-  if (!need) return SLO_OK;
+  if (!need && !n.whole) return SLO_OK;
   if (!scores) return fail(SLO_ERR_INVALID, "accumulate_attention: null pointer");
-  if (!a->workspace || a->workspace_bytes < need || reinterpret_cast<uintptr_t>(a->workspace) % 16)
+  if (need && (!a->workspace || a->workspace_bytes < need || reinterpret_cast<uintptr_t>(a->workspace) % 16))
     return fail(SLO_ERR_WORKSPACE, "accumulate_attention: workspace smaller than slo_accumulate_attention_workspace_bytes");
   ScoreParams p = {};
   p.q = static_cast<const uint16_t*>(a->q);
@@ -561,8 +688,7 @@ extern "C" int slo_accumulate_attention(const slo_paged_attention_args* a, float
   p.hq = a->num_heads;
   p.hkv = a->num_kv_heads;
   p.group = a->num_heads / a->num_kv_heads;
-  p.scale_log2 = (a->softmax_scale < 0 ? -a->softmax_scale : a->softmax_scale) * kLog2e;
-  p.q_sign = a->softmax_scale < 0 ? 0x80008000u : 0u;
+  p.scale_log2 = a->softmax_scale * kLog2e;
   p.scores = scores;
   char* ws = static_cast<char*>(a->workspace);
   ScoreParams d = p, f = p;

@@ -98,6 +98,8 @@ CASES = {
     "long_prefix": dict(lens=[], chunks=[(3, 2600)], hq=8, hkv=2),
     "mixed": dict(lens=[5, 700, 64], chunks=[(100, 0), (50, 333)], block=256),
     "negative_scale": dict(lens=[80], chunks=[(30, 20)], hq=8, hkv=2, scale=-0.11),
+    "rows_past_lds": dict(lens=[4500, 1, 1025, 0, 5000], hq=8, hkv=2, block=256, gain=4.0),
+    "rows_past_lds_group_16": dict(lens=[1500, 1030, 33], hq=16, hkv=1, block=64),
     "pages_not_in_the_pool": dict(lens=[200, 60], chunks=[(20, 140)], hq=8, hkv=2, holes=[(0, 1, -1), (1, 0, 10 ** 6), (2, 0, -5)]),
 }
 

@@ -131,7 +131,7 @@ def test_attention_refusals_without_a_gpu(over, code, word):
 def test_workspace_refusals_without_a_gpu():
     lib = _lib.load()
     need = ctypes.c_size_t(0)
-    a = attention_args()
+    a = attention_args(decode_table_width=64)
     assert lib.slo_accumulate_attention_workspace_bytes(bytes(a), ctypes.byref(need)) == 0 and need.value > 0
     a.workspace, a.workspace_bytes = 4096, need.value - 1
     assert lib.slo_accumulate_attention(bytes(a), 4096, None) == 3

@@ -326,6 +326,14 @@ score_decode_kernel(ScoreParams p) {
     if (token + i < g.lk) add_score(p, g, block, off + i, head, token + i, w[i]);
 }
 
+// Sum over 16 lanes by DPP, in each of them.
+__device__ __forceinline__ float row_sum16(float x) {
+  x += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0xb1, 0xf, 0xf, false));   // quad_perm 1, 0, 3, 2
+  x += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x4e, 0xf, 0xf, false));   // quad_perm 2, 3, 0, 1
+  x += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x141, 0xf, 0xf, false));  // row_half_mirror
+  return x + __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x140, 0xf, 0xf, false));  // row_mirror
+}
+
 // Prefill rows, first pass: 16 NT (query, head) columns of one row per
 // workgroup, its four wavefronts every fourth pair of 16-token tiles of their
 // keys, the next pair's loads ahead of the products.  A lane sums its own
@@ -335,7 +343,7 @@ score_decode_kernel(ScoreParams p) {
 template <int KV, int NT>
 __global__ void __launch_bounds__(256, 2)
 score_lse_kernel(ScoreParams p, int tiles) {
-  __shared__ float sm[NT][4][64], sl[NT][4][64];
+  __shared__ float sm[NT][4][16], sl[NT][4][16];
   const int head = blockIdx.x, r = blockIdx.z;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, kg = lane >> 4;
@@ -381,57 +389,83 @@ score_lse_kernel(ScoreParams p, int tiles) {
     const bool now = ok;
     if (at + 128 < kend) ok = load(at + 128);
     if (!now) continue;
+    // One block of products and weights without a branch, so that the matrix
+    // cores work on a column group while the last one's weights are taken.
+    f32x4 s[NT][2];
+    float sum[NT], most = 0.0f;
+    auto weights = [&](bool masked) {
+      most = 0.0f;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      f32x4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[0] = mfma16(a[0][i], q[n][i], s[0]);
-        s[1] = mfma16(a[1][i], q[n][i], s[1]);
-      }
-      float e[8];
-      auto weights = [&] {
+      for (int n = 0; n < NT; ++n) {
+        float e[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j >> 2][j & 3], f[j >> 2][j & 3], -m[n]));
-          if (at + 32 > full && at + 16 * (j >> 2) + 4 * kg + (j & 3) >= limit[n]) e[j] = 0.0f;
+          e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][j >> 2][j & 3], f[j >> 2][j & 3], -m[n]));
+          if (masked && at + 16 * (j >> 2) + 4 * kg + (j & 3) >= limit[n]) e[j] = 0.0f;
         }
-        return fmaxf(fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])), fmaxf(fmaxf(e[4], e[5]), fmaxf(e[6], e[7])));
-      };
-      // The weights themselves tell whether the reference has to move.
-      if (__any(weights() > 256.0f)) {
+        most = fmaxf(most, fmaxf(fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])), fmaxf(fmaxf(e[4], e[5]), fmaxf(e[6], e[7]))));
+        sum[n] = ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+      }
+    };
+    auto products = [&] {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        s[n][0] = s[n][1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[n][0] = mfma16(a[0][i], q[n][i], s[n][0]);
+          s[n][1] = mfma16(a[1][i], q[n][i], s[n][1]);
+        }
+      }
+    };
+    const bool masked = at + 32 > full;
+    if (masked) {
+      products();
+      weights(true);
+    } else {
+      products();
+      weights(false);
+    }
+    // The weights themselves tell whether a reference has to move.
+    if (__any(most > 256.0f)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
         float top = m[n];
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (at + 16 * (j >> 2) + 4 * kg + (j & 3) < limit[n]) top = fmaxf(top, s[j >> 2][j & 3] * f[j >> 2][j & 3]);
+          if (at + 16 * (j >> 2) + 4 * kg + (j & 3) < limit[n]) top = fmaxf(top, s[n][j >> 2][j & 3] * f[j >> 2][j & 3]);
         l[n] *= __builtin_amdgcn_exp2f(m[n] - top);
         m[n] = top;
-        weights();
       }
-      l[n] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+      weights(true);
     }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) l[n] += sum[n];
   }
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    sm[n][wave][lane] = m[n];
-    sl[n][wave][lane] = l[n];
+    const float2 e = column_lse(float2{m[n], l[n]});
+    if (lane < 16) {
+      sm[n][wave][lane] = e.x;
+      sl[n][wave][lane] = e.y;
+    }
   }
   __syncthreads();
   const int x = threadIdx.x, tok = t0 + x / p.group;
   if (x < per * p.group && tok < t1) {
     float mm = kNone, ll = 0.0f;
-    for (int w = 0; w < 4; ++w)
-      for (int j = 0; j < 4; ++j) absorb(mm, ll, sm[x >> 4][w][16 * j + (x & 15)], sl[x >> 4][w][16 * j + (x & 15)]);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) absorb(mm, ll, sm[x >> 4][w][x & 15], sl[x >> 4][w][x & 15]);
     p.lse[(g.q0 - p.first_row + tok) * p.hq + head * p.group + x % p.group] = mm + __builtin_amdgcn_logf(ll);
   }
 }
 
 // Prefill rows, second pass: a workgroup takes 64 keys of one (row, kv head),
-// held as operands in every wavefront's registers, and its six wavefronts every
-// sixth 16 of the columns that see one of them.  A lane sums its 16
+// held as operands in every wavefront's registers, and its eight wavefronts
+// every eighth 16 of the columns that see one of them.  A lane sums its 16
 // tokens' weights over its columns; lanes, then wavefronts, are added in order
 // at the end.
-constexpr int kSumWaves = 6, kSumKeys = 64, kSumDepth = 3;
+constexpr int kSumWaves = 8, kSumKeys = 64, kSumDepth = 2;
 
 // 16 columns as their lanes take them: four operands of q, and the log2-sums.
 // They arrive by LDS DMA, kSumDepth in flight.
@@ -441,7 +475,7 @@ struct Columns {
 };
 
 template <int KV>
-__global__ void __launch_bounds__(64 * kSumWaves, 3)
+__global__ void __launch_bounds__(64 * kSumWaves, 2)
 score_prefill_kernel(ScoreParams p) {
   __shared__ Columns ring[kSumWaves][kSumDepth];
   __shared__ float sums[kSumWaves][kSumKeys];
@@ -449,12 +483,14 @@ score_prefill_kernel(ScoreParams p) {
   const int head = blockIdx.x, r = blockIdx.z;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, kg = lane >> 4;
-  const Row g = row_of(p, r);
   const int at = blockIdx.y * kSumKeys;
-  if (at >= g.lk || g.lq <= 0) return;
   int off;
-  const int block = page_of(p, r, at, off);
-  if (block < 0) return;
+  const int block = page_of(p, r, at, off);  // inside the tables' width, whatever the row's length
+  const Row g = row_of(p, r);
+  if (at >= g.lk || g.lq <= 0 || block < 0) return;
+  Keys<KV> keys[4];
+#pragma unroll
+  for (int h = 0; h < 4; ++h) keys[h].template load<false>(p, block, off + 16 * h, head, lane);
   // This wavefront's columns first + stride i; the next ones' query and head by
   // addition.  A column past the last is read as the last and weighs nothing.
   const int columns = g.lq * p.group, stride = 16 * kSumWaves;
@@ -482,14 +518,12 @@ score_prefill_kernel(ScoreParams p) {
     }
   };
   int now_tok = tok, now_hh = hh, sent = 0;
-  for (; sent < kSumDepth - 1 && sent < count; ++sent) fetch();
+  for (; sent < kSumDepth && sent < count; ++sent) fetch();
   bf16x8 a[4][4];
 #pragma unroll
   for (int h = 0; h < 4; ++h) {
-    Keys<KV> k;
-    k.template load<false>(p, block, off + 16 * h, head, lane);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) a[h][i] = k.operand(i);
+    for (int i = 0; i < 4; ++i) a[h][i] = keys[h].operand(i);
   }
   if (KV == KV_FP8_E4M3FN) {
     if (threadIdx.x < kSumKeys)
@@ -498,62 +532,80 @@ score_prefill_kernel(ScoreParams p) {
     __syncthreads();
   }
   float w[4][4] = {};
+  // One step ahead: the next columns' products run on the matrix cores while
+  // this one's weights are taken.
+  f32x4 s[2][4];
+  float ref[2];
   int from = 0;
-  for (int c = 0; c < count; ++c) {
-    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the place that the next fetch fills has been read
-    if (sent < count) {
-      fetch();
-      ++sent;
-    }
-    const int ahead = sent - 1 - c;
+  auto wait = [&](int c) {  // for the columns of step c
     asm volatile("" ::: "memory");
-    if (ahead >= 2)
-      __builtin_amdgcn_s_waitcnt(vmcnt_imm(10));
-    else if (ahead == 1)
+    if (sent - 1 - c >= 1)
       __builtin_amdgcn_s_waitcnt(vmcnt_imm(5));
     else
       __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
     asm volatile("" ::: "memory");
+  };
+  auto products = [&](f32x4(&o)[4], float& l) {
     const Columns& x = ring[wave][from];
-    from = from == kSumDepth - 1 ? 0 : from + 1;
-    f32x4 s[4] = {};
+#pragma unroll
+    for (int h = 0; h < 4; ++h) o[h] = f32x4{0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const bf16x8 q = as_bf16x8(x.q[i][lane]);
 #pragma unroll
-      for (int h = 0; h < 4; ++h) s[h] = mfma16(a[h][i], q, s[h]);
+      for (int h = 0; h < 4; ++h) o[h] = mfma16(a[h][i], q, o[h]);
     }
-    const float ref = x.lse[lane];
-    const int limit = now_tok < g.lq ? min(g.prefix + now_tok + 1, g.lk) : 0;
-    now_tok += dt;
-    now_hh += dh;
-    if (now_hh >= p.group) {
-      now_hh -= p.group;
-      ++now_tok;
-    }
-    auto add = [&](bool masked) {
+    l = x.lse[lane];
+  };
+  auto add = [&](const f32x4(&x)[4], float l, bool masked, int limit) {
 #pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        const f32x4 f = KV == KV_FP8_E4M3FN ? factors[4 * h + kg] : f32x4{p.scale_log2, p.scale_log2, p.scale_log2, p.scale_log2};
+    for (int h = 0; h < 4; ++h) {
+      const f32x4 f = KV == KV_FP8_E4M3FN ? factors[4 * h + kg] : f32x4{p.scale_log2, p.scale_log2, p.scale_log2, p.scale_log2};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][i], f[i], -ref));
-          w[h][i] += masked && at + 16 * h + 4 * kg + i >= limit ? 0.0f : e;
-        }
+      for (int i = 0; i < 4; ++i) {
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[h][i], f[i], -l));
+        w[h][i] += masked && at + 16 * h + 4 * kg + i >= limit ? 0.0f : e;
       }
-    };
-    if (__any(limit < at + kSumKeys))
-      add(true);
-    else
-      add(false);
+    }
+  };
+  if (count) {
+    wait(0);
+    products(s[0], ref[0]);
+  }
+  for (int c0 = 0; c0 < count; c0 += 2) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int c = c0 + u;
+      if (c >= count) break;
+      from = from == kSumDepth - 1 ? 0 : from + 1;
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the place that the next fetch fills has been read
+      if (sent < count) {
+        fetch();
+        ++sent;
+      }
+      const int limit = now_tok < g.lq ? min(g.prefix + now_tok + 1, g.lk) : 0;
+      now_tok += dt;
+      now_hh += dh;
+      if (now_hh >= p.group) {
+        now_hh -= p.group;
+        ++now_tok;
+      }
+      const bool more = c + 1 < count;
+      if (more) wait(c + 1);
+      if (!__any(limit < at + kSumKeys) && more) {
+        products(s[u ^ 1], ref[u ^ 1]);
+        add(s[u], ref[u], false, limit);
+      } else {
+        if (more) products(s[u ^ 1], ref[u ^ 1]);
+        add(s[u], ref[u], true, limit);
+      }
+    }
   }
 #pragma unroll
   for (int h = 0; h < 4; ++h)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float e = w[h][i];
-#pragma unroll
-      for (int d = 1; d < 16; d <<= 1) e += __shfl_xor(e, d, 64);
+      const float e = row_sum16(w[h][i]);
       if (col == 0) sums[wave][16 * h + 4 * kg + i] = e;
     }
   __syncthreads();

@@ -406,7 +406,10 @@ fp4_decode_kernel(Fp4Params p) {
       read_step(t, ring[wave].steps[from], lane);
       from = from == kDepth - 1 ? 0 : from + 1;
       const int at = begin + WAVES * KT * i;
-      if (ok & 1) step<1>(t, at + KT > g.lk, q, a, p.scale_log2, at, limit, g.lk, lane);
+      // Every step runs, so that the accumulators stay where they are: one whose
+      // page is not in the pool has no keys.
+      const bool in = ok & 1;
+      step<1>(t, !in || at + KT > g.lk, q, a, p.scale_log2, in ? at : 1 << 30, limit, g.lk, lane);
     }
   }
   auto& so = ring;
@@ -672,9 +675,8 @@ __device__ __forceinline__ void run_tile(const Fp4Params& p, const Row& g, int r
                                          Stage (&st)[2], int& buf, bf16x8 (&q)[NT][4], Acc<NT>& a, int wave, int lane) {
   const int per = 16 * NT / p.group;
   const int t0 = w0 + wave * per, t1 = min(t0 + per, g.lq);
-  const int all = min(max(g.prefix + min(w0 + 4 * per, g.lq), 0), g.lk);  // keys that one of the tile's queries sees
-  const int kend = t0 < g.lq ? min(max(g.prefix + t1, 0), g.lk) : 0;      // that one of the wavefront's sees
-  const int full = min(g.prefix + t0 + 1, g.lk);                          // that all of them see
+  const int all = min(max(g.prefix + min(w0 + 4 * per, g.lq), 0), g.lk);  // keys that one of the queries sees
+  const int full = min(g.prefix + t0 + 1, g.lk);                          // that all of the wavefront's see
   const int col = lane & 15, kg = lane >> 4;
   int limit[NT];
 #pragma unroll
@@ -694,7 +696,9 @@ __device__ __forceinline__ void run_tile(const Fp4Params& p, const Row& g, int r
   bool ok, next_ok = false;
   load_quarter(t, p, w.row(ok), wave, lane);
   for (int at = k0; at < k1; at += 64, buf ^= 1) {
-    stage(st[buf], t, all - at, wave, lane);
+    // Every step runs, so that the accumulators stay where they are: one whose
+    // page is not in the pool has no keys.
+    stage(st[buf], t, ok ? all - at : 0, wave, lane);
     if (at + 64 < k1) {
       w.advance(64);
       load_quarter(t, p, w.row(next_ok), wave, lane);
@@ -703,7 +707,7 @@ __device__ __forceinline__ void run_tile(const Fp4Params& p, const Row& g, int r
     // next step's barrier, when every wavefront has left it.  The barrier
     // waits for LDS only: the loads of the next step stay in flight.
     lds_sync();
-    if (ok && at < kend) staged_step<NT>(st[buf], at + 64 > full, q, a, p.scale_log2, at, limit, lane);
+    staged_step<NT>(st[buf], !ok || at + 64 > full, q, a, p.scale_log2, ok ? at : 1 << 30, limit, lane);
     ok = next_ok;
   }
 }

@@ -107,17 +107,6 @@ __device__ __forceinline__ int units_of(const Fp4Params& p, int r) {
   return r < p.rows ? (min(max(p.lens[r], 0), cap) + 127) >> 7 : 0;
 }
 
-// Inclusive sum over the wavefront by DPP: within rows of 16 lanes, then the
-// rows' last lanes onto the rows behind them.
-__device__ __forceinline__ int wave_scan(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr 1
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast 15
-  return x + __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast 31
-}
-
 __device__ __forceinline__ int chunk_units(const Fp4Params& p, int lane) {
   int total = 0;  // at most 65,535 rows of 2^15 units
   for (int r = lane; r < p.rows; r += 64) total += units_of(p, r);

@@ -58,12 +58,7 @@ __device__ __forceinline__ uint32_t order_key(float w) {
 // Exclusive sum over the workgroup's threads; `total` receives the whole.
 __device__ __forceinline__ int block_scan(int x, int* sums, int& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int s = x;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(s, d, 64);
-    if (lane >= d) s += y;
-  }
+  const int s = wave_scan(x);
   __syncthreads();
   if (lane == 63) sums[wave] = s;
   __syncthreads();
@@ -116,7 +111,7 @@ evict_select_kernel(EvictParams p) {
   load_run(p, scores, r, head, tid * RUN, old, k);
   int need = p.budget - p.recent;  // still to choose among the keys that match `prefix`
   uint32_t prefix = 0;
-#pragma unroll
+#pragma unroll 1  // three copies of this code take longer to fetch than to run
   for (int step = 0; step < 3; ++step) {
     const int shift = step == 0 ? 21 : step == 1 ? 10 : 0, bins = step == 2 ? 1024 : 2048;
     const uint32_t known = step == 0 ? 0u : step == 1 ? 0xffe00000u : 0xfffffc00u;

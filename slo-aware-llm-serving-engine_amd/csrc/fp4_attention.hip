@@ -579,8 +579,8 @@ __device__ __forceinline__ int tiles_of(const Fp4Params& p, int per, int r) {
   return g.lq > 0 ? (g.lq + per - 1) / per : 0;
 }
 
-__device__ __forceinline__ int steps_of(const Row& g, int per, int t) {
-  return (max(min(g.prefix + min((t + 1) * per, g.lq), g.lk), 1) + 63) >> 6;
+__device__ __forceinline__ int steps_of(int lq, int prefix, int lk, int per, int t) {
+  return (max(min(prefix + min((t + 1) * per, lq), lk), 1) + 63) >> 6;
 }
 
 // Sum over a 256-thread workgroup, before this thread and in all.
@@ -592,70 +592,92 @@ __device__ __forceinline__ int group_scan(int x, int* sums, int& total) {
   __syncthreads();
   total = sums[0] + sums[1] + sums[2] + sums[3];
   int before = upto - x;
-  for (int w = 0; w < wave; ++w) before += sums[w];
+#pragma unroll
+  for (int w = 0; w < 3; ++w) before += w < wave ? sums[w] : 0;
   return before;
 }
 
 constexpr int kMaxPrefillRows = 1024;
 constexpr int kLeastSteps = 4;  // of a share
 
-struct Plan256 {
+struct Rows {
   int first[kMaxPrefillRows + 1];  // number of each row's first tile
+  int lq[kMaxPrefillRows], prefix[kMaxPrefillRows], lk[kMaxPrefillRows];
   int sums[4];
-  int row, tile, skip;  // where the share begins
-  int each;             // steps of a share
+  int row, tile, skip;
 };
 
-// The number of the tiles' row, tile `i` of all.
-__device__ __forceinline__ int row_of_tile(const Plan256& s, int rows, int i) {
-  int lo = 0, hi = rows;  // first[lo] <= i < first[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (s.first[mid] <= i) lo = mid; else hi = mid;
-  }
-  return lo;
-}
+// A workgroup's share: where it begins, its steps, and those of a whole one.
+struct Share {
+  int row, tile, skip, steps, each;
+};
 
-// Finds this workgroup's share; returns its number of steps.
-__device__ __forceinline__ int find_share(const Fp4Params& p, int per, int share, Plan256& s) {
+__device__ __forceinline__ Share find_share(const Fp4Params& p, int per, int share, Rows& s) {
   const int tid = threadIdx.x;
   int tiles = 0;
   for (int base = 0; base < p.rows; base += 256) {
-    int all;
-    const int n = base + tid < p.rows ? tiles_of(p, per, base + tid) : 0;
+    const int r = base + tid;
+    int all, n = 0;
+    if (r < p.rows) {
+      const Row g = row_of(p, r);
+      s.lq[r] = g.lq;
+      s.prefix[r] = g.prefix;
+      s.lk[r] = g.lk;
+      n = g.lq > 0 ? (g.lq + per - 1) / per : 0;
+    }
     const int before = group_scan(n, s.sums, all);
-    if (base + tid < p.rows) s.first[base + tid] = tiles + before;
+    if (r < p.rows) s.first[r] = tiles + before;
     tiles += all;
   }
   if (tid == 0) s.first[p.rows] = tiles;
   __syncthreads();
-  auto steps = [&](int i) {
+  // Tile i's row (first[row] <= i < first[row + 1]) and steps.
+  auto steps = [&](int i, int& row) {
     if (i >= tiles) return 0;
-    const int r = row_of_tile(s, p.rows, i);
-    return steps_of(row_of(p, r), per, i - s.first[r]);
+    int lo = 0, hi = p.rows;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (s.first[mid] <= i) lo = mid; else hi = mid;
+    }
+    row = lo;
+    return steps_of(s.lq[lo], s.prefix[lo], s.lk[lo], per, i - s.first[lo]);
   };
-  int mine = 0, total, ignored;
-  for (int i = tid; i < tiles; i += 256) mine += steps(i);
-  group_scan(mine, s.sums, total);
-  const int each = max((total + p.shares - 1) / p.shares, kLeastSteps);
-  if (tid == 0) s.each = each;
-  const int begin = share * each;
-  if (begin >= total) return 0;
-  int before = 0;
-  for (int base = 0; base < tiles; base += 256) {
-    const int n = steps(base + tid);
-    const int at = before + group_scan(n, s.sums, ignored);
-    if (at <= begin && begin < at + n) {
-      const int r = row_of_tile(s, p.rows, base + tid);
-      s.row = r;
-      s.tile = base + tid - s.first[r];
+  int row = 0, own = steps(tid, row), mine = own, total, at;
+  if (tiles > 256) {
+    int ignored;
+    for (int i = tid + 256; i < tiles; i += 256) mine += steps(i, ignored);
+  }
+  at = group_scan(mine, s.sums, total);
+  Share c = {0, 0, 0, 0, max((total + p.shares - 1) / p.shares, kLeastSteps)};
+  const int begin = share * c.each;
+  if (begin >= total) return c;
+  if (tiles <= 256) {
+    if (at <= begin && begin < at + own) {
+      s.row = row;
+      s.tile = tid - s.first[row];
       s.skip = begin - at;
     }
-    before += ignored;
-    if (before > begin) break;
+  } else {
+    int before = 0;
+    for (int base = 0; base < tiles && before <= begin; base += 256) {
+      int all;
+      const int n = steps(base + tid, row);
+      at = before + group_scan(n, s.sums, all);
+      if (at <= begin && begin < at + n) {
+        s.row = row;
+        s.tile = base + tid - s.first[row];
+        s.skip = begin - at;
+      }
+      before += all;
+    }
   }
   __syncthreads();
-  return min(each, total - begin);
+  c.row = s.row;
+  c.tile = s.tile;
+  c.skip = s.skip;
+  c.steps = min(c.each, total - begin);
+  __syncthreads();  // the steps' operands take this memory next
+  return c;
 }
 
 // Steps [from, to) of one tile for this wavefront's columns.
@@ -707,21 +729,25 @@ __device__ __forceinline__ void run_tile(const Fp4Params& p, const Row& g, int r
 template <int NT>
 __global__ void __launch_bounds__(256, 2)
 fp4_prefill_kernel(Fp4Params p) {
-  __shared__ Stage st[2];
-  __shared__ Plan256 plan;
+  __shared__ union {
+    Stage st[2];
+    Rows rows;
+  } lds;
   const int head = blockIdx.x, share = blockIdx.y;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int per = 4 * (16 * NT / p.group);
   Part& part = p.parts[(int64_t)share * p.hkv + head];
-  int left = find_share(p, per, share, plan);
-  int r = plan.row, tile = plan.tile, from = plan.skip, buf = 0;
+  const Share mine = find_share(p, per, share, lds.rows);
+  int left = __builtin_amdgcn_readfirstlane(mine.steps), r = __builtin_amdgcn_readfirstlane(mine.row);
+  int tile = __builtin_amdgcn_readfirstlane(mine.tile), from = __builtin_amdgcn_readfirstlane(mine.skip), buf = 0;
+  const int each = __builtin_amdgcn_readfirstlane(mine.each);
   int open_row = 0, open_tile = 0, open = 0;
   while (left > 0) {
     const Row g = row_of(p, r);
-    const int steps = steps_of(g, per, tile), to = min(steps, from + left);
+    const int steps = steps_of(g.lq, g.prefix, g.lk, per, tile), to = min(steps, from + left);
     bf16x8 q[NT][4];
     Acc<NT> a;
-    run_tile<NT>(p, g, r, head, tile * per, from, to, st, buf, q, a, wave, lane);
+    run_tile<NT>(p, g, r, head, tile * per, from, to, lds.st, buf, q, a, wave, lane);
     int c = lane & 15;
     asm("" : "+v"(c));  // found again here, so that the loop need not hold it in registers
     const int kg = lane >> 4;
@@ -771,54 +797,17 @@ fp4_prefill_kernel(Fp4Params p) {
   if (threadIdx.x == 0) {
     part.row = open_row;
     part.tile = open_tile;
-    part.count = open ? 1 + (open + plan.each - 1) / plan.each : 0;
+    part.count = open ? 1 + (open + each - 1) / each : 0;
   }
 }
 
-// Joins the parts of the tiles that were cut, in order: one workgroup per 16
-// columns of the tile that a share leaves open.
-template <int NT>
-__global__ void __launch_bounds__(256)
-fp4_join_prefill_kernel(Fp4Params p) {
-  const int head = blockIdx.x, share = blockIdx.y, block = blockIdx.z;
-  const Part* part = p.parts + (int64_t)share * p.hkv + head;
-  const int count = part->count;
-  if (count == 0) return;
-  const Row g = row_of(p, part->row);
-  const int quarter = 16 * NT / p.group;
-  const int lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
-  const int x = 16 * (block % NT) + col, tok = (part->tile * 4 + block / NT) * quarter + x / p.group;
-  if (x >= quarter * p.group || tok >= g.lq) return;
-  const int at = 16 * block + col;
-  float m = part->m[1][at];
-  for (int s = 1; s < count; ++s) m = fmaxf(m, part[(int64_t)s * p.hkv].m[0][at]);
-  f32x4 o[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-  float l = 0;
-#pragma unroll 2
-  for (int s = 0; s < count; ++s) {
-    const Part& e = part[(int64_t)s * p.hkv];
-    const int k = s == 0;
-    const float w = __builtin_amdgcn_exp2f(e.m[k][at] - m);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) o[j] += e.o[k][block][(threadIdx.x >> 6) + 4 * j][lane] * w;
-    l += e.l[k][at] * w;
-  }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  uint16_t* out = p.out + (g.q0 + tok) * p.out_stride + (head * p.group + x % p.group) * HD4 + 32 * kg;
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-    *reinterpret_cast<u32x2*>(out + 4 * ((threadIdx.x >> 6) + 4 * j)) =
-        u32x2{pack_bf16x2(o[j][0] * inv, o[j][1] * inv), pack_bf16x2(o[j][2] * inv, o[j][3] * inv)};
-}
-
-// Joins the partial results of a decode row's chunks: a workgroup per (row,
+// Joins the partial results of decode row r's chunks: a workgroup per (row,
 // head), four channels a lane.  Half wavefront i takes chunks i, i + 8, ... and
 // the eight sums meet in LDS in that order.
-__global__ void __launch_bounds__(256)
-fp4_join_decode_kernel(Fp4Params p) {
+__device__ __forceinline__ void join_decode(const Fp4Params& p, int r, int h) {
   __shared__ f32x4 so[8][32];
   __shared__ float sl[8];
-  const int lane = threadIdx.x & 31, i = threadIdx.x >> 5, h = blockIdx.x, r = blockIdx.y;
+  const int lane = threadIdx.x & 31, i = threadIdx.x >> 5;
   Chunk c;
   find_chunk(p, r, true, threadIdx.x & 63, c);
   if (c.count == 1) return;  // written by its only chunk
@@ -849,6 +838,54 @@ fp4_join_decode_kernel(Fp4Params p) {
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   *reinterpret_cast<u32x2*>(p.out + (int64_t)r * p.out_stride + h * HD4 + 4 * lane) =
       u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
+}
+
+// Joins the parts of the tile that a share leaves open, in order: a workgroup
+// per 16 of its columns.
+template <int NT>
+__device__ __forceinline__ void join_prefill(const Fp4Params& p, int share, int head, int block) {
+  const Part* part = p.parts + (int64_t)share * p.hkv + head;
+  const int count = part->count;
+  if (count == 0) return;
+  const Row g = row_of(p, part->row);
+  const int quarter = 16 * NT / p.group;
+  const int lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
+  const int x = 16 * (block % NT) + col, tok = (part->tile * 4 + block / NT) * quarter + x / p.group;
+  if (x >= quarter * p.group || tok >= g.lq) return;
+  const int at = 16 * block + col;
+  float m = part->m[1][at];
+  for (int s = 1; s < count; ++s) m = fmaxf(m, part[(int64_t)s * p.hkv].m[0][at]);
+  f32x4 o[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+  float l = 0;
+#pragma unroll 2
+  for (int s = 0; s < count; ++s) {
+    const Part& e = part[(int64_t)s * p.hkv];
+    const int k = s == 0;
+    const float w = __builtin_amdgcn_exp2f(e.m[k][at] - m);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) o[j] += e.o[k][block][(threadIdx.x >> 6) + 4 * j][lane] * w;
+    l += e.l[k][at] * w;
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  uint16_t* out = p.out + (g.q0 + tok) * p.out_stride + (head * p.group + x % p.group) * HD4 + 32 * kg;
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    *reinterpret_cast<u32x2*>(out + 4 * ((threadIdx.x >> 6) + 4 * j)) =
+        u32x2{pack_bf16x2(o[j][0] * inv, o[j][1] * inv), pack_bf16x2(o[j][2] * inv, o[j][3] * inv)};
+}
+
+// One launch joins both phases: workgroups below `decode` take decode rows.
+__global__ void __launch_bounds__(256)
+fp4_join_kernel(Fp4Params d, Fp4Params f, int decode) {
+  int i = blockIdx.x;
+  if (i < decode) {
+    join_decode(d, i / d.hq, i % d.hq);
+    return;
+  }
+  i -= decode;
+  const int blocks = 4 * kPrefillNT, block = i % blocks;
+  i /= blocks;
+  join_prefill<kPrefillNT>(f, i / f.hkv, i % f.hkv, block);
 }
 
 // Two prefill workgroups fit a CU (64 KiB of LDS and 256 registers each); all
@@ -970,36 +1007,33 @@ extern "C" int slo_paged_attention_fp4(const slo_paged_attention_args* a, slo_st
   p.group = a->num_heads / a->num_kv_heads;
   p.scale_log2 = (a->softmax_scale < 0 ? -a->softmax_scale : a->softmax_scale) * kLog2e;
   p.q_sign = a->softmax_scale < 0 ? 0x80008000u : 0u;
+  Fp4Params d = p, f = p;
   if (n.dwork) {
-    p.lens = a->decode_lens;
-    p.tables = a->decode_tables;
-    p.table_stride = a->decode_table_stride;
-    p.table_width = a->decode_table_width;
-    p.first_row = 0;
-    p.rows = a->num_decode;
-    p.budget = n.joined ? n.budget : 1;
-    p.partial = static_cast<float*>(a->workspace);
-    if (n.joined) {
-      hipLaunchKernelGGL(fp4_decode_kernel<4>, dim3(p.hkv, n.budget + p.rows), dim3(256), 0, s, p);
-      hipLaunchKernelGGL(fp4_join_decode_kernel, dim3(p.hq, p.rows), dim3(256), 0, s, p);
-    } else {
-      hipLaunchKernelGGL(fp4_decode_kernel<8>, dim3(p.hkv, p.rows), dim3(512), 0, s, p);
-    }
+    d.lens = a->decode_lens;
+    d.tables = a->decode_tables;
+    d.table_stride = a->decode_table_stride;
+    d.table_width = a->decode_table_width;
+    d.rows = a->num_decode;
+    d.budget = n.joined ? n.budget : 1;
+    d.partial = static_cast<float*>(a->workspace);
+    if (n.joined)
+      hipLaunchKernelGGL(fp4_decode_kernel<4>, dim3(d.hkv, n.budget + d.rows), dim3(256), 0, s, d);
+    else
+      hipLaunchKernelGGL(fp4_decode_kernel<8>, dim3(d.hkv, d.rows), dim3(512), 0, s, d);
   }
   if (n.shares) {
-    p.lens = nullptr;
-    p.cu_q = a->prefill_cu_q;
-    p.cu_k = a->prefill_cu_k;
-    p.tables = a->prefill_tables;
-    p.table_stride = a->prefill_table_stride;
-    p.table_width = a->prefill_table_width;
-    p.first_row = a->num_decode;
-    p.rows = a->num_prefill;
-    p.shares = n.shares;
-    p.parts = reinterpret_cast<Part*>(static_cast<char*>(a->workspace) + n.dbytes);
-    hipLaunchKernelGGL(fp4_prefill_kernel<kPrefillNT>, dim3(p.hkv, p.shares), dim3(256), 0, s, p);
-    if (p.shares > 1)
-      hipLaunchKernelGGL(fp4_join_prefill_kernel<kPrefillNT>, dim3(p.hkv, p.shares - 1, 4 * kPrefillNT), dim3(256), 0, s, p);
+    f.cu_q = a->prefill_cu_q;
+    f.cu_k = a->prefill_cu_k;
+    f.tables = a->prefill_tables;
+    f.table_stride = a->prefill_table_stride;
+    f.table_width = a->prefill_table_width;
+    f.first_row = a->num_decode;
+    f.rows = a->num_prefill;
+    f.shares = n.shares;
+    f.parts = reinterpret_cast<Part*>(static_cast<char*>(a->workspace) + n.dbytes);
+    hipLaunchKernelGGL(fp4_prefill_kernel<kPrefillNT>, dim3(f.hkv, f.shares), dim3(256), 0, s, f);
   }
+  const int decode = n.joined ? d.rows * d.hq : 0, prefill = n.shares > 1 ? (n.shares - 1) * f.hkv * 4 * kPrefillNT : 0;
+  if (decode + prefill) hipLaunchKernelGGL(fp4_join_kernel, dim3(decode + prefill), dim3(256), 0, s, d, f, decode);
   return check_launch("paged_attention_fp4");
 }

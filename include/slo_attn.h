@@ -337,7 +337,9 @@ int slo_load_kvcache(const void* k_cache, const void* v_cache, const void* k_sca
 /*
  * slo_paged_attention over a 4-bit pool: the same arguments (k_scale / v_scale
  * point to E8M0 bytes, kv_dtype is SLO_KV_FP4_E2M1) and the same rows, masks
- * and outputs; a row without keys gives zeros.  Prefill rows are read through
+ * and outputs; a row without keys gives zeros, and so do query rows past every
+ * row's.  At most 32,768 decode and 1,024 prefill rows; tables of up to 2^22
+ * tokens.  Prefill rows are read through
  * prefill_tables (without tables they read no pool: slo_paged_attention takes
  * them); store_slot_mapping must be NULL and softmax_scale not zero.  The
  * workspace (16-byte aligned, slo_paged_attention_fp4_workspace_bytes of the
@@ -359,8 +361,11 @@ int slo_paged_attention_fp4(const slo_paged_attention_args* args, slo_stream_t s
  * Rows, masks and K as in slo_paged_attention; V, out and the new_k / new_v
  * fields are not read.  K comes from a bf16, E4M3FN or 4-bit pool; prefill
  * rows need prefill_tables.  Rows that share an old page both count (fp32
- * atomic adds: there the order of the additions may vary).  Workspace as for
- * slo_paged_attention_fp4.
+ * atomic adds: there the order of the additions may vary).  softmax_scale may
+ * not be zero; at most 32,768 rows of either kind and 2^21 tokens a row.
+ * Workspace as for slo_paged_attention_fp4; rows whose tables span more than
+ * 16,384 / (num_heads / num_kv_heads) tokens need 4 bytes per (decode row,
+ * query head, token of the tables' width).
  */
 int slo_accumulate_attention_workspace_bytes(const slo_paged_attention_args* args, size_t* bytes);
 int slo_accumulate_attention(const slo_paged_attention_args* args, float* scores, slo_stream_t stream);
@@ -401,8 +406,9 @@ typedef struct slo_evict_kv_args {
  * row's first `budget` places, and the scores of its other places up to its
  * length become zero.  The kept positions are written to `kept`.  The pages
  * past the budget can then be freed.  Two rows may not share a page, or a row
- * hold one twice.  Tokens in no page of the pool weigh nothing and do not
- * move.
+ * hold one twice.  Tokens in no page of the pool weigh less than any other and
+ * do not move.  block_size must be a multiple of 64, scores lie on a 16-byte
+ * boundary, tables span at most 2^24 tokens.
  */
 int slo_evict_kv(const slo_evict_kv_args* args, slo_stream_t stream);
 

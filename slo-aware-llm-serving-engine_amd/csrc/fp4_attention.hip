@@ -60,6 +60,12 @@ struct Fp4Params {
   int hq, hkv, group;
   float scale_log2;  // |softmax scale| * log2(e)
   uint32_t q_sign;   // 0x80008000 where the scale is negative
+  // Query rows from first_idle + (ends ? *ends : 0) on belong to no row (the
+  // capacity padding of a captured step); the launch that has `idle` set gives
+  // them zeros, so every output row is defined.
+  const int32_t* ends;
+  int first_idle;
+  bool idle;
   int rows;
   int budget;      // decode rows: about so many chunks over all rows
   float* partial;  // decode rows: [chunks, hq] records
@@ -108,7 +114,7 @@ __device__ __forceinline__ int units_of(const Fp4Params& p, int r) {
 }
 
 __device__ __forceinline__ int chunk_units(const Fp4Params& p, int lane) {
-  int total = 0;  // at most 65,535 rows of 2^15 units
+  int total = 0;  // at most 2^15 rows of 2^15 units
   for (int r = lane; r < p.rows; r += 64) total += units_of(p, r);
   total = __builtin_amdgcn_readlane(wave_scan(total), 63);
   return max((total + p.budget - 1) / p.budget, 2);
@@ -176,6 +182,14 @@ __device__ __forceinline__ void read_step(Tile& t, const Step& s, int lane) {
     for (int i = 0; i < 4; ++i)
       t.v[4 * h + i] = *reinterpret_cast<const uint32_t*>(s.v + h * 1024 + kg * 256 + (i ^ kg) * 64 + c * 4);
   }
+}
+
+__device__ __forceinline__ void clear_idle(const Fp4Params& p) {
+  const int64_t from = (int64_t)p.first_idle + (p.ends ? max(*p.ends, 0) : 0);
+  const int per = p.hq * (HD4 / 8);  // 16-byte pieces of a row
+  const int64_t pieces = (p.num_q_rows - from) * per, stride = (int64_t)gridDim.x * gridDim.y * blockDim.x;
+  for (int64_t i = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x; i < pieces; i += stride)
+    *reinterpret_cast<u32x4*>(p.out + (from + i / per) * p.out_stride + 8 * (i % per)) = u32x4{0, 0, 0, 0};
 }
 
 template <int NT>
@@ -344,6 +358,7 @@ fp4_decode_kernel(Fp4Params p) {
   __shared__ float sm[WAVES][16], sl[WAVES][16];
   const int head = blockIdx.x;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (p.idle) clear_idle(p);
   Chunk chunk;
   if (!find_chunk(p, blockIdx.y, false, lane, chunk)) return;
   const int r = chunk.row;
@@ -794,6 +809,7 @@ fp4_prefill_kernel(Fp4Params p) {
       while (tiles_of(p, per, r) == 0);
     }
   }
+  if (p.idle) clear_idle(p);
   if (threadIdx.x == 0) {
     part.row = open_row;
     part.tile = open_tile;
@@ -940,8 +956,8 @@ int check_args(const slo_paged_attention_args* a) {
   if (!(a->softmax_scale != 0.0f) || a->softmax_scale - a->softmax_scale != 0.0f)
     return fail(SLO_ERR_INVALID, "paged_attention_fp4: softmax_scale must be finite and not zero");
   if (a->store_slot_mapping) return fail(SLO_ERR_INVALID, "paged_attention_fp4: store the new rows first");
-  if (a->num_decode > 65535 || a->num_prefill > kMaxPrefillRows)
-    return fail(SLO_ERR_UNSUPPORTED, "paged_attention_fp4: more than 65535 decode or 1024 prefill rows");
+  if (a->num_decode > 32768 || a->num_prefill > kMaxPrefillRows)
+    return fail(SLO_ERR_UNSUPPORTED, "paged_attention_fp4: more than 32768 decode or 1024 prefill rows");
   const bool dec = a->num_decode > 0 && (a->phases & SLO_PHASE_DECODE);
   const bool pre = a->num_prefill > 0 && (a->phases & SLO_PHASE_PREFILL);
   if (!dec && !pre) return SLO_OK;
@@ -1007,7 +1023,12 @@ extern "C" int slo_paged_attention_fp4(const slo_paged_attention_args* a, slo_st
   p.group = a->num_heads / a->num_kv_heads;
   p.scale_log2 = (a->softmax_scale < 0 ? -a->softmax_scale : a->softmax_scale) * kLog2e;
   p.q_sign = a->softmax_scale < 0 ? 0x80008000u : 0u;
+  const bool rows = a->num_prefill > 0 && a->prefill_cu_q;  // whatever the phases
+  p.ends = rows ? a->prefill_cu_q + a->num_prefill : nullptr;
+  p.first_idle = a->num_decode;
   Fp4Params d = p, f = p;
+  d.idle = !n.shares && a->num_q_rows > a->num_decode;
+  f.idle = true;
   if (n.dwork) {
     d.lens = a->decode_lens;
     d.tables = a->decode_tables;

@@ -661,8 +661,8 @@ int check_args(const slo_paged_attention_args* a) {
     return fail(SLO_ERR_INVALID, "accumulate_attention: bad row counts");
   if (!(a->softmax_scale != 0.0f) || a->softmax_scale - a->softmax_scale != 0.0f)
     return fail(SLO_ERR_INVALID, "accumulate_attention: softmax_scale must be finite and not zero");
-  if (a->num_decode > 65535 || a->num_prefill > 65535)
-    return fail(SLO_ERR_UNSUPPORTED, "accumulate_attention: more than 65535 rows");
+  if (a->num_decode > 32768 || a->num_prefill > 32768)
+    return fail(SLO_ERR_UNSUPPORTED, "accumulate_attention: more than 32768 rows");
   const bool dec = a->num_decode > 0 && (a->phases & SLO_PHASE_DECODE);
   const bool pre = a->num_prefill > 0 && (a->phases & SLO_PHASE_PREFILL);
   if (!dec && !pre) return SLO_OK;
@@ -675,13 +675,14 @@ int check_args(const slo_paged_attention_args* a) {
     return fail(SLO_ERR_INVALID, "accumulate_attention: the pool must be 16-byte aligned");
   if (a->block_size <= 0 || a->block_size % 64)
     return fail(SLO_ERR_UNSUPPORTED, "accumulate_attention: block_size must be a multiple of 64");
+  if (pre && a->max_q > (1 << 18)) return fail(SLO_ERR_UNSUPPORTED, "accumulate_attention: more than 2^18 queries a row");
   if (dec && (!a->decode_lens || !a->decode_tables || a->decode_table_width <= 0))
     return fail(SLO_ERR_INVALID, "accumulate_attention: missing decode metadata");
   if (pre && (!a->prefill_cu_q || !a->prefill_cu_k || !a->prefill_tables || a->prefill_table_width <= 0))
     return fail(SLO_ERR_INVALID, "accumulate_attention: missing prefill metadata");
-  if ((dec && (int64_t)a->decode_table_width * a->block_size > (1 << 24)) ||
-      (pre && (int64_t)a->prefill_table_width * a->block_size > (1 << 24)))
-    return fail(SLO_ERR_UNSUPPORTED, "accumulate_attention: tables span more than 2^24 tokens");
+  if ((dec && (int64_t)a->decode_table_width * a->block_size > (1 << 21)) ||
+      (pre && (int64_t)a->prefill_table_width * a->block_size > (1 << 21)))
+    return fail(SLO_ERR_UNSUPPORTED, "accumulate_attention: tables span more than 2^21 tokens");
   return SLO_OK;
 }
 

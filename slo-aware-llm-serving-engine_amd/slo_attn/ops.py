@@ -466,6 +466,11 @@ def _row_args(T, num_decode, decode_lens, decode_tables, num_prefill, cu_q, cu_k
     if not 0 <= num_decode <= T:
         raise ValueError("num_decode must be from 0 to the number of query rows")
     decode, prefill = (num_decode, None, None, 0, 0), (0, None, None, 0, 0, None, 0, 0)
+    if num_prefill and cu_q is not None:  # where the prefill rows end matters in either phase
+        _int32(cu_q, "cu_seqlens_q")
+        if cu_q.numel() < num_prefill + 1:
+            raise ValueError("cu_seqlens shorter than num_prefill + 1")
+        prefill = num_prefill, cu_q.data_ptr(), *prefill[2:]
     if num_decode and phases & _lib.PHASE_DECODE:
         _int32(decode_lens, "decode_lens")
         _int32(decode_tables, "decode_tables")

@@ -90,14 +90,15 @@ def i32(x, device):
 class Rows:
     """Decode rows of ``lens`` keys and prefill rows (queries, prefix) over one pool."""
 
-    def __init__(self, fmt, lens, chunks=(), hq=32, hkv=8, block=64, seed=0, gain=1.0, scale=D ** -0.5, holes=()):
+    def __init__(self, fmt, lens, chunks=(), hq=32, hkv=8, block=64, seed=0, gain=1.0, scale=D ** -0.5, holes=(),
+                 spare=1):
         g = torch.Generator().manual_seed(seed)
         self.lens, self.chunks, self.hq, self.hkv, self.block, self.scale = list(lens), list(chunks), hq, hkv, block, scale
         totals = self.lens + [max(n + p, 0) for n, p in self.chunks]
         pages = [-(-t // block) for t in totals]
         self.blocks = sum(pages) + 2
         order, at, self.tables = torch.randperm(self.blocks, generator=g).tolist(), 0, []
-        width = max(pages + [1]) + 1
+        width = max(pages + [1]) + spare
         for n in pages:
             self.tables.append(order[at:at + n] + [-1] * (width - n))
             at += n

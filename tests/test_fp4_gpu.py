@@ -100,6 +100,9 @@ CASES = {
     "negative_scale": dict(lens=[80], chunks=[(30, 20)], hq=8, hkv=2, scale=-0.11),
     "rows_past_lds": dict(lens=[4500, 1, 1025, 0, 5000], hq=8, hkv=2, block=256, gain=4.0),
     "rows_past_lds_group_16": dict(lens=[1500, 1030, 33], hq=16, hkv=1, block=64),
+    "many_rows": dict(lens=[(37 * i) % 130 for i in range(150)], chunks=[(i % 5, 3 * i) for i in range(70)], hq=4, hkv=2),
+    "many_tiles": dict(lens=[], chunks=[(2300, 30), (40, 0)], hq=16, hkv=1),
+    "tables_far_wider_than_the_rows": dict(lens=[100, 5, 0], chunks=[(9, 70), (2, 0)], hq=8, hkv=2, spare=90),
     "pages_not_in_the_pool": dict(lens=[200, 60], chunks=[(20, 140)], hq=8, hkv=2, holes=[(0, 1, -1), (1, 0, 10 ** 6), (2, 0, -5)]),
 }
 
@@ -134,6 +137,65 @@ def test_attention_of_views_into_a_wider_output(device):
         other = torch.ones(case.tokens, dtype=torch.bool)
         other[mine] = False
         assert torch.equal(o[mine], plain[mine]) and (o[other.to(device)] == 5).all()
+
+
+def test_rows_past_every_row_get_zeros_and_bounds_may_be_capacities(device):
+    case = Rows("fp4", [100, 30], [(17, 40), (5, 0)], hq=8, hkv=2, seed=4)
+    kc, vc, ks, vs = case.pool.device(device)
+    args = dict(num_kv_heads=2, k_scale=ks, v_scale=vs, **case.arguments(device))
+    q = torch.cat((case.q, torch.full((40, 8, D), float("nan"), dtype=torch.bfloat16))).to(device)
+    want, _, bound = case.attend()
+    args["max_q"], args["max_k"] = 60, 5000
+    for phases in (1, 2, 3):
+        out = torch.full(q.shape, 3.0, dtype=torch.bfloat16, device=device)
+        slo_attn.paged_attention(q, kc, vc, case.scale, out=out, phases=phases, **args)
+        assert not out[case.tokens:].any()
+        for bit, rows in ((1, slice(0, 2)), (2, slice(2, case.tokens))):
+            if phases & bit:
+                assert ((out[rows].double().cpu() - want[rows]).abs() <= bound[rows]).all()
+            else:
+                assert (out[rows] == 3).all()
+    decode = {k: v for k, v in args.items() if "prefill" not in k and "max" not in k}
+    out = slo_attn.paged_attention(q[:5], kc, vc, case.scale, out=torch.ones_like(q[:5]), **decode)
+    assert not out[2:].any() and out[:2].any()
+
+
+def test_captured_mixed_steps_on_a_4_bit_pool(device):
+    # a bucket's graph (metadata, store, attention, weights) against the same bucket run eagerly
+    hq, hkv, block, width = 8, 2, 64, 4
+    pool = slo_attn.KVPool(2, 24, block, hkv, D, "fp4_e2m1", device, track_scores=True)
+    layers = [slo_attn.Attention(hq, D, D ** -0.5, hkv) for _ in range(2)]
+    pool.attach(layers)
+    g = torch.Generator().manual_seed(3)
+    table = random_values(g, 50, hq + 2 * hkv, D).to(device)
+
+    def forward(ids, positions):
+        x = table[ids]
+        out = 0
+        for layer in layers:
+            out = out + layer(x[:, :hq].contiguous(), x[:, hq:hq + hkv], x[:, hq + hkv:])
+        return out
+
+    buf = slo_attn.MixedStepBuffers(4, 3, 120, width, block, width * block, device)
+    graph = slo_attn.MixedStepGraph(buf, forward)
+    pool.kv.zero_(), pool.scale.fill_(127), pool.scores.zero_()
+    steps = [([], [(0, 60), (0, 33)], [[0, 1], [2]], list(range(40)) + list(range(50)) + [7, 8, 9]),
+             ([60, 33], [(0, 20)], [[0, 1], [2], [5]], list(range(22))),
+             ([61, 34, 20], [(0, 1)], [[0, 1], [2], [5], [6]], [1, 2, 3, 4])]
+    for step in steps:
+        before = pool.kv.clone(), pool.scale.clone(), pool.scores.clone()
+        got = graph.run(*step).clone()
+        torch.cuda.synchronize()
+        after = pool.kv.clone(), pool.scale.clone(), pool.scores.clone()
+        for t, b in zip((pool.kv, pool.scale, pool.scores), before):
+            t.copy_(b)
+        buf.build()
+        buf.set_context(True)
+        want = forward(buf.input_ids, buf.positions)
+        slo_attn.reset_context()
+        assert torch.isfinite(want).all() and torch.equal(got, want)
+        assert all(torch.equal(x, y) for x, y in zip(after, (pool.kv, pool.scale, pool.scores)))
+    assert pool.scores.any()
 
 
 def test_pool_past_4_gib(device):

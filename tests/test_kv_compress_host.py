@@ -116,6 +116,7 @@ def attention_args(**over):
     (dict(q_row_stride=4100), 1, "aligned"), (dict(k_cache=0), 1, "pool"), (dict(k_scale=0), 1, "scale"),
     (dict(block_size=96), 4, "block_size"), (dict(decode_lens=0), 1, "metadata"), (dict(decode_table_width=0), 1, "metadata"),
     (dict(num_prefill=1, max_q=3), 1, "metadata"), (dict(decode_table_width=1 << 23), 4, "tokens"),
+    (dict(num_decode=40000, num_q_rows=40000), 4, "rows"), (dict(num_prefill=40000), 4, "rows"),
 ])
 def test_attention_refusals_without_a_gpu(over, code, word):
     lib = _lib.load()
@@ -177,9 +178,10 @@ def test_evict_refusals_without_a_gpu():
 
     assert lib.slo_evict_kv(None, None) == 1 and call(num_rows=0) == 0
     for over in (dict(budget=0), dict(recent=101), dict(recent=-1), dict(num_layers=0), dict(kv_dtype=3), dict(num_blocks=0),
-                 dict(k_scale=None), dict(scores=None), dict(kept=None), dict(k_cache=4104), dict(table_width=0)):
+                 dict(k_scale=None), dict(scores=None), dict(kept=None), dict(k_cache=4104), dict(table_width=0),
+                 dict(scores=4100)):
         assert call(**over) == 1, over
-    for over in (dict(head_dim=96), dict(num_rows=65536), dict(table_width=1 << 20)):
+    for over in (dict(head_dim=96), dict(num_rows=65536), dict(table_width=1 << 20), dict(block_size=96)):
         assert call(**over) == 4, over
 
 

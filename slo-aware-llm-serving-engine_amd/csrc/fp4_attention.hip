@@ -101,7 +101,7 @@ __device__ __forceinline__ Row row_of(const Fp4Params& p, int r) {
 // captured launch knows no more of them than its tables' width): chunks of one
 // length over all rows, in units of 128 tokens, such that there are about
 // `budget`; a row's own are equal.  Every wavefront works it out for itself, 64
-// rows at a time (0.3 us for up to 64 rows).
+// rows at a time.
 struct Chunk {
   int row, index, count;  // the row's chunk `index` of `count`
   int first;              // number of the row's first chunk
@@ -154,7 +154,7 @@ struct Step {
   uint8_t k[2048], v[2048], ks[128], vs[128];
 };
 // Two in flight leave room for four workgroups on a CU; three for three, which
-// took 43.9 us where two take 39.6.
+// took 43.9 us where two took 39.6 (the 64 rows below, by the same rule).
 constexpr int kDepth = 2, kStepLoads = 5;
 
 __device__ __forceinline__ void fetch(const Fp4Params& p, int64_t row, uint32_t to, int lane) {
@@ -163,8 +163,8 @@ __device__ __forceinline__ void fetch(const Fp4Params& p, int64_t row, uint32_t 
   const uint8_t *k = p.kc + row * 64, *v = p.vc + row * 64;
   dma16_nt_at(k, ko, to);
   dma16_nt_at(k, ko + 1024, to + 1024);
-  dma16_nt_at(v, vo, to + 2048);
-  dma16_nt_at(v, vo + 1024, to + 3072);
+  dma16_nt_at(v, vo, to + 2 * 1024);
+  dma16_nt_at(v, vo + 1024, to + 2 * 1024 + 1024);
   dma4((lane < 32 ? p.ks : p.vs) + row * 4 + (lane & 31) * 4, to + 4096);
 }
 
@@ -351,8 +351,8 @@ __device__ __forceinline__ void clear(Acc<NT>& a) {
 // Each wavefront fetches its own steps, so the loop has no barrier; the
 // wavefronts' results meet in LDS.  Bound by the read: 64 rows of 512-4,096
 // tokens and 8 kv heads, 172 MB, 36.5 us or 4.7 TB/s (31.5 us with the
-// arithmetic left out, 39.6 with the default cache policy); steps in registers
-// instead of LDS, at most three wavefronts a SIMD, 52 us.
+// arithmetic left out, 39.4 with the default cache policy).  With chunks of
+// another rule, steps in registers instead of LDS took 53 us where LDS took 40.
 template <int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, 4)
 fp4_decode_kernel(Fp4Params p) {
@@ -404,9 +404,7 @@ fp4_decode_kernel(Fp4Params p) {
       if (sent < steps) send();
       const int ahead = sent - 1 - i;
       asm volatile("" ::: "memory");
-      if (ahead >= 2)
-        __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * kStepLoads));
-      else if (ahead == 1)
+      if (ahead == 1)
         __builtin_amdgcn_s_waitcnt(vmcnt_imm(kStepLoads));
       else
         __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
@@ -745,11 +743,11 @@ __device__ __forceinline__ void run_tile(const Fp4Params& p, const Row& g, int r
 
 // A workgroup's four wavefronts turn each step's codes into operands together,
 // each a quarter, and each runs 16 NT columns over them; the next step's codes
-// load meanwhile.  (Every wavefront converting for itself, without LDS: 175 us
-// where this takes 51, chunks of 1,000, 300 and 77 queries on 3,500, 1,000 and
-// 3,077 keys, 16 query heads.)  A step of the two workgroups on a CU takes 2.3
-// us, of which the matrix cores work 0.9: operand reads from LDS, weights and
-// products of only two wavefronts a SIMD overlap little.
+// load meanwhile.  Chunks of 1,000, 300 and 77 queries on 3,500, 1,000 and
+// 3,077 keys, 16 query heads: every wavefront converting for itself 175 us,
+// staged 80, with equal shares 51.  Of the last, copies with a part removed save
+// 36 us without the steps, 9 without the operand reads from LDS, 6 without the
+// output products, 4 without the exponents, 5 without the conversion.
 template <int NT>
 __global__ void __launch_bounds__(256, 2)
 fp4_prefill_kernel(Fp4Params p) {

@@ -222,8 +222,8 @@ __device__ __forceinline__ float2 column_lse(float2 e) {
 // Decode rows whose logits fit LDS: a workgroup takes a (row, kv head) whole,
 // so one launch does, and K is all that moves.  64 rows of 512-4,096 tokens of
 // a 4-bit pool, 8 kv heads (86 MB of K): 30 us, against 37 and 11 in two
-// launches through memory; 22 without the second half, whose adds end with the
-// round trip to the scores' lines.
+// launches through memory; 25 without the adds to the scores, 23 without the
+// second half.
 constexpr int kRowLogits = 16384;
 
 template <int KV, int WAVES>
@@ -351,7 +351,7 @@ __device__ __forceinline__ float row_sum16(float x) {
 // only where that passes it by 2^8 (sums of weights up to 256 round like those
 // below 1); the lanes meet at the end.  1,024 queries on 2,048 keys and 500 on
 // 500, 32 heads, E4M3FN: 39 us (45 with two column groups a wavefront, whose
-// keys then serve half as many columns), 12 of them before the first product.
+// keys then serve half as many columns), 12 without the loop over the keys.
 template <int KV, int NT>
 __global__ void __launch_bounds__(256, 2)
 score_lse_kernel(ScoreParams p, int tiles) {
@@ -476,9 +476,9 @@ score_lse_kernel(ScoreParams p, int tiles) {
 // held as operands in every wavefront's registers, and its eight wavefronts
 // every eighth 16 of the columns that see one of them.  A lane sums its 16
 // tokens' weights over its columns; lanes, then wavefronts, are added in order
-// at the end.  The same queries and keys: 40 us, 10 of them before the first
-// product; three or four steps of columns in flight instead of two change
-// nothing, and neither do the exponents or products alone (2 us each).
+// at the end.  The same queries and keys: 40 us; three or four steps of columns
+// in flight instead of two 40 and 41.  Of 42 before the last change, the loop was
+// 27, the exponents alone 2 and the products alone 3.
 constexpr int kSumWaves = 8, kSumKeys = 64, kSumDepth = 2;
 
 // 16 columns as their lanes take them: four operands of q, and the log2-sums.

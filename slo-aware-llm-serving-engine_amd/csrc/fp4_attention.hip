@@ -591,7 +591,7 @@ __device__ __forceinline__ void staged_step(const Stage& st, bool masked, const 
 // for each workgroup of a kv head: causal tiles differ in length, a row may be
 // long and its queries few, and the lengths are known on the GPU only.  A tile
 // that lies in one share is written out; the parts of one that is cut meet in
-// fp4_join_prefill_kernel.
+// fp4_join_kernel.
 __device__ __forceinline__ int tiles_of(const Fp4Params& p, int per, int r) {
   const Row g = row_of(p, r);
   return g.lq > 0 ? (g.lq + per - 1) / per : 0;

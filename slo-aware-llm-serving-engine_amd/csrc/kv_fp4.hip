@@ -120,14 +120,21 @@ load_kv_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ 
             o[2 * i + h] = pack_bf16x2(__uint_as_float(b[h] << 16) * scale[d], __uint_as_float(b[h] & 0xffff0000u) * scale[d]);
         }
       }
-      reinterpret_cast<u32x4*>(t.is_v ? v_out : k_out)[(((int64_t)t.token * hkv + t.head) << shift) + t.j] = o;
+      u32x4* to = reinterpret_cast<u32x4*>(t.is_v ? v_out : k_out) + ((((int64_t)t.token * hkv + t.head) << shift) + t.j);
+      if constexpr (TOK > 1)
+        __builtin_nontemporal_store(o, to);
+      else
+        *to = o;
     }
   }
 }
 
 // Four tokens a workgroup, and four loads a lane in flight, from here on: the
 // read back of 262,144 tokens of 8 heads takes 347 us so and 376 us with one
-// token a workgroup, that of 4,096 tokens 8.7 and 7.0 us.
+// token a workgroup, that of 4,096 tokens 8.7 and 7.0 us.  What such a read back
+// writes is larger than the caches, so it is stored past them: 338 us, and what
+// the next kernel finds there is not displaced (a move of 16 rows in the pool
+// that was read back before takes 160 us instead of 184).
 constexpr int kManyTokens = 16384;
 
 }  // namespace slo

@@ -338,7 +338,8 @@ int slo_load_kvcache(const void* k_cache, const void* v_cache, const void* k_sca
  * slo_paged_attention over a 4-bit pool: the same arguments (k_scale / v_scale
  * point to E8M0 bytes, kv_dtype is SLO_KV_FP4_E2M1) and the same rows, masks
  * and outputs; a row without keys gives zeros, and so do query rows past every
- * row's.  At most 32,768 decode and 1,024 prefill rows; tables of up to 2^22
+ * row's.  max_q is not read and max_k may be 0 (it sizes the launch, never the
+ * result).  At most 32,768 decode and 1,024 prefill rows; tables of up to 2^22
  * tokens.  Prefill rows are read through
  * prefill_tables (without tables they read no pool: slo_paged_attention takes
  * them); store_slot_mapping must be NULL and softmax_scale not zero.  The

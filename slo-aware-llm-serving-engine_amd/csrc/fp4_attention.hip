@@ -939,9 +939,11 @@ Plan plan_of(const slo_paged_attention_args* a) {
     n.budget = n.joined ? (kDecodeChunks + a->num_kv_heads - 1) / a->num_kv_heads : 0;
     if (n.joined) n.dbytes = (size_t)(n.budget + a->num_decode) * a->num_heads * RECORD * 4;
   }
-  if (a->num_prefill > 0 && (a->phases & SLO_PHASE_PREFILL) && a->max_q > 0) {
+  if (a->num_prefill > 0 && (a->phases & SLO_PHASE_PREFILL)) {
     const int per = 4 * (16 * kPrefillNT / (a->num_heads / a->num_kv_heads));
-    const int64_t cap = (int64_t)a->prefill_table_width * a->block_size, keys = cap < a->max_k ? cap : a->max_k;
+    // max_k only keeps the shares of short rows in wide tables few: any number
+    // of them covers all steps, and without it the tables' width bounds the keys.
+    const int64_t cap = (int64_t)a->prefill_table_width * a->block_size, keys = a->max_k > 0 && a->max_k < cap ? a->max_k : cap;
     // The rows' queries together bound the tiles; no more shares than steps / kLeastSteps.
     const int64_t tiles = (a->num_q_rows - a->num_decode) / per + a->num_prefill, steps = tiles * ((keys + 63) / 64);
     const int64_t most = (steps + kLeastSteps - 1) / kLeastSteps, full = (kPrefillShares + a->num_kv_heads - 1) / a->num_kv_heads;

@@ -658,7 +658,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor | None, v_cache: torc
     for the decode rows and one for the prefill rows (and one that joins the
     parts of long rows); ``store_slot_mapping`` then stores first.  Prefill rows
     without tables read no pool and run as with any other.  ``noalloc`` is
-    refused.
+    refused.  ``max_q`` and ``max_k`` may be left out with any pool: results do
+    not depend on them.
 
     ``noalloc=True`` launches through ``slo_paged_attention_noalloc``, which
     uses the library's static per-GPU scratch instead of this module's

@@ -1,0 +1,28 @@
+"""Limits of the 4-bit attention and of the accumulated weights, on the CPU: what
+the C entries size and refuse."""
+import ctypes
+
+import pytest
+
+from slo_attn import _lib
+from test_kv_compress_host import attention_args
+
+
+def prefill_args(queries, rows, width, heads=32, kv_heads=8, **over):
+    return attention_args(**{**dict(num_decode=0, num_q_rows=queries, num_prefill=rows, prefill_cu_q=4096, prefill_cu_k=4096,
+                                    prefill_tables=4096, prefill_table_stride=width, prefill_table_width=width,
+                                    num_heads=heads, num_kv_heads=kv_heads, q_row_stride=heads * 128,
+                                    out_row_stride=heads * 128), **over})
+
+
+def workspace(call, a):
+    need = ctypes.c_size_t(0)
+    assert call(bytes(a), ctypes.byref(need)) == 0, _lib.load().slo_last_error()
+    return need.value
+
+
+@pytest.mark.parametrize("bounds", [(0, 0), (0, 900), (700, 0), (1, 1)])
+def test_4_bit_prefill_rows_have_a_plan_whatever_the_bounds(bounds):
+    call = _lib.load().slo_paged_attention_fp4_workspace_bytes
+    exact = workspace(call, prefill_args(700, 2, 16, max_q=700, max_k=900))
+    assert exact > 0 and workspace(call, prefill_args(700, 2, 16, max_q=bounds[0], max_k=bounds[1])) > 0

@@ -362,8 +362,9 @@ int slo_paged_attention_fp4(const slo_paged_attention_args* args, slo_stream_t s
  * Rows, masks and K as in slo_paged_attention; V, out and the new_k / new_v
  * fields are not read.  K comes from a bf16, E4M3FN or 4-bit pool; prefill
  * rows need prefill_tables.  Rows that share an old page both count (fp32
- * atomic adds: there the order of the additions may vary).  softmax_scale may
- * not be zero; at most 32,768 rows of either kind, 2^21 tokens a row and 2^17
+ * atomic adds: there the order of the additions may vary).  max_q and max_k
+ * size the launches (0: the queries and the tables' width do), never the
+ * result.  softmax_scale may not be zero; at most 32,768 rows of either kind, 2^21 tokens a row and 2^17
  * queries a prefill row.
  * Workspace as for slo_paged_attention_fp4; rows whose tables span more than
  * 16,384 / (num_heads / num_kv_heads) tokens need 4 bytes per (decode row,

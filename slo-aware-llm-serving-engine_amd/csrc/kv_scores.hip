@@ -353,16 +353,11 @@ __device__ __forceinline__ float row_sum16(float x) {
 // 500, 32 heads, E4M3FN: 39 us (45 with two column groups a wavefront, whose
 // keys then serve half as many columns), 12 without the loop over the keys.
 template <int KV, int NT>
-__global__ void __launch_bounds__(256, 2)
-score_lse_kernel(ScoreParams p, int tiles) {
+__device__ __forceinline__ void find_lse(const ScoreParams& p, const Row& g, int r, int head, int per, int t0) {
   __shared__ float sm[NT][4][16], sl[NT][4][16];
-  const int head = blockIdx.x, r = blockIdx.z;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, kg = lane >> 4;
-  const int per = 16 * NT / p.group;
-  const Row g = row_of(p, r);
-  const int t0 = (tiles - 1 - (int)blockIdx.y) * per, t1 = min(t0 + per, g.lq);
-  if (t0 >= g.lq) return;
+  const int t1 = min(t0 + per, g.lq);
   const int kend = min(max(g.prefix + t1, 0), g.lk);
   bf16x8 q[NT][4];
   int limit[NT];
@@ -472,6 +467,19 @@ score_lse_kernel(ScoreParams p, int tiles) {
   }
 }
 
+// One tile a workgroup; those of a row with more queries than the launch was
+// sized for (max_q) go round.
+template <int KV, int NT>
+__global__ void __launch_bounds__(256, 2)
+score_lse_kernel(ScoreParams p, int tiles) {
+  const int head = blockIdx.x, r = blockIdx.z, per = 16 * NT / p.group;
+  const Row g = row_of(p, r);
+  for (int t0 = (tiles - 1 - (int)blockIdx.y) * per; t0 < g.lq; t0 += tiles * per) {
+    find_lse<KV, NT>(p, g, r, head, per, t0);
+    __syncthreads();  // the maxima and sums have been read
+  }
+}
+
 // Prefill rows, second pass: a workgroup takes 64 keys of one (row, kv head),
 // held as operands in every wavefront's registers, and its eight wavefronts
 // every eighth 16 of the columns that see one of them.  A lane sums its 16
@@ -488,20 +496,14 @@ struct Columns {
   float lse[64];
 };
 
+// The keys from token `at` of row r, in page `block` from place `off` on.
 template <int KV>
-__global__ void __launch_bounds__(64 * kSumWaves, 2)
-score_prefill_kernel(ScoreParams p) {
+__device__ __forceinline__ void weigh_keys(const ScoreParams& p, const Row& g, int head, int at, int block, int off) {
   __shared__ Columns ring[kSumWaves][kSumDepth];
   __shared__ float sums[kSumWaves][kSumKeys];
   __shared__ f32x4 factors[KV == KV_FP8_E4M3FN ? kSumKeys / 4 : 1];  // E4M3FN scales, in LDS to save registers
-  const int head = blockIdx.x, r = blockIdx.z;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, kg = lane >> 4;
-  const int at = blockIdx.y * kSumKeys;
-  int off;
-  const int block = page_of(p, r, at, off);  // inside the tables' width, whatever the row's length
-  const Row g = row_of(p, r);
-  if (at >= g.lk || g.lq <= 0 || block < 0) return;
   Keys<KV> keys[4];
 #pragma unroll
   for (int h = 0; h < 4; ++h) keys[h].template load<false>(p, block, off + 16 * h, head, lane);
@@ -632,7 +634,27 @@ score_prefill_kernel(ScoreParams p) {
   }
 }
 
+template <int KV>
+__global__ void __launch_bounds__(64 * kSumWaves, 2)
+score_prefill_kernel(ScoreParams p) {
+  const int head = blockIdx.x, r = blockIdx.z;
+  int at = blockIdx.y * kSumKeys, off;
+  int block = page_of(p, r, at, off);  // inside the tables' width, whatever the row's length
+  const Row g = row_of(p, r);
+  if (g.lq <= 0) return;
+  // 64 keys a workgroup; those of a row with more keys than the launch was sized
+  // for (max_k) go round.
+  while (at < g.lk) {
+    if (block >= 0) weigh_keys<KV>(p, g, head, at, block, off);
+    at += gridDim.y * kSumKeys;
+    if (at >= g.lk) return;
+    block = page_of(p, r, at, off);
+    __syncthreads();  // the last keys' sums and factors have been read
+  }
+}
+
 constexpr int kLseNT = 4;
+constexpr int kMostQueries = 1 << 17;  // of a row
 
 struct Plan {
   bool whole;  // decode rows in one launch
@@ -655,9 +677,12 @@ Plan plan_of(const slo_paged_attention_args* a) {
     if (!n.whole) n.logits = up256((size_t)a->num_decode * a->num_heads * cap * 4);
     if (!n.whole) n.partial = up256((size_t)a->num_decode * a->num_heads * n.splits * 8);
   }
-  if (a->num_prefill > 0 && (a->phases & SLO_PHASE_PREFILL) && a->max_q > 0) {
+  if (a->num_prefill > 0 && (a->phases & SLO_PHASE_PREFILL) && a->num_q_rows > a->num_decode) {
+    // max_q and max_k size the two launches, whose workgroups go round where a
+    // row is longer; without them the queries and the tables bound the rows.
     const int per = 16 * kLseNT / (a->num_heads / a->num_kv_heads);
-    n.tiles = (a->max_q + per - 1) / per;
+    const int all = a->num_q_rows - a->num_decode, most = a->max_q > 0 && a->max_q < all ? a->max_q : all;
+    n.tiles = ((most < kMostQueries ? most : kMostQueries) + per - 1) / per;
     n.lse = up256((size_t)(a->num_q_rows - a->num_decode) * a->num_heads * 4);
   }
   return n;
@@ -689,7 +714,7 @@ int check_args(const slo_paged_attention_args* a) {
     return fail(SLO_ERR_INVALID, "accumulate_attention: the pool must be 16-byte aligned");
   if (a->block_size <= 0 || a->block_size % 64)
     return fail(SLO_ERR_UNSUPPORTED, "accumulate_attention: block_size must be a multiple of 64");
-  if (pre && a->max_q > (1 << 17)) return fail(SLO_ERR_UNSUPPORTED, "accumulate_attention: more than 2^17 queries a row");
+  if (pre && a->max_q > kMostQueries) return fail(SLO_ERR_UNSUPPORTED, "accumulate_attention: more than 2^17 queries a row");
   if (dec && (!a->decode_lens || !a->decode_tables || a->decode_table_width <= 0))
     return fail(SLO_ERR_INVALID, "accumulate_attention: missing decode metadata");
   if (pre && (!a->prefill_cu_q || !a->prefill_cu_k || !a->prefill_tables || a->prefill_table_width <= 0))
@@ -715,7 +740,7 @@ void launch(const ScoreParams& d, const ScoreParams& f, const slo_paged_attentio
   if (n.tiles) {
     hipLaunchKernelGGL((score_lse_kernel<KV, kLseNT>), dim3(f.hkv, n.tiles, a->num_prefill), dim3(256), 0, s, f, n.tiles);
     const int64_t most = (int64_t)f.table_width * f.block_size;
-    const int64_t keys = a->max_k > 0 ? ((int64_t)a->max_k + 63) / 64 * 64 : 64;
+    const int64_t keys = a->max_k > 0 ? ((int64_t)a->max_k + 63) / 64 * 64 : most;
     const int cap = (int)(most < keys ? most : keys);
     hipLaunchKernelGGL(score_prefill_kernel<KV>, dim3(f.hkv, cap / kSumKeys, a->num_prefill), dim3(64 * kSumWaves), 0, s, f);
   }

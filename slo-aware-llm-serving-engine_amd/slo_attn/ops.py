@@ -546,7 +546,8 @@ def accumulate_attention(q: torch.Tensor, k_cache: torch.Tensor, kv_scores: torc
     last ``cu_q[r+1] - cu_q[r]`` of a prefill row) start from that sum, whatever
     their slots held.  A cached prefix that was never weighed has to be zero
     (``KVPool.reset_blocks``).  Rows of one call may share old pages: each adds
-    its weights, in an order that is not fixed.  ``evict_kv`` reads the scores.
+    its weights, in an order that is not fixed.  ``max_q`` and ``max_k`` only
+    size the launches; given, they keep them small.  ``evict_kv`` reads the scores.
     """
     index, geometry = _check_query(q, num_kv_heads, k_cache, k_scale, None, None, False, kv_scores, decode_lens, decode_tables,
                                    prefill_cu_q, prefill_cu_k, prefill_tables)

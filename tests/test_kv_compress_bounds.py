@@ -26,3 +26,10 @@ def test_4_bit_prefill_rows_have_a_plan_whatever_the_bounds(bounds):
     call = _lib.load().slo_paged_attention_fp4_workspace_bytes
     exact = workspace(call, prefill_args(700, 2, 16, max_q=700, max_k=900))
     assert exact > 0 and workspace(call, prefill_args(700, 2, 16, max_q=bounds[0], max_k=bounds[1])) > 0
+
+
+@pytest.mark.parametrize("bounds", [(0, 0), (0, 900), (700, 0), (1, 1), (1 << 17, 1 << 21)])
+def test_weights_keep_a_place_for_every_query_whatever_the_bounds(bounds):
+    call = _lib.load().slo_accumulate_attention_workspace_bytes
+    exact = workspace(call, prefill_args(700, 2, 16, max_q=700, max_k=900))
+    assert exact >= 700 * 32 * 4 and workspace(call, prefill_args(700, 2, 16, max_q=bounds[0], max_k=bounds[1])) == exact

@@ -931,6 +931,16 @@ struct Plan {
   size_t dbytes, pbytes;
 };
 
+// Prefill rows' shares are numbered steps of all tiles together, in 32 bits on
+// the GPU (find_share adds up to two shares' steps to their sum).
+constexpr int64_t kMaxSteps = 1 << 30;
+
+int64_t prefill_tiles(const slo_paged_attention_args* a) {
+  // The rows' queries together bound the tiles.
+  const int per = 4 * (16 * kPrefillNT / (a->num_heads / a->num_kv_heads));
+  return (int64_t)(a->num_q_rows - a->num_decode) / per + a->num_prefill;
+}
+
 Plan plan_of(const slo_paged_attention_args* a) {
   Plan n = {false, false, 0, 0, 0, 0};
   if (a->num_decode > 0 && (a->phases & SLO_PHASE_DECODE)) {
@@ -940,12 +950,11 @@ Plan plan_of(const slo_paged_attention_args* a) {
     if (n.joined) n.dbytes = (size_t)(n.budget + a->num_decode) * a->num_heads * RECORD * 4;
   }
   if (a->num_prefill > 0 && (a->phases & SLO_PHASE_PREFILL)) {
-    const int per = 4 * (16 * kPrefillNT / (a->num_heads / a->num_kv_heads));
     // max_k only keeps the shares of short rows in wide tables few: any number
     // of them covers all steps, and without it the tables' width bounds the keys.
     const int64_t cap = (int64_t)a->prefill_table_width * a->block_size, keys = a->max_k > 0 && a->max_k < cap ? a->max_k : cap;
-    // The rows' queries together bound the tiles; no more shares than steps / kLeastSteps.
-    const int64_t tiles = (a->num_q_rows - a->num_decode) / per + a->num_prefill, steps = tiles * ((keys + 63) / 64);
+    // No more shares than steps / kLeastSteps.
+    const int64_t steps = prefill_tiles(a) * ((keys + 63) / 64);
     const int64_t most = (steps + kLeastSteps - 1) / kLeastSteps, full = (kPrefillShares + a->num_kv_heads - 1) / a->num_kv_heads;
     n.shares = (int)(most < 1 ? 1 : most < full ? most : full);
     n.pbytes = (size_t)n.shares * a->num_kv_heads * sizeof(Part);
@@ -990,6 +999,8 @@ int check_args(const slo_paged_attention_args* a) {
   if ((dec && (int64_t)a->decode_table_width * a->block_size > (1 << 22)) ||
       (pre && (int64_t)a->prefill_table_width * a->block_size > (1 << 22)))
     return fail(SLO_ERR_UNSUPPORTED, "paged_attention_fp4: tables span more than 2^22 tokens");
+  if (pre && prefill_tiles(a) * ((int64_t)a->prefill_table_width * a->block_size / 64) > kMaxSteps)
+    return fail(SLO_ERR_UNSUPPORTED, "paged_attention_fp4: prefill queries times the tables' tokens past 2^30 steps of a tile");
   return SLO_OK;
 }
 

@@ -33,3 +33,18 @@ def test_weights_keep_a_place_for_every_query_whatever_the_bounds(bounds):
     call = _lib.load().slo_accumulate_attention_workspace_bytes
     exact = workspace(call, prefill_args(700, 2, 16, max_q=700, max_k=900))
     assert exact >= 700 * 32 * 4 and workspace(call, prefill_args(700, 2, 16, max_q=bounds[0], max_k=bounds[1])) == exact
+
+
+@pytest.mark.parametrize("heads,kv_heads,rows,most", [(64, 4, 1, 131071), (64, 4, 129, 130047), (32, 8, 1, 524287), (28, 4, 7, 262047)])
+def test_4_bit_prefill_steps_stay_in_32_bits(heads, kv_heads, rows, most):
+    # Tiles of 4 floor(32 / group) queries, and one more a row, times 65,536 steps of 64 keys: 2^30 at most, so 2^14 tiles.
+    lib = _lib.load()
+    need = ctypes.c_size_t(0)
+    for n in (most, most + 1):
+        a = prefill_args(n, rows, 16384, heads, kv_heads)
+        rc = lib.slo_paged_attention_fp4_workspace_bytes(bytes(a), ctypes.byref(need))
+        assert rc == (0 if n == most else 4), lib.slo_last_error()
+        if rc:
+            assert lib.slo_paged_attention_fp4(bytes(a), None) == 4 and b"2^30" in lib.slo_last_error()
+    # a captured step's capacities are far below
+    assert lib.slo_paged_attention_fp4_workspace_bytes(bytes(prefill_args(65536, 1024, 640)), ctypes.byref(need)) == 0

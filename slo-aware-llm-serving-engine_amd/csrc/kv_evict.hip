@@ -186,8 +186,8 @@ evict_select_kernel(EvictParams p) {
 // rows: `unit` bytes of a lane, `units` lanes a token.
 struct Stream {
   uint8_t* base;
-  int64_t layer_bytes, page_bytes;
-  int head_bytes, token_bytes, unit, units;
+  int64_t layer_bytes, page_bytes, head_bytes;  // 2^24 tokens of 128 bytes are 2^31
+  int token_bytes, unit, units;
 };
 
 constexpr int kMaxStreams = 20, kDepth = 8;
@@ -212,7 +212,7 @@ struct MoveParams {
 template <typename U>
 __device__ __forceinline__ void move_stream(const EvictParams& p, const Stream& s, int r, int head, int layer) {
   const int32_t* kept = p.kept + (((int64_t)layer * p.rows + r) * p.hkv + head) * p.budget;
-  uint8_t* base = s.base + layer * s.layer_bytes + (int64_t)head * s.head_bytes;
+  uint8_t* base = s.base + layer * s.layer_bytes + head * s.head_bytes;
   const int shift = s.units == 4 ? 2 : s.units == 2 ? 1 : 0;  // 1, 2 or 4 lanes a token
   const int part = (threadIdx.x & (s.units - 1)) * (int)sizeof(U), tile = (256 >> shift) * kDepth;
   for (int i0 = 0; i0 < p.budget; i0 += tile) {
@@ -321,8 +321,9 @@ extern "C" int slo_evict_kv(const slo_evict_kv_args* a, slo_stream_t stream) {
     const int unit = row % 16 == 0 ? 16 : row % 4 == 0 ? 4 : 2, most = 4 * unit;
     for (int at = 0; at < row; at += most) {
       const int bytes = row - at < most ? row - at : most;
-      m.s[streams++] = Stream{static_cast<uint8_t*>(base) + at, page * a->num_blocks, page, by_head ? a->block_size * row : row,
-                              by_head ? row : a->num_kv_heads * row, unit, bytes / unit};
+      m.s[streams++] = Stream{static_cast<uint8_t*>(base) + at, page * a->num_blocks, page,
+                              by_head ? (int64_t)a->block_size * row : row, by_head ? row : a->num_kv_heads * row, unit,
+                              bytes / unit};
     }
   };
   const int row = a->kv_dtype == KV_BF16 ? 2 * a->head_dim : fp4 ? a->head_dim / 2 : a->head_dim;

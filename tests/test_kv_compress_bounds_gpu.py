@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import slo_attn
-from fp4_cases import Rows
+from fp4_cases import Rows, i32
 from test_fp4_gpu import CASES
 from test_kv_scores_gpu import expected
 
@@ -42,3 +42,25 @@ def test_weights_do_not_depend_on_the_bounds(device, fmt, name, bounds):
     slo_attn.accumulate_attention(case.q.to(device), kc, got, case.scale, num_kv_heads=case.hkv, k_scale=ks,
                                   **without_bounds(case, device), **bounds)
     assert torch.isfinite(got).all() and ((got.double().cpu() - want).abs() <= bound).all()
+
+
+def test_eviction_in_a_page_whose_heads_lie_2_gib_apart(device):
+    # one page of 2^24 tokens of a 4-bit pool with head_dim 256: a head's codes are 2^31 bytes
+    block, n, budget, recent = 1 << 24, 700, 300, 40
+    g = torch.Generator().manual_seed(3)
+    small = [torch.randint(0, 256, (1, 2, 768, w), generator=g, dtype=torch.uint8).to(device) for w in (128, 128, 8, 8)]
+    weights = torch.randint(0, 9, (1, 2, 768), generator=g).float().to(device)
+    big = [torch.zeros(1, 2, block, t.shape[-1], dtype=torch.uint8, device=device) for t in small]
+    scores = torch.zeros(1, 2, block, device=device)
+    scores[:, :, :768] = weights
+    for b, t in zip(big, small):
+        b[:, :, :768] = t
+    lens, table = i32([n], device), i32([[0]], device)
+    results = []
+    for (k, v, ks, vs), w in ((small, weights), (big, scores)):
+        k, v = (t.view(torch.float4_e2m1fn_x2) for t in (k, v))
+        results.append(slo_attn.evict_kv(k, v, w, lens, table, budget, recent, ks, vs))
+    assert torch.equal(results[0][1], results[1][1]) and results[1][0].tolist() == [budget]
+    for b, t in zip([*big, scores[..., None]], [*small, weights[..., None]]):
+        assert torch.equal(b[:, :, :768], t)
+        assert not b[:, :, 768:1 << 16].any() and not b[:, :, -(1 << 16):].any()

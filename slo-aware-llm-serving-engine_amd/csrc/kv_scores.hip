@@ -369,7 +369,9 @@ __device__ __forceinline__ void find_lse(const ScoreParams& p, const Row& g, int
     limit[n] = live ? min(g.prefix + tok + 1, g.lk) : 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) q[n][i] = load_q<KV>(p, g.q0 + tok, head * p.group + x % p.group, i, kg, live);
-    m[n] = kNone;
+    // A column of no query has scores of zero: from a reference of zero its
+    // weights of 1 do not look like a maximum that moved.
+    m[n] = live ? kNone : 0.0f;
     l[n] = 0.0f;
   }
   const int full = min(g.prefix + t0 + 1, g.lk);

@@ -64,3 +64,15 @@ def test_eviction_in_a_page_whose_heads_lie_2_gib_apart(device):
     for b, t in zip([*big, scores[..., None]], [*small, weights[..., None]]):
         assert torch.equal(b[:, :, :768], t)
         assert not b[:, :, 768:1 << 16].any() and not b[:, :, -(1 << 16):].any()
+
+
+@pytest.mark.parametrize("fmt,group", [("bf16", 3), ("fp8", 5), ("fp4", 6), ("bf16", 9), ("fp8", 11), ("fp4", 13), ("bf16", 15)])
+def test_weights_of_groups_that_leave_columns_empty(device, fmt, group):
+    # groups that do not divide a tile's 64 columns, and last tiles of few queries, over keys that every query sees
+    case = Rows(fmt, [], [(37, 300), (1, 129), (9, 0)], hq=2 * group, hkv=2, seed=group, gain=8.0)
+    kc, _, ks, _ = case.pool.device(device)
+    start = torch.zeros(case.blocks, 2, case.block)
+    want, bound = expected(case, start)
+    got = start.to(device)
+    slo_attn.accumulate_attention(case.q.to(device), kc, got, case.scale, num_kv_heads=2, k_scale=ks, **case.arguments(device))
+    assert torch.isfinite(got).all() and ((got.double().cpu() - want).abs() <= bound).all()

@@ -16,8 +16,9 @@ runner assigns uint8 / float8_e4m3fn ``k_cache`` / ``v_cache`` views; with
 float4_e2m1fn_x2 views they are the E8M0 scales of a 4-bit pool (``KVPool``
 allocates either).  An optional ``kv_scores`` attribute (fp32 ``[num_blocks,
 num_kv_heads, block_size]``) has every step add its attention weights to the
-scores of the cached tokens (``accumulate_attention``); all rows then need
-block tables.
+scores of the cached tokens (``accumulate_attention``, from the pool's keys).
+Prompts that come without block tables are whole: the slots that their tokens
+were written to say which pages they have.
 ``forward(q, k, v, kv_stored=True)`` skips the KV write, for callers whose
 ``qk_norm_rope_store`` already wrote this step's K/V into the pool.
 """
@@ -36,6 +37,16 @@ __all__ = ["Attention", "store_kvcache"]
 
 def _stored(*args):
     """store_fn for a step whose K/V are already in the pool."""
+
+
+def _pages_of_slots(slots: torch.Tensor, cu_k: torch.Tensor, max_k: int, block_size: int) -> torch.Tensor:
+    """Block tables int32 ``[rows, pages of max_k]``, -1 padded, of cold prefill rows: token j of row r went
+    to ``slots[cu_k[r] + j]``, and every ``block_size``-th token begins a page.  Without ``max_k`` the slots bound the rows."""
+    if not slots.numel():
+        return torch.full((cu_k.numel() - 1, 1), -1, dtype=torch.int32, device=cu_k.device)
+    first = torch.arange(0, max_k if max_k > 0 else slots.numel(), block_size, dtype=cu_k.dtype, device=cu_k.device) + cu_k[:-1, None]
+    slot = slots[first.clamp(max=slots.numel() - 1)]
+    return torch.where((first < cu_k[1:, None]) & (slot >= 0), slot // block_size, -1)
 
 
 class Attention(nn.Module):
@@ -64,7 +75,7 @@ class Attention(nn.Module):
                 self._weigh(q, num_decode=meta.num_decode, decode_lens=meta.decode_lens, decode_tables=meta.decode_tables,
                             num_prefill=meta.prefill_cu_q.numel() - 1 if meta.num_prefill_tokens else 0,
                             prefill_cu_q=meta.prefill_cu_q, prefill_cu_k=meta.prefill_cu_k, max_q=meta.max_q,
-                            max_k=meta.max_k, prefill_tables=meta.prefill_tables)
+                            max_k=meta.max_k, prefill_tables=meta.prefill_tables, slots=context.slot_mapping)
             return o
         have_cache = bool(k_cache.numel() and v_cache.numel())
         # The pool is written inside the attention launch (same result, one
@@ -98,7 +109,8 @@ class Attention(nn.Module):
                 phases=_lib.PHASE_ALL if paged else _lib.PHASE_ALL | _lib.NEW_ROWS_STRIDED, **store)
             if self.kv_scores is not None and have_cache:
                 self._weigh(q, num_prefill=rows, prefill_cu_q=context.cu_seqlens_q, prefill_cu_k=context.cu_seqlens_k,
-                            max_q=context.max_seqlen_q, max_k=context.max_seqlen_k, prefill_tables=context.block_tables)
+                            max_q=context.max_seqlen_q, max_k=context.max_seqlen_k, prefill_tables=context.block_tables,
+                            slots=context.slot_mapping)
             return o
         o = paged_attention(
             q, k_cache, v_cache, self.scale, num_kv_heads=self.num_kv_heads,
@@ -109,7 +121,10 @@ class Attention(nn.Module):
             self._weigh(q, num_decode=q.shape[0], decode_lens=context.context_lens, decode_tables=context.block_tables)
         return o.unsqueeze(1)
 
-    def _weigh(self, q, **rows):
-        """The step's attention weights into ``kv_scores``."""
+    def _weigh(self, q, slots=None, **rows):
+        """The step's attention weights into ``kv_scores``; ``slots`` are the new tokens', decode rows first."""
+        if rows.get("num_prefill") and rows["prefill_tables"] is None and slots is not None:
+            rows["prefill_tables"] = _pages_of_slots(slots[rows.get("num_decode", 0):], rows["prefill_cu_k"], rows["max_k"],
+                                                     self.kv_scores.shape[2])
         accumulate_attention(q, self.k_cache, self.kv_scores, self.scale, num_kv_heads=self.num_kv_heads,
                              k_scale=self.k_scale, **rows)

@@ -3,8 +3,10 @@ the C entries size and refuse."""
 import ctypes
 
 import pytest
+import torch
 
 from slo_attn import _lib
+from slo_attn.attention import _pages_of_slots
 from test_kv_compress_host import attention_args
 
 
@@ -48,3 +50,23 @@ def test_4_bit_prefill_steps_stay_in_32_bits(heads, kv_heads, rows, most):
             assert lib.slo_paged_attention_fp4(bytes(a), None) == 4 and b"2^30" in lib.slo_last_error()
     # a captured step's capacities are far below
     assert lib.slo_paged_attention_fp4_workspace_bytes(bytes(prefill_args(65536, 1024, 640)), ctypes.byref(need)) == 0
+
+
+@pytest.mark.parametrize("lens,block", [([1], 64), ([130, 0, 64, 65], 64), ([300, 17], 128), ([0, 0], 64)])
+def test_pages_of_a_cold_prompts_slots(lens, block):
+    pages = [-(-n // block) for n in lens]
+    order, tables = list(range(40))[::-1], []
+    width = max(pages + [1])
+    for n in pages:
+        tables.append([order.pop(0) for _ in range(n)] + [-1] * (width - n))
+    slots = torch.tensor([t[j // block] * block + j % block for t, n in zip(tables, lens) for j in range(n)], dtype=torch.int32)
+    cu_k = torch.tensor([0] + [sum(lens[:i + 1]) for i in range(len(lens))], dtype=torch.int32)
+    got = _pages_of_slots(slots, cu_k, max(lens), block)
+    assert got.dtype == torch.int32 and got.tolist() == tables
+    # tokens that were not stored are in no page; padding behind the last row is no row's
+    if slots.numel():
+        padded = torch.cat((torch.full_like(slots, -1), slots))
+        assert (_pages_of_slots(padded[:slots.numel()], cu_k, max(lens), block) == -1).all()
+        assert _pages_of_slots(torch.cat((slots, slots)), cu_k, max(lens), block).tolist() == tables
+        unbounded = _pages_of_slots(slots, cu_k, 0, block)
+        assert unbounded[:, :width].tolist() == tables and (unbounded[:, width:] == -1).all()

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import slo_attn
-from fp4_cases import Rows, i32
+from fp4_cases import D, Rows, i32, random_values
 from test_fp4_gpu import CASES
 from test_kv_scores_gpu import expected
 
@@ -76,3 +76,44 @@ def test_weights_of_groups_that_leave_columns_empty(device, fmt, group):
     got = start.to(device)
     slo_attn.accumulate_attention(case.q.to(device), kc, got, case.scale, num_kv_heads=2, k_scale=ks, **case.arguments(device))
     assert torch.isfinite(got).all() and ((got.double().cpu() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("mixed", [False, True], ids=["v0", "mixed"])
+@pytest.mark.parametrize("fmt", ["bf16", "fp8_e4m3fn", "fp4_e2m1"])
+def test_cold_prompts_without_tables_are_weighed(device, fmt, mixed):
+    # whole prompts attend to their new rows; their weights go to the pages that their slots say
+    hq, hkv, block, lens = 8, 2, 64, [130, 1, 64]
+    tables = [[4, 0, 7], [2, -1, -1], [5, -1, -1]]
+    pool = slo_attn.KVPool(1, 9, block, hkv, D, fmt, device, track_scores=True)
+    layer = slo_attn.Attention(hq, D, D ** -0.5, hkv)
+    pool.attach([layer])
+    pool.kv.zero_()
+    pool.scores.fill_(50.0)
+    g = torch.Generator().manual_seed(6)
+    n = sum(lens) + mixed
+    q, k, v = (random_values(g, n, h, D).to(device) for h in (hq, hkv, hkv))
+    slots = [t[j // block] * block + j % block for t, m in zip(tables, lens) for j in range(m)]
+    cu = i32([0, 130, 131, 195], device)
+    if mixed:  # a decode row's first token beside them, in block 8
+        meta = slo_attn.MixedAttentionContext(1, n - 1, i32([1], device), i32([[8]], device), cu, cu, None, 130, 130, False)
+        slo_attn.set_context(False, slot_mapping=i32([8 * block] + slots, device), mixed=meta)
+    else:
+        slo_attn.set_context(True, cu, cu, 130, 130, i32(slots, device), None, None)
+    out = layer(q, k, v)
+    slo_attn.reset_context()
+    got = pool.scores[0].clone()
+    # the same call with the tables written out
+    kc, _, ks, _ = pool.layer(0)
+    want = torch.full_like(got, 50.0)
+    slo_attn.accumulate_attention(q[mixed:], kc, want, D ** -0.5, num_kv_heads=hkv, k_scale=ks, num_prefill=3, prefill_cu_q=cu,
+                                  prefill_cu_k=cu, max_q=130, max_k=130, prefill_tables=i32(tables, device))
+    if mixed:
+        want[8, :, 0] = 4.0  # the only key of the group's four heads
+        got[8, :, 0] = got[8, :, 0].round(decimals=5)
+    assert torch.equal(got, want)
+    for t, m in zip(tables, lens):
+        row = torch.stack([got[t[j // block], :, j % block] for j in range(m)])
+        assert torch.allclose(row.sum(0), torch.full((hkv,), 4.0 * m, device=device), rtol=1e-4)
+    alone = slo_attn.paged_attention(q[mixed:], None, None, D ** -0.5, num_kv_heads=hkv, num_prefill=3, prefill_cu_q=cu,
+                                     prefill_cu_k=cu, max_q=130, max_k=130, k=k[mixed:], v=v[mixed:])
+    assert torch.equal(out[mixed:], alone)

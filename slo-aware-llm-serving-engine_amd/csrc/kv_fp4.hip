@@ -29,8 +29,9 @@ __device__ __forceinline__ Unit unit_of(int u, int hkv, int shift, int tokens) {
 // Slot-mapped write into a 4-bit pool (format and scale rule: fp4.h): 16 bytes
 // a lane in, the group's largest magnitude over 4 lanes by DPP, 4 code bytes
 // out; the first of the 4 lanes writes the scale byte.  Bound by the round trip
-// to memory at a decode step's size (24 tokens of 8 heads 2.9 us) and by HBM
-// above a few thousand tokens (4,096 tokens, 21 MB, 7.4 us).
+// to memory at a decode step's size (24 tokens of 8 heads 2.9 us) and still by
+// two of them at a prompt's (4,096 tokens, 21 MB, 7.4 us or 2.9 TB/s; 262,144
+// tokens, 1.36 GB, 267 us or 5.1 TB/s).
 template <int TOK, int DEPTH>
 __global__ void __launch_bounds__(256)
 store_fp4_kernel(const uint16_t* __restrict__ key, int64_t key_stride, const uint16_t* __restrict__ value,
@@ -67,7 +68,7 @@ store_fp4_kernel(const uint16_t* __restrict__ key, int64_t key_stride, const uin
 
 // Cached tokens as bf16 rows.  E4M3FN values are code * scale in fp32, rounded
 // once; 4-bit values are exact.  A slot outside the pool gives zeros.
-template <int KV, int TOK, int DEPTH>
+template <int KV, int TOK, int DEPTH, bool NT>
 __global__ void __launch_bounds__(256)
 load_kv_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v_cache,
                const void* __restrict__ k_scale, const void* __restrict__ v_scale,
@@ -121,7 +122,7 @@ load_kv_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ 
         }
       }
       u32x4* to = reinterpret_cast<u32x4*>(t.is_v ? v_out : k_out) + ((((int64_t)t.token * hkv + t.head) << shift) + t.j);
-      if constexpr (TOK > 1)
+      if constexpr (NT)
         __builtin_nontemporal_store(o, to);
       else
         *to = o;
@@ -129,13 +130,39 @@ load_kv_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ 
   }
 }
 
-// Four tokens a workgroup, and four loads a lane in flight, from here on: the
-// read back of 262,144 tokens of 8 heads takes 347 us so and 376 us with one
-// token a workgroup, that of 4,096 tokens 8.7 and 7.0 us.  What such a read back
-// writes is larger than the caches, so it is stored past them: 338 us, and what
-// the next kernel finds there is not displaced (a move of 16 rows in the pool
-// that was read back before takes 160 us instead of 184).
-constexpr int kManyTokens = 16384;
+// Four tokens a workgroup, and four loads a lane in flight, from 16,384 tokens
+// on where one token leaves lanes of a workgroup idle or, packed, just fills it;
+// with more heads a token's workgroup has loads enough, and bf16's are four
+// times a code's.  us with one token / with four, at head_dim 128:
+//   store       8 heads: 16,384 tokens 18.2 / 18.4, 65,536 78 / 65, 262,144
+//               302 / 267; 1 head 65,536 34 / 24; 16 heads 65,536 137 / 137
+//   read back   4 bits, 8 heads: 16,384 17.1 / 17.0, 262,144 408 / 335; 1 head
+//               65,536 23 / 14; 16 heads 65,536 165 / 173
+//               E4M3FN, 8 heads: 262,144 324 / 291; 16 heads 65,536 142 / 155
+//               bf16, 4 heads: 131,072 104 / 95; 8 heads 262,144 355 / 379
+// A grid holds less than 2^32 threads, so from 2^24 tokens on there are always
+// four.
+constexpr int kManyTokens = 16384, kMostSingle = 1 << 24;
+
+static bool four_tokens(int tokens, int64_t lanes, bool bf16) {
+  return tokens >= kMostSingle || (tokens >= kManyTokens && lanes <= (bf16 ? 128 : 256));
+}
+
+// A read back that writes 256 MiB and more, the size of the last-level cache,
+// passes it by: little of it would be found there by what reads it next, and the
+// pool would be displaced.  us of a read back and a copy of what it wrote, through the
+// cache / past it, 8 heads of 4 bits: 67 MB 37 / 43, 134 MB 82 / 84, 268 MB 195
+// / 184, 1,074 MB 745 / 725; E4M3FN 37 / 42, 81 / 87, 184 / 178, 696 / 687.  bf16
+// reads as much as it writes and gains nothing: 200 / 204 and 781 / 795.
+constexpr int64_t kPastCache = 256ll << 20;
+
+template <int KV>
+static auto* load_kernel(bool four, bool past) {
+  if constexpr (KV != KV_BF16) {
+    if (four && past) return load_kv_kernel<KV, 4, 4, true>;
+  }
+  return four ? load_kv_kernel<KV, 4, 4, false> : load_kv_kernel<KV, 1, 1, false>;
+}
 
 }  // namespace slo
 
@@ -165,8 +192,8 @@ extern "C" int slo_store_kvcache_fp4(const void* key, int64_t key_row_stride, co
   const int64_t per = 2 * (int64_t)num_kv_heads * (head_dim / 8);
   if (per > 65536) return fail(SLO_ERR_UNSUPPORTED, "store_kvcache_fp4: too many heads");
   const int shift = head_dim == 64 ? 3 : head_dim == 128 ? 4 : 5;
-  const bool many = num_tokens >= kManyTokens;
-  hipLaunchKernelGGL((many ? store_fp4_kernel<4, 4> : store_fp4_kernel<1, 1>), dim3(many ? (num_tokens + 3) / 4 : num_tokens),
+  const bool four = four_tokens(num_tokens, per, false);
+  hipLaunchKernelGGL((four ? store_fp4_kernel<4, 4> : store_fp4_kernel<1, 1>), dim3(four ? (num_tokens + 3) / 4 : num_tokens),
                      dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<const uint16_t*>(key), key_row_stride,
                      static_cast<const uint16_t*>(value), value_row_stride, slot_mapping, num_tokens, num_kv_heads, shift,
                      static_cast<uint8_t*>(k_cache), static_cast<uint8_t*>(v_cache), static_cast<uint8_t*>(k_scale),
@@ -192,11 +219,11 @@ extern "C" int slo_load_kvcache(const void* k_cache, const void* v_cache, const 
   const int64_t per = 2 * (int64_t)num_kv_heads * (head_dim / 8);
   if (per > 65536) return fail(SLO_ERR_UNSUPPORTED, "load_kvcache: too many heads");
   const int shift = head_dim == 64 ? 3 : head_dim == 128 ? 4 : 5;
-  const bool many = num_tokens >= kManyTokens;
-  auto* kernel = kv_dtype == KV_BF16         ? (many ? load_kv_kernel<KV_BF16, 4, 4> : load_kv_kernel<KV_BF16, 1, 1>)
-                 : kv_dtype == KV_FP8_E4M3FN ? (many ? load_kv_kernel<KV_FP8_E4M3FN, 4, 4> : load_kv_kernel<KV_FP8_E4M3FN, 1, 1>)
-                                             : (many ? load_kv_kernel<KV_FP4_E2M1, 4, 4> : load_kv_kernel<KV_FP4_E2M1, 1, 1>);
-  hipLaunchKernelGGL(kernel, dim3(many ? (num_tokens + 3) / 4 : num_tokens), dim3(256), 0, static_cast<hipStream_t>(stream),
+  const bool four = four_tokens(num_tokens, per, kv_dtype == KV_BF16), past = 16 * per * num_tokens >= kPastCache;
+  auto* kernel = kv_dtype == KV_BF16         ? load_kernel<KV_BF16>(four, past)
+                 : kv_dtype == KV_FP8_E4M3FN ? load_kernel<KV_FP8_E4M3FN>(four, past)
+                                             : load_kernel<KV_FP4_E2M1>(four, past);
+  hipLaunchKernelGGL(kernel, dim3(four ? (num_tokens + 3) / 4 : num_tokens), dim3(256), 0, static_cast<hipStream_t>(stream),
                      static_cast<const uint8_t*>(k_cache), static_cast<const uint8_t*>(v_cache), k_scale, v_scale, slot_mapping,
                      num_tokens, num_kv_heads, shift, (int64_t)num_blocks * block_size, block_size,
                      static_cast<uint16_t*>(k_out), static_cast<uint16_t*>(v_out));

@@ -368,9 +368,10 @@ int slo_paged_attention_fp4(const slo_paged_attention_args* args, slo_stream_t s
  * size the launches (0: the queries and the tables' width do), never the
  * result.  softmax_scale may not be zero; at most 32,768 rows of either kind, 2^21 tokens a row and 2^17
  * queries a prefill row.
- * Workspace as for slo_paged_attention_fp4; rows whose tables span more than
- * 16,384 / (num_heads / num_kv_heads) tokens need 4 bytes per (decode row,
- * query head, token of the tables' width).
+ * Workspace as for slo_paged_attention_fp4; decode rows whose tables span more
+ * than 16,384 / (num_heads / num_kv_heads) tokens, or 512 KiB of K of a kv head
+ * where the rows times kv heads are fewer than 256, need 4 bytes per (decode
+ * row, query head, token of the tables' width).
  */
 int slo_accumulate_attention_workspace_bytes(const slo_paged_attention_args* args, size_t* bytes);
 int slo_accumulate_attention(const slo_paged_attention_args* args, float* scores, slo_stream_t stream);

@@ -219,12 +219,21 @@ __device__ __forceinline__ float2 column_lse(float2 e) {
   return float2{m, col_sum(e.y * __builtin_amdgcn_exp2f(e.x - m))};
 }
 
-// Decode rows whose logits fit LDS: a workgroup takes a (row, kv head) whole,
+// Decode rows whose logits fit LDS (by the tables' width, as a captured launch
+// knows no more): a workgroup takes a (row, kv head) whole,
 // so one launch does, and K is all that moves.  64 rows of 512-4,096 tokens of
 // a 4-bit pool, 8 kv heads (86 MB of K): 30 us, against 37 and 11 in two
 // launches through memory; 25 without the adds to the scores, 23 without the
 // second half.
 constexpr int kRowLogits = 16384;
+// With fewer (row, kv head) pairs than CUs, rows of 512 KiB of K and more take
+// the two launches: a workgroup a pair reads too slowly.  us whole / in two, one
+// row and 16 of them, 8 kv heads: bf16, 1,024 tokens 12.2 / 15.6 and 13.7 / 16.0,
+// 2,048 18.7 / 15.7 and 21.9 / 20.9, 16,384 (group 1) 120 / 16 and 168 / 142;
+// E4M3FN, 2,048 13.6 / 16.3 and 16.8 / 17.7, 4,096 22.3 / 16.2 and 28.3 / 27.5;
+// 4 bits, 4,096 14.4 / 17.5 and 20.0 / 21.5, 8,192 23.3 / 17.2 and 34.8 / 32.8.
+// 64 rows of 2,048-4,096 tokens fill the CUs: bf16 113 / 154, 4 bits 46 / 65.
+constexpr int kFullGroups = 256, kLongRow = 512 << 10;
 
 template <int KV, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, 4)
@@ -670,7 +679,8 @@ Plan plan_of(const slo_paged_attention_args* a) {
   Plan n = {false, 1, 1 << 30, 0, 0, 0, 0};
   if (a->num_decode > 0 && (a->phases & SLO_PHASE_DECODE)) {
     const int64_t cap = (int64_t)a->decode_table_width * a->block_size, groups = (int64_t)a->num_decode * a->num_kv_heads;
-    n.whole = cap * (a->num_heads / a->num_kv_heads) <= kRowLogits;
+    const int64_t row = cap * (a->kv_dtype == KV_BF16 ? 256 : a->kv_dtype == KV_FP8_E4M3FN ? 128 : 64);
+    n.whole = cap * (a->num_heads / a->num_kv_heads) <= kRowLogits && (groups >= kFullGroups || row < kLongRow);
     const int64_t want = (2048 + groups - 1) / groups;
     int64_t c = ((cap + want - 1) / want + 127) / 128 * 128;
     if (c < 256) c = 256;

@@ -70,3 +70,19 @@ def test_pages_of_a_cold_prompts_slots(lens, block):
         assert _pages_of_slots(torch.cat((slots, slots)), cu_k, max(lens), block).tolist() == tables
         unbounded = _pages_of_slots(slots, cu_k, 0, block)
         assert unbounded[:, :width].tolist() == tables and (unbounded[:, width:] == -1).all()
+
+
+@pytest.mark.parametrize("kv_dtype,row_bytes", [(0, 256), (1, 128), (2, 64)])
+def test_few_long_decode_rows_are_cut(kv_dtype, row_bytes):
+    # one launch and no workspace below 512 KiB of K a (row, kv head), or where these fill the CUs
+    call = _lib.load().slo_accumulate_attention_workspace_bytes
+
+    def need(rows, tokens):
+        return workspace(call, attention_args(num_decode=rows, num_q_rows=rows, decode_table_width=tokens // 64, block_size=64,
+                                              num_heads=8, q_row_stride=8 * 128, kv_dtype=kv_dtype))
+
+    long = (512 << 10) // row_bytes
+    assert need(1, long - 64) == 0 and need(31, long - 64) == 0 and need(32, long) == 0 and need(32, 16384) == 0
+    for rows in (1, 31):
+        assert need(rows, long) >= rows * 8 * long * 4
+    assert need(32, 16384 + 64) > 0

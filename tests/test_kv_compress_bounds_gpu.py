@@ -117,3 +117,15 @@ def test_cold_prompts_without_tables_are_weighed(device, fmt, mixed):
     alone = slo_attn.paged_attention(q[mixed:], None, None, D ** -0.5, num_kv_heads=hkv, num_prefill=3, prefill_cu_q=cu,
                                      prefill_cu_k=cu, max_q=130, max_k=130, k=k[mixed:], v=v[mixed:])
     assert torch.equal(out[mixed:], alone)
+
+
+@pytest.mark.parametrize("fmt,lens,hq,hkv,width", [("bf16", [2047, 5], 2, 2, 33), ("bf16", [1983], 2, 2, 31), ("fp8", [4100, 0, 64], 4, 4, 65),
+                                                   ("fp4", [8200], 1, 1, 129), ("fp4", [8000, 9], 2, 1, 126)])
+def test_few_long_decode_rows(device, fmt, lens, hq, hkv, width):
+    case = Rows(fmt, lens, hq=hq, hkv=hkv, seed=width, gain=3.0, spare=width - max(-(-n // 64) for n in lens))
+    kc, _, ks, _ = case.pool.device(device)
+    start = torch.rand(case.blocks, hkv, case.block, generator=torch.Generator().manual_seed(2))
+    want, bound = expected(case, start)
+    got = start.to(device)
+    slo_attn.accumulate_attention(case.q.to(device), kc, got, case.scale, num_kv_heads=hkv, k_scale=ks, **case.arguments(device))
+    assert torch.isfinite(got).all() and ((got.double().cpu() - want).abs() <= bound).all()

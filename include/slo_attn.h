@@ -338,16 +338,17 @@ int slo_load_kvcache(const void* k_cache, const void* v_cache, const void* k_sca
  * slo_paged_attention over a 4-bit pool: the same arguments (k_scale / v_scale
  * point to E8M0 bytes, kv_dtype is SLO_KV_FP4_E2M1) and the same rows, masks
  * and outputs; a row without keys gives zeros, and so do query rows past every
- * row's.  max_q is not read and max_k may be 0 (it sizes the launch, never the
- * result).  At most 32,768 decode and 1,024 prefill rows; tables of up to 2^22
- * tokens; (prefill queries / (4 * floor(32 / (num_heads / num_kv_heads))) +
- * prefill rows) * the tables' tokens / 64 at most 2^30 (2^19 queries of four
- * heads a kv head with the widest tables).  Prefill rows are read through
- * prefill_tables (without tables they read no pool: slo_paged_attention takes
- * them); store_slot_mapping must be NULL and softmax_scale not zero.  The
- * workspace (16-byte aligned, slo_paged_attention_fp4_workspace_bytes of the
- * same arguments; it need not be cleared and holds nothing between calls) may
- * not be used by two calls that overlap.
+ * row's (a call without rows of its phases writes nothing).  max_q is not read
+ * and max_k may be 0 (it sizes the launch, never the result).  At most 32,768
+ * decode and 1,024 prefill rows; tables of up to 2^22 tokens; (prefill queries
+ * / (4 * floor(32 / (num_heads / num_kv_heads))) + prefill rows) * the tables'
+ * tokens / 64 at most 2^30 (2^19 queries of four heads a kv head with the
+ * widest tables).  Prefill rows are read through prefill_tables (without tables
+ * they read no pool: slo_paged_attention takes them); store_slot_mapping must
+ * be NULL and softmax_scale not zero.  The workspace (16-byte aligned,
+ * slo_paged_attention_fp4_workspace_bytes of the same arguments; it need not be
+ * cleared and holds nothing between calls) may not be used by two calls that
+ * overlap.
  */
 int slo_paged_attention_fp4_workspace_bytes(const slo_paged_attention_args* args, size_t* bytes);
 int slo_paged_attention_fp4(const slo_paged_attention_args* args, slo_stream_t stream);

@@ -665,18 +665,19 @@ score_prefill_kernel(ScoreParams p) {
 }
 
 constexpr int kLseNT = 4;
-constexpr int kMostQueries = 1 << 17;  // of a row
+constexpr int kMostQueries = 1 << 17;  // of a row, where max_q is given
+constexpr int kUnbounded = 1 << 15;
 
 struct Plan {
   bool whole;  // decode rows in one launch
-  int splits, chunk, tiles;
+  int splits, chunk, tiles, keys;
   size_t logits, partial, lse;
 };
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 Plan plan_of(const slo_paged_attention_args* a) {
-  Plan n = {false, 1, 1 << 30, 0, 0, 0, 0};
+  Plan n = {false, 1, 1 << 30, 0, 0, 0, 0, 0};
   if (a->num_decode > 0 && (a->phases & SLO_PHASE_DECODE)) {
     const int64_t cap = (int64_t)a->decode_table_width * a->block_size, groups = (int64_t)a->num_decode * a->num_kv_heads;
     const int64_t row = cap * (a->kv_dtype == KV_BF16 ? 256 : a->kv_dtype == KV_FP8_E4M3FN ? 128 : 64);
@@ -691,11 +692,16 @@ Plan plan_of(const slo_paged_attention_args* a) {
   }
   if (a->num_prefill > 0 && (a->phases & SLO_PHASE_PREFILL) && a->num_q_rows > a->num_decode) {
     // max_q and max_k size the two launches, whose workgroups go round where a
-    // row is longer; without them the queries and the tables bound the rows.
-    const int per = 16 * kLseNT / (a->num_heads / a->num_kv_heads);
-    const int all = a->num_q_rows - a->num_decode, most = a->max_q > 0 && a->max_q < all ? a->max_q : all;
-    n.tiles = ((most < kMostQueries ? most : kMostQueries) + per - 1) / per;
-    n.lse = up256((size_t)(a->num_q_rows - a->num_decode) * a->num_heads * 4);
+    // row is longer.  Without them the queries and the tables' width bound a row,
+    // and a launch has kUnbounded workgroups or 16 a (row, kv head).
+    const int per = 16 * kLseNT / (a->num_heads / a->num_kv_heads), all = a->num_q_rows - a->num_decode;
+    const int64_t pairs = (int64_t)a->num_prefill * a->num_kv_heads, few = kUnbounded / pairs > 16 ? kUnbounded / pairs : 16;
+    const int64_t cap = (int64_t)a->prefill_table_width * a->block_size / kSumKeys;
+    const int64_t tiles = ((a->max_q > 0 && a->max_q < all ? a->max_q : all) + per - 1) / per;
+    const int64_t keys = a->max_k > 0 ? ((int64_t)a->max_k + kSumKeys - 1) / kSumKeys : few;
+    n.tiles = (int)(a->max_q > 0 || tiles < few ? tiles : few);
+    n.keys = (int)(keys < cap ? keys : cap);
+    n.lse = up256((size_t)all * a->num_heads * 4);
   }
   return n;
 }
@@ -751,10 +757,7 @@ void launch(const ScoreParams& d, const ScoreParams& f, const slo_paged_attentio
   }
   if (n.tiles) {
     hipLaunchKernelGGL((score_lse_kernel<KV, kLseNT>), dim3(f.hkv, n.tiles, a->num_prefill), dim3(256), 0, s, f, n.tiles);
-    const int64_t most = (int64_t)f.table_width * f.block_size;
-    const int64_t keys = a->max_k > 0 ? ((int64_t)a->max_k + 63) / 64 * 64 : most;
-    const int cap = (int)(most < keys ? most : keys);
-    hipLaunchKernelGGL(score_prefill_kernel<KV>, dim3(f.hkv, cap / kSumKeys, a->num_prefill), dim3(64 * kSumWaves), 0, s, f);
+    hipLaunchKernelGGL(score_prefill_kernel<KV>, dim3(f.hkv, n.keys, a->num_prefill), dim3(64 * kSumWaves), 0, s, f);
   }
 }
 

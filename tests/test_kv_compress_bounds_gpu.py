@@ -66,6 +66,17 @@ def test_eviction_in_a_page_whose_heads_lie_2_gib_apart(device):
         assert not b[:, :, 768:1 << 16].any() and not b[:, :, -(1 << 16):].any()
 
 
+def test_weights_of_many_rows_without_bounds(device):
+    # 1,102 rows in tables of 41 pages: 29 workgroups a row, which go round the longest one's keys
+    case = Rows("fp4", [], [(300, 2200), (1, 5)] + [(1 + i % 2, i % 7) for i in range(1100)], hq=2, hkv=1, seed=8, block=64)
+    kc, _, ks, _ = case.pool.device(device)
+    args, start = case.arguments(device), torch.zeros(case.blocks, 1, case.block, device=device)
+    given = start.clone()
+    slo_attn.accumulate_attention(case.q.to(device), kc, given, case.scale, num_kv_heads=1, k_scale=ks, **args)
+    slo_attn.accumulate_attention(case.q.to(device), kc, start, case.scale, num_kv_heads=1, k_scale=ks, **without_bounds(case, device))
+    assert torch.equal(given, start) and given.sum().item() == pytest.approx(2 * case.tokens, rel=1e-4)
+
+
 @pytest.mark.parametrize("fmt,group", [("bf16", 3), ("fp8", 5), ("fp4", 6), ("bf16", 9), ("fp8", 11), ("fp4", 13), ("bf16", 15)])
 def test_weights_of_groups_that_leave_columns_empty(device, fmt, group):
     # groups that do not divide a tile's 64 columns, and last tiles of few queries, over keys that every query sees

@@ -18,6 +18,10 @@
 // turn channel pairs into token pairs.  Probabilities are rounded to bf16 and
 // their sum is taken of the rounded values (one more row of the second
 // product, of ones), so a weight's rounding cancels where one key dominates.
+// The rounding is the matrix operand's, and that of the attention over the other
+// pools: outputs are off by 0.0020-0.0023 of their size where 32-bit
+// probabilities leave 0.0016-0.0017, the rounding of the output alone; a second
+// operand with what was rounded off would double the second product.
 // Sums, maxima and outputs are fp32 until the one rounding at the end.
 #include "capi_internal.h"
 #include "fp4.h"
@@ -145,8 +149,9 @@ __device__ __forceinline__ bool find_chunk(const Fp4Params& p, int i, bool by_ro
 }
 
 // A decode wavefront's steps arrive in LDS by DMA, kDepth in flight.  Codes
-// land as their lanes fetch them, so the lanes fetch in an order that lets both
-// operands be read without a bank conflict: of K, 16-byte part p of token t
+// land as their lanes fetch them, so the lanes fetch in an order that spreads
+// both operands' reads over the banks (of about 47 LDS cycles a step 9 are
+// conflicts; the other conflicts are where the wavefronts meet): of K, 16-byte part p of token t
 // lies at part p ^ (t / 4 mod 4) of its place; of V, token t lies at place
 // t ^ (t / 4 mod 4).  Both stay within the 256 bytes of four tokens, so a
 // fetch still takes whole lines.
@@ -353,6 +358,7 @@ __device__ __forceinline__ void clear(Acc<NT>& a) {
 // tokens and 8 kv heads, 172 MB, 36.5 us or 4.7 TB/s (31.5 us with the
 // arithmetic left out, 39.4 with the default cache policy).  With chunks of
 // another rule, steps in registers instead of LDS took 53 us where LDS took 40.
+// 172.6 MB are fetched for 170.9 of codes and scales.
 template <int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, 4)
 fp4_decode_kernel(Fp4Params p) {
@@ -463,7 +469,8 @@ fp4_decode_kernel(Fp4Params p) {
 
 // One 64-token step of a workgroup as bf16 operands in LDS, in the order in
 // which lanes read them (16 bytes a lane, no bank twice): K's four operands of
-// each 16 tokens, V's eight of each 32 tokens.
+// each 16 tokens, V's eight of each 32 tokens.  Half a V operand is written at a
+// time, two lanes to a bank: 32 of a step's 226 LDS cycles.
 struct Stage {
   u32x4 k[4][4][64], v[2][8][64];
 };
@@ -921,8 +928,11 @@ constexpr int kPrefillShares = 512;
 // and 5.1 us to join them, 38.1 + 6.6 with twice as many, 42.1 + 6.8 with four
 // times; three rows of 20,000-60,000 30.2 + 4.2, 32.1 + 5.8, 35.9 + 7.2.
 constexpr int kDecodeChunks = 1024;
-// Rows of at most this many tokens are not cut, and eight wavefronts take each:
-// one row of 1,000 6.7 us, 5.4 + 4.4 us as two chunks and their join.
+// Where the tables span at most this many tokens rows are not cut, and eight
+// wavefronts take each: one row of 1,000 6.7 us, 5.4 + 4.4 us as two chunks and
+// their join.  The launch knows the tables' width only, so in wider tables (a
+// captured step's) such a row is cut into chunks of 256 tokens and more and
+// joined: 20.9 us a call in tables of 4,096 and of 40,960 tokens, 15.9 in 1,024.
 constexpr int kWholeRow = 1024;
 
 struct Plan {

@@ -205,10 +205,11 @@ struct MoveParams {
 // streams, so each keeps kDepth loads a lane in flight (a tile is 512 tokens of
 // 64 bytes).  One row cut from 1,500 to 1,024 bf16 tokens: 8.8 us (10.6 with
 // four in flight, 39 with four and whole rows); 16 rows to 2,048 tokens in 8
-// layers of a 4-bit pool: 161 us for 0.57 GB, 3.5 TB/s; the
-// counters show 0.25 GB read and 0.31 written, so no line is read in vain.  (When
-// read backs were stored through the caches: 184, 213 with four in flight, 199
-// with four and twice the lanes, 6.7 there for the one row.)
+// layers of a 4-bit pool: 161 us for 0.57 GB, 3.5 TB/s.  What it moves is 0.81
+// GB, 5.0 TB/s: 0.31 GB are written, but 0.50 GB read for 0.29, in lines of 128
+// bytes, as the 64-byte rows that stay lie one or two to a line.  (When read
+// backs were stored through the caches: 184, 213 with four in flight, 199 with
+// four and twice the lanes, 6.7 there for the one row.)
 template <typename U>
 __device__ __forceinline__ void move_stream(const EvictParams& p, const Stream& s, int r, int head, int layer) {
   const int32_t* kept = p.kept + (((int64_t)layer * p.rows + r) * p.hkv + head) * p.budget;

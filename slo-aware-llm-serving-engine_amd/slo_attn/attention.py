@@ -40,8 +40,11 @@ def _stored(*args):
 
 
 def _pages_of_slots(slots: torch.Tensor, cu_k: torch.Tensor, max_k: int, block_size: int) -> torch.Tensor:
-    """Block tables int32 ``[rows, pages of max_k]``, -1 padded, of cold prefill rows: token j of row r went
-    to ``slots[cu_k[r] + j]``, and every ``block_size``-th token begins a page.  Without ``max_k`` the slots bound the rows."""
+    """Block tables int32 ``[rows, pages of max_k]``, -1 padded, of cold prefill rows.
+
+    Token j of row r went to ``slots[cu_k[r] + j]``, and every ``block_size``-th
+    token begins a page.  Without ``max_k`` the slots bound the rows.
+    """
     if not slots.numel():
         return torch.full((cu_k.numel() - 1, 1), -1, dtype=torch.int32, device=cu_k.device)
     first = torch.arange(0, max_k if max_k > 0 else slots.numel(), block_size, dtype=cu_k.dtype, device=cu_k.device) + cu_k[:-1, None]

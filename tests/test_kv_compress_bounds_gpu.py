@@ -140,3 +140,43 @@ def test_few_long_decode_rows(device, fmt, lens, hq, hkv, width):
     got = start.to(device)
     slo_attn.accumulate_attention(case.q.to(device), kc, got, case.scale, num_kv_heads=hkv, k_scale=ks, **case.arguments(device))
     assert torch.isfinite(got).all() and ((got.double().cpu() - want).abs() <= bound).all()
+
+
+def test_captured_cold_prompts_are_weighed_on_every_replay(device):
+    # the pages come from the slots inside the graph: a replay goes where the slots then say
+    hq, hkv, block, lens = 8, 2, 64, [70, 33]
+    pool = slo_attn.KVPool(1, 6, block, hkv, D, "bf16", device, track_scores=True)
+    layer = slo_attn.Attention(hq, D, D ** -0.5, hkv)
+    pool.attach([layer])
+    pool.kv.zero_()
+    g = torch.Generator().manual_seed(9)
+    q, k, v = (random_values(g, sum(lens), h, D).to(device) for h in (hq, hkv, hkv))
+    cu, slots = i32([0, 70, 103], device), torch.full((sum(lens),), -1, dtype=torch.int32, device=device)
+
+    def step():
+        slo_attn.set_context(True, cu, cu, 70, 70, slots, None, None)
+        try:
+            return layer(q, k, v)
+        finally:
+            slo_attn.reset_context()
+
+    step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        captured = step()
+    for tables in ([[0, 3], [5]], [[4, 1], [2]], [[0, 3], [5]]):
+        slots.copy_(i32([t[j // block] * block + j % block for t, n in zip(tables, lens) for j in range(n)], device))
+        pool.scores.fill_(9.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = captured.clone(), pool.scores.clone()
+        pool.scores.fill_(9.0)
+        want = step()
+        assert torch.equal(got[0], want) and torch.equal(got[1], pool.scores)
+        live = torch.zeros_like(got[1], dtype=torch.bool)
+        for t, n in zip(tables, lens):
+            for j in range(n):
+                live[0, t[j // block], :, j % block] = True
+        assert (got[1][~live] == 9).all() and got[1][live].sum().item() == pytest.approx(hq * sum(lens), rel=1e-4)

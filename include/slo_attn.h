@@ -109,6 +109,24 @@ int slo_qk_norm_rope_store(const void* qkv, int64_t qkv_row_stride, const int64_
                            int64_t num_slots, float scale_floor, slo_stream_t stream);
 
 /*
+ * The same step in the other rotary layouts, with or without the norms.  The
+ * first rotary_dim channels of a q or k head (a multiple of 8 up to head_dim)
+ * turn in pairs: neighbours (2i, 2i + 1) when `interleaved`, else
+ * (i, i + rotary_dim / 2); row p of cos_sin, fp32 [max_position, rotary_dim],
+ * holds the pairs' cosines, then their sines.  Both norm weights (bf16
+ * [head_dim]), or neither (NULL: no norm, eps not read).  Norm and rotation are
+ * computed in fp32 and rounded once.  head_dim 64, 128 or 256; any number of
+ * heads; num_slots 0 (k_cache and v_cache may be NULL) writes q and k only.
+ */
+int slo_rope_store(const void* qkv, int64_t qkv_row_stride, const int64_t* positions,
+                   int32_t num_tokens, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                   const void* q_norm_weight, const void* k_norm_weight, float eps,
+                   const float* cos_sin, int32_t max_position, int32_t rotary_dim,
+                   int32_t interleaved, void* q_out, void* k_out, const int32_t* slot_mapping,
+                   int32_t kv_dtype, void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                   int64_t num_slots, float scale_floor, slo_stream_t stream);
+
+/*
  * LM head on the sampled rows with the greedy argmax fused in.
  *
  * Replaces compute_logits on the sampled hidden rows and the greedy argmax of
@@ -352,6 +370,25 @@ int slo_load_kvcache(const void* k_cache, const void* v_cache, const void* k_sca
  */
 int slo_paged_attention_fp4_workspace_bytes(const slo_paged_attention_args* args, size_t* bytes);
 int slo_paged_attention_fp4(const slo_paged_attention_args* args, slo_stream_t stream);
+
+/*
+ * slo_paged_attention with a sliding window: the query at position t of its row
+ * (t = prefix + its place in the row's chunk; a decode row's is its last key)
+ * sees the keys j <= t with j > t - window or j < sinks (window > 0, sinks >=
+ * 0).  Arguments, rows and outputs as in slo_paged_attention, over a bf16,
+ * E4M3FN or 4-bit pool (kv_dtype; k_scale / v_scale point to fp32 or E8M0
+ * scales) and, without prefill_tables, over the contiguous bf16 rows k and v;
+ * store_slot_mapping must be NULL and softmax_scale not zero.  Pages without a
+ * visible key are not read: their table entries may be anything.  Entries that
+ * are not in the pool count as keys that no query sees.  A query without keys
+ * gives zeros, and so do query rows past every row's.  max_q and max_k are not
+ * read.  At most 32,768 decode and 1,024 prefill rows, tables of up to 2^22
+ * tokens, 2^24 rows of k and v.  Workspace as for slo_paged_attention_fp4.
+ */
+int slo_paged_attention_window_workspace_bytes(const slo_paged_attention_args* args, int32_t window,
+                                               int32_t sinks, size_t* bytes);
+int slo_paged_attention_window(const slo_paged_attention_args* args, int32_t window, int32_t sinks,
+                               slo_stream_t stream);
 
 /*
  * Adds the attention weights of a step's queries to the scores of the cached

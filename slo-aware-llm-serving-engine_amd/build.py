@@ -18,7 +18,8 @@ CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "slo_attn")
 LIB = os.path.join(OUT_DIR, "libslo_attn.so")
 SOURCES = ["store_kv.hip", "qk_norm_rope.hip", "lm_head.hip", "metadata.hip", "paged_attention.hip",
-           "kv_fp4.hip", "fp4_attention.hip", "kv_scores.hip", "kv_evict.hip", "capi.cpp"]
+           "kv_fp4.hip", "fp4_attention.hip", "kv_scores.hip", "kv_evict.hip", "rope_store.hip", "window_attention.hip",
+           "capi.cpp"]
 ARCH = "gfx950"
 FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-fPIC", "-std=c++17",
@@ -41,7 +42,7 @@ def hipcc() -> str:
 
 # Kernels whose every instantiation must keep its registers out of scratch
 # memory (a spill there puts per-lane memory traffic into the tile loops).
-NO_SCRATCH = {"paged_attention.hip", "fp4_attention.hip", "kv_scores.hip"}
+NO_SCRATCH = {"paged_attention.hip", "fp4_attention.hip", "kv_scores.hip", "window_attention.hip"}
 
 
 def _compile(src: str, obj: str) -> None:

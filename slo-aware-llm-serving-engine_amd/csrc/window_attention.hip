@@ -1,0 +1,1152 @@
+// Ragged paged attention with a sliding window and a few first tokens that
+// stay visible (gfx950).
+//
+// out[t, h] = sum_j softmax_j(scale q[t, h] . k[j]) v[j] over the keys j that
+// the query at position t of its row sees: j <= t and (j > t - window or
+// j < sinks).  One pass over those keys with a running maximum and sum per
+// (query, head); pages and steps without a visible key are not read, so that a
+// row costs what its window does, however long it is.
+//
+//   S^T = K q^T      A = K (rows: 16 tokens), B = q (columns: 16 queries or heads)
+//   O^T += V^T P^T   A = V^T (rows: 16 channels), B = P (columns: the same 16)
+//
+// Transposed products keep a column's statistics in the lanes that hold its
+// scores and outputs.  Lane (c, kg), c = lane % 16 and kg = lane / 16, has of
+// each 16 tokens K's channels 32 kg .. 32 kg + 31 of token c (four operands of
+// 8), and V's channels 8 c .. 8 c + 7 of tokens 4 kg .. 4 kg + 3, of which two
+// v_perm_b32 per channel pair make the operand that has those tokens side by
+// side; a lane's scores are of tokens 4 kg .. 4 kg + 3 and are, exponentiated,
+// the other operand as they lie.  Pools of all three formats take this one
+// order: codes are converted to bf16 operands exactly (E4M3FN scales multiply
+// scores and weights, E8M0 ones go in with the conversion).
+// Sums, maxima and outputs are fp32 until the one rounding at the end.
+#include "capi_internal.h"
+#include "fp4.h"
+#include "tile_io.h"
+#include <algorithm>
+
+namespace slo {
+namespace {
+
+constexpr int RECORD = HD + 4;   // floats of a decode chunk's partial result: outputs, maximum, sum, 2 unused
+constexpr float kNone = -1e30f;  // running maximum before the first key
+constexpr float kSumMax = 224.0f;  // largest sum of a lane's weights in a step before the reference moves
+constexpr int NT = 2;            // 16-column blocks of a prefill wavefront
+constexpr int kWaves = 4;
+
+// Partial result of a part of a prefill tile, as it lies in the registers of
+// its lanes (four channels a piece).
+struct Part {
+  f32x4 o[kWaves * NT][8][64];
+  float m[64 * NT], l[64 * NT];
+};
+
+struct WinParams {
+  const uint16_t* q;
+  int64_t q_stride;
+  uint16_t* out;
+  int64_t out_stride;
+  int num_q_rows;
+  const uint8_t *kc, *vc;  // pool, or the step's own rows (no prefill tables)
+  const void *ks, *vs;
+  int num_blocks, block_size;
+  uint32_t tpb, tpb_inv;  // 64-token tiles per block, ceil(2^32 / tpb)
+  int hq, hkv, group;
+  float scale_log2;  // |softmax scale| * log2(e)
+  uint32_t q_sign;   // 0x80008000 where the scale is negative
+  int window, sinks;
+  // decode rows
+  const int32_t* lens;
+  const int32_t* dtables;
+  int dstride, dwidth, drows, chunks;
+  float* records;  // [rows, kv heads, chunks, group] records
+  // prefill rows
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  const int32_t* ptables;
+  int pstride, pwidth, prows, splits, items;
+  Part* parts;  // [items, kv heads, splits]
+  const uint8_t *rk, *rv;  // without tables: bf16 rows, byte strides
+  int64_t rk_stride, rv_stride;
+  int num_kv_rows;
+  int first_row;  // query row of the first prefill row's first query
+  // Query rows from first_idle + (ends ? *ends : 0) on belong to no row (the
+  // capacity padding of a captured step) and are given zeros.
+  const int32_t* ends;
+  int first_idle;
+  bool idle;
+};
+
+__device__ __forceinline__ void clear_idle(const WinParams& p) {
+  const int64_t from = (int64_t)p.first_idle + (p.ends ? max(*p.ends, 0) : 0);
+  const int per = p.hq * (HD / 8);  // 16-byte pieces of a row
+  const int64_t pieces = (p.num_q_rows - from) * per, stride = (int64_t)gridDim.x * blockDim.x;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < pieces; i += stride)
+    *reinterpret_cast<u32x4*>(p.out + (from + i / per) * p.out_stride + 8 * (i % per)) = u32x4{0, 0, 0, 0};
+}
+
+// The steps of T keys that hold what queries at positions [x0, x1] see of a
+// row of lk keys: `sink` steps from key 0 on, then those from key `start` on.
+struct Span {
+  int first, end;  // keys of the window part
+  int sink, start, steps;
+};
+template <int T>
+__device__ __forceinline__ Span span_of(const WinParams& p, int x0, int x1, int lk) {
+  Span s;
+  s.end = max(min(x1 + 1, lk), 0);
+  s.first = max(x0 - p.window + 1, 0);
+  const int f = s.first / T;
+  s.sink = min((min(p.sinks, s.end) + T - 1) / T, f);
+  s.start = f * T;
+  s.steps = s.sink + max((s.end + T - 1) / T - f, 0);
+  return s;
+}
+template <int T>
+__device__ __forceinline__ int key_of(const Span& s, int i) {
+  return i < s.sink ? i * T : s.start + (i - s.sink) * T;
+}
+
+// The pool row (token * kv heads, or the head's own token) of a row's key.
+__device__ __forceinline__ const __attribute__((address_space(4))) int32_t* scalar(const int32_t* x) {
+  return (const __attribute__((address_space(4))) int32_t*)(uintptr_t)x;
+}
+template <int F>
+__device__ __forceinline__ int64_t pool_row(const WinParams& p, const int32_t* table, int head, int key, bool& ok) {
+  const uint32_t t = (uint32_t)key / 64;
+  const int page = p.tpb == 1 ? (int)t : (int)__umulhi(t, p.tpb_inv);
+  const int b = scalar(table)[page], off = key - page * p.block_size;
+  ok = b >= 0 && b < p.num_blocks;
+  const int64_t block = ok ? b : 0;
+  if (F == KV_FP4_E2M1) return (block * p.hkv + head) * p.block_size + off;
+  return (block * p.block_size + off) * p.hkv + head;
+}
+
+__device__ __forceinline__ bf16x8 load_q(const WinParams& p, int64_t row, int h, int channel, bool live) {
+  u32x4 x = {0, 0, 0, 0};
+  if (live) x = ld16(p.q + row * p.q_stride + h * HD + channel);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] ^= p.q_sign;
+  return as_bf16x8(x);
+}
+
+// Four tokens' channel pairs as two channels' token quadruples.
+__device__ __forceinline__ u32x2 evens(const uint32_t (&w)[4]) {
+  return u32x2{__builtin_amdgcn_perm(w[1], w[0], 0x05040100u), __builtin_amdgcn_perm(w[3], w[2], 0x05040100u)};
+}
+__device__ __forceinline__ u32x2 odds(const uint32_t (&w)[4]) {
+  return u32x2{__builtin_amdgcn_perm(w[1], w[0], 0x07060302u), __builtin_amdgcn_perm(w[3], w[2], 0x07060302u)};
+}
+
+// ------------------------------------------------------------- decode rows
+// A wavefront's steps of T tokens arrive in LDS by non-temporal DMA, two in
+// flight, as their lanes fetch them: 16-byte pieces of K's rows in an order
+// that spreads the operands' reads over the banks, V's rows as they are.
+template <int F> struct Step;
+template <> struct Step<KV_BF16> {
+  static constexpr int T = 16, LOADS = 8;
+  uint8_t k[T * 256], v[T * 256];
+};
+template <> struct Step<KV_FP8_E4M3FN> {
+  static constexpr int T = 32, LOADS = 9;
+  uint8_t k[T * 128], v[T * 128];
+  float s[2 * T];
+};
+template <> struct Step<KV_FP4_E2M1> {
+  static constexpr int T = 32, LOADS = 5;
+  uint8_t k[T * 64], v[T * 64], ks[T * 4], vs[T * 4];
+};
+
+template <int F>
+__device__ __forceinline__ void fetch(const WinParams& p, int64_t row, uint32_t to, int lane) {
+  if constexpr (F == KV_BF16) {
+    const uint32_t stride = p.hkv * 256, r = lane >> 4, c = lane & 15;
+    const uint8_t *k = p.kc + row * 256, *v = p.vc + row * 256;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dma16_nt_at(k, (4 * i + r) * stride + 16 * (c ^ (4 * i + r)), to + 1024 * i);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dma16_nt_at(v, (4 * i + r) * stride + 16 * c, to + 4096 + 1024 * i);
+  } else if constexpr (F == KV_FP8_E4M3FN) {
+    const uint32_t stride = p.hkv * 128, r = lane >> 3, c = lane & 7;
+    const uint8_t *k = p.kc + row * 128, *v = p.vc + row * 128;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dma16_nt_at(k, (8 * i + r) * stride + 16 * (c ^ r), to + 1024 * i);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dma16_nt_at(v, (8 * i + r) * stride + 16 * c, to + 4096 + 1024 * i);
+    dma4(static_cast<const float*>(lane < 32 ? p.ks : p.vs) + row + (int64_t)(lane & 31) * p.hkv, to + 8192);
+  } else {
+    // Of K, 16-byte part x of token t lies at part x ^ (t / 4 mod 4) of its
+    // place; of V, token t lies at place t ^ (t / 4 mod 4).
+    const uint32_t t = lane >> 2, x = (lane >> 4) & 3;
+    const uint32_t ko = t * 64 + ((lane & 3) ^ x) * 16, vo = (t ^ x) * 64 + (lane & 3) * 16;
+    const uint8_t *k = p.kc + row * 64, *v = p.vc + row * 64;
+    dma16_nt_at(k, ko, to);
+    dma16_nt_at(k, ko + 1024, to + 1024);
+    dma16_nt_at(v, vo, to + 2048);
+    dma16_nt_at(v, vo + 1024, to + 2048 + 1024);
+    dma4(static_cast<const uint8_t*>(lane < 32 ? p.ks : p.vs) + row * 4 + (lane & 31) * 4, to + 4096);
+  }
+}
+
+struct DecodeAcc {
+  f32x4 o[8];
+  float m, l;  // l: this lane's own tokens
+};
+
+// Weights of H x 4 scores (log2 domain) of a lane's tokens; the reference of
+// the column moves only where a score passes it by 2^8.
+template <int H>
+__device__ __forceinline__ void weigh(f32x4 (&s)[H], DecodeAcc& a) {
+  float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
+  if constexpr (H == 2) top = fmaxf(top, fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+  if (__any(top > a.m + 8.0f)) {
+    const float m = fmaxf(a.m, col_max(top)), w = __builtin_amdgcn_exp2f(a.m - m);
+    a.m = m;
+    a.l *= w;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) a.o[e] *= w;
+  }
+#pragma unroll
+  for (int h = 0; h < H; ++h)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[h][i] = __builtin_amdgcn_exp2f(s[h][i] - a.m);
+      a.l += s[h][i];
+    }
+}
+
+// A weight as two bf16 terms, which carry it to 2^-17: the decode steps wait
+// for memory, not for the second product.
+template <int H>
+__device__ __forceinline__ void split(const f32x4 (&e)[H], uint32_t (&hi)[2 * H], uint32_t (&lo)[2 * H]) {
+#pragma unroll
+  for (int h = 0; h < H; ++h)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float x = e[h][2 * i], y = e[h][2 * i + 1];
+      const uint32_t w = pack_bf16x2(x, y);
+      hi[2 * h + i] = w;
+      lo[2 * h + i] = pack_bf16x2(x - __uint_as_float(w << 16), y - __uint_as_float(w & 0xffff0000u));
+    }
+}
+
+// One landed step: token i of half h of a lane is seen where bit 4 h + i of
+// `seen` is set.  (A token that is not seen may be anything in the pages.)
+template <int F>
+__device__ __forceinline__ void decode_step(const WinParams& p, const Step<F>& st, uint32_t seen, const bf16x8 (&q)[4],
+                                            DecodeAcc& a, int lane) {
+  constexpr int H = Step<F>::T / 16;
+  const int c = lane & 15, kg = lane >> 4;
+  const bool masked = __any(seen != (1u << (4 * H)) - 1);
+  f32x4 s[H];
+  if constexpr (F == KV_BF16) {
+    u32x4 k[4], v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) k[i] = ld16(st.k + c * 256 + 16 * ((4 * kg + i) ^ c));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = ld16(st.v + (4 * kg + i) * 256 + 16 * c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[0] = mfma16(as_bf16x8(k[i]), q[i], i ? s[0] : f32x4{0, 0, 0, 0});
+    s[0] *= p.scale_log2;
+    if (masked) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (!(seen >> i & 1)) {
+          s[0][i] = -INFINITY;
+          v[i] = u32x4{0, 0, 0, 0};
+        }
+    }
+    weigh<1>(s, a);
+    uint32_t hi[2], lo[2];
+    split<1>(s, hi, lo);
+    const s16x4 ph = __builtin_bit_cast(s16x4, u32x2{hi[0], hi[1]}), pl = __builtin_bit_cast(s16x4, u32x2{lo[0], lo[1]});
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const uint32_t w[4] = {v[0][b], v[1][b], v[2][b], v[3][b]};
+      const s16x4 e = __builtin_bit_cast(s16x4, evens(w)), o = __builtin_bit_cast(s16x4, odds(w));
+      a.o[2 * b] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(e, ph, a.o[2 * b], 0, 0, 0);
+      a.o[2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(o, ph, a.o[2 * b + 1], 0, 0, 0);
+      a.o[2 * b] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(e, pl, a.o[2 * b], 0, 0, 0);
+      a.o[2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(o, pl, a.o[2 * b + 1], 0, 0, 0);
+    }
+  } else {
+    u32x4 v[8];  // 8 channels of 8 tokens: 4 kg + i and 16 + 4 kg + i
+    f32x4 vs[2];
+    if constexpr (F == KV_FP8_E4M3FN) {
+      u32x2 raw[8];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const u32x4 k = ld16(st.k + (16 * h + c) * 128 + 16 * ((2 * kg + i) ^ (c & 7)));
+          s[h] = mfma16(as_bf16x8(fp8x8_to_bf16x8(u32x2{k[0], k[1]})), q[2 * i], i ? s[h] : f32x4{0, 0, 0, 0});
+          s[h] = mfma16(as_bf16x8(fp8x8_to_bf16x8(u32x2{k[2], k[3]})), q[2 * i + 1], s[h]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) raw[4 * h + i] = ld8(st.v + (16 * h + 4 * kg + i) * 128 + 8 * c);
+      }
+      const f32x4* ks = reinterpret_cast<const f32x4*>(st.s);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        s[h] *= p.scale_log2 * ks[4 * h + kg];
+        vs[h] = ks[8 + 4 * h + kg];
+      }
+      if (masked) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (!(seen >> j & 1)) {
+            raw[j] = u32x2{0, 0};
+            vs[j >> 2][j & 3] = 0.0f;
+          }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = fp8x8_to_bf16x8(raw[j]);
+    } else {
+      uint32_t raw[8];
+      float sc[8];
+      const int turn = (9 + 8 * (c >> 2)) & 31;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const u32x4 k = ld16(st.k + h * 1024 + c * 64 + (kg ^ (c >> 2)) * 16);
+        const float ks = e8m0(st.ks[h * 64 + c * 4 + kg]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[h] = mfma16(as_bf16x8(e2m1_decode8(k[i], ks)), q[i], i ? s[h] : f32x4{0, 0, 0, 0});
+        s[h] *= p.scale_log2;
+        // The conversion reads nothing but the exponent of its scale.
+        const u32x4 x = ld16(st.vs + h * 64 + kg * 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          raw[4 * h + i] = *reinterpret_cast<const uint32_t*>(st.v + h * 1024 + kg * 256 + (i ^ kg) * 64 + c * 4);
+          sc[4 * h + i] = __uint_as_float(__builtin_amdgcn_alignbit(x[i], x[i], turn));
+        }
+      }
+      if (masked) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (!(seen >> j & 1)) sc[j] = 0.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = e2m1_decode8(raw[j], sc[j]);
+    }
+    if (masked) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (!(seen >> j & 1)) s[j >> 2][j & 3] = -INFINITY;
+    }
+    weigh<2>(s, a);
+    if constexpr (F == KV_FP8_E4M3FN) {
+      s[0] *= vs[0];
+      s[1] *= vs[1];
+    }
+    uint32_t hi[4], lo[4];
+    split<2>(s, hi, lo);
+    const bf16x8 ph = as_bf16x8(u32x4{hi[0], hi[1], hi[2], hi[3]}), pl = as_bf16x8(u32x4{lo[0], lo[1], lo[2], lo[3]});
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const uint32_t w0[4] = {v[0][b], v[1][b], v[2][b], v[3][b]}, w1[4] = {v[4][b], v[5][b], v[6][b], v[7][b]};
+      const u32x2 e0 = evens(w0), e1 = evens(w1), o0 = odds(w0), o1 = odds(w1);
+      const bf16x8 e = as_bf16x8(u32x4{e0.x, e0.y, e1.x, e1.y}), o = as_bf16x8(u32x4{o0.x, o0.y, o1.x, o1.y});
+      a.o[2 * b] = mfma16(e, ph, a.o[2 * b]);
+      a.o[2 * b + 1] = mfma16(o, ph, a.o[2 * b + 1]);
+      a.o[2 * b] = mfma16(e, pl, a.o[2 * b]);
+      a.o[2 * b + 1] = mfma16(o, pl, a.o[2 * b + 1]);
+    }
+  }
+}
+
+// A decode row's chunks: `count` of equal steps, no shorter than 256 keys.
+template <int F>
+struct Chunks {
+  Span s;
+  int len, count, per;
+};
+template <int F>
+__device__ __forceinline__ Chunks<F> chunks_of(const WinParams& p, int r) {
+  constexpr int T = Step<F>::T;
+  Chunks<F> c;
+  c.len = min(max(scalar(p.lens)[r], 0), p.dwidth * p.block_size);
+  c.s = span_of<T>(p, c.len - 1, c.len - 1, c.len);
+  c.count = max(1, min(p.chunks, (c.s.steps * T + 255) / 256));
+  c.per = (c.s.steps + c.count - 1) / c.count;
+  return c;
+}
+
+template <int F>
+struct DecodeLds {
+  union {
+    Step<F> steps[2];
+    float o[16][HD];
+  } ring[kWaves];
+  float m[kWaves][16], l[kWaves][16];
+};
+
+// One chunk of one (row, kv head) a workgroup, its four wavefronts every fourth
+// step, all heads of the group as columns.  Each wavefront fetches its own
+// steps, so the loop has no barrier; the wavefronts' results meet in LDS.
+template <int F>
+__device__ void decode_item(const WinParams& p, DecodeLds<F>& lds, int r, int chunk, int head) {
+  constexpr int T = Step<F>::T, H = T / 16;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, kg = lane >> 4;
+  bf16x8 q[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) q[i] = load_q(p, r, head * p.group + c, 32 * kg + 8 * i, c < p.group);
+  const Chunks<F> ch = chunks_of<F>(p, r);
+  if (chunk >= ch.count) return;
+  const int begin = chunk * ch.per + wave, end = min((chunk + 1) * ch.per, ch.s.steps);
+  DecodeAcc a;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) a.o[e] = f32x4{0, 0, 0, 0};
+  a.m = kNone;
+  a.l = 0.0f;
+  const int steps = end > begin ? (end - begin + kWaves - 1) / kWaves : 0;
+  if (steps > 0) {
+    const int32_t* table = p.dtables + (int64_t)r * p.dstride;
+    const uint32_t ring = lds_addr(&lds.ring[wave]);
+    int key[2];   // of the steps in flight; past every key where the page is not in the pool
+    auto send = [&](int i) {
+      bool ok;
+      const int k = key_of<T>(ch.s, begin + kWaves * i);
+      const int64_t row = pool_row<F>(p, table, head, k, ok);
+      fetch<F>(p, row, ring + (i & 1) * (uint32_t)sizeof(Step<F>), lane);
+      return ok ? k : ch.len;
+    };
+    key[1] = send(0);
+    for (int i = 0; i < steps; ++i) {
+      key[0] = key[1];
+      // The place that the next fetch fills was read in the last iteration; its
+      // reads have returned.
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+      const bool more = i + 1 < steps;
+      if (more) key[1] = send(i + 1);
+      asm volatile("" ::: "memory");
+      if (more)
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(Step<F>::LOADS));
+      else
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+      asm volatile("" ::: "memory");
+      uint32_t seen = 0;
+#pragma unroll
+      for (int j = 0; j < 4 * H; ++j) {
+        const int k = key[0] + 16 * (j >> 2) + 4 * kg + (j & 3);
+        seen |= (uint32_t)(k < ch.len && (k >= ch.s.first || k < p.sinks)) << j;
+      }
+      decode_step<F>(p, lds.ring[wave].steps[i & 1], seen, q, a, lane);
+    }
+  }
+  a.l = col_sum(a.l);
+  if (c < p.group) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; e += 4)
+        *reinterpret_cast<f32x4*>(&lds.ring[wave].o[c][32 * kg + 8 * i + e]) =
+            f32x4{a.o[e][i], a.o[e + 1][i], a.o[e + 2][i], a.o[e + 3][i]};
+    if (kg == 0) {
+      lds.m[wave][c] = a.m;
+      lds.l[wave][c] = a.l;
+    }
+  }
+  __syncthreads();
+  for (int x = threadIdx.x; x < p.group * (HD / 4); x += 64 * kWaves) {
+    const int h = x >> 5, d = (x & 31) * 4;
+    float m = lds.m[0][h];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) m = fmaxf(m, lds.m[w][h]);
+    f32x4 o = {0, 0, 0, 0};
+    float l = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = __builtin_amdgcn_exp2f(lds.m[w][h] - m);
+      o += *reinterpret_cast<const f32x4*>(&lds.ring[w].o[h][d]) * f;
+      l += lds.l[w][h] * f;
+    }
+    if (ch.count == 1) {
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      *reinterpret_cast<u32x2*>(p.out + (int64_t)r * p.out_stride + (head * p.group + h) * HD + d) =
+          u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
+    } else {
+      float* rec = p.records + ((((int64_t)r * p.hkv + head) * p.chunks + chunk) * p.group + h) * RECORD;
+      *reinterpret_cast<f32x4*>(rec + d) = o;
+      if (d == 0) {
+        rec[HD] = m;
+        rec[HD + 1] = l;
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------ prefill rows
+// One 64-token step of a workgroup as bf16 operands in LDS, in the order in
+// which lanes read them (16 bytes a lane, no bank twice): K's four operands of
+// each 16 tokens, V's eight of each 32 tokens, and E4M3FN's scales.
+template <int F>
+struct Stage {
+  u32x4 k[4][4][64], v[2][8][64];
+  float s[F == KV_FP8_E4M3FN ? 2 : 1][64];
+};
+
+// A wavefront's quarter of a step, 16 tokens, as loaded.
+template <int F> struct Quarter;
+template <> struct Quarter<KV_BF16> {
+  u32x4 k[4], v[4];
+};
+template <> struct Quarter<KV_FP8_E4M3FN> {
+  u32x4 k[2];
+  u32x2 v[4];
+  float s;
+};
+template <> struct Quarter<KV_FP4_E2M1> {
+  u32x4 k, vs;
+  uint32_t ks, v[4];
+};
+
+struct PrefillRow {
+  int64_t q0;  // first query row
+  int lq, lk, prefix, k0;
+};
+
+__device__ __forceinline__ PrefillRow prefill_row(const WinParams& p, int r) {
+  PrefillRow g;
+  const int start = p.cu_q[r], k0 = p.cu_k[r], k = p.cu_k[r + 1] - k0;
+  g.q0 = (int64_t)p.first_row + start;
+  g.lq = p.cu_q[r + 1] - start;
+  g.prefix = k - g.lq;
+  g.k0 = k0;
+  g.lk = p.ptables ? min(k, p.pwidth * p.block_size) : min(k, p.num_kv_rows - k0);
+  if (!p.ptables && k0 < 0) g.lk = 0;
+  if (start < 0 || g.q0 + g.lq > p.num_q_rows) g.lq = 0;
+  return g;
+}
+
+// The 16 tokens from `key` + 16 wave on; `left`: keys of the row from `key` on
+// (rows without a pool are not read past their end).
+template <int F>
+__device__ __forceinline__ void load_quarter(Quarter<F>& t, const WinParams& p, const PrefillRow& g, const int32_t* table,
+                                             int head, int key, int wave, int lane, bool& ok) {
+  const int c = lane & 15, kg = lane >> 4;
+  if constexpr (F == KV_BF16) {
+    const uint8_t *k, *v;
+    int64_t ks, vs;
+    int last = 63;
+    ok = true;
+    if (p.ptables) {
+      const int64_t row = pool_row<F>(p, table, head, key, ok);
+      k = p.kc + row * 256;
+      v = p.vc + row * 256;
+      ks = vs = p.hkv * 256;
+    } else {
+      const int64_t row = (int64_t)g.k0 + key;
+      k = p.rk + row * p.rk_stride + head * 256;
+      v = p.rv + row * p.rv_stride + head * 256;
+      ks = p.rk_stride;
+      vs = p.rv_stride;
+      last = g.lk - 1 - key;
+    }
+    k += min(16 * wave + c, last) * ks + 64 * kg;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t.k[i] = ld16(k + 16 * i);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t.v[i] = ld16(v + min(16 * wave + 4 * kg + i, last) * vs + 16 * c);
+  } else if constexpr (F == KV_FP8_E4M3FN) {
+    const int64_t row = pool_row<F>(p, table, head, key, ok) + 16 * wave * p.hkv;
+    const uint8_t *k = p.kc + row * 128, *v = p.vc + row * 128;
+    const uint32_t stride = p.hkv * 128;
+    t.k[0] = ld16(k + (c * stride + 32 * kg));
+    t.k[1] = ld16(k + (c * stride + 32 * kg + 16));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t.v[i] = ld8(v + ((4 * kg + i) * stride + 8 * c));
+    t.s = static_cast<const float*>(lane & 16 ? p.vs : p.ks)[row + c * p.hkv];
+  } else {
+    const int64_t row = pool_row<F>(p, table, head, key, ok) + 16 * wave;
+    const uint8_t *k = p.kc + row * 64, *v = p.vc + row * 64;
+    const uint8_t *ks = static_cast<const uint8_t*>(p.ks) + row * 4, *vs = static_cast<const uint8_t*>(p.vs) + row * 4;
+    t.k = ld16(k + (c * 64 + kg * 16));
+    t.ks = ks[c * 4 + kg];
+    t.vs = ld16(vs + kg * 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t.v[i] = *reinterpret_cast<const uint32_t*>(v + (kg * 256 + c * 4 + i * 64));
+  }
+}
+
+// `seen`: which of the lane's four V tokens one of the tile's queries sees.  The
+// others may be anything in the pages, and a weight of zero must not make that
+// a NaN.
+template <int F>
+__device__ __forceinline__ void stage(Stage<F>& s, const Quarter<F>& t, uint32_t seen, int wave, int lane) {
+  const int c = lane & 15;
+  u32x4 v[4];
+  if constexpr (F == KV_BF16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s.k[wave][i][lane] = t.k[i];
+      v[i] = t.v[i];
+    }
+    if (__any(seen != 15)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (!(seen >> i & 1)) v[i] = u32x4{0, 0, 0, 0};
+    }
+  } else if constexpr (F == KV_FP8_E4M3FN) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      s.k[wave][2 * i][lane] = fp8x8_to_bf16x8(u32x2{t.k[i][0], t.k[i][1]});
+      s.k[wave][2 * i + 1][lane] = fp8x8_to_bf16x8(u32x2{t.k[i][2], t.k[i][3]});
+    }
+    if (lane < 32) s.s[lane >> 4][16 * wave + c] = t.s;
+    u32x2 raw[4] = {t.v[0], t.v[1], t.v[2], t.v[3]};
+    if (__any(seen != 15)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (!(seen >> i & 1)) raw[i] = u32x2{0, 0};
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = fp8x8_to_bf16x8(raw[i]);
+  } else {
+    const float sc = e8m0(t.ks);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s.k[wave][i][lane] = e2m1_decode8(t.k[i], sc);
+    float vs[4];
+    const int turn = (9 + 8 * (c >> 2)) & 31;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) vs[i] = __uint_as_float(__builtin_amdgcn_alignbit(t.vs[i], t.vs[i], turn));
+    if (__any(seen != 15)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (!(seen >> i & 1)) vs[i] = 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = e2m1_decode8(t.v[i], vs[i]);
+  }
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    const uint32_t w[4] = {v[0][b], v[1][b], v[2][b], v[3][b]};
+    reinterpret_cast<u32x2*>(&s.v[wave >> 1][2 * b][lane])[wave & 1] = evens(w);
+    reinterpret_cast<u32x2*>(&s.v[wave >> 1][2 * b + 1][lane])[wave & 1] = odds(w);
+  }
+}
+
+struct Acc {
+  f32x4 o[NT][8];
+  float ncm[NT], l[NT];  // minus the reference in the log2 domain (+inf before the first key), this lane's sum
+};
+
+// 64 tokens of a wavefront's columns against the staged operands, read four
+// ahead of the products.  at[n]: position of column block n's query; keys from
+// `kend` on are not the row's.
+template <int F>
+__device__ __forceinline__ void staged_step(const WinParams& p, const Stage<F>& st, bool masked, const bf16x8 (&q)[NT][4],
+                                            Acc& a, int kv0, const int (&at)[NT], int kend, int lane) {
+  const int kg = lane >> 4;
+  f32x4 s[NT][4];
+  bf16x8 x[2][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[0][i] = as_bf16x8(st.k[0][i][lane]);
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[(t + 1) & 1][i] = as_bf16x8(t < 3 ? st.k[t + 1][i][lane] : st.v[0][i][lane]);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[n][t] = mfma16(x[t & 1][i], q[n][i], i ? s[n][t] : f32x4{0, 0, 0, 0});
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  if constexpr (F == KV_FP8_E4M3FN) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const f32x4 ks = *reinterpret_cast<const f32x4*>(&st.s[0][16 * t + 4 * kg]);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[n][t] *= ks;
+    }
+  }
+  if (masked) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int k = kv0 + 16 * t + 4 * kg + i;
+          if (!(k <= at[n] && k < kend && (k > at[n] - p.window || k < p.sinks))) s[n][t][i] = -INFINITY;
+        }
+  }
+  // No maximum is formed: a reference that is too low shows in the sum of a
+  // lane's weights (inf or NaN while it is unset).  Only then are the columns'
+  // maxima found and the weights taken again.
+  const float c = p.scale_log2;
+  f32x4 e[NT][4];
+  float rs[NT];
+  bool over = false;
+  auto exponents = [&](int n, float ncm) {
+    rs[n] = 0.0f;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        e[n][t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][t][i], c, ncm));
+        rs[n] += e[n][t][i];
+      }
+  };
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    exponents(n, a.ncm[n]);
+    over = over || !(rs[n] <= kSumMax);
+  }
+  if (__any(over)) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const bool mine = !(rs[n] <= kSumMax);
+      if (!__any(mine)) continue;
+      const bool grow = col_max(mine ? 1.0f : 0.0f) > 0.0f;
+      float top = s[n][0][0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) top = fmaxf(top, s[n][i >> 2][i & 3]);
+      top = col_max(top);
+      const float next = grow && top != -INFINITY ? fminf(a.ncm[n], -c * top) : a.ncm[n];
+      const float use = next == INFINITY ? 0.0f : next;  // no key yet: weights of zero
+      const float w = grow ? __builtin_amdgcn_exp2f(use - a.ncm[n]) : 1.0f;
+      exponents(n, use);
+      a.l[n] *= w;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a.o[n][i] *= w;
+      a.ncm[n] = next;
+    }
+  }
+  bf16x8 pr[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    a.l[n] += rs[n];
+    if constexpr (F == KV_FP8_E4M3FN) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        f32x4 vs = *reinterpret_cast<const f32x4*>(&st.s[1][16 * t + 4 * kg]);
+        if (masked) {  // of tokens that may be anything
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (e[n][t][i] == 0.0f) vs[i] = 0.0f;
+        }
+        e[n][t] *= vs;
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+      pr[n][g] = as_bf16x8(u32x4{pack_bf16x2(e[n][2 * g][0], e[n][2 * g][1]), pack_bf16x2(e[n][2 * g][2], e[n][2 * g][3]),
+                                 pack_bf16x2(e[n][2 * g + 1][0], e[n][2 * g + 1][1]),
+                                 pack_bf16x2(e[n][2 * g + 1][2], e[n][2 * g + 1][3])});
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {  // V's operands, four at a time
+    const int g = j >> 1;
+    if (j < 3) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[(j + 1) & 1][i] = as_bf16x8(st.v[(j + 1) >> 1][4 * ((j + 1) & 1) + i][lane]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) a.o[n][4 * (j & 1) + i] = mfma16(x[j & 1][i], pr[n][g], a.o[n][4 * (j & 1) + i]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// Item i's row and tile: the rows' tiles in order, each row's last one (the
+// longest, where the window has not filled) first.
+__device__ __forceinline__ bool find_tile(const WinParams& p, int per, int item, int lane, int& row, int& tile) {
+  int before = 0;
+  for (int base = 0; base < p.prows; base += 64) {
+    int n = 0;
+    if (base + lane < p.prows) {
+      const int lq = prefill_row(p, base + lane).lq;
+      n = lq > 0 ? (lq + per - 1) / per : 0;
+    }
+    const int upto = wave_scan(n);
+    const uint64_t past = __ballot(before + upto > item);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      row = base + at;
+      tile = before + __builtin_amdgcn_readlane(upto, at) - 1 - item;
+      return true;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  return false;
+}
+
+// Tile `item`, part `part` of its steps, kv head `head`.  The four wavefronts
+// turn each step into operands together, a quarter each, and each runs 16 NT
+// columns, (query, head of the group) pairs of consecutive queries, over them;
+// the next step loads meanwhile.
+template <int F>
+__device__ void prefill_item(const WinParams& p, Stage<F> (&st)[2], int item, int part, int head) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, kg = lane >> 4;
+  const int each = 16 * NT / p.group, per = kWaves * each;  // queries of a wavefront, of a tile
+  int r = 0, tile = 0;
+  if (!find_tile(p, per, item, lane, r, tile)) return;
+  r = __builtin_amdgcn_readfirstlane(r);
+  tile = __builtin_amdgcn_readfirstlane(tile);
+  const PrefillRow g = prefill_row(p, r);
+  const int w0 = tile * per, w1 = min(w0 + per, g.lq);
+  const Span s = span_of<64>(p, g.prefix + w0, g.prefix + w1 - 1, g.lk);
+  const int from = (int)((int64_t)s.steps * part / p.splits), to = (int)((int64_t)s.steps * (part + 1) / p.splits);
+  // Queries of this wavefront [t0, t1); columns past them repeat the last one's
+  // mask with a query of zeros.
+  const int t0 = min(w0 + wave * each, w1 - 1), t1 = max(min(w0 + wave * each + each, w1), t0 + 1);
+  int at[NT];
+  bf16x8 q[NT][4];
+  Acc a;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int x = 16 * n + c, tok = w0 + wave * each + x / p.group;
+    const bool live = x < each * p.group && tok < w1;
+    at[n] = g.prefix + min(tok, t1 - 1);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[n][i] = load_q(p, g.q0 + tok, head * p.group + x % p.group, 32 * kg + 8 * i, live);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a.o[n][i] = f32x4{0, 0, 0, 0};
+    a.ncm[n] = INFINITY;
+    a.l[n] = 0.0f;
+  }
+  if (from < to) {
+    const int32_t* table = p.ptables ? p.ptables + (int64_t)r * p.pstride : nullptr;
+    const int x0 = g.prefix + t0, x1 = g.prefix + t1 - 1;
+    Quarter<F> t;
+    bool ok, next_ok = false;
+    int key = key_of<64>(s, from), next = key;
+    load_quarter<F>(t, p, g, table, head, key, wave, lane, ok);
+    for (int i = from; i < to; ++i) {
+      const int buf = (i - from) & 1;
+      uint32_t seen = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int k = key + 16 * wave + 4 * kg + j;
+        seen |= (uint32_t)(ok && k < s.end && (k >= s.first || k < p.sinks)) << j;
+      }
+      stage<F>(st[buf], t, seen, wave, lane);
+      if (i + 1 < to) {
+        next = key_of<64>(s, i + 1);
+        load_quarter<F>(t, p, g, table, head, next, wave, lane, next_ok);
+      }
+      // Two buffers: a wavefront comes to write this one again only past the
+      // next step's barrier, when every wavefront has left it.  The barrier
+      // waits for LDS only: the loads of the next step stay in flight.
+      lds_sync();
+      const bool all = ok && key + 63 <= x0 && key + 64 <= g.lk && (key > x1 - p.window || key + 64 <= p.sinks);
+      staged_step<F>(p, st[buf], !all, q, a, ok ? key : 1 << 30, at, g.lk, lane);
+      key = next;
+      ok = next_ok;
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const float l = col_sum(a.l[n]);
+    if (p.splits == 1) {
+      const int x = 16 * n + c, tok = w0 + wave * each + x / p.group, h = head * p.group + x % p.group;
+      if (x >= each * p.group || tok >= w1) continue;
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      uint16_t* out = p.out + (g.q0 + tok) * p.out_stride + h * HD + 32 * kg;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<u32x4*>(out + 8 * i) =
+            u32x4{pack_bf16x2(a.o[n][0][i] * inv, a.o[n][1][i] * inv), pack_bf16x2(a.o[n][2][i] * inv, a.o[n][3][i] * inv),
+                  pack_bf16x2(a.o[n][4][i] * inv, a.o[n][5][i] * inv), pack_bf16x2(a.o[n][6][i] * inv, a.o[n][7][i] * inv)};
+    } else {
+      Part& out = p.parts[((int64_t)item * p.hkv + head) * p.splits + part];
+      const int block = NT * wave + n;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; e += 4)
+          out.o[block][2 * i + (e >> 2)][lane] = f32x4{a.o[n][e][i], a.o[n][e + 1][i], a.o[n][e + 2][i], a.o[n][e + 3][i]};
+      if (kg == 0) {
+        out.m[16 * block + c] = a.ncm[n] == INFINITY ? kNone : -a.ncm[n];
+        out.l[16 * block + c] = l;
+      }
+    }
+  }
+}
+
+// Both phases in one launch, prefill items first.
+template <int F>
+__global__ void __launch_bounds__(64 * kWaves, 2)
+window_attention_kernel(WinParams p) {
+  __shared__ union {
+    Stage<F> st[2];
+    DecodeLds<F> dec;
+  } lds;
+  int i = blockIdx.x;
+  const int head = i % p.hkv;
+  i /= p.hkv;
+  const int prefill = p.items * p.splits;
+  if (i < prefill)
+    prefill_item<F>(p, lds.st, i / p.splits, i % p.splits, head);
+  else
+    decode_item<F>(p, lds.dec, (i - prefill) / p.chunks, (i - prefill) % p.chunks, head);
+  if (p.idle) clear_idle(p);
+}
+
+// Joins the chunks of decode rows (workgroups below `decode`, one per row and
+// kv head) and the parts of prefill tiles (one per item, kv head and 16
+// columns).
+template <int F>
+__global__ void __launch_bounds__(256)
+window_join_kernel(WinParams p, int decode) {
+  int i = blockIdx.x;
+  if (i < decode) {
+    const int r = i / p.hkv, head = i % p.hkv;
+    const int count = chunks_of<F>(p, r).count;
+    if (count == 1) return;  // written by its only chunk
+    const float* rec = p.records + (int64_t)i * p.chunks * p.group * RECORD;
+    const int64_t stride = (int64_t)p.group * RECORD;
+    for (int x = threadIdx.x; x < p.group * (HD / 4); x += 256) {
+      const int h = x >> 5, d = (x & 31) * 4;
+      const float* e = rec + h * RECORD;
+      float m = kNone;
+      for (int s = 0; s < count; ++s) m = fmaxf(m, e[s * stride + HD]);
+      f32x4 o = {0, 0, 0, 0};
+      float l = 0;
+      for (int s = 0; s < count; ++s) {
+        const float w = __builtin_amdgcn_exp2f(e[s * stride + HD] - m);
+        o += *reinterpret_cast<const f32x4*>(e + s * stride + d) * w;
+        l += e[s * stride + HD + 1] * w;
+      }
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      *reinterpret_cast<u32x2*>(p.out + (int64_t)r * p.out_stride + (head * p.group + h) * HD + d) =
+          u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
+    }
+    return;
+  }
+  i -= decode;
+  const int block = i % (kWaves * NT), head = i / (kWaves * NT) % p.hkv, item = i / (kWaves * NT) / p.hkv;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, kg = lane >> 4;
+  const int each = 16 * NT / p.group, per = kWaves * each;
+  int r = 0, tile = 0;
+  if (!find_tile(p, per, item, lane, r, tile)) return;
+  const PrefillRow g = prefill_row(p, r);
+  const int x = 16 * (block % NT) + c, tok = tile * per + block / NT * each + x / p.group;
+  if (x >= each * p.group || tok >= g.lq) return;
+  const Part* part = p.parts + ((int64_t)item * p.hkv + head) * p.splits;
+  const int at = 16 * block + c;
+  float m = kNone;
+  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, part[s].m[at]);
+  f32x4 o[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+  float l = 0;
+  for (int s = 0; s < p.splits; ++s) {
+    const float w = __builtin_amdgcn_exp2f(part[s].m[at] - m);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) o[j] += part[s].o[block][wave + 4 * j][lane] * w;
+    l += part[s].l[at] * w;
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  uint16_t* out = p.out + (g.q0 + tok) * p.out_stride + (head * p.group + x % p.group) * HD + 32 * kg;
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    *reinterpret_cast<u32x2*>(out + 4 * (wave + 4 * j)) =
+        u32x2{pack_bf16x2(o[j][0] * inv, o[j][1] * inv), pack_bf16x2(o[j][2] * inv, o[j][3] * inv)};
+}
+
+// ------------------------------------------------------------------- launch
+constexpr int kMaxPrefillRows = 1024;
+constexpr int kSlots = 512;  // two workgroups fit a CU
+
+struct Plan {
+  bool dwork, pwork;
+  int chunks, items, splits;
+  size_t dbytes, pbytes;
+};
+
+// Steps of 64 keys that queries at `n` consecutive positions may need.
+int64_t most_steps(int64_t window, int64_t sinks, int64_t n, int64_t cap) {
+  const int64_t keys = std::min(window + n, cap);
+  return std::min((keys + 63) / 64 + 1 + (sinks + 63) / 64, (cap + 63) / 64);
+}
+
+Plan plan_of(const slo_paged_attention_args* a, int window, int sinks) {
+  Plan n = {false, false, 0, 0, 1, 0, 0};
+  const int group = a->num_heads / a->num_kv_heads;
+  if (a->num_decode > 0 && (a->phases & SLO_PHASE_DECODE)) {
+    n.dwork = true;
+    const int64_t pairs = (int64_t)a->num_decode * a->num_kv_heads;
+    const int64_t steps = most_steps(window, sinks, 1, (int64_t)a->decode_table_width * a->block_size);
+    n.chunks = (int)std::max<int64_t>(1, std::min((kSlots + pairs - 1) / pairs, (steps + 3) / 4));
+    if (n.chunks > 1) n.dbytes = (size_t)pairs * n.chunks * group * RECORD * 4;
+  }
+  if (a->num_prefill > 0 && (a->phases & SLO_PHASE_PREFILL)) {
+    n.pwork = true;
+    // The rows' queries together bound the tiles.
+    const int per = kWaves * (16 * NT / group);
+    n.items = (int)((int64_t)(a->num_q_rows - a->num_decode) / per + a->num_prefill);
+    const int64_t cap = a->prefill_tables ? (int64_t)a->prefill_table_width * a->block_size : a->num_kv_rows;
+    const int64_t steps = most_steps(window, sinks, per, cap);
+    const int64_t wgs = (int64_t)n.items * a->num_kv_heads;
+    n.splits = (int)std::max<int64_t>(1, std::min(kSlots / wgs, steps / 8));
+    if (n.splits > 1) n.pbytes = (size_t)wgs * n.splits * sizeof(Part);
+  }
+  return n;
+}
+
+int64_t workgroups(const slo_paged_attention_args* a, const Plan& n) {
+  const int64_t joined = (n.chunks > 1 ? a->num_decode : 0) + (n.splits > 1 ? (int64_t)n.items * kWaves * NT : 0);
+  return std::max((int64_t)n.items * n.splits + (int64_t)a->num_decode * n.chunks, joined) * a->num_kv_heads;
+}
+
+int check_args(const slo_paged_attention_args* a, int window, int sinks) {
+  if (!a) return fail(SLO_ERR_INVALID, "paged_attention_window: null args");
+  if (window <= 0 || sinks < 0) return fail(SLO_ERR_INVALID, "paged_attention_window: window must be positive and sinks not negative");
+  if (a->head_dim != HD) return fail(SLO_ERR_UNSUPPORTED, "paged_attention_window: head_dim must be 128");
+  if (a->num_heads <= 0 || a->num_kv_heads <= 0 || a->num_heads % a->num_kv_heads)
+    return fail(SLO_ERR_INVALID, "paged_attention_window: num_heads must be a multiple of num_kv_heads");
+  if (a->num_heads / a->num_kv_heads > 16)
+    return fail(SLO_ERR_UNSUPPORTED, "paged_attention_window: at most 16 query heads per kv head");
+  if (a->num_kv_heads > 4096) return fail(SLO_ERR_UNSUPPORTED, "paged_attention_window: more than 4096 kv heads");
+  if (a->kv_dtype < KV_BF16 || a->kv_dtype > KV_FP4_E2M1) return fail(SLO_ERR_INVALID, "paged_attention_window: bad kv_dtype");
+  if (a->num_q_rows < 0 || a->num_decode < 0 || a->num_prefill < 0 || a->num_decode > a->num_q_rows)
+    return fail(SLO_ERR_INVALID, "paged_attention_window: bad row counts");
+  if (!(a->softmax_scale != 0.0f) || a->softmax_scale - a->softmax_scale != 0.0f)
+    return fail(SLO_ERR_INVALID, "paged_attention_window: softmax_scale must be finite and not zero");
+  if (a->store_slot_mapping) return fail(SLO_ERR_INVALID, "paged_attention_window: store the new rows first");
+  if (a->num_decode > 32768 || a->num_prefill > kMaxPrefillRows)
+    return fail(SLO_ERR_UNSUPPORTED, "paged_attention_window: more than 32768 decode or 1024 prefill rows");
+  const bool dec = a->num_decode > 0 && (a->phases & SLO_PHASE_DECODE);
+  const bool pre = a->num_prefill > 0 && (a->phases & SLO_PHASE_PREFILL);
+  if (!dec && !pre) return SLO_OK;
+  if (!a->q || !a->out) return fail(SLO_ERR_INVALID, "paged_attention_window: null pointer");
+  if ((a->q_row_stride % 8) || (a->out_row_stride % 8) || a->q_row_stride < a->num_heads * HD ||
+      a->out_row_stride < a->num_heads * HD || (reinterpret_cast<uintptr_t>(a->q) % 16) ||
+      (reinterpret_cast<uintptr_t>(a->out) % 16))
+    return fail(SLO_ERR_INVALID, "paged_attention_window: q and out rows must be 16-byte aligned");
+  if (dec || (pre && a->prefill_tables)) {
+    const bool scaled = a->kv_dtype != KV_BF16;
+    if (!a->k_cache || !a->v_cache || a->num_blocks <= 0 || (scaled && (!a->k_scale || !a->v_scale)))
+      return fail(SLO_ERR_INVALID, "paged_attention_window: no KV pool or no scales");
+    if ((reinterpret_cast<uintptr_t>(a->k_cache) % 16) || (reinterpret_cast<uintptr_t>(a->v_cache) % 16) ||
+        (scaled && ((reinterpret_cast<uintptr_t>(a->k_scale) % 16) || (reinterpret_cast<uintptr_t>(a->v_scale) % 16))))
+      return fail(SLO_ERR_INVALID, "paged_attention_window: pools and scales must be 16-byte aligned");
+    if (a->block_size <= 0 || a->block_size % 64)
+      return fail(SLO_ERR_UNSUPPORTED, "paged_attention_window: block_size must be a multiple of 64");
+  }
+  if (dec && (!a->decode_lens || !a->decode_tables || a->decode_table_width <= 0))
+    return fail(SLO_ERR_INVALID, "paged_attention_window: missing decode metadata");
+  if (pre && (!a->prefill_cu_q || !a->prefill_cu_k || (a->prefill_tables && a->prefill_table_width <= 0)))
+    return fail(SLO_ERR_INVALID, "paged_attention_window: missing prefill metadata");
+  if (pre && !a->prefill_tables) {
+    if (!a->k || !a->v || a->num_kv_rows <= 0) return fail(SLO_ERR_INVALID, "paged_attention_window: prefill rows without tables need k and v");
+    if ((a->k_row_stride % 8) || (a->v_row_stride % 8) || a->k_row_stride < a->num_kv_heads * HD ||
+        a->v_row_stride < a->num_kv_heads * HD || (reinterpret_cast<uintptr_t>(a->k) % 16) ||
+        (reinterpret_cast<uintptr_t>(a->v) % 16))
+      return fail(SLO_ERR_INVALID, "paged_attention_window: k and v rows must be 16-byte aligned, num_kv_heads * 128 elements or more apart");
+  }
+  if ((dec && (int64_t)a->decode_table_width * a->block_size > (1 << 22)) ||
+      (pre && a->prefill_tables && (int64_t)a->prefill_table_width * a->block_size > (1 << 22)) ||
+      (pre && !a->prefill_tables && a->num_kv_rows > (1 << 24)))
+    return fail(SLO_ERR_UNSUPPORTED, "paged_attention_window: tables span more than 2^22 tokens, or more than 2^24 k rows");
+  // A grid holds less than 2^32 threads.
+  if (workgroups(a, plan_of(a, window, sinks)) >= 1 << 24)
+    return fail(SLO_ERR_UNSUPPORTED, "paged_attention_window: too many rows times kv heads in one call");
+  return SLO_OK;
+}
+
+template <int F>
+void launch(const WinParams& p, hipStream_t s) {
+  const unsigned blocks = (unsigned)(((int64_t)p.items * p.splits + (int64_t)p.drows * p.chunks) * p.hkv);
+  hipLaunchKernelGGL(window_attention_kernel<F>, dim3(blocks), dim3(64 * kWaves), 0, s, p);
+  const int decode = p.chunks > 1 ? p.drows * p.hkv : 0;
+  const int prefill = p.splits > 1 ? p.items * p.hkv * kWaves * NT : 0;
+  if (decode + prefill) hipLaunchKernelGGL(window_join_kernel<F>, dim3(decode + prefill), dim3(256), 0, s, p, decode);
+}
+
+}  // namespace
+}  // namespace slo
+
+using namespace slo;
+
+extern "C" int slo_paged_attention_window_workspace_bytes(const slo_paged_attention_args* a, int32_t window, int32_t sinks,
+                                                          size_t* bytes) {
+  if (!bytes) return fail(SLO_ERR_INVALID, "paged_attention_window: null pointer");
+  const int rc = check_args(a, window, sinks);
+  if (rc) return rc;
+  const Plan n = plan_of(a, window, sinks);
+  *bytes = n.dbytes + n.pbytes;
+  return SLO_OK;
+}
+
+extern "C" int slo_paged_attention_window(const slo_paged_attention_args* a, int32_t window, int32_t sinks,
+                                          slo_stream_t stream) {
+  const int rc = check_args(a, window, sinks);
+  if (rc) return rc;
+  const Plan n = plan_of(a, window, sinks);
+  if (n.dbytes + n.pbytes > 0 && (!a->workspace || a->workspace_bytes < n.dbytes + n.pbytes ||
+                                  reinterpret_cast<uintptr_t>(a->workspace) % 16))
+    return fail(SLO_ERR_WORKSPACE, "paged_attention_window: workspace smaller than slo_paged_attention_window_workspace_bytes");
+  if (!n.dwork && !n.pwork) return SLO_OK;
+  WinParams p = {};
+  p.q = static_cast<const uint16_t*>(a->q);
+  p.q_stride = a->q_row_stride;
+  p.out = static_cast<uint16_t*>(a->out);
+  p.out_stride = a->out_row_stride;
+  p.num_q_rows = a->num_q_rows;
+  p.kc = static_cast<const uint8_t*>(a->k_cache);
+  p.vc = static_cast<const uint8_t*>(a->v_cache);
+  p.ks = a->k_scale;
+  p.vs = a->v_scale;
+  p.num_blocks = a->num_blocks;
+  p.block_size = a->block_size;
+  p.tpb = a->block_size > 0 ? a->block_size / 64 : 1;
+  p.tpb_inv = (uint32_t)((0xffffffffull + p.tpb) / p.tpb);
+  p.hq = a->num_heads;
+  p.hkv = a->num_kv_heads;
+  p.group = a->num_heads / a->num_kv_heads;
+  p.scale_log2 = (a->softmax_scale < 0 ? -a->softmax_scale : a->softmax_scale) * kLog2e;
+  p.q_sign = a->softmax_scale < 0 ? 0x80008000u : 0u;
+  p.window = std::min(window, 1 << 26);
+  p.sinks = std::min(sinks, 1 << 26);
+  const bool rows = a->num_prefill > 0 && a->prefill_cu_q;  // whatever the phases
+  p.ends = rows ? a->prefill_cu_q + a->num_prefill : nullptr;
+  p.first_idle = p.first_row = a->num_decode;
+  p.idle = n.pwork || a->num_q_rows > a->num_decode;
+  p.chunks = p.splits = 1;
+  if (n.dwork) {
+    p.lens = a->decode_lens;
+    p.dtables = a->decode_tables;
+    p.dstride = a->decode_table_stride;
+    p.dwidth = a->decode_table_width;
+    p.drows = a->num_decode;
+    p.chunks = n.chunks;
+    p.records = static_cast<float*>(a->workspace);
+  }
+  if (n.pwork) {
+    p.cu_q = a->prefill_cu_q;
+    p.cu_k = a->prefill_cu_k;
+    p.ptables = a->prefill_tables;
+    p.pstride = a->prefill_table_stride;
+    p.pwidth = a->prefill_table_width;
+    p.prows = a->num_prefill;
+    p.items = n.items;
+    p.splits = n.splits;
+    p.parts = reinterpret_cast<Part*>(static_cast<char*>(a->workspace) + n.dbytes);
+    p.rk = static_cast<const uint8_t*>(a->k);
+    p.rv = static_cast<const uint8_t*>(a->v);
+    p.rk_stride = 2 * a->k_row_stride;
+    p.rv_stride = 2 * a->v_row_stride;
+    p.num_kv_rows = a->num_kv_rows;
+  }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (n.pwork && !p.ptables && a->kv_dtype != KV_BF16) {
+    // The step's own rows are bf16 whatever the pool's format.
+    WinParams cold = p;
+    cold.drows = 0;
+    launch<KV_BF16>(cold, s);
+    p.items = 0;
+    p.splits = 1;
+    p.idle = false;
+  }
+  if (p.items || p.drows) {
+    if (a->kv_dtype == KV_BF16) launch<KV_BF16>(p, s);
+    else if (a->kv_dtype == KV_FP8_E4M3FN) launch<KV_FP8_E4M3FN>(p, s);
+    else launch<KV_FP4_E2M1>(p, s);
+  }
+  return check_launch("paged_attention_window");
+}

@@ -91,6 +91,7 @@ _lib = None
 EXPORTS = (
     "slo_store_kvcache",
     "slo_qk_norm_rope_store",
+    "slo_rope_store",
     "slo_lm_head_argmax",
     "slo_build_mixed_metadata",
     "slo_attention_workspace_bytes",
@@ -101,6 +102,8 @@ EXPORTS = (
     "slo_load_kvcache",
     "slo_paged_attention_fp4_workspace_bytes",
     "slo_paged_attention_fp4",
+    "slo_paged_attention_window_workspace_bytes",
+    "slo_paged_attention_window",
     "slo_accumulate_attention_workspace_bytes",
     "slo_accumulate_attention",
     "slo_evict_kv",
@@ -132,6 +135,11 @@ def load() -> ctypes.CDLL:
             _c_void_p, _c_int64, _c_void_p, _c_int32, _c_int32, _c_int32, _c_int32, _c_void_p, _c_void_p,
             ctypes.c_float, _c_void_p, _c_int32, _c_void_p, _c_void_p, _c_void_p, _c_int32, _c_void_p, _c_void_p,
             _c_void_p, _c_void_p, _c_int64, ctypes.c_float, _c_void_p]
+        lib.slo_rope_store.restype = ctypes.c_int
+        lib.slo_rope_store.argtypes = [
+            _c_void_p, _c_int64, _c_void_p, _c_int32, _c_int32, _c_int32, _c_int32, _c_void_p, _c_void_p,
+            ctypes.c_float, _c_void_p, _c_int32, _c_int32, _c_int32, _c_void_p, _c_void_p, _c_void_p, _c_int32, _c_void_p,
+            _c_void_p, _c_void_p, _c_void_p, _c_int64, ctypes.c_float, _c_void_p]
         lib.slo_lm_head_argmax.restype = ctypes.c_int
         lib.slo_lm_head_argmax.argtypes = [
             _c_void_p, _c_int64, _c_int32, _c_void_p, _c_int64, _c_int32, _c_int32, _c_void_p, _c_int64,
@@ -162,6 +170,11 @@ def load() -> ctypes.CDLL:
             getattr(lib, name).argtypes = [ctypes.c_char_p, ctypes.POINTER(ctypes.c_size_t)]
         lib.slo_paged_attention_fp4.restype = ctypes.c_int
         lib.slo_paged_attention_fp4.argtypes = [ctypes.c_char_p, _c_void_p]
+        lib.slo_paged_attention_window_workspace_bytes.restype = ctypes.c_int
+        lib.slo_paged_attention_window_workspace_bytes.argtypes = [ctypes.c_char_p, _c_int32, _c_int32,
+                                                                   ctypes.POINTER(ctypes.c_size_t)]
+        lib.slo_paged_attention_window.restype = ctypes.c_int
+        lib.slo_paged_attention_window.argtypes = [ctypes.c_char_p, _c_int32, _c_int32, _c_void_p]
         lib.slo_accumulate_attention.restype = ctypes.c_int
         lib.slo_accumulate_attention.argtypes = [ctypes.c_char_p, _c_void_p, _c_void_p]
         lib.slo_evict_kv.restype = ctypes.c_int

@@ -21,6 +21,9 @@ Prompts that come without block tables are whole: the slots that their tokens
 were written to say which pages they have.
 ``forward(q, k, v, kv_stored=True)`` skips the KV write, for callers whose
 ``qk_norm_rope_store`` already wrote this step's K/V into the pool.
+``Attention(..., window=W, sinks=S)`` is a layer with a sliding window: a query
+sees the W newest tokens up to its own and the row's first S.  Its KV write is a
+launch of its own, and it takes no ``kv_scores``.
 """
 from __future__ import annotations
 
@@ -54,8 +57,10 @@ def _pages_of_slots(slots: torch.Tensor, cu_k: torch.Tensor, max_k: int, block_s
 
 class Attention(nn.Module):
 
-    def __init__(self, num_heads, head_dim, scale, num_kv_heads):
+    def __init__(self, num_heads, head_dim, scale, num_kv_heads, window=0, sinks=0):
         super().__init__()
+        if window < 0 or sinks < 0 or (sinks and not window):
+            raise ValueError("window must be positive (0 without sinks: no window) and sinks not negative")
         self.num_heads = num_heads
         self.head_dim = head_dim
         self.scale = scale
@@ -63,6 +68,7 @@ class Attention(nn.Module):
         self.k_cache = self.v_cache = torch.tensor([])
         self.k_scale = self.v_scale = None
         self.kv_scores = None
+        self.window, self.sinks = window, sinks
 
     def _scales(self):
         return () if self.k_scale is None else (self.k_scale, self.v_scale)
@@ -70,9 +76,12 @@ class Attention(nn.Module):
     def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_stored: bool = False):
         context = get_context()
         k_cache, v_cache = self.k_cache, self.v_cache
+        span = dict(window=self.window, sinks=self.sinks)
+        if self.window and self.kv_scores is not None:
+            raise ValueError("a layer with a window takes no kv_scores: attach a pool without track_scores")
         if context.mixed is not None:
             o = forward_mixed(q, k, v, k_cache, v_cache, context, self.scale,
-                              _stored if kv_stored else store_kvcache, self.k_scale, self.v_scale)
+                              _stored if kv_stored else store_kvcache, self.k_scale, self.v_scale, **span)
             if self.kv_scores is not None:
                 meta = context.mixed
                 self._weigh(q, num_decode=meta.num_decode, decode_lens=meta.decode_lens, decode_tables=meta.decode_tables,
@@ -91,7 +100,7 @@ class Attention(nn.Module):
         # write their own tokens.  A prefill step that reads the pool hands over
         # contiguous bf16 rows only; otherwise the store kernel runs first.
         paged = context.is_prefill and context.block_tables is not None
-        fold = have_cache and not kv_stored and (
+        fold = have_cache and not kv_stored and not self.window and (
             (self.k_scale is None and not is_fp4(k_cache) and foldable(k, v))
             or (not paged and folds_alone(q, k, v, k_cache, self.k_scale)))
         if fold:
@@ -109,7 +118,7 @@ class Attention(nn.Module):
                 prefill_cu_q=context.cu_seqlens_q, prefill_cu_k=context.cu_seqlens_k,
                 max_q=context.max_seqlen_q, max_k=context.max_seqlen_k,
                 prefill_tables=context.block_tables, k=None if paged else k, v=None if paged else v,
-                phases=_lib.PHASE_ALL if paged else _lib.PHASE_ALL | _lib.NEW_ROWS_STRIDED, **store)
+                phases=_lib.PHASE_ALL if paged else _lib.PHASE_ALL | _lib.NEW_ROWS_STRIDED, **store, **span)
             if self.kv_scores is not None and have_cache:
                 self._weigh(q, num_prefill=rows, prefill_cu_q=context.cu_seqlens_q, prefill_cu_k=context.cu_seqlens_k,
                             max_q=context.max_seqlen_q, max_k=context.max_seqlen_k, prefill_tables=context.block_tables,
@@ -119,7 +128,7 @@ class Attention(nn.Module):
             q, k_cache, v_cache, self.scale, num_kv_heads=self.num_kv_heads,
             k_scale=self.k_scale, v_scale=self.v_scale, num_decode=q.shape[0],
             decode_lens=context.context_lens, decode_tables=context.block_tables,
-            phases=_lib.PHASE_ALL | _lib.NEW_ROWS_STRIDED, **store)
+            phases=_lib.PHASE_ALL | _lib.NEW_ROWS_STRIDED, **store, **span)
         if self.kv_scores is not None:
             self._weigh(q, num_decode=q.shape[0], decode_lens=context.context_lens, decode_tables=context.block_tables)
         return o.unsqueeze(1)

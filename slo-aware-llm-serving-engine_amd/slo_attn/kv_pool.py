@@ -64,6 +64,17 @@ def num_kv_blocks(total: int, used: int, peak: int, current: int, gpu_memory_uti
     return count
 
 
+def window_blocks(length: int, window: int, sinks: int, block_size: int) -> range:
+    """Places in the block table of a row of ``length`` cached tokens whose pages no later token sees.
+
+    A token at position t >= ``length`` sees the keys j > t - window and j <
+    sinks.  An engine gives these pages back (or to another row) and puts -1 in
+    their places: attention with the window does not read them."""
+    if window <= 0 or sinks < 0 or block_size <= 0:
+        raise ValueError("window and block_size must be positive and sinks not negative")
+    return range(-(-sinks // block_size), max(length - window + 1, 0) // block_size)
+
+
 class KVPool:
     """One pool for all layers: codes or bf16 values, and the scales of the quantised formats.
 

@@ -32,7 +32,7 @@ class MixedAttentionContext:
 
 
 def forward_mixed(q, k, v, k_cache, v_cache, context, scale, store_fn,
-                  k_scale=None, v_scale=None, phases=_lib.PHASE_ALL):
+                  k_scale=None, v_scale=None, phases=_lib.PHASE_ALL, window=0, sinks=0):
     """Write all new K/V first, then attend: decode rows first, prefill after.
 
     Same arguments as the reference (mixed_attention.py:29).  ``k_scale`` /
@@ -40,7 +40,8 @@ def forward_mixed(q, k, v, k_cache, v_cache, context, scale, store_fn,
     a 4-bit cache.  ``phases``
     restricts the launch to decode or prefill rows (the split mode that mirrors
     the reference's per-phase calls); rows of the other phase are left
-    untouched in the returned tensor.
+    untouched in the returned tensor.  ``window`` and ``sinks`` are
+    ``paged_attention``'s.
     """
     meta = context.mixed
     if not k_cache.numel() or not v_cache.numel():
@@ -58,8 +59,8 @@ def forward_mixed(q, k, v, k_cache, v_cache, context, scale, store_fn,
     # tokens' tiles in every item (24 decode rows and two chunks, one after a
     # 1,024-token prefix: 108 against 72 us).  Any other store_fn runs first.
     alone = not meta.num_prefill_tokens or (not meta.num_decode and not meta.prefill_has_history)
-    # A 4-bit pool keeps the store kernel: its launches read pages only.
-    fold = (store_fn is store_kvcache and phases == _lib.PHASE_ALL and not is_fp4(k_cache)
+    # A 4-bit pool and a window keep the store kernel: their launches read pages only.
+    fold = (store_fn is store_kvcache and phases == _lib.PHASE_ALL and not is_fp4(k_cache) and not window
             and ((foldable(k, v)
                   and (k_scale is None or (q.shape[1] <= 8 * k.shape[1] and not meta.num_prefill_tokens)))
                  or (alone and folds_alone(q, k, v, k_cache, k_scale))))
@@ -84,4 +85,4 @@ def forward_mixed(q, k, v, k_cache, v_cache, context, scale, store_fn,
         prefill_tables=meta.prefill_tables if history else None,
         k=None if history else k[d:], v=None if history else v[d:], phases=phases,
         store_slot_mapping=context.slot_mapping if fold else None, new_k=k if fold else None,
-        new_v=v if fold else None)
+        new_v=v if fold else None, window=window, sinks=sinks)

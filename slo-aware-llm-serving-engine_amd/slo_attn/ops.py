@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import math
 import threading
 
 import torch
@@ -276,24 +277,71 @@ def load_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: tor
 
 
 # ------------------------------------------- fused q/k norm + RoPE + KV write
-def rope_cos_sin(head_dim: int, max_position: int, base: float, device) -> torch.Tensor:
-    """fp32 [max_position, head_dim] table: cos(p * inv_freq) then sin(p * inv_freq).
+def _inverse_frequencies(dim: int, base: float, scaling: dict) -> tuple[torch.Tensor, float]:
+    """fp64 frequencies of ``dim / 2`` channel pairs, and the table's factor, after ``scaling``."""
+    i = torch.arange(0, dim, 2, dtype=torch.float64)
+    freq = base ** (-i / dim)
+    kind = scaling.get("rope_type", scaling.get("type", "default"))
+    if kind == "default":
+        return freq, 1.0
+    if kind not in ("linear", "yarn"):
+        raise ValueError(f"rope scaling {kind!r} is not default, linear or yarn")
+    factor = float(scaling["factor"])
+    if not factor >= 1.0 or factor == float("inf"):
+        raise ValueError("the rope scaling factor must be finite and at least 1")
+    if kind == "linear":
+        return freq / factor, 1.0
+    trained = scaling["original_max_position_embeddings"]
+    size = scaling.get("attention_factor")
+    if size is None:
+        size = 0.1 * math.log(factor) + 1.0
 
-    The cos_sin_cache of RotaryEmbedding (nanovllm/layers/rotary_embedding.py:27-35),
-    built with the same torch operations on ``device``.
+    def channel(turns):  # the pair that turns so many times in the trained positions
+        return dim * math.log(trained / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+    low = max(math.floor(channel(scaling.get("beta_fast") or 32.0)), 0)
+    high = min(math.ceil(channel(scaling.get("beta_slow") or 1.0)), dim - 1)
+    ramp = ((i / 2 - low) / max(high - low, 0.001)).clamp(0, 1)
+    return freq / factor * ramp + freq * (1 - ramp), float(size)
+
+
+def rope_cos_sin(head_dim: int, max_position: int, base: float, device, rotary_dim: int | None = None,
+                 scaling: dict | None = None) -> torch.Tensor:
+    """fp32 [max_position, rotary_dim] table: cos(p * inv_freq) then sin(p * inv_freq).
+
+    Without ``rotary_dim`` and ``scaling``, the cos_sin_cache of RotaryEmbedding
+    (nanovllm/layers/rotary_embedding.py:27-35), built with the same torch
+    operations on ``device``.  Otherwise the angles are taken in 64 bits and the
+    table rounded once: 32 bits leave an angle of 10^5 positions off by 0.004.
+    ``rotary_dim``: the channels of a head that turn (default all of them).
+    ``scaling``: a model configuration's rope scaling, by its ``rope_type``:
+    "linear" divides every frequency by ``factor``; "yarn" only those of pairs
+    that turn less than ``beta_slow`` (1) times in
+    ``original_max_position_embeddings`` positions, leaves those that turn more
+    than ``beta_fast`` (32) times, goes from one to the other linearly over the
+    pairs between, and multiplies the table by ``attention_factor`` (0.1
+    ln(factor) + 1).
     """
+    if rotary_dim is not None or scaling is not None:
+        dim = head_dim if rotary_dim is None else rotary_dim
+        if not 0 < dim <= head_dim or dim % 2:
+            raise ValueError("rotary_dim must be even, from 2 to head_dim")
+        freq, size = _inverse_frequencies(dim, float(base), scaling or {})
+        angle = torch.arange(max_position, dtype=torch.float64, device=device)[:, None] * freq.to(device)
+        return (torch.cat((angle.cos(), angle.sin()), dim=-1) * size).float()
     inv_freq = 1.0 / (base ** (torch.arange(0, head_dim, 2, dtype=torch.float, device=device) / head_dim))
     t = torch.arange(max_position, dtype=torch.float, device=device)
     freqs = torch.einsum("i,j -> ij", t, inv_freq)
     return torch.cat((freqs.cos(), freqs.sin()), dim=-1).contiguous()
 
 
-def qk_norm_rope_store(qkv: torch.Tensor, positions: torch.Tensor, q_norm_weight: torch.Tensor,
-                       k_norm_weight: torch.Tensor, eps: float, cos_sin: torch.Tensor, num_heads: int,
+def qk_norm_rope_store(qkv: torch.Tensor, positions: torch.Tensor, q_norm_weight: torch.Tensor | None,
+                       k_norm_weight: torch.Tensor | None, eps: float, cos_sin: torch.Tensor, num_heads: int,
                        num_kv_heads: int, k_cache: torch.Tensor, v_cache: torch.Tensor,
                        slot_mapping: torch.Tensor, k_scale: torch.Tensor | None = None,
                        v_scale: torch.Tensor | None = None, head_dim: int = 128,
-                       scale_floor: float = _lib.FP8_SCALE_FLOOR):
+                       scale_floor: float = _lib.FP8_SCALE_FLOOR, *, rotary_dim: int | None = None,
+                       interleaved: bool = False):
     """q_norm, k_norm, rotary_emb and the KV write of one layer in one launch.
 
     Covers nanovllm/models/qwen3.py:80-86 up to the attention call, and the
@@ -304,7 +352,19 @@ def qk_norm_rope_store(qkv: torch.Tensor, positions: torch.Tensor, q_norm_weight
     The pool receives the rotated k and v at ``slot_mapping`` (bf16, or
     E4M3FN or 4 bits with ``k_scale``/``v_scale``), as ``store_kvcache`` writes
     them; into a 4-bit pool they go in a second launch.
+
+    ``rotary_dim`` (a multiple of 8; default ``head_dim``): only so many first
+    channels of a head turn, and ``cos_sin`` has as many columns.
+    ``interleaved``: the channels turn in pairs (2i, 2i + 1) instead of
+    (i, i + rotary_dim / 2).  Norm weights of None: q and k are only rotated.
+    ``head_dim`` is 64, 128 or 256.  In these layouts norm and rotation are
+    computed in fp32 and rounded once; the reference's (128 channels in halves,
+    both norms) keeps the reference's roundings to bf16 after each step.
     """
+    rot = head_dim if rotary_dim is None else int(rotary_dim)
+    if interleaved or rot != head_dim or head_dim != 128 or q_norm_weight is None or k_norm_weight is None:
+        return _rope_store(qkv, positions, q_norm_weight, k_norm_weight, eps, cos_sin, num_heads, num_kv_heads, k_cache, v_cache,
+                           slot_mapping, k_scale, v_scale, head_dim, scale_floor, rot, interleaved)
     if qkv.dim() != 2 or qkv.stride(-1) != 1:
         raise ValueError("qkv must be a [tokens, width] tensor with contiguous rows")
     N = qkv.shape[0]
@@ -352,6 +412,45 @@ def qk_norm_rope_store(qkv: torch.Tensor, positions: torch.Tensor, q_norm_weight
         _ptr(k_norm_weight), float(eps), _ptr(cos_sin), cos_sin.shape[0], _ptr(q), _ptr(k), _ptr(slot_mapping),
         _lib.KV_BF16 if fp4 else code, _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), num_slots,
         float(scale_floor), _stream(device)), "slo_qk_norm_rope_store")
+    v = qkv[:, (num_heads + num_kv_heads) * head_dim:].view(N, num_kv_heads, head_dim)
+    if fp4:
+        store_kvcache(k, v, k_cache, v_cache, slot_mapping, k_scale, v_scale, scale_floor)
+    return q, k, v
+
+
+def _rope_store(qkv, positions, q_norm_weight, k_norm_weight, eps, cos_sin, num_heads, num_kv_heads, k_cache, v_cache,
+                slot_mapping, k_scale, v_scale, head_dim, scale_floor, rot, interleaved):
+    """``qk_norm_rope_store`` in any layout but the reference's."""
+    width = (num_heads + 2 * num_kv_heads) * head_dim
+    if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] != width:
+        raise ValueError(f"qkv must be [tokens, {width}] with contiguous rows")
+    if not 0 < rot <= head_dim or rot % 8:
+        raise ValueError("rotary_dim must be a multiple of 8 up to head_dim")
+    index = _one_device(qkv, positions, q_norm_weight, k_norm_weight, cos_sin, k_cache, v_cache, slot_mapping, k_scale, v_scale)
+    N = qkv.shape[0]
+    if qkv.dtype != torch.bfloat16:
+        raise TypeError("qkv must be bf16")
+    if positions.dtype != torch.int64 or positions.numel() != N or not positions.is_contiguous():
+        raise ValueError("positions must be a contiguous int64 [tokens] tensor")
+    if (q_norm_weight is None) != (k_norm_weight is None):
+        raise ValueError("the norms of both q and k, or of neither")
+    for w in (q_norm_weight, k_norm_weight):
+        if w is not None and (w.dtype != torch.bfloat16 or w.numel() != head_dim or not w.is_contiguous()):
+            raise ValueError("norm weights must be contiguous bf16 [head_dim] tensors")
+    if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or cos_sin.shape[1] != rot or not cos_sin.is_contiguous():
+        raise ValueError("cos_sin must be a contiguous fp32 [max_position, rotary_dim] table")
+    code, blocks, block, heads, d = _pool_geometry(k_cache, k_scale, v_cache, v_scale)
+    if (heads, d) != (num_kv_heads, head_dim):
+        raise ValueError(f"KV pool holds {heads} kv heads of {d}, not {num_kv_heads} of {head_dim}")
+    if slot_mapping.dtype != torch.int32 or slot_mapping.numel() != N or not slot_mapping.is_contiguous():
+        raise ValueError("slot_mapping must be a contiguous int32 [tokens] tensor")
+    q = torch.empty((N, num_heads, head_dim), dtype=torch.bfloat16, device=qkv.device)
+    k = torch.empty((N, num_kv_heads, head_dim), dtype=torch.bfloat16, device=qkv.device)
+    fp4 = code == _lib.KV_FP4_E2M1  # the kernel then writes q and k only: a pool of no slots
+    _launch(index, "slo_rope_store", qkv.data_ptr(), qkv.stride(0) if N > 1 else width, positions.data_ptr(), N, num_heads,
+            num_kv_heads, head_dim, _ptr(q_norm_weight), _ptr(k_norm_weight), eps, cos_sin.data_ptr(), cos_sin.shape[0], rot,
+            interleaved, q.data_ptr(), k.data_ptr(), slot_mapping.data_ptr(), _lib.KV_BF16 if fp4 else code, k_cache.data_ptr(),
+            v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), 0 if fp4 else blocks * block, scale_floor)
     v = qkv[:, (num_heads + num_kv_heads) * head_dim:].view(N, num_kv_heads, head_dim)
     if fp4:
         store_kvcache(k, v, k_cache, v_cache, slot_mapping, k_scale, v_scale, scale_floor)
@@ -496,19 +595,21 @@ def _row_args(T, num_decode, decode_lens, decode_tables, num_prefill, cu_q, cu_k
 _NO_ROWS, _NO_STORE = (None, 0, None, 0, 0), (None, None, 0, None, 0, 0, 0.0)
 
 
-def _pool_call(what, extra, index, device, q, out, k_cache, v_cache, k_scale, v_scale, geometry, rows, scale, phases):
+def _pool_call(what, extra, index, device, q, out, k_cache, v_cache, k_scale, v_scale, geometry, rows, scale, phases, sized=(),
+               own=(0, 0, 0, 0, 0)):
     """Calls ``what`` over a pool with a workspace of the call's own, from torch's allocator: calls on several streams,
-    and graphs captured apart, do not share one, and it need not be cleared."""
+    and graphs captured apart, do not share one, and it need not be cleared.  ``sized``: what its size depends on
+    besides the arguments; ``own``: k, v, their strides and rows where prefill rows have no tables."""
     code, blocks, block, heads, head_dim = geometry
     T, num_heads, _ = q.shape
     decode, prefill = rows
     fields = (q.data_ptr(), q.stride(0) if T > 1 else num_heads * head_dim, _ptr(out) or 0,
-              0 if out is None else out.stride(0) if T > 1 else num_heads * head_dim, T, k_cache.data_ptr(), _ptr(v_cache) or 0,
+              0 if out is None else out.stride(0) if T > 1 else num_heads * head_dim, T, _ptr(k_cache) or 0, _ptr(v_cache) or 0,
               _ptr(k_scale) or 0, _ptr(v_scale) or 0, code, blocks, block, *(x or 0 for x in decode), *(x or 0 for x in prefill),
-              0, 0, 0, 0, 0, num_heads, heads, head_dim, scale)
+              *own, num_heads, heads, head_dim, scale)
     args = _lib.pack_attention_args(*fields, 0, 0, phases, 0, 0, 0, 0, 0, 0, 0.0)
-    need = _workspace_need(args, what, T, num_heads, heads, code, block, phases, decode[0], decode[4], prefill[0], prefill[3],
-                           prefill[4], prefill[7])
+    need = _workspace_need(args, sized, what, T, num_heads, heads, code, block, phases, decode[0], decode[4], prefill[0],
+                           prefill[3], prefill[4], prefill[7], own[4])
     if need:
         ws = torch.empty(need, dtype=torch.uint8, device=device)
         args = _lib.pack_attention_args(*fields, ws.data_ptr(), need, phases, 0, 0, 0, 0, 0, 0, 0.0)
@@ -518,12 +619,12 @@ def _pool_call(what, extra, index, device, q, out, k_cache, v_cache, k_scale, v_
 _sizes: dict[tuple, int] = {}  # workspace bytes by entry point and sizes
 
 
-def _workspace_need(args, *key) -> int:
-    what = key[0]
+def _workspace_need(args, sized, *key) -> int:
+    what, key = key[0], (*key, *sized)
     need = _sizes.get(key)
     if need is None:
         size = ctypes.c_size_t(0)
-        _lib.check(getattr(_lib.load(), what + "_workspace_bytes")(args, ctypes.byref(size)), what)
+        _lib.check(getattr(_lib.load(), what + "_workspace_bytes")(args, *sized, ctypes.byref(size)), what)
         if len(_sizes) >= 4096:
             _sizes.clear()
         need = _sizes[key] = size.value
@@ -637,7 +738,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor | None, v_cache: torc
                     phases: int = _lib.PHASE_ALL, out: torch.Tensor | None = None,
                     store_slot_mapping: torch.Tensor | None = None, new_k: torch.Tensor | None = None,
                     new_v: torch.Tensor | None = None, noalloc: bool = False,
-                    store_scale_floor: float = _lib.FP8_SCALE_FLOOR) -> torch.Tensor:
+                    store_scale_floor: float = _lib.FP8_SCALE_FLOOR, window: int = 0, sinks: int = 0) -> torch.Tensor:
     """One ragged launch: decode rows ``q[:num_decode]``, then prefill rows.
 
     Decode row b attends to ``decode_lens[b]`` cached tokens through
@@ -665,7 +766,17 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor | None, v_cache: torc
     ``noalloc=True`` launches through ``slo_paged_attention_noalloc``, which
     uses the library's static per-GPU scratch instead of this module's
     workspace (pass ``out`` as well and nothing is allocated).
+
+    With ``window`` (0: none) the query at position t sees the keys j <= t with
+    j > t - window or j < ``sinks`` only, over a pool of any format and over the
+    contiguous ``k``/``v``.  Pages without a visible key are not read: an engine
+    may have given them back (``window_blocks``) and put -1 in their places of
+    the tables.  ``store_slot_mapping`` then stores first; ``noalloc`` is refused.
     """
+    if window or sinks:
+        return _paged_attention_window(q, k_cache, v_cache, softmax_scale, num_kv_heads, k_scale, v_scale, num_decode,
+                                       decode_lens, decode_tables, num_prefill, prefill_cu_q, prefill_cu_k, prefill_tables, k, v,
+                                       phases, out, store_slot_mapping, new_k, new_v, noalloc, store_scale_floor, window, sinks)
     if is_fp4(k_cache):
         return _paged_attention_fp4(q, k_cache, v_cache, softmax_scale, num_kv_heads, k_scale, v_scale, num_decode, decode_lens,
                                     decode_tables, num_prefill, prefill_cu_q, prefill_cu_k, max_q, max_k, prefill_tables, k, v,
@@ -794,4 +905,64 @@ def _paged_attention_fp4(q, k_cache, v_cache, softmax_scale, num_kv_heads, k_sca
     rows = _row_args(q.shape[0], num_decode, decode_lens, decode_tables, num_prefill, cu_q, cu_k, max_q, max_k, tables, phases)
     _pool_call("slo_paged_attention_fp4", (), index, q.device, q, out, k_cache, v_cache, k_scale, v_scale, geometry, rows,
                float(softmax_scale), phases)
+    return out
+
+
+def _paged_attention_window(q, k_cache, v_cache, softmax_scale, num_kv_heads, k_scale, v_scale, num_decode, decode_lens,
+                            decode_tables, num_prefill, cu_q, cu_k, tables, k, v, phases, out, slot_mapping, new_k, new_v,
+                            noalloc, scale_floor, window, sinks):
+    """``paged_attention`` with a sliding window, over a pool of any format or the step's own rows."""
+    if window <= 0 or sinks < 0:
+        raise ValueError("window must be positive (0 without sinks: no window) and sinks not negative")
+    if noalloc:
+        raise ValueError("noalloc launches take no window")
+    phases &= _lib.PHASE_ALL
+    pre = num_prefill and phases & _lib.PHASE_PREFILL
+    cold = pre and tables is None
+    pool = k_cache is not None and k_cache.numel()
+    if not pool:
+        if (num_decode and phases & _lib.PHASE_DECODE) or (pre and not cold) or slot_mapping is not None:
+            raise ValueError("decode rows, and prefill rows with block tables, need a KV pool")
+        k_cache = v_cache = k_scale = v_scale = None
+        if q.dim() != 3:
+            raise ValueError("q must be [tokens, num_heads, head_dim]")
+        index = _one_device(q, cu_q, cu_k, k, v, out)
+        if q.dtype != torch.bfloat16:
+            raise TypeError("q must be bf16")
+        if q.stride(2) != 1 or q.stride(1) != q.shape[2]:
+            raise ValueError("q rows must hold contiguous heads")
+        geometry = (_lib.KV_BF16, 0, 0, num_kv_heads, q.shape[2])
+    else:
+        index, geometry = _check_query(q, num_kv_heads, k_cache, k_scale, v_cache, v_scale, True, decode_lens, decode_tables,
+                                       cu_q, cu_k, tables, k, v, out)
+    if out is None:
+        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+    elif out.dtype != torch.bfloat16:
+        raise TypeError("out must be bf16")
+    elif out.shape != q.shape or out.stride(2) != 1 or out.stride(1) != q.shape[2]:
+        raise ValueError("out must be [tokens, num_heads, head_dim] with contiguous heads")
+    own = (0, 0, 0, 0, 0)
+    if cold:
+        if k is None or v is None:
+            raise ValueError("prefill without block tables needs contiguous k and v")
+        for name, t in (("k", k), ("v", v)):
+            if t.dtype != torch.bfloat16 or t.dim() != 3 or t.shape[1:] != (num_kv_heads, q.shape[2]) or t.stride(2) != 1 or \
+                    t.stride(1) != q.shape[2]:
+                raise ValueError(f"{name} must be bf16 [tokens, num_kv_heads, head_dim] rows")
+        width = num_kv_heads * q.shape[2]
+        own = (k.data_ptr(), k.stride(0) if k.shape[0] > 1 else width, v.data_ptr(), v.stride(0) if v.shape[0] > 1 else width,
+               min(k.shape[0], v.shape[0]))
+        decode, _ = _row_args(q.shape[0], num_decode, decode_lens, decode_tables, 0, None, None, 0, 0, None, phases)
+        _int32(cu_q, "cu_seqlens_q")
+        _int32(cu_k, "cu_seqlens_k")
+        if cu_q.numel() < num_prefill + 1 or cu_k.numel() < num_prefill + 1:
+            raise ValueError("cu_seqlens shorter than num_prefill + 1")
+        rows = decode, (num_prefill, cu_q.data_ptr(), cu_k.data_ptr(), 0, 0, None, 0, 0)
+    else:
+        rows = _row_args(q.shape[0], num_decode, decode_lens, decode_tables, num_prefill, cu_q, cu_k, 0, 0, tables, phases)
+    if slot_mapping is not None:
+        store_kvcache(new_k, new_v, k_cache, v_cache, slot_mapping, k_scale, v_scale, scale_floor)
+    size = min(int(window), 1 << 30), min(int(sinks), 1 << 30)
+    _pool_call("slo_paged_attention_window", size, index, q.device, q, out, k_cache, v_cache, k_scale, v_scale, geometry, rows,
+               float(softmax_scale), phases, size, own)
     return out

@@ -118,13 +118,30 @@ int slo_qk_norm_rope_store(const void* qkv, int64_t qkv_row_stride, const int64_
  * computed in fp32 and rounded once.  head_dim 64, 128 or 256; any number of
  * heads; num_slots 0 (k_cache and v_cache may be NULL) writes q and k only.
  */
-int slo_rope_store(const void* qkv, int64_t qkv_row_stride, const int64_t* positions,
-                   int32_t num_tokens, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
-                   const void* q_norm_weight, const void* k_norm_weight, float eps,
-                   const float* cos_sin, int32_t max_position, int32_t rotary_dim,
-                   int32_t interleaved, void* q_out, void* k_out, const int32_t* slot_mapping,
-                   int32_t kv_dtype, void* k_cache, void* v_cache, float* k_scale, float* v_scale,
-                   int64_t num_slots, float scale_floor, slo_stream_t stream);
+typedef struct slo_rope_store_args {
+  const void* qkv;
+  int64_t qkv_row_stride;
+  const int64_t* positions;
+  int32_t num_tokens, num_heads, num_kv_heads, head_dim;
+  const void* q_norm_weight; /* or NULL, both */
+  const void* k_norm_weight;
+  float eps;
+  int32_t max_position;
+  const float* cos_sin; /* [max_position, rotary_dim] */
+  int32_t rotary_dim, interleaved;
+  void* q_out;
+  void* k_out;
+  const int32_t* slot_mapping;
+  int32_t kv_dtype;
+  float scale_floor;
+  void* k_cache;
+  void* v_cache;
+  float* k_scale;
+  float* v_scale;
+  int64_t num_slots;
+} slo_rope_store_args;
+
+int slo_rope_store(const slo_rope_store_args* args, slo_stream_t stream);
 
 /*
  * LM head on the sampled rows with the greedy argmax fused in.
@@ -457,6 +474,7 @@ typedef struct slo_evict_kv_args {
 int slo_evict_kv(const slo_evict_kv_args* args, slo_stream_t stream);
 
 /* Size of slo_evict_kv_args, for binding checks. */
+size_t slo_rope_store_args_size(void);
 size_t slo_evict_kv_args_size(void);
 
 /* Description of the last error on the calling thread ("" if none). */

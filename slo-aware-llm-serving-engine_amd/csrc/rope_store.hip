@@ -186,39 +186,39 @@ inline bool unaligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) %
 
 using namespace slo;
 
-extern "C" int slo_rope_store(const void* qkv, int64_t qkv_row_stride, const int64_t* positions, int32_t num_tokens,
-                              int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, const void* q_norm_weight,
-                              const void* k_norm_weight, float eps, const float* cos_sin, int32_t max_position,
-                              int32_t rotary_dim, int32_t interleaved, void* q_out, void* k_out,
-                              const int32_t* slot_mapping, int32_t kv_dtype, void* k_cache, void* v_cache, float* k_scale,
-                              float* v_scale, int64_t num_slots, float scale_floor, slo_stream_t stream) {
-  if (num_tokens < 0 || num_heads <= 0 || num_kv_heads <= 0) return fail(SLO_ERR_INVALID, "rope_store: bad token/head count");
-  if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+extern "C" int slo_rope_store(const slo_rope_store_args* a, slo_stream_t stream) {
+  if (!a) return fail(SLO_ERR_INVALID, "rope_store: null args");
+  if (a->num_tokens < 0 || a->num_heads <= 0 || a->num_kv_heads <= 0)
+    return fail(SLO_ERR_INVALID, "rope_store: bad token/head count");
+  if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256)
     return fail(SLO_ERR_UNSUPPORTED, "rope_store: head_dim must be 64, 128 or 256");
-  if (rotary_dim <= 0 || rotary_dim > head_dim || rotary_dim % 8)
+  if (a->rotary_dim <= 0 || a->rotary_dim > a->head_dim || a->rotary_dim % 8)
     return fail(SLO_ERR_INVALID, "rope_store: rotary_dim must be a multiple of 8 up to head_dim");
-  if (kv_dtype != KV_BF16 && kv_dtype != KV_FP8_E4M3FN) return fail(SLO_ERR_INVALID, "rope_store: bad kv_dtype");
-  if (max_position <= 0 || num_slots < 0) return fail(SLO_ERR_INVALID, "rope_store: max_position must be positive");
-  if ((int64_t)num_heads + 2 * (int64_t)num_kv_heads > 65536) return fail(SLO_ERR_UNSUPPORTED, "rope_store: too many heads");
-  if ((q_norm_weight == nullptr) != (k_norm_weight == nullptr))
-    return fail(SLO_ERR_INVALID, "rope_store: weights of both norms, or of neither");
-  if (q_norm_weight && !(eps >= 0.0f)) return fail(SLO_ERR_INVALID, "rope_store: eps must be >= 0");
-  if (num_tokens == 0) return SLO_OK;
-  if (!qkv || !positions || !cos_sin || !q_out || !k_out || !slot_mapping || (num_slots && (!k_cache || !v_cache)))
+  const bool fp8 = a->kv_dtype == KV_FP8_E4M3FN;
+  if (a->kv_dtype != KV_BF16 && !fp8) return fail(SLO_ERR_INVALID, "rope_store: bad kv_dtype");
+  if (a->max_position <= 0 || a->num_slots < 0)
+    return fail(SLO_ERR_INVALID, "rope_store: max_position must be positive and num_slots not negative");
+  if ((int64_t)a->num_heads + 2 * (int64_t)a->num_kv_heads > 65536) return fail(SLO_ERR_UNSUPPORTED, "rope_store: too many heads");
+  if (!a->q_norm_weight != !a->k_norm_weight) return fail(SLO_ERR_INVALID, "rope_store: weights of both norms, or of neither");
+  if (a->q_norm_weight && !(a->eps >= 0.0f)) return fail(SLO_ERR_INVALID, "rope_store: eps must be >= 0");
+  if (a->num_tokens == 0) return SLO_OK;
+  if (!a->qkv || !a->positions || !a->cos_sin || !a->q_out || !a->k_out || !a->slot_mapping ||
+      (a->num_slots && (!a->k_cache || !a->v_cache)))
     return fail(SLO_ERR_INVALID, "rope_store: null pointer");
-  if (kv_dtype == KV_FP8_E4M3FN && (!k_scale || !v_scale)) return fail(SLO_ERR_INVALID, "rope_store: FP8 needs scale pools");
-  if (kv_dtype == KV_FP8_E4M3FN && !(scale_floor > 0.0f)) return fail(SLO_ERR_INVALID, "rope_store: scale_floor must be > 0");
-  if ((qkv_row_stride % 8) || qkv_row_stride < (int64_t)(num_heads + 2 * num_kv_heads) * head_dim || unaligned16(qkv) ||
-      unaligned16(q_out) || unaligned16(k_out) || unaligned16(k_cache) || unaligned16(v_cache) || unaligned16(cos_sin) ||
-      unaligned16(q_norm_weight) || unaligned16(k_norm_weight))
+  if (fp8 && (!a->k_scale || !a->v_scale)) return fail(SLO_ERR_INVALID, "rope_store: FP8 needs scale pools");
+  if (fp8 && !(a->scale_floor > 0.0f)) return fail(SLO_ERR_INVALID, "rope_store: scale_floor must be > 0");
+  if ((a->qkv_row_stride % 8) || a->qkv_row_stride < ((int64_t)a->num_heads + 2 * (int64_t)a->num_kv_heads) * a->head_dim ||
+      unaligned16(a->qkv) || unaligned16(a->q_out) || unaligned16(a->k_out) || unaligned16(a->k_cache) ||
+      unaligned16(a->v_cache) || unaligned16(a->cos_sin) || unaligned16(a->q_norm_weight) || unaligned16(a->k_norm_weight))
     return fail(SLO_ERR_INVALID, "rope_store: rows and tables must be 16-byte aligned");
-  const RopeParams p = {static_cast<const uint16_t*>(qkv), qkv_row_stride, positions, num_tokens, num_heads, num_kv_heads,
-                        static_cast<const uint16_t*>(q_norm_weight), static_cast<const uint16_t*>(k_norm_weight), eps, cos_sin,
-                        max_position, rotary_dim, static_cast<uint16_t*>(q_out), static_cast<uint16_t*>(k_out), slot_mapping,
-                        kv_dtype, k_cache, v_cache, k_scale, v_scale, num_slots, scale_floor};
+  const RopeParams p = {static_cast<const uint16_t*>(a->qkv), a->qkv_row_stride, a->positions, a->num_tokens, a->num_heads,
+                        a->num_kv_heads, static_cast<const uint16_t*>(a->q_norm_weight),
+                        static_cast<const uint16_t*>(a->k_norm_weight), a->eps, a->cos_sin, a->max_position, a->rotary_dim,
+                        static_cast<uint16_t*>(a->q_out), static_cast<uint16_t*>(a->k_out), a->slot_mapping, a->kv_dtype,
+                        a->k_cache, a->v_cache, a->k_scale, a->v_scale, a->num_slots, a->scale_floor};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (head_dim == 64) launch_rope<64>(p, interleaved != 0, s);
-  else if (head_dim == 128) launch_rope<128>(p, interleaved != 0, s);
-  else launch_rope<256>(p, interleaved != 0, s);
+  if (a->head_dim == 64) launch_rope<64>(p, a->interleaved != 0, s);
+  else if (a->head_dim == 128) launch_rope<128>(p, a->interleaved != 0, s);
+  else launch_rope<256>(p, a->interleaved != 0, s);
   return check_launch("rope_store");
 }

@@ -24,6 +24,7 @@
 #include "fp4.h"
 #include "tile_io.h"
 #include <algorithm>
+#include <type_traits>
 
 namespace slo {
 namespace {
@@ -32,7 +33,7 @@ constexpr int RECORD = HD + 4;   // floats of a decode chunk's partial result: o
 constexpr float kNone = -1e30f;  // running maximum before the first key
 constexpr float kSumMax = 224.0f;  // largest sum of a lane's weights in a step before the reference moves
 constexpr int NT = 2;            // 16-column blocks of a prefill wavefront
-constexpr int kWaves = 4;
+constexpr int kWaves = 4;        // wavefronts that run a tile
 
 // Partial result of a part of a prefill tile, as it lies in the registers of
 // its lanes (four channels a piece).
@@ -52,6 +53,7 @@ struct WinParams {
   int num_blocks, block_size;
   uint32_t tpb, tpb_inv;  // 64-token tiles per block, ceil(2^32 / tpb)
   int hq, hkv, group;
+  uint32_t group_inv;  // ceil(2^16 / group)
   float scale_log2;  // |softmax scale| * log2(e)
   uint32_t q_sign;   // 0x80008000 where the scale is negative
   int window, sinks;
@@ -100,6 +102,12 @@ __device__ __forceinline__ Span span_of(const WinParams& p, int x0, int x1, int 
   s.sink = min((min(p.sinks, s.end) + T - 1) / T, f);
   s.start = f * T;
   s.steps = s.sink + max((s.end + T - 1) / T - f, 0);
+  // (Said to be uniform, or what follows from them is computed lane by lane.)
+  s.first = __builtin_amdgcn_readfirstlane(s.first);
+  s.end = __builtin_amdgcn_readfirstlane(s.end);
+  s.sink = __builtin_amdgcn_readfirstlane(s.sink);
+  s.start = __builtin_amdgcn_readfirstlane(s.start);
+  s.steps = __builtin_amdgcn_readfirstlane(s.steps);
   return s;
 }
 template <int T>
@@ -112,7 +120,7 @@ __device__ __forceinline__ const __attribute__((address_space(4))) int32_t* scal
   return (const __attribute__((address_space(4))) int32_t*)(uintptr_t)x;
 }
 template <int F>
-__device__ __forceinline__ int64_t pool_row(const WinParams& p, const int32_t* table, int head, int key, bool& ok) {
+__device__ __forceinline__ int64_t pool_row(const WinParams& p, const int32_t* table, int head, int key, int& ok) {
   const uint32_t t = (uint32_t)key / 64;
   const int page = p.tpb == 1 ? (int)t : (int)__umulhi(t, p.tpb_inv);
   const int b = scalar(table)[page], off = key - page * p.block_size;
@@ -122,12 +130,20 @@ __device__ __forceinline__ int64_t pool_row(const WinParams& p, const int32_t* t
   return (block * p.block_size + off) * p.hkv + head;
 }
 
-__device__ __forceinline__ bf16x8 load_q(const WinParams& p, int64_t row, int h, int channel, bool live) {
-  u32x4 x = {0, 0, 0, 0};
-  if (live) x = ld16(p.q + row * p.q_stride + h * HD + channel);
+// Four operands of a query, channels 32 kg .. 32 kg + 31; zeros where not live.
+__device__ __forceinline__ void load_q(bf16x8 (&q)[4], const WinParams& p, int64_t row, int h, int kg, bool live) {
+  u32x4 x[4] = {};
+  if (live) {
+    const uint16_t* from = p.q + row * p.q_stride + h * HD + 32 * kg;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] ^= p.q_sign;
-  return as_bf16x8(x);
+    for (int i = 0; i < 4; ++i) x[i] = ld16(from + 8 * i);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[i][j] ^= p.q_sign;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) q[i] = as_bf16x8(x[i]);
 }
 
 // Four tokens' channel pairs as two channels' token quadruples.
@@ -371,26 +387,25 @@ __device__ __forceinline__ Chunks<F> chunks_of(const WinParams& p, int r) {
   return c;
 }
 
-template <int F>
+template <int F, int WAVES>
 struct DecodeLds {
   union {
     Step<F> steps[2];
     float o[16][HD];
-  } ring[kWaves];
-  float m[kWaves][16], l[kWaves][16];
+  } ring[WAVES];
+  float m[WAVES][16], l[WAVES][16];
 };
 
-// One chunk of one (row, kv head) a workgroup, its four wavefronts every fourth
-// step, all heads of the group as columns.  Each wavefront fetches its own
+// One chunk of one (row, kv head) a workgroup, its wavefronts a step each in
+// turn, all heads of the group as columns.  Each wavefront fetches its own
 // steps, so the loop has no barrier; the wavefronts' results meet in LDS.
-template <int F>
-__device__ void decode_item(const WinParams& p, DecodeLds<F>& lds, int r, int chunk, int head) {
+template <int F, int WAVES>
+__device__ void decode_item(const WinParams& p, DecodeLds<F, WAVES>& lds, int r, int chunk, int head) {
   constexpr int T = Step<F>::T, H = T / 16;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, kg = lane >> 4;
   bf16x8 q[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) q[i] = load_q(p, r, head * p.group + c, 32 * kg + 8 * i, c < p.group);
+  load_q(q, p, r, head * p.group + c, kg, c < p.group);
   const Chunks<F> ch = chunks_of<F>(p, r);
   if (chunk >= ch.count) return;
   const int begin = chunk * ch.per + wave, end = min((chunk + 1) * ch.per, ch.s.steps);
@@ -399,14 +414,14 @@ __device__ void decode_item(const WinParams& p, DecodeLds<F>& lds, int r, int ch
   for (int e = 0; e < 8; ++e) a.o[e] = f32x4{0, 0, 0, 0};
   a.m = kNone;
   a.l = 0.0f;
-  const int steps = end > begin ? (end - begin + kWaves - 1) / kWaves : 0;
+  const int steps = end > begin ? (end - begin + WAVES - 1) / WAVES : 0;
   if (steps > 0) {
     const int32_t* table = p.dtables + (int64_t)r * p.dstride;
     const uint32_t ring = lds_addr(&lds.ring[wave]);
     int key[2];   // of the steps in flight; past every key where the page is not in the pool
     auto send = [&](int i) {
-      bool ok;
-      const int k = key_of<T>(ch.s, begin + kWaves * i);
+      int ok;
+      const int k = key_of<T>(ch.s, begin + WAVES * i);
       const int64_t row = pool_row<F>(p, table, head, k, ok);
       fetch<F>(p, row, ring + (i & 1) * (uint32_t)sizeof(Step<F>), lane);
       return ok ? k : ch.len;
@@ -448,15 +463,15 @@ __device__ void decode_item(const WinParams& p, DecodeLds<F>& lds, int r, int ch
     }
   }
   __syncthreads();
-  for (int x = threadIdx.x; x < p.group * (HD / 4); x += 64 * kWaves) {
+  for (int x = threadIdx.x; x < p.group * (HD / 4); x += 64 * WAVES) {
     const int h = x >> 5, d = (x & 31) * 4;
     float m = lds.m[0][h];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) m = fmaxf(m, lds.m[w][h]);
+    for (int w = 1; w < WAVES; ++w) m = fmaxf(m, lds.m[w][h]);
     f32x4 o = {0, 0, 0, 0};
     float l = 0;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
       const float f = __builtin_amdgcn_exp2f(lds.m[w][h] - m);
       o += *reinterpret_cast<const f32x4*>(&lds.ring[w].o[h][d]) * f;
       l += lds.l[w][h] * f;
@@ -494,86 +509,138 @@ template <> struct Quarter<KV_BF16> {
 template <> struct Quarter<KV_FP8_E4M3FN> {
   u32x4 k[2];
   u32x2 v[4];
-  float s;
+  float ks, vs;  // of token c
 };
 template <> struct Quarter<KV_FP4_E2M1> {
   u32x4 k, vs;
   uint32_t ks, v[4];
 };
 
+// x / group of a tile's column (x < 64).
+__device__ __forceinline__ int by_group(const WinParams& p, int x) { return x * p.group_inv >> 16; }
+
 struct PrefillRow {
-  int64_t q0;  // first query row
+  int q0;  // first query row of the row
   int lq, lk, prefix, k0;
 };
 
 __device__ __forceinline__ PrefillRow prefill_row(const WinParams& p, int r) {
   PrefillRow g;
   const int start = p.cu_q[r], k0 = p.cu_k[r], k = p.cu_k[r + 1] - k0;
-  g.q0 = (int64_t)p.first_row + start;
+  g.q0 = p.first_row + start;
   g.lq = p.cu_q[r + 1] - start;
   g.prefix = k - g.lq;
   g.k0 = k0;
-  g.lk = p.ptables ? min(k, p.pwidth * p.block_size) : min(k, p.num_kv_rows - k0);
-  if (!p.ptables && k0 < 0) g.lk = 0;
-  if (start < 0 || g.q0 + g.lq > p.num_q_rows) g.lq = 0;
+  g.lk = p.ptables ? min(k, p.pwidth * p.block_size) : k0 < 0 ? 0 : min(k, p.num_kv_rows - k0);
+  if (start < 0 || (int64_t)g.q0 + g.lq > p.num_q_rows) g.lq = 0;
   return g;
 }
 
-// The 16 tokens from `key` + 16 wave on; `left`: keys of the row from `key` on
-// (rows without a pool are not read past their end).
+// Byte offsets of a lane's pieces (of V, of the first of its four tokens) from
+// its step's first token: the same at every step, so that a load is a uniform
+// base and one of these.
+struct Lanes {
+  uint32_t k, v;
+};
+template <int F>
+__device__ __forceinline__ Lanes lanes_of(const WinParams& p, int wave, int lane) {
+  const uint32_t c = lane & 15, kg = lane >> 4, row = F == KV_BF16 ? 256 : F == KV_FP8_E4M3FN ? 128 : 64;
+  const bool rows = F == KV_BF16 && !p.ptables;
+  const uint32_t stride = F == KV_FP4_E2M1 ? row : p.hkv * row;
+  Lanes l;
+  l.k = (16 * wave + c) * (rows ? (uint32_t)p.rk_stride : stride) + kg * (row / 4);
+  l.v = (16 * wave + 4 * kg) * (rows ? (uint32_t)p.rv_stride : stride) + c * (row / 16);
+  return l;
+}
+
+// A load at a uniform base plus a lane's 32-bit offset.  (The offset is found
+// again at each step: extended to 64 bits before the loop, it would take two
+// registers and the load a lane address.)
+template <typename T>
+__device__ __forceinline__ T load(const void* base, uint32_t off, int more = 0) {
+  asm("" : "+v"(off));
+  return *reinterpret_cast<const T*>(static_cast<const uint8_t*>(base) + off + more);
+}
+
+// This wavefront's 16 of the 64 tokens from `key` on.
 template <int F>
 __device__ __forceinline__ void load_quarter(Quarter<F>& t, const WinParams& p, const PrefillRow& g, const int32_t* table,
-                                             int head, int key, int wave, int lane, bool& ok) {
+                                             int head, int key, const Lanes& l, int wave, int lane, int& ok) {
   const int c = lane & 15, kg = lane >> 4;
   if constexpr (F == KV_BF16) {
     const uint8_t *k, *v;
-    int64_t ks, vs;
-    int last = 63;
+    uint32_t stride = p.hkv * 256;
     ok = true;
     if (p.ptables) {
       const int64_t row = pool_row<F>(p, table, head, key, ok);
       k = p.kc + row * 256;
       v = p.vc + row * 256;
-      ks = vs = p.hkv * 256;
     } else {
+      stride = p.rv_stride;
       const int64_t row = (int64_t)g.k0 + key;
       k = p.rk + row * p.rk_stride + head * 256;
       v = p.rv + row * p.rv_stride + head * 256;
-      ks = p.rk_stride;
-      vs = p.rv_stride;
-      last = g.lk - 1 - key;
+      const int last = g.lk - 1 - key;
+      if (last < 63) {  // nothing is read past the rows' end
+        k += min(16 * wave + c, last) * (uint32_t)p.rk_stride;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          t.k[i] = ld16(k + 64 * kg + 16 * i);
+          t.v[i] = ld16(v + min(16 * wave + 4 * kg + i, last) * stride + 16 * c);
+        }
+        return;
+      }
     }
-    k += min(16 * wave + c, last) * ks + 64 * kg;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) t.k[i] = ld16(k + 16 * i);
+    for (int i = 0; i < 4; ++i) t.k[i] = load<u32x4>(k, l.k, 16 * i);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) t.v[i] = ld16(v + min(16 * wave + 4 * kg + i, last) * vs + 16 * c);
+    for (int i = 0; i < 4; ++i) t.v[i] = load<u32x4>(v + i * stride, l.v);
   } else if constexpr (F == KV_FP8_E4M3FN) {
-    const int64_t row = pool_row<F>(p, table, head, key, ok) + 16 * wave * p.hkv;
+    const int64_t row = pool_row<F>(p, table, head, key, ok);
     const uint8_t *k = p.kc + row * 128, *v = p.vc + row * 128;
-    const uint32_t stride = p.hkv * 128;
-    t.k[0] = ld16(k + (c * stride + 32 * kg));
-    t.k[1] = ld16(k + (c * stride + 32 * kg + 16));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) t.v[i] = ld8(v + ((4 * kg + i) * stride + 8 * c));
-    t.s = static_cast<const float*>(lane & 16 ? p.vs : p.ks)[row + c * p.hkv];
+    for (int i = 0; i < 2; ++i) t.k[i] = load<u32x4>(k, l.k, 16 * i);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t.v[i] = load<u32x2>(v + i * (uint32_t)(p.hkv * 128), l.v);
+    const uint32_t at = 4 * (16 * wave + c) * p.hkv;
+    t.ks = load<float>(static_cast<const float*>(p.ks) + row, at);
+    t.vs = load<float>(static_cast<const float*>(p.vs) + row, at);
   } else {
-    const int64_t row = pool_row<F>(p, table, head, key, ok) + 16 * wave;
-    const uint8_t *k = p.kc + row * 64, *v = p.vc + row * 64;
+    const int64_t row = pool_row<F>(p, table, head, key, ok);
     const uint8_t *ks = static_cast<const uint8_t*>(p.ks) + row * 4, *vs = static_cast<const uint8_t*>(p.vs) + row * 4;
-    t.k = ld16(k + (c * 64 + kg * 16));
-    t.ks = ks[c * 4 + kg];
-    t.vs = ld16(vs + kg * 16);
+    t.k = load<u32x4>(p.kc + row * 64, l.k);
+    t.ks = load<uint8_t>(ks, 64 * wave + c * 4 + kg);
+    t.vs = load<u32x4>(vs, 64 * wave + kg * 16);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) t.v[i] = *reinterpret_cast<const uint32_t*>(v + (kg * 256 + c * 4 + i * 64));
+    for (int i = 0; i < 4; ++i) t.v[i] = load<uint32_t>(p.vc + row * 64, l.v, 64 * i);
   }
 }
 
-// `seen`: which of the lane's four V tokens one of the tile's queries sees.  The
-// others may be anything in the pages, and a weight of zero must not make that
-// a NaN.
+// Clears the V tokens that none of the tile's queries sees, of a step from
+// `key` on that may hold some.  They may be anything in the pages, and a weight
+// of zero must not make that a NaN.
 template <int F>
-__device__ __forceinline__ void stage(Stage<F>& s, const Quarter<F>& t, uint32_t seen, int wave, int lane) {
+__device__ __forceinline__ void clear_unseen(Quarter<F>& t, int key, int first, int end, int sinks, int wave, int lane) {
+  const int k = key + 16 * wave + 4 * (lane >> 4);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool seen = (k + i < end) & ((k + i >= first) | (k + i < sinks));
+    if constexpr (F == KV_BF16) {
+      t.v[i] = seen ? t.v[i] : u32x4{0, 0, 0, 0};
+    } else if constexpr (F == KV_FP8_E4M3FN) {
+      t.v[i] = seen ? t.v[i] : u32x2{0, 0};
+    } else {
+      t.vs[i] = seen ? t.vs[i] : 0;
+    }
+  }
+  if constexpr (F == KV_FP8_E4M3FN) {
+    const int k = key + 16 * wave + (lane & 15);
+    if (!((k < end) & ((k >= first) | (k < sinks)))) t.vs = 0.0f;
+  }
+}
+
+template <int F>
+__device__ __forceinline__ void stage(Stage<F>& s, const Quarter<F>& t, int wave, int lane) {
   const int c = lane & 15;
   u32x4 v[4];
   if constexpr (F == KV_BF16) {
@@ -582,41 +649,25 @@ __device__ __forceinline__ void stage(Stage<F>& s, const Quarter<F>& t, uint32_t
       s.k[wave][i][lane] = t.k[i];
       v[i] = t.v[i];
     }
-    if (__any(seen != 15)) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (!(seen >> i & 1)) v[i] = u32x4{0, 0, 0, 0};
-    }
   } else if constexpr (F == KV_FP8_E4M3FN) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       s.k[wave][2 * i][lane] = fp8x8_to_bf16x8(u32x2{t.k[i][0], t.k[i][1]});
       s.k[wave][2 * i + 1][lane] = fp8x8_to_bf16x8(u32x2{t.k[i][2], t.k[i][3]});
     }
-    if (lane < 32) s.s[lane >> 4][16 * wave + c] = t.s;
-    u32x2 raw[4] = {t.v[0], t.v[1], t.v[2], t.v[3]};
-    if (__any(seen != 15)) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (!(seen >> i & 1)) raw[i] = u32x2{0, 0};
+    if (lane < 16) {
+      s.s[0][16 * wave + c] = t.ks;
+      s.s[1][16 * wave + c] = t.vs;
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = fp8x8_to_bf16x8(raw[i]);
+    for (int i = 0; i < 4; ++i) v[i] = fp8x8_to_bf16x8(t.v[i]);
   } else {
     const float sc = e8m0(t.ks);
 #pragma unroll
     for (int i = 0; i < 4; ++i) s.k[wave][i][lane] = e2m1_decode8(t.k[i], sc);
-    float vs[4];
-    const int turn = (9 + 8 * (c >> 2)) & 31;
+    const int turn = (9 + 8 * (c >> 2)) & 31;  // the lane's scale byte to the exponent's place
 #pragma unroll
-    for (int i = 0; i < 4; ++i) vs[i] = __uint_as_float(__builtin_amdgcn_alignbit(t.vs[i], t.vs[i], turn));
-    if (__any(seen != 15)) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (!(seen >> i & 1)) vs[i] = 0.0f;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = e2m1_decode8(t.v[i], vs[i]);
+    for (int i = 0; i < 4; ++i) v[i] = e2m1_decode8(t.v[i], __uint_as_float(__builtin_amdgcn_alignbit(t.vs[i], t.vs[i], turn)));
   }
 #pragma unroll
   for (int b = 0; b < 4; ++b) {
@@ -631,13 +682,17 @@ struct Acc {
   float ncm[NT], l[NT];  // minus the reference in the log2 domain (+inf before the first key), this lane's sum
 };
 
-// 64 tokens of a wavefront's columns against the staged operands, read four
-// ahead of the products.  at[n]: position of column block n's query; keys from
-// `kend` on are not the row's.
+// 64 tokens from `key` on of a wavefront's columns against the staged operands,
+// read four ahead of the products.  The further a wavefront is from the step's
+// end the higher its priority, so that the two of a SIMD do not fall into step
+// (4,096 queries on 8,191 keys 282 -> 268 us; any one phase raised 271-282).  at[n]: position of column block n's query;
+// keys from `kend` on are not the row's.  A step before the window part (`sink`)
+// shows a query nothing but sinks.
 template <int F>
-__device__ __forceinline__ void staged_step(const WinParams& p, const Stage<F>& st, bool masked, const bf16x8 (&q)[NT][4],
-                                            Acc& a, int kv0, const int (&at)[NT], int kend, int lane) {
+__device__ __forceinline__ void staged_step(const WinParams& p, const Stage<F>& st, bool masked, bool sink, const bf16x8 (&q)[NT][4],
+                                            Acc& a, int key, const int (&at)[NT], int kend, int lane) {
   const int kg = lane >> 4;
+  __builtin_amdgcn_s_setprio(3);
   f32x4 s[NT][4];
   bf16x8 x[2][4];
 #pragma unroll
@@ -653,53 +708,53 @@ __device__ __forceinline__ void staged_step(const WinParams& p, const Stage<F>& 
       for (int n = 0; n < NT; ++n) s[n][t] = mfma16(x[t & 1][i], q[n][i], i ? s[n][t] : f32x4{0, 0, 0, 0});
     __builtin_amdgcn_sched_barrier(0);
   }
-  if constexpr (F == KV_FP8_E4M3FN) {
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const f32x4 ks = *reinterpret_cast<const f32x4*>(&st.s[0][16 * t + 4 * kg]);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) s[n][t] *= ks;
-    }
-  }
-  if (masked) {
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int k = kv0 + 16 * t + 4 * kg + i;
-          if (!(k <= at[n] && k < kend && (k > at[n] - p.window || k < p.sinks))) s[n][t][i] = -INFINITY;
-        }
-  }
+  __builtin_amdgcn_s_setprio(2);
   // No maximum is formed: a reference that is too low shows in the sum of a
   // lane's weights (inf or NaN while it is unset).  Only then are the columns'
   // maxima found and the weights taken again.
   const float c = p.scale_log2;
-  f32x4 e[NT][4];
-  float rs[NT];
-  bool over = false;
-  auto exponents = [&](int n, float ncm) {
-    rs[n] = 0.0f;
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        e[n][t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][t][i], c, ncm));
-        rs[n] += e[n][t][i];
-      }
-  };
+  const int few = sink ? 0 : p.sinks - key;  // sinks among the window part's keys
+  bf16x8 pr[NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    exponents(n, a.ncm[n]);
-    over = over || !(rs[n] <= kSumMax);
-  }
-  if (__any(over)) {
+    if constexpr (F == KV_FP8_E4M3FN) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const bool mine = !(rs[n] <= kSumMax);
-      if (!__any(mine)) continue;
-      const bool grow = col_max(mine ? 1.0f : 0.0f) > 0.0f;
+      for (int t = 0; t < 4; ++t) s[n][t] *= *reinterpret_cast<const f32x4*>(&st.s[0][16 * t + 4 * kg]);
+    }
+    if (masked) {
+      const int hi = min(at[n], (sink ? min(kend, p.sinks) : kend) - 1) - key - 4 * kg;
+      const int lo = (sink ? 0 : max(at[n] - p.window + 1 - key, 0)) - 4 * kg;
+      if (few <= 0) {
+        const uint32_t span = max(hi - lo + 1, 0), from = -lo;  // tokens below lo wrap past every span
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[n][t][i] = from + (16 * t + i) < span ? s[n][t][i] : -INFINITY;
+      } else {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int k = 16 * t + i;
+            s[n][t][i] = (k <= hi) & ((k >= lo) | (k < few - 4 * kg)) ? s[n][t][i] : -INFINITY;
+          }
+      }
+    }
+    f32x4 e[4];
+    float rs;
+    auto exponents = [&](float ncm) {
+      rs = 0.0f;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          e[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][t][i], c, ncm));
+          rs += e[t][i];
+        }
+    };
+    exponents(a.ncm[n]);
+    if (__any(!(rs <= kSumMax))) {
+      const bool grow = col_max(rs <= kSumMax ? 0.0f : 1.0f) > 0.0f;
       float top = s[n][0][0];
 #pragma unroll
       for (int i = 1; i < 16; ++i) top = fmaxf(top, s[n][i >> 2][i & 3]);
@@ -707,35 +762,24 @@ __device__ __forceinline__ void staged_step(const WinParams& p, const Stage<F>& 
       const float next = grow && top != -INFINITY ? fminf(a.ncm[n], -c * top) : a.ncm[n];
       const float use = next == INFINITY ? 0.0f : next;  // no key yet: weights of zero
       const float w = grow ? __builtin_amdgcn_exp2f(use - a.ncm[n]) : 1.0f;
-      exponents(n, use);
+      exponents(use);
       a.l[n] *= w;
 #pragma unroll
       for (int i = 0; i < 8; ++i) a.o[n][i] *= w;
       a.ncm[n] = next;
     }
-  }
-  bf16x8 pr[NT][2];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    a.l[n] += rs[n];
+    a.l[n] += rs;
     if constexpr (F == KV_FP8_E4M3FN) {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        f32x4 vs = *reinterpret_cast<const f32x4*>(&st.s[1][16 * t + 4 * kg]);
-        if (masked) {  // of tokens that may be anything
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (e[n][t][i] == 0.0f) vs[i] = 0.0f;
-        }
-        e[n][t] *= vs;
-      }
+      for (int t = 0; t < 4; ++t) e[t] *= *reinterpret_cast<const f32x4*>(&st.s[1][16 * t + 4 * kg]);
     }
 #pragma unroll
     for (int g = 0; g < 2; ++g)
-      pr[n][g] = as_bf16x8(u32x4{pack_bf16x2(e[n][2 * g][0], e[n][2 * g][1]), pack_bf16x2(e[n][2 * g][2], e[n][2 * g][3]),
-                                 pack_bf16x2(e[n][2 * g + 1][0], e[n][2 * g + 1][1]),
-                                 pack_bf16x2(e[n][2 * g + 1][2], e[n][2 * g + 1][3])});
+      pr[n][g] = as_bf16x8(u32x4{pack_bf16x2(e[2 * g][0], e[2 * g][1]), pack_bf16x2(e[2 * g][2], e[2 * g][3]),
+                                 pack_bf16x2(e[2 * g + 1][0], e[2 * g + 1][1]), pack_bf16x2(e[2 * g + 1][2], e[2 * g + 1][3])});
+    __builtin_amdgcn_sched_barrier(0);
   }
+  __builtin_amdgcn_s_setprio(1);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {  // V's operands, four at a time
     const int g = j >> 1;
@@ -750,24 +794,32 @@ __device__ __forceinline__ void staged_step(const WinParams& p, const Stage<F>& 
       for (int n = 0; n < NT; ++n) a.o[n][4 * (j & 1) + i] = mfma16(x[j & 1][i], pr[n][g], a.o[n][4 * (j & 1) + i]);
     __builtin_amdgcn_sched_barrier(0);
   }
+  __builtin_amdgcn_s_setprio(0);
 }
 
 // Item i's row and tile: the rows' tiles in order, each row's last one (the
 // longest, where the window has not filled) first.
-__device__ __forceinline__ bool find_tile(const WinParams& p, int per, int item, int lane, int& row, int& tile) {
+__device__ __forceinline__ bool find_tile(const WinParams& p, int per, int item, int lane, int& row, int& tile, PrefillRow& g) {
   int before = 0;
   for (int base = 0; base < p.prows; base += 64) {
     int n = 0;
+    PrefillRow x = {};
     if (base + lane < p.prows) {
-      const int lq = prefill_row(p, base + lane).lq;
-      n = lq > 0 ? (lq + per - 1) / per : 0;
+      x = prefill_row(p, base + lane);
+      n = x.lq > 0 ? (int)((uint32_t)(x.lq + per - 1) / (uint32_t)per) : 0;
     }
     const int upto = wave_scan(n);
     const uint64_t past = __ballot(before + upto > item);
     if (past) {
-      const int at = __builtin_ctzll(past);
-      row = base + at;
-      tile = before + __builtin_amdgcn_readlane(upto, at) - 1 - item;
+      const int at = __builtin_amdgcn_readfirstlane(__builtin_ctzll(past));
+      auto of = [&](int v) { return __builtin_amdgcn_readfirstlane(__builtin_amdgcn_readlane(v, at)); };
+      row = __builtin_amdgcn_readfirstlane(base + at);
+      tile = __builtin_amdgcn_readfirstlane(before + __builtin_amdgcn_readlane(upto, at) - 1 - item);
+      g.q0 = of(x.q0);
+      g.lq = of(x.lq);
+      g.lk = of(x.lk);
+      g.prefix = of(x.prefix);
+      g.k0 = of(x.k0);
       return true;
     }
     before += __builtin_amdgcn_readlane(upto, 63);
@@ -775,23 +827,36 @@ __device__ __forceinline__ bool find_tile(const WinParams& p, int per, int item,
   return false;
 }
 
-// Tile `item`, part `part` of its steps, kv head `head`.  The four wavefronts
-// turn each step into operands together, a quarter each, and each runs 16 NT
-// columns, (query, head of the group) pairs of consecutive queries, over them;
-// the next step loads meanwhile.
-template <int F>
-__device__ void prefill_item(const WinParams& p, Stage<F> (&st)[2], int item, int part, int head) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+// What a second half of a workgroup leaves for the first.
+struct Half {
+  f32x4 o[kWaves][NT][8][64];
+  float ncm[kWaves][NT][64], l[kWaves][NT][64];
+};
+template <int F, int HALVES>
+union PrefillLds {
+  Stage<F> st[HALVES][2];
+  std::conditional_t<HALVES == 2, Half, char> half;
+};
+
+// Tile `item`, part `part` of its steps, kv head `head`.  Four wavefronts turn a
+// step into operands together, a quarter each, and each runs 16 NT columns,
+// (query, head of the group) pairs of consecutive queries, over them; the next
+// step loads meanwhile.  With two halves of four wavefronts each half takes
+// every other step.
+template <int F, int HALVES>
+__device__ void prefill_item(const WinParams& p, PrefillLds<F, HALVES>& lds, int item, int part, int head) {
+  const int lane = threadIdx.x & 63, any = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = any & (kWaves - 1), half = any / kWaves;
   const int c = lane & 15, kg = lane >> 4;
-  const int each = 16 * NT / p.group, per = kWaves * each;  // queries of a wavefront, of a tile
+  const int each = by_group(p, 16 * NT), per = kWaves * each;  // queries of a wavefront, of a tile
   int r = 0, tile = 0;
-  if (!find_tile(p, per, item, lane, r, tile)) return;
-  r = __builtin_amdgcn_readfirstlane(r);
-  tile = __builtin_amdgcn_readfirstlane(tile);
-  const PrefillRow g = prefill_row(p, r);
+  PrefillRow g;
+  if (!find_tile(p, per, item, lane, r, tile, g)) return;
   const int w0 = tile * per, w1 = min(w0 + per, g.lq);
   const Span s = span_of<64>(p, g.prefix + w0, g.prefix + w1 - 1, g.lk);
-  const int from = (int)((int64_t)s.steps * part / p.splits), to = (int)((int64_t)s.steps * (part + 1) / p.splits);
+  // (At most 2^18 steps, 512 parts.)
+  const int from = __builtin_amdgcn_readfirstlane((uint32_t)s.steps * part / p.splits);
+  const int to = __builtin_amdgcn_readfirstlane((uint32_t)s.steps * (part + 1) / p.splits);
   // Queries of this wavefront [t0, t1); columns past them repeat the last one's
   // mask with a query of zeros.
   const int t0 = min(w0 + wave * each, w1 - 1), t1 = max(min(w0 + wave * each + each, w1), t0 + 1);
@@ -800,11 +865,9 @@ __device__ void prefill_item(const WinParams& p, Stage<F> (&st)[2], int item, in
   Acc a;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const int x = 16 * n + c, tok = w0 + wave * each + x / p.group;
-    const bool live = x < each * p.group && tok < w1;
+    const int x = 16 * n + c, y = by_group(p, x), tok = w0 + wave * each + y;
     at[n] = g.prefix + min(tok, t1 - 1);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) q[n][i] = load_q(p, g.q0 + tok, head * p.group + x % p.group, 32 * kg + 8 * i, live);
+    load_q(q[n], p, g.q0 + tok, head * p.group + x - y * p.group, kg, y < each && tok < w1);
 #pragma unroll
     for (int i = 0; i < 8; ++i) a.o[n][i] = f32x4{0, 0, 0, 0};
     a.ncm[n] = INFINITY;
@@ -813,41 +876,66 @@ __device__ void prefill_item(const WinParams& p, Stage<F> (&st)[2], int item, in
   if (from < to) {
     const int32_t* table = p.ptables ? p.ptables + (int64_t)r * p.pstride : nullptr;
     const int x0 = g.prefix + t0, x1 = g.prefix + t1 - 1;
+    const Lanes lanes = lanes_of<F>(p, wave, lane);
     Quarter<F> t;
-    bool ok, next_ok = false;
-    int key = key_of<64>(s, from), next = key;
-    load_quarter<F>(t, p, g, table, head, key, wave, lane, ok);
-    for (int i = from; i < to; ++i) {
-      const int buf = (i - from) & 1;
-      uint32_t seen = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int k = key + 16 * wave + 4 * kg + j;
-        seen |= (uint32_t)(ok && k < s.end && (k >= s.first || k < p.sinks)) << j;
-      }
-      stage<F>(st[buf], t, seen, wave, lane);
-      if (i + 1 < to) {
-        next = key_of<64>(s, i + 1);
-        load_quarter<F>(t, p, g, table, head, next, wave, lane, next_ok);
+    int in = 0;
+    if (from + half < to) load_quarter<F>(t, p, g, table, head, key_of<64>(s, from + half), lanes, wave, lane, in);
+    for (int i = from + half; i < to + half; i += HALVES) {
+      Stage<F>& st = lds.st[half][(i - from) / HALVES & 1];
+      const bool mine = HALVES == 1 || i < to;  // the last turn may have steps for one half only
+      const int key = key_of<64>(s, i);
+      const int ok = in;  // whether the step's page is in the pool
+      if (mine) {
+        if (!ok || key + 64 > s.end || (key < s.first && key + 64 > p.sinks))
+          clear_unseen<F>(t, key, s.first, ok ? s.end : 0, p.sinks, wave, lane);
+        stage<F>(st, t, wave, lane);
+        if (i + HALVES < to) load_quarter<F>(t, p, g, table, head, key_of<64>(s, i + HALVES), lanes, wave, lane, in);
       }
       // Two buffers: a wavefront comes to write this one again only past the
       // next step's barrier, when every wavefront has left it.  The barrier
       // waits for LDS only: the loads of the next step stay in flight.
       lds_sync();
-      const bool all = ok && key + 63 <= x0 && key + 64 <= g.lk && (key > x1 - p.window || key + 64 <= p.sinks);
-      staged_step<F>(p, st[buf], !all, q, a, ok ? key : 1 << 30, at, g.lk, lane);
-      key = next;
-      ok = next_ok;
+      if (mine) {
+        const bool all = ok && key + 63 <= x0 && key + 64 <= g.lk && (key > x1 - p.window || key + 64 <= p.sinks);
+        staged_step<F>(p, st, !all, i < s.sink, q, a, key, at, ok ? g.lk : 0, lane);
+      }
     }
   }
+  if constexpr (HALVES == 2) {
+    Half& h = lds.half;
+    __syncthreads();
+    if (half == 1) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h.o[wave][n][e][lane] = a.o[n][e];
+        h.ncm[wave][n][lane] = a.ncm[n];
+        h.l[wave][n][lane] = a.l[n];
+      }
+    }
+    __syncthreads();
+    if (half == 1) return;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const float other = h.ncm[wave][n][lane], ncm = fminf(a.ncm[n], other);
+      const float mine = a.ncm[n] == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ncm - a.ncm[n]);
+      const float w = other == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ncm - other);
+      a.ncm[n] = ncm;
+      a.l[n] = a.l[n] * mine + h.l[wave][n][lane] * w;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) a.o[n][e] = a.o[n][e] * mine + h.o[wave][n][e][lane] * w;
+    }
+  }
+  int col = lane & 15;
+  asm("" : "+v"(col));  // found again here, so that the loop need not hold what follows from it in registers
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const float l = col_sum(a.l[n]);
     if (p.splits == 1) {
-      const int x = 16 * n + c, tok = w0 + wave * each + x / p.group, h = head * p.group + x % p.group;
-      if (x >= each * p.group || tok >= w1) continue;
+      const int x = 16 * n + col, y = by_group(p, x), tok = w0 + wave * each + y, h = head * p.group + x - y * p.group;
+      if (y >= each || tok >= w1) continue;
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      uint16_t* out = p.out + (g.q0 + tok) * p.out_stride + h * HD + 32 * kg;
+      uint16_t* out = p.out + (int64_t)(g.q0 + tok) * p.out_stride + h * HD + 32 * kg;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         *reinterpret_cast<u32x4*>(out + 8 * i) =
@@ -862,78 +950,104 @@ __device__ void prefill_item(const WinParams& p, Stage<F> (&st)[2], int item, in
         for (int e = 0; e < 8; e += 4)
           out.o[block][2 * i + (e >> 2)][lane] = f32x4{a.o[n][e][i], a.o[n][e + 1][i], a.o[n][e + 2][i], a.o[n][e + 3][i]};
       if (kg == 0) {
-        out.m[16 * block + c] = a.ncm[n] == INFINITY ? kNone : -a.ncm[n];
-        out.l[16 * block + c] = l;
+        out.m[16 * block + col] = a.ncm[n] == INFINITY ? kNone : -a.ncm[n];
+        out.l[16 * block + col] = l;
       }
     }
   }
 }
 
 // Both phases in one launch, prefill items first.
-template <int F>
-__global__ void __launch_bounds__(64 * kWaves, 2)
+template <int F, int HALVES>
+__global__ void __launch_bounds__(64 * kWaves * HALVES, 2)
 window_attention_kernel(WinParams p) {
   __shared__ union {
-    Stage<F> st[2];
-    DecodeLds<F> dec;
+    PrefillLds<F, HALVES> pre;
+    DecodeLds<F, kWaves * HALVES> dec;
   } lds;
-  int i = blockIdx.x;
-  const int head = i % p.hkv;
-  i /= p.hkv;
-  const int prefill = p.items * p.splits;
-  if (i < prefill)
-    prefill_item<F>(p, lds.st, i / p.splits, i % p.splits, head);
-  else
-    decode_item<F>(p, lds.dec, (i - prefill) / p.chunks, (i - prefill) % p.chunks, head);
+  // (Quotients are said to be uniform, or what follows from them is computed
+  // lane by lane.)
+  auto div = [](uint32_t x, uint32_t y) { return (int)__builtin_amdgcn_readfirstlane(x / y); };
+  int i = div(blockIdx.x, p.hkv);
+  const int head = blockIdx.x - i * p.hkv, prefill = p.items * p.splits;
+  if (i < prefill) {
+    const int item = div(i, p.splits);
+    prefill_item<F, HALVES>(p, lds.pre, item, i - item * p.splits, head);
+  } else {
+    i -= prefill;
+    const int r = div(i, p.chunks);
+    decode_item<F, kWaves * HALVES>(p, lds.dec, r, i - r * p.chunks, head);
+  }
   if (p.idle) clear_idle(p);
 }
 
+// Joins the chunks of decode row r, query head h: half wavefront i takes chunks
+// i, i + 8, ..., four channels a lane, and the eight sums meet in LDS in order.
+template <int F>
+__device__ __forceinline__ void join_decode(const WinParams& p, int r, int h) {
+  __shared__ f32x4 so[8][32];
+  __shared__ float sl[8];
+  const int lane = threadIdx.x & 31, i = threadIdx.x >> 5, head = h / p.group;
+  const int count = chunks_of<F>(p, r).count;
+  if (count == 1) return;  // written by its only chunk
+  const float* rec = p.records + (((int64_t)r * p.hkv + head) * p.chunks * p.group + h - head * p.group) * RECORD;
+  const int64_t stride = (int64_t)p.group * RECORD;
+  float m = kNone;
+  for (int s = lane; s < count; s += 32) m = fmaxf(m, rec[s * stride + HD]);
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) m = wave_max_xor(m, d);
+  f32x4 o = {0, 0, 0, 0};
+  float l = 0;
+#pragma unroll 4
+  for (int s = i; s < count; s += 8) {
+    const float* e = rec + s * stride;
+    const float w = __builtin_amdgcn_exp2f(e[HD] - m);
+    o += *reinterpret_cast<const f32x4*>(e + 4 * lane) * w;
+    l += e[HD + 1] * w;
+  }
+  so[i][lane] = o;
+  if (lane == 0) sl[i] = l;
+  __syncthreads();
+  if (i) return;
+#pragma unroll
+  for (int k = 1; k < 8; ++k) {
+    o += so[k][lane];
+    l += sl[k];
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  *reinterpret_cast<u32x2*>(p.out + (int64_t)r * p.out_stride + h * HD + 4 * lane) =
+      u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
+}
+
 // Joins the chunks of decode rows (workgroups below `decode`, one per row and
-// kv head) and the parts of prefill tiles (one per item, kv head and 16
+// query head) and the parts of prefill tiles (one per item, kv head and 16
 // columns).
 template <int F>
 __global__ void __launch_bounds__(256)
 window_join_kernel(WinParams p, int decode) {
   int i = blockIdx.x;
   if (i < decode) {
-    const int r = i / p.hkv, head = i % p.hkv;
-    const int count = chunks_of<F>(p, r).count;
-    if (count == 1) return;  // written by its only chunk
-    const float* rec = p.records + (int64_t)i * p.chunks * p.group * RECORD;
-    const int64_t stride = (int64_t)p.group * RECORD;
-    for (int x = threadIdx.x; x < p.group * (HD / 4); x += 256) {
-      const int h = x >> 5, d = (x & 31) * 4;
-      const float* e = rec + h * RECORD;
-      float m = kNone;
-      for (int s = 0; s < count; ++s) m = fmaxf(m, e[s * stride + HD]);
-      f32x4 o = {0, 0, 0, 0};
-      float l = 0;
-      for (int s = 0; s < count; ++s) {
-        const float w = __builtin_amdgcn_exp2f(e[s * stride + HD] - m);
-        o += *reinterpret_cast<const f32x4*>(e + s * stride + d) * w;
-        l += e[s * stride + HD + 1] * w;
-      }
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      *reinterpret_cast<u32x2*>(p.out + (int64_t)r * p.out_stride + (head * p.group + h) * HD + d) =
-          u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
-    }
+    const int r = i / p.hq;
+    join_decode<F>(p, r, i - r * p.hq);
     return;
   }
   i -= decode;
   const int block = i % (kWaves * NT), head = i / (kWaves * NT) % p.hkv, item = i / (kWaves * NT) / p.hkv;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, kg = lane >> 4;
-  const int each = 16 * NT / p.group, per = kWaves * each;
+  const int each = by_group(p, 16 * NT), per = kWaves * each;
   int r = 0, tile = 0;
-  if (!find_tile(p, per, item, lane, r, tile)) return;
-  const PrefillRow g = prefill_row(p, r);
-  const int x = 16 * (block % NT) + c, tok = tile * per + block / NT * each + x / p.group;
-  if (x >= each * p.group || tok >= g.lq) return;
+  PrefillRow g;
+  if (!find_tile(p, per, item, lane, r, tile, g)) return;
+  const int x = 16 * (block % NT) + c, y = by_group(p, x), tok = tile * per + block / NT * each + y;
+  if (y >= each || tok >= g.lq) return;
   const Part* part = p.parts + ((int64_t)item * p.hkv + head) * p.splits;
   const int at = 16 * block + c;
   float m = kNone;
+#pragma unroll 4
   for (int s = 0; s < p.splits; ++s) m = fmaxf(m, part[s].m[at]);
   f32x4 o[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
   float l = 0;
+#pragma unroll 4
   for (int s = 0; s < p.splits; ++s) {
     const float w = __builtin_amdgcn_exp2f(part[s].m[at] - m);
 #pragma unroll
@@ -941,7 +1055,7 @@ window_join_kernel(WinParams p, int decode) {
     l += part[s].l[at] * w;
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  uint16_t* out = p.out + (g.q0 + tok) * p.out_stride + (head * p.group + x % p.group) * HD + 32 * kg;
+  uint16_t* out = p.out + (int64_t)(g.q0 + tok) * p.out_stride + (head * p.group + x - y * p.group) * HD + 32 * kg;
 #pragma unroll
   for (int j = 0; j < 2; ++j)
     *reinterpret_cast<u32x2*>(out + 4 * (wave + 4 * j)) =
@@ -954,7 +1068,7 @@ constexpr int kSlots = 512;  // two workgroups fit a CU
 
 struct Plan {
   bool dwork, pwork;
-  int chunks, items, splits;
+  int halves, chunks, items, splits;
   size_t dbytes, pbytes;
 };
 
@@ -965,7 +1079,7 @@ int64_t most_steps(int64_t window, int64_t sinks, int64_t n, int64_t cap) {
 }
 
 Plan plan_of(const slo_paged_attention_args* a, int window, int sinks) {
-  Plan n = {false, false, 0, 0, 1, 0, 0};
+  Plan n = {false, false, 1, 0, 0, 1, 0, 0};
   const int group = a->num_heads / a->num_kv_heads;
   if (a->num_decode > 0 && (a->phases & SLO_PHASE_DECODE)) {
     n.dwork = true;
@@ -981,16 +1095,19 @@ Plan plan_of(const slo_paged_attention_args* a, int window, int sinks) {
     n.items = (int)((int64_t)(a->num_q_rows - a->num_decode) / per + a->num_prefill);
     const int64_t cap = a->prefill_tables ? (int64_t)a->prefill_table_width * a->block_size : a->num_kv_rows;
     const int64_t steps = most_steps(window, sinks, per, cap);
-    const int64_t wgs = (int64_t)n.items * a->num_kv_heads;
-    n.splits = (int)std::max<int64_t>(1, std::min(kSlots / wgs, steps / 8));
-    if (n.splits > 1) n.pbytes = (size_t)wgs * n.splits * sizeof(Part);
+    // Tiles, if every row's are full ones (workgroups past the last tile end at once).
+    const int64_t tiles = std::max<int64_t>(1, (a->num_q_rows - a->num_decode + per - 1) / per) * a->num_kv_heads;
+    n.halves = tiles + (n.dwork ? (int64_t)a->num_decode * a->num_kv_heads : 0) <= kSlots / 2 ? 2 : 1;
+    if (n.halves == 2) n.splits = (int)std::max<int64_t>(1, std::min(kSlots / 2 / tiles, steps / 16));
+    if (n.splits > 1) n.pbytes = (size_t)n.items * a->num_kv_heads * n.splits * sizeof(Part);
   }
   return n;
 }
 
 int64_t workgroups(const slo_paged_attention_args* a, const Plan& n) {
-  const int64_t joined = (n.chunks > 1 ? a->num_decode : 0) + (n.splits > 1 ? (int64_t)n.items * kWaves * NT : 0);
-  return std::max((int64_t)n.items * n.splits + (int64_t)a->num_decode * n.chunks, joined) * a->num_kv_heads;
+  const int64_t heads = a->num_kv_heads;
+  const int64_t joined = (n.chunks > 1 ? (int64_t)a->num_decode * a->num_heads : 0) + (n.splits > 1 ? n.items * heads * kWaves * NT : 0);
+  return std::max((int64_t)n.items * n.splits * heads * n.halves + (int64_t)a->num_decode * n.chunks * heads * n.halves, joined);
 }
 
 int check_args(const slo_paged_attention_args* a, int window, int sinks) {
@@ -1035,9 +1152,9 @@ int check_args(const slo_paged_attention_args* a, int window, int sinks) {
   if (pre && !a->prefill_tables) {
     if (!a->k || !a->v || a->num_kv_rows <= 0) return fail(SLO_ERR_INVALID, "paged_attention_window: prefill rows without tables need k and v");
     if ((a->k_row_stride % 8) || (a->v_row_stride % 8) || a->k_row_stride < a->num_kv_heads * HD ||
-        a->v_row_stride < a->num_kv_heads * HD || (reinterpret_cast<uintptr_t>(a->k) % 16) ||
-        (reinterpret_cast<uintptr_t>(a->v) % 16))
-      return fail(SLO_ERR_INVALID, "paged_attention_window: k and v rows must be 16-byte aligned, num_kv_heads * 128 elements or more apart");
+        a->v_row_stride < a->num_kv_heads * HD || a->k_row_stride >= 1 << 25 || a->v_row_stride >= 1 << 25 ||
+        (reinterpret_cast<uintptr_t>(a->k) % 16) || (reinterpret_cast<uintptr_t>(a->v) % 16))
+      return fail(SLO_ERR_INVALID, "paged_attention_window: k and v rows must be 16-byte aligned, from num_kv_heads * 128 to 2^25 elements apart");
   }
   if ((dec && (int64_t)a->decode_table_width * a->block_size > (1 << 22)) ||
       (pre && a->prefill_tables && (int64_t)a->prefill_table_width * a->block_size > (1 << 22)) ||
@@ -1050,10 +1167,13 @@ int check_args(const slo_paged_attention_args* a, int window, int sinks) {
 }
 
 template <int F>
-void launch(const WinParams& p, hipStream_t s) {
+void launch(const WinParams& p, int halves, hipStream_t s) {
   const unsigned blocks = (unsigned)(((int64_t)p.items * p.splits + (int64_t)p.drows * p.chunks) * p.hkv);
-  hipLaunchKernelGGL(window_attention_kernel<F>, dim3(blocks), dim3(64 * kWaves), 0, s, p);
-  const int decode = p.chunks > 1 ? p.drows * p.hkv : 0;
+  if (halves == 2)
+    hipLaunchKernelGGL((window_attention_kernel<F, 2>), dim3(blocks), dim3(64 * kWaves * 2), 0, s, p);
+  else
+    hipLaunchKernelGGL((window_attention_kernel<F, 1>), dim3(blocks), dim3(64 * kWaves), 0, s, p);
+  const int decode = p.chunks > 1 ? p.drows * p.hq : 0;
   const int prefill = p.splits > 1 ? p.items * p.hkv * kWaves * NT : 0;
   if (decode + prefill) hipLaunchKernelGGL(window_join_kernel<F>, dim3(decode + prefill), dim3(256), 0, s, p, decode);
 }
@@ -1099,6 +1219,7 @@ extern "C" int slo_paged_attention_window(const slo_paged_attention_args* a, int
   p.hq = a->num_heads;
   p.hkv = a->num_kv_heads;
   p.group = a->num_heads / a->num_kv_heads;
+  p.group_inv = ((1 << 16) + p.group - 1) / p.group;
   p.scale_log2 = (a->softmax_scale < 0 ? -a->softmax_scale : a->softmax_scale) * kLog2e;
   p.q_sign = a->softmax_scale < 0 ? 0x80008000u : 0u;
   p.window = std::min(window, 1 << 26);
@@ -1138,15 +1259,15 @@ extern "C" int slo_paged_attention_window(const slo_paged_attention_args* a, int
     // The step's own rows are bf16 whatever the pool's format.
     WinParams cold = p;
     cold.drows = 0;
-    launch<KV_BF16>(cold, s);
+    launch<KV_BF16>(cold, n.halves, s);
     p.items = 0;
     p.splits = 1;
     p.idle = false;
   }
   if (p.items || p.drows) {
-    if (a->kv_dtype == KV_BF16) launch<KV_BF16>(p, s);
-    else if (a->kv_dtype == KV_FP8_E4M3FN) launch<KV_FP8_E4M3FN>(p, s);
-    else launch<KV_FP4_E2M1>(p, s);
+    if (a->kv_dtype == KV_BF16) launch<KV_BF16>(p, n.halves, s);
+    else if (a->kv_dtype == KV_FP8_E4M3FN) launch<KV_FP8_E4M3FN>(p, n.halves, s);
+    else launch<KV_FP4_E2M1>(p, n.halves, s);
   }
   return check_launch("paged_attention_window");
 }

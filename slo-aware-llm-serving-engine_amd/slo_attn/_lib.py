@@ -71,6 +71,22 @@ _CODES = {_c_void_p: "P", _c_int64: "q", _c_int32: "i", ctypes.c_float: "f", cty
 pack_attention_args = struct.Struct("@" + "".join(_CODES[t] for _, t in PagedAttentionArgs._fields_) + "0P").pack
 
 
+class RopeStoreArgs(ctypes.Structure):
+    """Mirror of ``slo_rope_store_args`` (include/slo_attn.h)."""
+
+    _fields_ = [
+        ("qkv", _c_void_p), ("qkv_row_stride", _c_int64), ("positions", _c_void_p),
+        ("num_tokens", _c_int32), ("num_heads", _c_int32), ("num_kv_heads", _c_int32), ("head_dim", _c_int32),
+        ("q_norm_weight", _c_void_p), ("k_norm_weight", _c_void_p), ("eps", ctypes.c_float), ("max_position", _c_int32),
+        ("cos_sin", _c_void_p), ("rotary_dim", _c_int32), ("interleaved", _c_int32), ("q_out", _c_void_p), ("k_out", _c_void_p),
+        ("slot_mapping", _c_void_p), ("kv_dtype", _c_int32), ("scale_floor", ctypes.c_float), ("k_cache", _c_void_p),
+        ("v_cache", _c_void_p), ("k_scale", _c_void_p), ("v_scale", _c_void_p), ("num_slots", _c_int64),
+    ]
+
+
+pack_rope_args = struct.Struct("@" + "".join(_CODES[t] for _, t in RopeStoreArgs._fields_) + "0P").pack
+
+
 class EvictKvArgs(ctypes.Structure):
     """Mirror of ``slo_evict_kv_args`` (include/slo_attn.h)."""
 
@@ -92,6 +108,7 @@ EXPORTS = (
     "slo_store_kvcache",
     "slo_qk_norm_rope_store",
     "slo_rope_store",
+    "slo_rope_store_args_size",
     "slo_lm_head_argmax",
     "slo_build_mixed_metadata",
     "slo_attention_workspace_bytes",
@@ -136,10 +153,9 @@ def load() -> ctypes.CDLL:
             ctypes.c_float, _c_void_p, _c_int32, _c_void_p, _c_void_p, _c_void_p, _c_int32, _c_void_p, _c_void_p,
             _c_void_p, _c_void_p, _c_int64, ctypes.c_float, _c_void_p]
         lib.slo_rope_store.restype = ctypes.c_int
-        lib.slo_rope_store.argtypes = [
-            _c_void_p, _c_int64, _c_void_p, _c_int32, _c_int32, _c_int32, _c_int32, _c_void_p, _c_void_p,
-            ctypes.c_float, _c_void_p, _c_int32, _c_int32, _c_int32, _c_void_p, _c_void_p, _c_void_p, _c_int32, _c_void_p,
-            _c_void_p, _c_void_p, _c_void_p, _c_int64, ctypes.c_float, _c_void_p]
+        lib.slo_rope_store.argtypes = [ctypes.c_char_p, _c_void_p]
+        lib.slo_rope_store_args_size.restype = ctypes.c_size_t
+        lib.slo_rope_store_args_size.argtypes = []
         lib.slo_lm_head_argmax.restype = ctypes.c_int
         lib.slo_lm_head_argmax.argtypes = [
             _c_void_p, _c_int64, _c_int32, _c_void_p, _c_int64, _c_int32, _c_int32, _c_void_p, _c_int64,
@@ -189,6 +205,8 @@ def load() -> ctypes.CDLL:
             raise RuntimeError("slo_paged_attention_args layout mismatch between header and binding")
         if lib.slo_evict_kv_args_size() != ctypes.sizeof(EvictKvArgs):
             raise RuntimeError("slo_evict_kv_args layout mismatch between header and binding")
+        if lib.slo_rope_store_args_size() != ctypes.sizeof(RopeStoreArgs):
+            raise RuntimeError("slo_rope_store_args layout mismatch between header and binding")
         _lib = lib
         return lib
 

@@ -8,7 +8,6 @@ There is no CPU path: CPU tensors are rejected.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 import threading
@@ -118,11 +117,17 @@ def _one_device(first: torch.Tensor, *others) -> int:
     return device.index
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def _launch(index: int, what: str, *args) -> None:
     """Calls an entry point on the current stream of GPU ``index``, which need not be the current one."""
-    lib = _lib.load()
-    with contextlib.nullcontext() if torch.cuda.current_device() == index else torch.cuda.device(index):
-        rc = getattr(lib, what)(*args, _raw_stream(index))
+    call = getattr(_lib.load(), what)
+    if _current_device() == index:  # (the tensors that came here have initialised the device)
+        rc = call(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = call(*args, _raw_stream(index))
     if rc:
         _lib.check(rc, what)
 
@@ -447,10 +452,12 @@ def _rope_store(qkv, positions, q_norm_weight, k_norm_weight, eps, cos_sin, num_
     q = torch.empty((N, num_heads, head_dim), dtype=torch.bfloat16, device=qkv.device)
     k = torch.empty((N, num_kv_heads, head_dim), dtype=torch.bfloat16, device=qkv.device)
     fp4 = code == _lib.KV_FP4_E2M1  # the kernel then writes q and k only: a pool of no slots
-    _launch(index, "slo_rope_store", qkv.data_ptr(), qkv.stride(0) if N > 1 else width, positions.data_ptr(), N, num_heads,
-            num_kv_heads, head_dim, _ptr(q_norm_weight), _ptr(k_norm_weight), eps, cos_sin.data_ptr(), cos_sin.shape[0], rot,
-            interleaved, q.data_ptr(), k.data_ptr(), slot_mapping.data_ptr(), _lib.KV_BF16 if fp4 else code, k_cache.data_ptr(),
-            v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), 0 if fp4 else blocks * block, scale_floor)
+    args = _lib.pack_rope_args(
+        qkv.data_ptr(), qkv.stride(0) if N > 1 else width, positions.data_ptr(), N, num_heads, num_kv_heads, head_dim,
+        _ptr(q_norm_weight) or 0, _ptr(k_norm_weight) or 0, eps, cos_sin.shape[0], cos_sin.data_ptr(), rot, interleaved,
+        q.data_ptr(), k.data_ptr(), slot_mapping.data_ptr(), _lib.KV_BF16 if fp4 else code, scale_floor, k_cache.data_ptr(),
+        v_cache.data_ptr(), _ptr(k_scale) or 0, _ptr(v_scale) or 0, 0 if fp4 else blocks * block)
+    _launch(index, "slo_rope_store", args)
     v = qkv[:, (num_heads + num_kv_heads) * head_dim:].view(N, num_kv_heads, head_dim)
     if fp4:
         store_kvcache(k, v, k_cache, v_cache, slot_mapping, k_scale, v_scale, scale_floor)
@@ -603,32 +610,30 @@ def _pool_call(what, extra, index, device, q, out, k_cache, v_cache, k_scale, v_
     code, blocks, block, heads, head_dim = geometry
     T, num_heads, _ = q.shape
     decode, prefill = rows
-    fields = (q.data_ptr(), q.stride(0) if T > 1 else num_heads * head_dim, _ptr(out) or 0,
-              0 if out is None else out.stride(0) if T > 1 else num_heads * head_dim, T, _ptr(k_cache) or 0, _ptr(v_cache) or 0,
-              _ptr(k_scale) or 0, _ptr(v_scale) or 0, code, blocks, block, *(x or 0 for x in decode), *(x or 0 for x in prefill),
-              *own, num_heads, heads, head_dim, scale)
-    args = _lib.pack_attention_args(*fields, 0, 0, phases, 0, 0, 0, 0, 0, 0, 0.0)
-    need = _workspace_need(args, sized, what, T, num_heads, heads, code, block, phases, decode[0], decode[4], prefill[0],
-                           prefill[3], prefill[4], prefill[7], own[4])
-    if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=device)
-        args = _lib.pack_attention_args(*fields, ws.data_ptr(), need, phases, 0, 0, 0, 0, 0, 0, 0.0)
+    width = num_heads * head_dim
+    fields = (q.data_ptr(), q.stride(0) if T > 1 else width, _ptr(out) or 0, 0 if out is None else out.stride(0) if T > 1 else width,
+              T, _ptr(k_cache) or 0, _ptr(v_cache) or 0, _ptr(k_scale) or 0, _ptr(v_scale) or 0, code, blocks, block,
+              *(x or 0 for x in decode), *(x or 0 for x in prefill), *own, num_heads, heads, head_dim, scale)
+    key = (what, T, num_heads, heads, code, block, phases, decode[0], decode[4], prefill[0], prefill[3], prefill[4], prefill[7],
+           own[4], *sized)
+    need = _sizes.get(key)
+    if need is None:
+        need = _workspace_need(what, _lib.pack_attention_args(*fields, 0, 0, phases, 0, 0, 0, 0, 0, 0, 0.0), sized)
+        if len(_sizes) >= 4096:
+            _sizes.clear()
+        _sizes[key] = need
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    args = _lib.pack_attention_args(*fields, ws.data_ptr() if need else 0, need, phases, 0, 0, 0, 0, 0, 0, 0.0)
     _launch(index, what, args, *extra)
 
 
 _sizes: dict[tuple, int] = {}  # workspace bytes by entry point and sizes
 
 
-def _workspace_need(args, sized, *key) -> int:
-    what, key = key[0], (*key, *sized)
-    need = _sizes.get(key)
-    if need is None:
-        size = ctypes.c_size_t(0)
-        _lib.check(getattr(_lib.load(), what + "_workspace_bytes")(args, *sized, ctypes.byref(size)), what)
-        if len(_sizes) >= 4096:
-            _sizes.clear()
-        need = _sizes[key] = size.value
-    return need
+def _workspace_need(what, args, sized) -> int:
+    size = ctypes.c_size_t(0)
+    _lib.check(getattr(_lib.load(), what + "_workspace_bytes")(args, *sized, ctypes.byref(size)), what)
+    return size.value
 
 
 def accumulate_attention(q: torch.Tensor, k_cache: torch.Tensor, kv_scores: torch.Tensor, softmax_scale: float, *,

@@ -140,17 +140,32 @@ def test_window_sizes_without_a_gpu():
 def test_rope_store_refusals_without_a_gpu():
     lib = _lib.load()
 
-    def call(n=4, hq=32, hkv=8, d=128, qw=4096, kw=4096, eps=1e-6, far=100, rot=64, kv=1, qkv=4096, stride=6144, table=4096,
-             ks=4096, slots=100, floor=2.0 ** -64, kc=4096):
-        return lib.slo_rope_store(qkv, stride, 4096, n, hq, hkv, d, qw, kw, eps, table, far, rot, 1, 4096, 4096, 4096, kv, kc, 4096,
-                                  ks, 4096, slots, floor, None)
+    def call(**over):
+        a = _lib.RopeStoreArgs()
+        a.num_tokens, a.num_heads, a.num_kv_heads, a.head_dim, a.rotary_dim, a.interleaved = 4, 32, 8, 128, 64, 1
+        a.qkv_row_stride, a.eps, a.max_position, a.kv_dtype, a.num_slots, a.scale_floor = 6144, 1e-6, 100, 1, 100, 2.0 ** -64
+        for name, kind in a._fields_:
+            if kind is ctypes.c_void_p:
+                setattr(a, name, 4096)
+        for name, value in over.items():
+            setattr(a, name, value)
+        return lib.slo_rope_store(bytes(a), None)
 
-    assert call(n=0) == 0
-    for over in (dict(n=-1), dict(hq=0), dict(hkv=0), dict(qw=None), dict(eps=-1.0), dict(eps=float("nan")), dict(far=0), dict(rot=0),
-                 dict(rot=60), dict(rot=136), dict(kv=2), dict(qkv=None), dict(qkv=4104), dict(stride=6136), dict(stride=6148),
-                 dict(table=4100), dict(ks=None), dict(floor=0.0), dict(slots=-1), dict(kc=None), dict(kc=4104)):
+    assert lib.slo_rope_store(None, None) == 1 and call(num_tokens=0) == 0
+    for over in (dict(num_tokens=-1), dict(num_heads=0), dict(num_kv_heads=0), dict(q_norm_weight=None), dict(eps=-1.0),
+                 dict(eps=float("nan")), dict(max_position=0), dict(rotary_dim=0), dict(rotary_dim=60), dict(rotary_dim=136),
+                 dict(kv_dtype=2), dict(qkv=None), dict(qkv=4104), dict(qkv_row_stride=6136), dict(qkv_row_stride=6148),
+                 dict(cos_sin=4100), dict(k_scale=None), dict(scale_floor=0.0), dict(num_slots=-1), dict(k_cache=None),
+                 dict(k_cache=4104), dict(slot_mapping=None)):
         assert call(**over) == 1, over
-    assert call(d=96) == 4 and call(hq=65537, stride=1 << 24) == 4
+    assert call(head_dim=96) == 4 and call(num_heads=65537, qkv_row_stride=1 << 24) == 4
+
+
+def test_packed_rope_arguments_are_the_struct():
+    a = _lib.RopeStoreArgs()
+    for i, (name, _) in enumerate(a._fields_, 1):
+        setattr(a, name, i)
+    assert _lib.pack_rope_args(*range(1, len(a._fields_) + 1)) == bytes(a)
 
 
 def test_layer_refuses_a_window_that_is_none():

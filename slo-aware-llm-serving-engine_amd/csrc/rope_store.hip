@@ -17,8 +17,14 @@
 namespace slo {
 namespace {
 
-constexpr int RS_NT = 512;  // threads per workgroup
-constexpr int RS_U = 2;     // heads that a lane group has in flight
+// Threads per workgroup, and heads that a lane group has in flight.  Up to 1,024
+// tokens all workgroups of 512 threads are on the GPU at once, and a token's
+// heads side by side end soonest; past that, small ones that hold more heads a
+// lane keep more loads in flight.  us for 512 x 2 / 128 x 3, 32 and 8 heads of
+// 128: 128 tokens 3.5 / 4.8, 768 6.9 / 8.2, 2,000 12.5 / 11.0, 8,192 (221 MB) 60.6
+// / 44.8 (4.9 TB/s; 256 x 3 45.3, 128 x 6 43.0 but 11.7 for the 2,000); 16 and 1 heads,
+// 8,192 28.0 / 16.6; heads of 64 29.2 / 21.1; E4M3FN, 4,096 29.9 / 28.0.
+constexpr int kFewThreads = 512, kFewHeads = 2, kManyThreads = 128, kManyHeads = 3, kMany = 1024;
 
 struct RopeParams {
   const uint16_t* qkv;
@@ -64,10 +70,10 @@ __device__ __forceinline__ void unpack4(const u32x2& w, float* f) {
 // channels in two pieces of 4: lane j of a head has channels 8j.. and 8j + 4..,
 // or, with FAR pairs on a rotated lane (j < R / 8), 4j.. and R / 2 + 4j.., so
 // that both channels of a pair are in one lane in either layout.
-template <int D, bool FAR>
-__global__ void __launch_bounds__(RS_NT)
+template <int D, bool FAR, int THREADS, int U>
+__global__ void __launch_bounds__(THREADS)
 rope_store_kernel(RopeParams p) {
-  constexpr int LANES = D / 8, GROUPS = RS_NT / LANES;
+  constexpr int LANES = D / 8, GROUPS = THREADS / LANES;
   const int j = threadIdx.x % LANES, grp = threadIdx.x / LANES;
   const int heads = p.num_heads + 2 * p.num_kv_heads, qk = p.num_heads + p.num_kv_heads;
   const bool turned = 8 * j < p.rot;
@@ -92,10 +98,10 @@ rope_store_kernel(RopeParams p) {
       cs = *reinterpret_cast<const f32x4*>(t);
       sn = *reinterpret_cast<const f32x4*>(t + p.rot / 2);
     }
-    for (int h0 = 0; h0 < heads; h0 += GROUPS * RS_U) {
-      u32x2 x[RS_U][2];
+    for (int h0 = 0; h0 < heads; h0 += GROUPS * U) {
+      u32x2 x[U][2];
 #pragma unroll
-      for (int u = 0; u < RS_U; ++u) {
+      for (int u = 0; u < U; ++u) {
         const int h = h0 + GROUPS * u + grp;
         // V keeps its order: its lanes hold 8 channels side by side.
         const int a = h < qk ? c0 : 8 * j, b = h < qk ? c1 : 8 * j + 4;
@@ -106,7 +112,7 @@ rope_store_kernel(RopeParams p) {
         }
       }
 #pragma unroll
-      for (int u = 0; u < RS_U; ++u) {
+      for (int u = 0; u < U; ++u) {
         const int h = h0 + GROUPS * u + grp;
         if (h >= heads) continue;
         int a = 8 * j, b = 8 * j + 4;
@@ -168,15 +174,21 @@ rope_store_kernel(RopeParams p) {
 }
 
 // A grid holds less than 2^32 threads: past so many tokens workgroups go round.
-constexpr int RS_GRID = 1 << 20;
+constexpr int kGrid = 1 << 20;
+
+template <int D, bool FAR>
+void launch_rope(const RopeParams& p, hipStream_t s) {
+  const dim3 grid(p.tokens < kGrid ? p.tokens : kGrid);
+  if (p.tokens > kMany)
+    hipLaunchKernelGGL((rope_store_kernel<D, FAR, kManyThreads, kManyHeads>), grid, dim3(kManyThreads), 0, s, p);
+  else
+    hipLaunchKernelGGL((rope_store_kernel<D, FAR, kFewThreads, kFewHeads>), grid, dim3(kFewThreads), 0, s, p);
+}
 
 template <int D>
 void launch_rope(const RopeParams& p, bool interleaved, hipStream_t s) {
-  const dim3 grid(p.tokens < RS_GRID ? p.tokens : RS_GRID);
-  if (interleaved)
-    hipLaunchKernelGGL((rope_store_kernel<D, false>), grid, dim3(RS_NT), 0, s, p);
-  else
-    hipLaunchKernelGGL((rope_store_kernel<D, true>), grid, dim3(RS_NT), 0, s, p);
+  if (interleaved) launch_rope<D, false>(p, s);
+  else launch_rope<D, true>(p, s);
 }
 
 inline bool unaligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; }

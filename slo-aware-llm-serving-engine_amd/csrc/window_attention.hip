@@ -981,6 +981,17 @@ window_attention_kernel(WinParams p) {
   if (p.idle) clear_idle(p);
 }
 
+// Decode rows alone.
+template <int F, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, 2)
+window_decode_kernel(WinParams p) {
+  __shared__ DecodeLds<F, WAVES> lds;
+  auto div = [](uint32_t x, uint32_t y) { return (int)__builtin_amdgcn_readfirstlane(x / y); };
+  const int i = div(blockIdx.x, p.hkv), r = div(i, p.chunks);
+  decode_item<F, WAVES>(p, lds, r, i - r * p.chunks, blockIdx.x - i * p.hkv);
+  if (p.idle) clear_idle(p);
+}
+
 // Joins the chunks of decode row r, query head h: half wavefront i takes chunks
 // i, i + 8, ..., four channels a lane, and the eight sums meet in LDS in order.
 template <int F>
@@ -1078,15 +1089,32 @@ int64_t most_steps(int64_t window, int64_t sinks, int64_t n, int64_t cap) {
   return std::min((keys + 63) / 64 + 1 + (sinks + 63) / 64, (cap + 63) / 64);
 }
 
+// Chunks of a decode row that sees up to so many keys, by the (row, kv head)
+// pairs.  A cut spreads few pairs over the GPU and costs the join (4-5 us).  us
+// in 1, 2, 3, 4, 6 and 8 chunks:
+//   8 pairs, 1,028 keys, bf16        13.4  11.7  10.1   9.4   9.0   9.0
+//   16 pairs, 8,196 keys, bf16       90.5  51.2  37.5  30.6  23.8  20.5
+//   64 pairs, 1,028 keys, bf16       16.5  15.0  13.0  12.4  14.5  14.4
+//   128 pairs, 1,028 keys, bf16      20.5  19.1  20.9  19.3  20.8  20.9
+//   128 pairs, 516 keys, bf16        11.8  13.3  14.8  15.0
+//   320 pairs, 4,100 keys, E4M3FN    94.6  85.2  82.3  80.7  84.2  85.9
+//   512 pairs, 4,100 keys, bf16       163   171   173   175   180   186
+// 32 pairs of 8,256 keys, E4M3FN: 8 chunks 22.4, 16 24.6, 32 32.3.
+int decode_chunks(int64_t pairs, int64_t keys) {
+  if (pairs >= kSlots) return 1;
+  const int64_t wanted = pairs >= 128 && keys >= 2048 ? 768 : 256;
+  const int64_t chunks = std::min((wanted + pairs - 1) / pairs, (keys + 255) / 256);
+  return chunks > 1 && keys - keys / chunks >= 512 ? (int)chunks : 1;
+}
+
 Plan plan_of(const slo_paged_attention_args* a, int window, int sinks) {
   Plan n = {false, false, 1, 0, 0, 1, 0, 0};
   const int group = a->num_heads / a->num_kv_heads;
   if (a->num_decode > 0 && (a->phases & SLO_PHASE_DECODE)) {
     n.dwork = true;
-    const int64_t pairs = (int64_t)a->num_decode * a->num_kv_heads;
-    const int64_t steps = most_steps(window, sinks, 1, (int64_t)a->decode_table_width * a->block_size);
-    n.chunks = (int)std::max<int64_t>(1, std::min((kSlots + pairs - 1) / pairs, (steps + 3) / 4));
-    if (n.chunks > 1) n.dbytes = (size_t)pairs * n.chunks * group * RECORD * 4;
+    n.chunks = decode_chunks((int64_t)a->num_decode * a->num_kv_heads,
+                             64 * most_steps(window, sinks, 1, (int64_t)a->decode_table_width * a->block_size));
+    if (n.chunks > 1) n.dbytes = (size_t)a->num_decode * a->num_heads * n.chunks * RECORD * 4;
   }
   if (a->num_prefill > 0 && (a->phases & SLO_PHASE_PREFILL)) {
     n.pwork = true;
@@ -1167,9 +1195,14 @@ int check_args(const slo_paged_attention_args* a, int window, int sinks) {
 }
 
 template <int F>
+constexpr int kDecodeWaves = 4;
+
+template <int F>
 void launch(const WinParams& p, int halves, hipStream_t s) {
   const unsigned blocks = (unsigned)(((int64_t)p.items * p.splits + (int64_t)p.drows * p.chunks) * p.hkv);
-  if (halves == 2)
+  if (!p.items)
+    hipLaunchKernelGGL((window_decode_kernel<F, kDecodeWaves<F>>), dim3(blocks), dim3(64 * kDecodeWaves<F>), 0, s, p);
+  else if (halves == 2)
     hipLaunchKernelGGL((window_attention_kernel<F, 2>), dim3(blocks), dim3(64 * kWaves * 2), 0, s, p);
   else
     hipLaunchKernelGGL((window_attention_kernel<F, 1>), dim3(blocks), dim3(64 * kWaves), 0, s, p);

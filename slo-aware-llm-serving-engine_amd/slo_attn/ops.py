@@ -449,8 +449,7 @@ def _rope_store(qkv, positions, q_norm_weight, k_norm_weight, eps, cos_sin, num_
         raise ValueError(f"KV pool holds {heads} kv heads of {d}, not {num_kv_heads} of {head_dim}")
     if slot_mapping.dtype != torch.int32 or slot_mapping.numel() != N or not slot_mapping.is_contiguous():
         raise ValueError("slot_mapping must be a contiguous int32 [tokens] tensor")
-    q = torch.empty((N, num_heads, head_dim), dtype=torch.bfloat16, device=qkv.device)
-    k = torch.empty((N, num_kv_heads, head_dim), dtype=torch.bfloat16, device=qkv.device)
+    q, k = qkv.new_empty((N, num_heads, head_dim)), qkv.new_empty((N, num_kv_heads, head_dim))
     fp4 = code == _lib.KV_FP4_E2M1  # the kernel then writes q and k only: a pool of no slots
     args = _lib.pack_rope_args(
         qkv.data_ptr(), qkv.stride(0) if N > 1 else width, positions.data_ptr(), N, num_heads, num_kv_heads, head_dim,
@@ -458,7 +457,8 @@ def _rope_store(qkv, positions, q_norm_weight, k_norm_weight, eps, cos_sin, num_
         q.data_ptr(), k.data_ptr(), slot_mapping.data_ptr(), _lib.KV_BF16 if fp4 else code, scale_floor, k_cache.data_ptr(),
         v_cache.data_ptr(), _ptr(k_scale) or 0, _ptr(v_scale) or 0, 0 if fp4 else blocks * block)
     _launch(index, "slo_rope_store", args)
-    v = qkv[:, (num_heads + num_kv_heads) * head_dim:].view(N, num_kv_heads, head_dim)
+    v = qkv.as_strided((N, num_kv_heads, head_dim), (qkv.stride(0), head_dim, 1),
+                       qkv.storage_offset() + (num_heads + num_kv_heads) * head_dim)
     if fp4:
         store_kvcache(k, v, k_cache, v_cache, slot_mapping, k_scale, v_scale, scale_floor)
     return q, k, v
@@ -941,7 +941,7 @@ def _paged_attention_window(q, k_cache, v_cache, softmax_scale, num_kv_heads, k_
         index, geometry = _check_query(q, num_kv_heads, k_cache, k_scale, v_cache, v_scale, True, decode_lens, decode_tables,
                                        cu_q, cu_k, tables, k, v, out)
     if out is None:
-        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+        out = q.new_empty(q.shape)
     elif out.dtype != torch.bfloat16:
         raise TypeError("out must be bf16")
     elif out.shape != q.shape or out.stride(2) != 1 or out.stride(1) != q.shape[2]:

@@ -130,20 +130,24 @@ __device__ __forceinline__ int64_t pool_row(const WinParams& p, const int32_t* t
   return (block * p.block_size + off) * p.hkv + head;
 }
 
-// Four operands of a query, channels 32 kg .. 32 kg + 31; zeros where not live.
-__device__ __forceinline__ void load_q(bf16x8 (&q)[4], const WinParams& p, int64_t row, int h, int kg, bool live) {
-  u32x4 x[4] = {};
+// Four operands of a query, channels 32 kg .. 32 kg + 31 (zeros where not live):
+// the load, and, once what else is to be loaded is on its way, the sign.
+__device__ __forceinline__ void load_q(u32x4 (&x)[4], const WinParams& p, int64_t row, int h, int kg, bool live) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = u32x4{0, 0, 0, 0};
   if (live) {
     const uint16_t* from = p.q + row * p.q_stride + h * HD + 32 * kg;
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = ld16(from + 8 * i);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[i][j] ^= p.q_sign;
   }
+}
+__device__ __forceinline__ void operands(bf16x8 (&q)[4], u32x4 (&x)[4], const WinParams& p) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) q[i] = as_bf16x8(x[i]);
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[i][j] ^= p.q_sign;
+    q[i] = as_bf16x8(x[i]);
+  }
 }
 
 // Four tokens' channel pairs as two channels' token quadruples.
@@ -404,10 +408,12 @@ __device__ void decode_item(const WinParams& p, DecodeLds<F, WAVES>& lds, int r,
   constexpr int T = Step<F>::T, H = T / 16;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, kg = lane >> 4;
-  bf16x8 q[4];
-  load_q(q, p, r, head * p.group + c, kg, c < p.group);
+  u32x4 raw[4];
+  load_q(raw, p, r, head * p.group + c, kg, c < p.group);
   const Chunks<F> ch = chunks_of<F>(p, r);
   if (chunk >= ch.count) return;
+  bf16x8 q[4];
+  operands(q, raw, p);
   const int begin = chunk * ch.per + wave, end = min((chunk + 1) * ch.per, ch.s.steps);
   DecodeAcc a;
 #pragma unroll
@@ -861,13 +867,13 @@ __device__ void prefill_item(const WinParams& p, PrefillLds<F, HALVES>& lds, int
   // mask with a query of zeros.
   const int t0 = min(w0 + wave * each, w1 - 1), t1 = max(min(w0 + wave * each + each, w1), t0 + 1);
   int at[NT];
-  bf16x8 q[NT][4];
+  u32x4 raw[NT][4];
   Acc a;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int x = 16 * n + c, y = by_group(p, x), tok = w0 + wave * each + y;
     at[n] = g.prefix + min(tok, t1 - 1);
-    load_q(q[n], p, g.q0 + tok, head * p.group + x - y * p.group, kg, y < each && tok < w1);
+    load_q(raw[n], p, g.q0 + tok, head * p.group + x - y * p.group, kg, y < each && tok < w1);
 #pragma unroll
     for (int i = 0; i < 8; ++i) a.o[n][i] = f32x4{0, 0, 0, 0};
     a.ncm[n] = INFINITY;
@@ -880,6 +886,9 @@ __device__ void prefill_item(const WinParams& p, PrefillLds<F, HALVES>& lds, int
     Quarter<F> t;
     int in = 0;
     if (from + half < to) load_quarter<F>(t, p, g, table, head, key_of<64>(s, from + half), lanes, wave, lane, in);
+    bf16x8 q[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) operands(q[n], raw[n], p);
     for (int i = from + half; i < to + half; i += HALVES) {
       Stage<F>& st = lds.st[half][(i - from) / HALVES & 1];
       const bool mine = HALVES == 1 || i < to;  // the last turn may have steps for one half only

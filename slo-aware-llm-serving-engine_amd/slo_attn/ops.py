@@ -453,7 +453,7 @@ def _rope_store(qkv, positions, q_norm_weight, k_norm_weight, eps, cos_sin, num_
     fp4 = code == _lib.KV_FP4_E2M1  # the kernel then writes q and k only: a pool of no slots
     args = _lib.pack_rope_args(
         qkv.data_ptr(), qkv.stride(0) if N > 1 else width, positions.data_ptr(), N, num_heads, num_kv_heads, head_dim,
-        _ptr(q_norm_weight) or 0, _ptr(k_norm_weight) or 0, eps, cos_sin.shape[0], cos_sin.data_ptr(), rot, interleaved,
+        _ptr(q_norm_weight) or 0, _ptr(k_norm_weight) or 0, 0.0 if q_norm_weight is None else eps, cos_sin.shape[0], cos_sin.data_ptr(), rot, interleaved,
         q.data_ptr(), k.data_ptr(), slot_mapping.data_ptr(), _lib.KV_BF16 if fp4 else code, scale_floor, k_cache.data_ptr(),
         v_cache.data_ptr(), _ptr(k_scale) or 0, _ptr(v_scale) or 0, 0 if fp4 else blocks * block)
     _launch(index, "slo_rope_store", args)

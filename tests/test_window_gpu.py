@@ -149,6 +149,80 @@ def test_captured_step_replays(device, fmt):
         assert torch.equal(captured, step())
 
 
+def test_two_captured_graphs_replay_at_once(device):
+    # each graph has its own workspace: cut decode rows, halves of tiles and cut tiles
+    cases = [WindowRows("bf16", [2500, 900], [(60, 1900)], hq=8, hkv=2, seed=s, window=1800) for s in (31, 32)]
+    states = [(c.q.to(device), c.pool.device(device), c.arguments(device)) for c in cases]
+
+    def run(i):
+        q, (kc, vc, _, _), args = states[i]
+        return slo_attn.paged_attention(q, kc, vc, cases[i].scale, num_kv_heads=2, window=1800, sinks=4, **args)
+
+    want = [run(0), run(1)]
+    torch.cuda.synchronize()
+    graphs, got = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], [None, None]
+    for i in (0, 1):
+        with torch.cuda.graph(graphs[i]):
+            got[i] = run(i)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        run(0)
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "fp8_e4m3fn"])
+def test_captured_mixed_steps_of_windowed_layers(device, fmt):
+    # a bucket's graph (metadata, store, attention; padded rows and tokens) against the same bucket run eagerly
+    hq, hkv, block, width = 8, 2, 64, 6
+    pool = slo_attn.KVPool(2, 24, block, hkv, D, fmt, device)
+    layers = [slo_attn.Attention(hq, D, D ** -0.5, hkv, window=w, sinks=3) for w in (33, 100)]
+    pool.attach(layers)
+    g = torch.Generator().manual_seed(3)
+    table = random_values(g, 50, hq + 2 * hkv, D).to(device)
+
+    def forward(ids, positions):
+        x = table[ids]
+        out = 0
+        for layer in layers:
+            out = out + layer(x[:, :hq].contiguous(), x[:, hq:hq + hkv], x[:, hq + hkv:])
+        return out
+
+    buf = slo_attn.MixedStepBuffers(4, 3, 150, width, block, width * block, device)
+    graph = slo_attn.MixedStepGraph(buf, forward, exact_history=fmt != "bf16")
+    pool.kv.zero_()
+    rows = [[0, 1, 7], [2], [5], [6]]
+    steps = [([], [(0, 60), (0, 33)], [[0, 1], [2]], [i % 50 for i in range(93)]),
+             ([60, 33], [(0, 20)], [[0, 1], [2], [5]], list(range(22))),
+             ([61, 34, 20], [(0, 1)], [[0, 1], [2], [5], [6]], [1, 2, 3, 4]),
+             ([35, 21], [(62, 100)], [[2], [5], rows[0]], [i % 50 for i in range(102)])]
+    for step in steps:
+        before = pool.kv.clone(), None if pool.scale is None else pool.scale.clone()
+        got = graph.run(*step).clone()
+        torch.cuda.synchronize()
+        after = pool.kv.clone()
+        pool.kv.copy_(before[0])
+        if before[1] is not None:
+            pool.scale.copy_(before[1])
+        buf.build()
+        buf.set_context(fmt == "bf16" or any(s for s, n in step[1] if n))
+        want = forward(buf.input_ids, buf.positions)
+        slo_attn.reset_context()
+        assert torch.isfinite(want).all() and torch.equal(got, want) and torch.equal(after, pool.kv)
+
+
+def test_rows_do_not_depend_on_their_neighbours(device):
+    # a row alone takes other launch shapes (halves, cuts) than among many: both within the bound of the same result
+    case = WindowRows("bf16", [1200, 700] * 20, [(50, 600), (33, 0)] * 6, hq=16, hkv=4, seed=6, window=500)
+    want, bound = case.attend()
+    check(call(case, device), want, bound)
+    one = WindowRows("bf16", [], [(50, 600)], hq=16, hkv=4, seed=7, window=500)
+    check(call(one, device), *one.attend())
+
+
 def test_two_streams_at_once(device):
     cases = [WindowRows("bf16", [2500, 300], [(60, 900)], hq=16, hkv=4, seed=s, window=1400) for s in (21, 22)]
     states = [(c.q.to(device), c.pool.device(device), c.arguments(device)) for c in cases]

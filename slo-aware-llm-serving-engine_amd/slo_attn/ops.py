@@ -106,15 +106,15 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
 
 def _one_device(first: torch.Tensor, *others) -> int:
     """The index of the GPU that holds all tensors (None: left out)."""
-    device = first.device
-    if device.type != "cuda":
+    index = first.get_device()  # (an int, -1 on the CPU; a device object takes twice as long to compare)
+    if index < 0:
         raise RuntimeError("slo_attn kernels need GPU tensors; there is no CPU fallback")
     for t in others:
-        if t is not None and t.device != device:
+        if t is not None and t.get_device() != index:
             if t.device.type != "cuda":
                 raise RuntimeError("slo_attn kernels need GPU tensors; there is no CPU fallback")
-            raise RuntimeError(f"tensors on different devices: {device} vs {t.device}")
-    return device.index
+            raise RuntimeError(f"tensors on different devices: {first.device} vs {t.device}")
+    return index
 
 
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
@@ -135,7 +135,8 @@ def _launch(index: int, what: str, *args) -> None:
 def _int32(t: torch.Tensor, name: str) -> torch.Tensor:
     if t.dtype != torch.int32:
         raise TypeError(f"{name} must be int32, got {t.dtype}")
-    if t.dim() == 1 and t.stride(0) != 1:
+    stride = t.stride()
+    if len(stride) == 1 and stride[0] != 1:
         raise ValueError(f"{name} must be contiguous")
     return t
 
@@ -571,7 +572,7 @@ def _row_args(T, num_decode, decode_lens, decode_tables, num_prefill, cu_q, cu_k
     ``PagedAttentionArgs``: those of the decode rows, then those of the prefill rows."""
     if not 0 <= num_decode <= T:
         raise ValueError("num_decode must be from 0 to the number of query rows")
-    decode, prefill = (num_decode, None, None, 0, 0), (0, None, None, 0, 0, None, 0, 0)
+    decode, prefill = (num_decode, 0, 0, 0, 0), (0, 0, 0, 0, 0, 0, 0, 0)
     if num_prefill and cu_q is not None:  # where the prefill rows end matters in either phase
         _int32(cu_q, "cu_seqlens_q")
         if cu_q.numel() < num_prefill + 1:
@@ -599,9 +600,6 @@ def _row_args(T, num_decode, decode_lens, decode_tables, num_prefill, cu_q, cu_k
     return decode, prefill
 
 
-_NO_ROWS, _NO_STORE = (None, 0, None, 0, 0), (None, None, 0, None, 0, 0, 0.0)
-
-
 def _pool_call(what, extra, index, device, q, out, k_cache, v_cache, k_scale, v_scale, geometry, rows, scale, phases, sized=(),
                own=(0, 0, 0, 0, 0)):
     """Calls ``what`` over a pool with a workspace of the call's own, from torch's allocator: calls on several streams,
@@ -611,9 +609,11 @@ def _pool_call(what, extra, index, device, q, out, k_cache, v_cache, k_scale, v_
     T, num_heads, _ = q.shape
     decode, prefill = rows
     width = num_heads * head_dim
-    fields = (q.data_ptr(), q.stride(0) if T > 1 else width, _ptr(out) or 0, 0 if out is None else out.stride(0) if T > 1 else width,
-              T, _ptr(k_cache) or 0, _ptr(v_cache) or 0, _ptr(k_scale) or 0, _ptr(v_scale) or 0, code, blocks, block,
-              *(x or 0 for x in decode), *(x or 0 for x in prefill), *own, num_heads, heads, head_dim, scale)
+    fields = (q.data_ptr(), q.stride(0) if T > 1 else width, 0 if out is None else out.data_ptr(),
+              0 if out is None else out.stride(0) if T > 1 else width, T, 0 if k_cache is None else k_cache.data_ptr(),
+              0 if v_cache is None else v_cache.data_ptr(), 0 if k_scale is None else k_scale.data_ptr(),
+              0 if v_scale is None else v_scale.data_ptr(), code, blocks, block, *decode, *prefill, *own, num_heads, heads,
+              head_dim, scale)
     key = (what, T, num_heads, heads, code, block, phases, decode[0], decode[4], prefill[0], prefill[3], prefill[4], prefill[7],
            own[4], *sized)
     need = _sizes.get(key)
@@ -962,7 +962,7 @@ def _paged_attention_window(q, k_cache, v_cache, softmax_scale, num_kv_heads, k_
         _int32(cu_k, "cu_seqlens_k")
         if cu_q.numel() < num_prefill + 1 or cu_k.numel() < num_prefill + 1:
             raise ValueError("cu_seqlens shorter than num_prefill + 1")
-        rows = decode, (num_prefill, cu_q.data_ptr(), cu_k.data_ptr(), 0, 0, None, 0, 0)
+        rows = decode, (num_prefill, cu_q.data_ptr(), cu_k.data_ptr(), 0, 0, 0, 0, 0)
     else:
         rows = _row_args(q.shape[0], num_decode, decode_lens, decode_tables, num_prefill, cu_q, cu_k, 0, 0, tables, phases)
     if slot_mapping is not None:

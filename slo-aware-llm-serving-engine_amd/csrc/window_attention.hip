@@ -19,7 +19,11 @@
 // the other operand as they lie.  Pools of all three formats take this one
 // order: codes are converted to bf16 operands exactly (E4M3FN scales multiply
 // scores and weights, E8M0 ones go in with the conversion).
-// Sums, maxima and outputs are fp32 until the one rounding at the end.
+// Sums, maxima and outputs are fp32 until the one rounding at the end.  Weights
+// are rounded to bf16 for the second product: in two terms, which carry them to
+// 2^-17, for decode rows, whose outputs are then off by the output's rounding alone
+// (0.0016-0.0017 of their size); in one for prefill rows (0.0021-0.0023), where a
+// second term would double that product.
 #include "capi_internal.h"
 #include "fp4.h"
 #include "tile_io.h"
@@ -31,7 +35,10 @@ namespace {
 
 constexpr int RECORD = HD + 4;   // floats of a decode chunk's partial result: outputs, maximum, sum, 2 unused
 constexpr float kNone = -1e30f;  // running maximum before the first key
-constexpr float kSumMax = 224.0f;  // largest sum of a lane's weights in a step before the reference moves
+// Largest sum of a prefill lane's weights in a step before its column's
+// reference moves to the step's maximum, so that most steps need no maximum:
+// weights keep their relative rounding up to there, sums far from overflow.
+constexpr float kSumMax = 224.0f;
 constexpr int NT = 2;            // 16-column blocks of a prefill wavefront
 constexpr int kWaves = 4;        // wavefronts that run a tile
 
@@ -403,6 +410,11 @@ struct DecodeLds {
 // One chunk of one (row, kv head) a workgroup, its wavefronts a step each in
 // turn, all heads of the group as columns.  Each wavefront fetches its own
 // steps, so the loop has no barrier; the wavefronts' results meet in LDS.
+// Bound by the read: 64 rows under 1,024 keys and 4 sinks, 8 kv heads of bf16
+// (268 MB), 47.5 us or 5.6 TB/s, 47.0 with the arithmetic left out and about 4 of
+// them before the first key (length, page, key); E4M3FN 33.9 (32.2); 4 bits under
+// 2,048 keys (138 MB) 32.5 (28.6).  Eight wavefronts: bf16 49.4, 4 bits 34; four of
+// the 4-bit steps in flight 35.5.
 template <int F, int WAVES>
 __device__ void decode_item(const WinParams& p, DecodeLds<F, WAVES>& lds, int r, int chunk, int head) {
   constexpr int T = Step<F>::T, H = T / 16;
@@ -848,7 +860,14 @@ union PrefillLds {
 // step into operands together, a quarter each, and each runs 16 NT columns,
 // (query, head of the group) pairs of consecutive queries, over them; the next
 // step loads meanwhile.  With two halves of four wavefronts each half takes
-// every other step.
+// every other step.  4,096 queries of 32 heads under 4,096 keys run 270 us, 1,020
+// TFLOP/s (a library product of 8,192^3: 1,406): matrix cores busy 46% of the
+// time, LDS 40%, and lane operations (exponents, sums, masks, packing) most of the
+// rest, which two wavefronts a SIMD hardly overlap.  Four column blocks a wavefront
+// and one wavefront a SIMD took 566, no scheduling barriers 288 for 283, products
+// in four independent chains no less.  A launch of few steps mostly waits: 2.5 us
+// to the tile, 3.2 for queries and output, 2.5 for page and first keys, 2.8 for the
+// first step, 1 of them for the first maximum.
 template <int F, int HALVES>
 __device__ void prefill_item(const WinParams& p, PrefillLds<F, HALVES>& lds, int item, int part, int head) {
   const int lane = threadIdx.x & 63, any = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1116,6 +1135,21 @@ int decode_chunks(int64_t pairs, int64_t keys) {
   return chunks > 1 && keys - keys / chunks >= 512 ? (int)chunks : 1;
 }
 
+// Where all tiles fit one to a CU, beside the decode rows' workgroups, a second
+// half of each takes every other step: no records and no join.  us with one
+// half / two, 32 and 8 heads of bf16 behind 6,000 keys: 512 queries under 512 keys
+// 25.3 / 22.9, under 1,024 37.8 / 31.8, 960 under 1,024 38.8 / 34.3, 2,000 (504
+// tiles) 52.3 / 64.3; 24 decode rows and two chunks of 512 32.2 / 38.2.
+// Few tiles are cut into parts besides, as far as CUs are left: of 4 steps or
+// more where there is room for four parts (32 queries, 8 tiles: under 512 keys whole
+// 21.4, so 18.9; under 1,024 30.2, parts of 8, 6, 4 steps 22.9, 20.7, 17.7; under
+// 4,096 parts of 16, 8, 4 steps 32.7, 24.7, 24.2), else of 12 (512 queries, 128
+// tiles: under 512 keys whole 22.8, parts of 4 steps 27.9; under 1,024 31.5, parts
+// of 6 32.5; under 4,096 whole 85.6, in two 55.8).
+int tile_parts(int64_t tiles, int64_t steps) {
+  return (int)std::max<int64_t>(1, std::min(kSlots / 2 / tiles, steps / (4 * tiles <= kSlots / 2 ? 4 : 12)));
+}
+
 Plan plan_of(const slo_paged_attention_args* a, int window, int sinks) {
   Plan n = {false, false, 1, 0, 0, 1, 0, 0};
   const int group = a->num_heads / a->num_kv_heads;
@@ -1129,13 +1163,14 @@ Plan plan_of(const slo_paged_attention_args* a, int window, int sinks) {
     n.pwork = true;
     // The rows' queries together bound the tiles.
     const int per = kWaves * (16 * NT / group);
-    n.items = (int)((int64_t)(a->num_q_rows - a->num_decode) / per + a->num_prefill);
+    const int64_t tokens = a->num_q_rows - a->num_decode;
+    n.items = (int)(tokens / per + a->num_prefill);
     const int64_t cap = a->prefill_tables ? (int64_t)a->prefill_table_width * a->block_size : a->num_kv_rows;
     const int64_t steps = most_steps(window, sinks, per, cap);
-    // Tiles, if every row's are full ones (workgroups past the last tile end at once).
-    const int64_t tiles = std::max<int64_t>(1, (a->num_q_rows - a->num_decode + per - 1) / per) * a->num_kv_heads;
+    // About the tiles there are; workgroups past the last one end at once.
+    const int64_t tiles = std::max<int64_t>(a->num_prefill, (tokens + per - 1) / per) * a->num_kv_heads;
     n.halves = tiles + (n.dwork ? (int64_t)a->num_decode * a->num_kv_heads : 0) <= kSlots / 2 ? 2 : 1;
-    if (n.halves == 2) n.splits = (int)std::max<int64_t>(1, std::min(kSlots / 2 / tiles, steps / 16));
+    if (n.halves == 2) n.splits = tile_parts(tiles, steps);
     if (n.splits > 1) n.pbytes = (size_t)n.items * a->num_kv_heads * n.splits * sizeof(Part);
   }
   return n;

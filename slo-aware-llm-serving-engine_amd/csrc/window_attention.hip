@@ -510,20 +510,25 @@ __device__ void decode_item(const WinParams& p, DecodeLds<F, WAVES>& lds, int r,
 }
 
 // ------------------------------------------------------------ prefill rows
-// One 64-token step of a workgroup as bf16 operands in LDS, in the order in
-// which lanes read them (16 bytes a lane, no bank twice): K's four operands of
-// each 16 tokens, V's eight of each 32 tokens, and E4M3FN's scales.
+// One 64-token step of a workgroup in LDS.  Quantised: as bf16 operands in the
+// order in which lanes read them (16 bytes a lane, no bank twice): K's four
+// operands of each 16 tokens, V's eight of each 32 tokens, and E4M3FN's scales.
 template <int F>
 struct Stage {
   u32x4 k[4][4][64], v[2][8][64];
   float s[F == KV_FP8_E4M3FN ? 2 : 1][64];
 };
+// bf16 needs no conversion: rows as they are, sent there by the memory system in
+// whole rows, 16-byte part x of token t at part x ^ (t mod 16) so that no read has
+// a bank twice, V turned as it is read.  (By way of registers, a lane 64 bytes of a
+// K row and 16 of four V rows, 4,096 queries on 8,191 keys took 276 us for 258, cold
+// rows of 7,733 tokens 149 for 137, 24 decode rows and two chunks of 512 28.9 for 26.5.)
+template <> struct Stage<KV_BF16> {
+  u32x4 k[64][16], v[64][16];
+};
 
 // A wavefront's quarter of a step, 16 tokens, as loaded.
-template <int F> struct Quarter;
-template <> struct Quarter<KV_BF16> {
-  u32x4 k[4], v[4];
-};
+template <int F> struct Quarter {};
 template <> struct Quarter<KV_FP8_E4M3FN> {
   u32x4 k[2];
   u32x2 v[4];
@@ -563,11 +568,15 @@ struct Lanes {
 template <int F>
 __device__ __forceinline__ Lanes lanes_of(const WinParams& p, int wave, int lane) {
   const uint32_t c = lane & 15, kg = lane >> 4, row = F == KV_BF16 ? 256 : F == KV_FP8_E4M3FN ? 128 : 64;
-  const bool rows = F == KV_BF16 && !p.ptables;
   const uint32_t stride = F == KV_FP4_E2M1 ? row : p.hkv * row;
   Lanes l;
-  l.k = (16 * wave + c) * (rows ? (uint32_t)p.rk_stride : stride) + kg * (row / 4);
-  l.v = (16 * wave + 4 * kg) * (rows ? (uint32_t)p.rv_stride : stride) + c * (row / 16);
+  if constexpr (F == KV_BF16) {  // tokens kg, kg + 4, .. of 16, whole rows by 16 lanes
+    l.k = (16 * wave + kg) * (p.ptables ? stride : (uint32_t)p.rk_stride);
+    l.v = (16 * wave + kg) * (p.ptables ? stride : (uint32_t)p.rv_stride);
+  } else {
+    l.k = (16 * wave + c) * stride + kg * (row / 4);
+    l.v = (16 * wave + 4 * kg) * stride + c * (row / 16);
+  }
   return l;
 }
 
@@ -580,40 +589,52 @@ __device__ __forceinline__ T load(const void* base, uint32_t off, int more = 0) 
   return *reinterpret_cast<const T*>(static_cast<const uint8_t*>(base) + off + more);
 }
 
+// This wavefront's 16 of the 64 tokens from `key` on, bf16, straight to LDS.
+__device__ __forceinline__ void send_quarter(Stage<KV_BF16>& s, const WinParams& p, const PrefillRow& g, const int32_t* table,
+                                             int head, int key, const Lanes& l, int wave, int lane, int& ok) {
+  const uint32_t kg = lane >> 4, part = 16 * ((lane & 15) ^ kg);
+  const uint32_t tk = lds_addr(&s.k[16 * wave]), tv = lds_addr(&s.v[16 * wave]);
+  const uint8_t *k, *v;
+  uint32_t ks = p.hkv * 256, vs = ks;
+  ok = true;
+  if (p.ptables) {
+    const int64_t row = pool_row<KV_BF16>(p, table, head, key, ok);
+    k = p.kc + row * 256;
+    v = p.vc + row * 256;
+  } else {
+    ks = p.rk_stride;
+    vs = p.rv_stride;
+    const int64_t row = (int64_t)g.k0 + key;
+    k = p.rk + row * p.rk_stride + head * 256;
+    v = p.rv + row * p.rv_stride + head * 256;
+    const int last = g.lk - 1 - key;
+    if (last < 63) {  // nothing is read past the rows' end
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t t = min((int)(16 * wave + 4 * i + kg), last);
+        dma16(k + t * ks + (part ^ 64 * i), tk + 1024 * i);
+        dma16(v + t * vs + (part ^ 64 * i), tv + 1024 * i);
+      }
+      return;
+    }
+  }
+  int a[4], b[4];  // (a row is 256 bytes or more from the next: none is negative)
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t x = part ^ 64 * i;
+    a[i] = l.k + x + i * (4 * ks - 1024);
+    b[i] = l.v + x + i * (4 * vs - 1024);
+  }
+  dma16x4_at(k, a, tk);
+  dma16x4_at(v, b, tv);
+}
+
 // This wavefront's 16 of the 64 tokens from `key` on.
 template <int F>
-__device__ __forceinline__ void load_quarter(Quarter<F>& t, const WinParams& p, const PrefillRow& g, const int32_t* table,
-                                             int head, int key, const Lanes& l, int wave, int lane, int& ok) {
+__device__ __forceinline__ void load_quarter(Quarter<F>& t, const WinParams& p, const int32_t* table, int head, int key,
+                                             const Lanes& l, int wave, int lane, int& ok) {
   const int c = lane & 15, kg = lane >> 4;
-  if constexpr (F == KV_BF16) {
-    const uint8_t *k, *v;
-    uint32_t stride = p.hkv * 256;
-    ok = true;
-    if (p.ptables) {
-      const int64_t row = pool_row<F>(p, table, head, key, ok);
-      k = p.kc + row * 256;
-      v = p.vc + row * 256;
-    } else {
-      stride = p.rv_stride;
-      const int64_t row = (int64_t)g.k0 + key;
-      k = p.rk + row * p.rk_stride + head * 256;
-      v = p.rv + row * p.rv_stride + head * 256;
-      const int last = g.lk - 1 - key;
-      if (last < 63) {  // nothing is read past the rows' end
-        k += min(16 * wave + c, last) * (uint32_t)p.rk_stride;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          t.k[i] = ld16(k + 64 * kg + 16 * i);
-          t.v[i] = ld16(v + min(16 * wave + 4 * kg + i, last) * stride + 16 * c);
-        }
-        return;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) t.k[i] = load<u32x4>(k, l.k, 16 * i);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) t.v[i] = load<u32x4>(v + i * stride, l.v);
-  } else if constexpr (F == KV_FP8_E4M3FN) {
+  if constexpr (F == KV_FP8_E4M3FN) {
     const int64_t row = pool_row<F>(p, table, head, key, ok);
     const uint8_t *k = p.kc + row * 128, *v = p.vc + row * 128;
 #pragma unroll
@@ -637,15 +658,20 @@ __device__ __forceinline__ void load_quarter(Quarter<F>& t, const WinParams& p, 
 // Clears the V tokens that none of the tile's queries sees, of a step from
 // `key` on that may hold some.  They may be anything in the pages, and a weight
 // of zero must not make that a NaN.
+__device__ __forceinline__ void clear_unseen(Stage<KV_BF16>& s, int key, int first, int end, int sinks, int wave, int lane) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int t = 16 * wave + 4 * i + (lane >> 4), k = key + t;
+    if (!((k < end) & ((k >= first) | (k < sinks)))) s.v[t][lane & 15] = u32x4{0, 0, 0, 0};
+  }
+}
 template <int F>
 __device__ __forceinline__ void clear_unseen(Quarter<F>& t, int key, int first, int end, int sinks, int wave, int lane) {
   const int k = key + 16 * wave + 4 * (lane >> 4);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const bool seen = (k + i < end) & ((k + i >= first) | (k + i < sinks));
-    if constexpr (F == KV_BF16) {
-      t.v[i] = seen ? t.v[i] : u32x4{0, 0, 0, 0};
-    } else if constexpr (F == KV_FP8_E4M3FN) {
+    if constexpr (F == KV_FP8_E4M3FN) {
       t.v[i] = seen ? t.v[i] : u32x2{0, 0};
     } else {
       t.vs[i] = seen ? t.vs[i] : 0;
@@ -661,13 +687,7 @@ template <int F>
 __device__ __forceinline__ void stage(Stage<F>& s, const Quarter<F>& t, int wave, int lane) {
   const int c = lane & 15;
   u32x4 v[4];
-  if constexpr (F == KV_BF16) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      s.k[wave][i][lane] = t.k[i];
-      v[i] = t.v[i];
-    }
-  } else if constexpr (F == KV_FP8_E4M3FN) {
+  if constexpr (F == KV_FP8_E4M3FN) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       s.k[wave][2 * i][lane] = fp8x8_to_bf16x8(u32x2{t.k[i][0], t.k[i][1]});
@@ -695,6 +715,25 @@ __device__ __forceinline__ void stage(Stage<F>& s, const Quarter<F>& t, int wave
   }
 }
 
+// K's operand i of 16 tokens t, V's operand i of 32 tokens g.
+template <int F>
+__device__ __forceinline__ bf16x8 k_operand(const Stage<F>& s, int t, int i, int lane) {
+  if constexpr (F == KV_BF16) return as_bf16x8(s.k[16 * t + (lane & 15)][(4 * (lane >> 4) + i) ^ (lane & 15)]);
+  else return as_bf16x8(s.k[t][i][lane]);
+}
+template <int F>
+__device__ __forceinline__ bf16x8 v_operand(const Stage<F>& s, int g, int i, int lane) {
+  if constexpr (F == KV_BF16) {
+    // The lanes of a column group read 4 tokens' 8 channels at 8 i and 64 + 8 i
+    // and receive a channel's 4 tokens each.
+    const int t = 4 * (lane >> 4) + ((lane & 15) >> 2), x = (4 * (lane & 2) + i) ^ t;
+    const uint8_t* from = reinterpret_cast<const uint8_t*>(&s.v[32 * g + t][x]) + 8 * (lane & 1);
+    return join_tr(lds_tr16(from), lds_tr16(from + 16 * 256));
+  } else {
+    return as_bf16x8(s.v[g][i][lane]);
+  }
+}
+
 struct Acc {
   f32x4 o[NT][8];
   float ncm[NT], l[NT];  // minus the reference in the log2 domain (+inf before the first key), this lane's sum
@@ -714,11 +753,11 @@ __device__ __forceinline__ void staged_step(const WinParams& p, const Stage<F>& 
   f32x4 s[NT][4];
   bf16x8 x[2][4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) x[0][i] = as_bf16x8(st.k[0][i][lane]);
+  for (int i = 0; i < 4; ++i) x[0][i] = k_operand<F>(st, 0, i, lane);
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[(t + 1) & 1][i] = as_bf16x8(t < 3 ? st.k[t + 1][i][lane] : st.v[0][i][lane]);
+    for (int i = 0; i < 4; ++i) x[(t + 1) & 1][i] = t < 3 ? k_operand<F>(st, t + 1, i, lane) : v_operand<F>(st, 0, i, lane);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -803,7 +842,7 @@ __device__ __forceinline__ void staged_step(const WinParams& p, const Stage<F>& 
     const int g = j >> 1;
     if (j < 3) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[(j + 1) & 1][i] = as_bf16x8(st.v[(j + 1) >> 1][4 * ((j + 1) & 1) + i][lane]);
+      for (int i = 0; i < 4; ++i) x[(j + 1) & 1][i] = v_operand<F>(st, (j + 1) >> 1, 4 * ((j + 1) & 1) + i, lane);
     }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -904,26 +943,39 @@ __device__ void prefill_item(const WinParams& p, PrefillLds<F, HALVES>& lds, int
     const Lanes lanes = lanes_of<F>(p, wave, lane);
     Quarter<F> t;
     int in = 0;
-    if (from + half < to) load_quarter<F>(t, p, g, table, head, key_of<64>(s, from + half), lanes, wave, lane, in);
+    auto get = [&](int i, int to_buffer) {
+      if constexpr (F == KV_BF16) send_quarter(lds.st[half][to_buffer], p, g, table, head, key_of<64>(s, i), lanes, wave, lane, in);
+      else load_quarter<F>(t, p, table, head, key_of<64>(s, i), lanes, wave, lane, in);
+    };
+    if (from + half < to) get(from + half, 0);
     bf16x8 q[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) operands(q[n], raw[n], p);
     for (int i = from + half; i < to + half; i += HALVES) {
-      Stage<F>& st = lds.st[half][(i - from) / HALVES & 1];
+      const int buffer = (i - from) / HALVES & 1;
+      Stage<F>& st = lds.st[half][buffer];
       const bool mine = HALVES == 1 || i < to;  // the last turn may have steps for one half only
       const int key = key_of<64>(s, i);
       const int ok = in;  // whether the step's page is in the pool
       if (mine) {
-        if (!ok || key + 64 > s.end || (key < s.first && key + 64 > p.sinks))
-          clear_unseen<F>(t, key, s.first, ok ? s.end : 0, p.sinks, wave, lane);
-        stage<F>(st, t, wave, lane);
-        if (i + HALVES < to) load_quarter<F>(t, p, g, table, head, key_of<64>(s, i + HALVES), lanes, wave, lane, in);
+        const bool unseen = !ok || key + 64 > s.end || (key < s.first && key + 64 > p.sinks);
+        if constexpr (F == KV_BF16) {
+          __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // this wavefront's quarter has come
+          if (unseen) clear_unseen(st, key, s.first, ok ? s.end : 0, p.sinks, wave, lane);
+        } else {
+          if (unseen) clear_unseen<F>(t, key, s.first, ok ? s.end : 0, p.sinks, wave, lane);
+          stage<F>(st, t, wave, lane);
+          if (i + HALVES < to) get(i + HALVES, 0);
+        }
       }
-      // Two buffers: a wavefront comes to write this one again only past the
+      // Two buffers: a wavefront comes to fill this one again only past the
       // next step's barrier, when every wavefront has left it.  The barrier
       // waits for LDS only: the loads of the next step stay in flight.
       lds_sync();
       if (mine) {
+        if constexpr (F == KV_BF16) {
+          if (i + HALVES < to) get(i + HALVES, buffer ^ 1);
+        }
         const bool all = ok && key + 63 <= x0 && key + 64 <= g.lk && (key > x1 - p.window || key + 64 <= p.sinks);
         staged_step<F>(p, st, !all, i < s.sink, q, a, key, at, ok ? g.lk : 0, lane);
       }
@@ -961,22 +1013,41 @@ __device__ void prefill_item(const WinParams& p, PrefillLds<F, HALVES>& lds, int
     const float l = col_sum(a.l[n]);
     if (p.splits == 1) {
       const int x = 16 * n + col, y = by_group(p, x), tok = w0 + wave * each + y, h = head * p.group + x - y * p.group;
-      if (y >= each || tok >= w1) continue;
+      const bool live = y < each && tok < w1;
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      uint16_t* out = p.out + (int64_t)(g.q0 + tok) * p.out_stride + h * HD + 32 * kg;
+      uint16_t* out = p.out + (int64_t)(g.q0 + tok) * p.out_stride + h * HD;
+      if constexpr (F == KV_BF16) {
+        // A lane's 4 channels at 64 (kg / 2) + 8 e + 4 (kg mod 2): lanes of
+        // neighbouring kg exchange theirs of two e.
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const f32x4 v = a.o[n][e] * inv, w = a.o[n][e + 1] * inv;
+          const auto x = __builtin_amdgcn_permlane16_swap(pack_bf16x2(v[0], v[1]), pack_bf16x2(w[0], w[1]), false, false);
+          const auto y = __builtin_amdgcn_permlane16_swap(pack_bf16x2(v[2], v[3]), pack_bf16x2(w[2], w[3]), false, false);
+          if (live) *reinterpret_cast<u32x4*>(out + 64 * (kg >> 1) + 8 * (e + (kg & 1))) = u32x4{x[0], y[0], x[1], y[1]};
+        }
+        continue;
+      }
+      if (!live) continue;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<u32x4*>(out + 8 * i) =
+        *reinterpret_cast<u32x4*>(out + 32 * kg + 8 * i) =
             u32x4{pack_bf16x2(a.o[n][0][i] * inv, a.o[n][1][i] * inv), pack_bf16x2(a.o[n][2][i] * inv, a.o[n][3][i] * inv),
                   pack_bf16x2(a.o[n][4][i] * inv, a.o[n][5][i] * inv), pack_bf16x2(a.o[n][6][i] * inv, a.o[n][7][i] * inv)};
     } else {
       Part& out = p.parts[((int64_t)item * p.hkv + head) * p.splits + part];
       const int block = NT * wave + n;
+      if constexpr (F == KV_BF16) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int e = 0; e < 8; ++e)
+          out.o[block][2 * (e & 3) + (kg & 1)][col + 16 * (2 * (kg >> 1) + (e >> 2))] = a.o[n][e];
+      } else {
 #pragma unroll
-        for (int e = 0; e < 8; e += 4)
-          out.o[block][2 * i + (e >> 2)][lane] = f32x4{a.o[n][e][i], a.o[n][e + 1][i], a.o[n][e + 2][i], a.o[n][e + 3][i]};
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 8; e += 4)
+            out.o[block][2 * i + (e >> 2)][lane] = f32x4{a.o[n][e][i], a.o[n][e + 1][i], a.o[n][e + 2][i], a.o[n][e + 3][i]};
+      }
       if (kg == 0) {
         out.m[16 * block + col] = a.ncm[n] == INFINITY ? kNone : -a.ncm[n];
         out.l[16 * block + col] = l;

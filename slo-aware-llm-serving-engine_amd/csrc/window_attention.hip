@@ -521,7 +521,7 @@ struct Stage {
 // bf16 needs no conversion: rows as they are, sent there by the memory system in
 // whole rows, 16-byte part x of token t at part x ^ (t mod 16) so that no read has
 // a bank twice, V turned as it is read.  (By way of registers, a lane 64 bytes of a
-// K row and 16 of four V rows, 4,096 queries on 8,191 keys took 276 us for 258, cold
+// K row and 16 of four V rows, 4,096 queries under 4,096 keys took 276 us for 258, cold
 // rows of 7,733 tokens 149 for 137, 24 decode rows and two chunks of 512 28.9 for 26.5.)
 template <> struct Stage<KV_BF16> {
   u32x4 k[64][16], v[64][16];
@@ -740,16 +740,16 @@ struct Acc {
 };
 
 // 64 tokens from `key` on of a wavefront's columns against the staged operands,
-// read four ahead of the products.  The further a wavefront is from the step's
-// end the higher its priority, so that the two of a SIMD do not fall into step
-// (4,096 queries on 8,191 keys 282 -> 268 us; any one phase raised 271-282).  at[n]: position of column block n's query;
-// keys from `kend` on are not the row's.  A step before the window part (`sink`)
-// shows a query nothing but sinks.
+// read four ahead of the products.  A wavefront at its score products goes before
+// the other one of its SIMD, so that the two do not fall into step (4,096 queries
+// under 4,096 keys 254 us; no priorities, or others, 257-263).  at[n]: position of
+// column block n's query; keys from `kend` on are not the row's.  A step before the
+// window part (`sink`) shows a query nothing but sinks.
 template <int F>
 __device__ __forceinline__ void staged_step(const WinParams& p, const Stage<F>& st, bool masked, bool sink, const bf16x8 (&q)[NT][4],
                                             Acc& a, int key, const int (&at)[NT], int kend, int lane) {
   const int kg = lane >> 4;
-  __builtin_amdgcn_s_setprio(3);
+  __builtin_amdgcn_s_setprio(1);
   f32x4 s[NT][4];
   bf16x8 x[2][4];
 #pragma unroll
@@ -765,7 +765,7 @@ __device__ __forceinline__ void staged_step(const WinParams& p, const Stage<F>& 
       for (int n = 0; n < NT; ++n) s[n][t] = mfma16(x[t & 1][i], q[n][i], i ? s[n][t] : f32x4{0, 0, 0, 0});
     __builtin_amdgcn_sched_barrier(0);
   }
-  __builtin_amdgcn_s_setprio(2);
+  __builtin_amdgcn_s_setprio(0);
   // No maximum is formed: a reference that is too low shows in the sum of a
   // lane's weights (inf or NaN while it is unset).  Only then are the columns'
   // maxima found and the weights taken again.
@@ -836,7 +836,6 @@ __device__ __forceinline__ void staged_step(const WinParams& p, const Stage<F>& 
                                  pack_bf16x2(e[2 * g + 1][0], e[2 * g + 1][1]), pack_bf16x2(e[2 * g + 1][2], e[2 * g + 1][3])});
     __builtin_amdgcn_sched_barrier(0);
   }
-  __builtin_amdgcn_s_setprio(1);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {  // V's operands, four at a time
     const int g = j >> 1;
@@ -851,7 +850,6 @@ __device__ __forceinline__ void staged_step(const WinParams& p, const Stage<F>& 
       for (int n = 0; n < NT; ++n) a.o[n][4 * (j & 1) + i] = mfma16(x[j & 1][i], pr[n][g], a.o[n][4 * (j & 1) + i]);
     __builtin_amdgcn_sched_barrier(0);
   }
-  __builtin_amdgcn_s_setprio(0);
 }
 
 // Item i's row and tile: the rows' tiles in order, each row's last one (the
@@ -899,12 +897,13 @@ union PrefillLds {
 // step into operands together, a quarter each, and each runs 16 NT columns,
 // (query, head of the group) pairs of consecutive queries, over them; the next
 // step loads meanwhile.  With two halves of four wavefronts each half takes
-// every other step.  4,096 queries of 32 heads under 4,096 keys run 270 us, 1,020
-// TFLOP/s (a library product of 8,192^3: 1,406): matrix cores busy 46% of the
-// time, LDS 40%, and lane operations (exponents, sums, masks, packing) most of the
-// rest, which two wavefronts a SIMD hardly overlap.  Four column blocks a wavefront
-// and one wavefront a SIMD took 566, no scheduling barriers 288 for 283, products
-// in four independent chains no less.  A launch of few steps mostly waits: 2.5 us
+// every other step.  4,096 queries of 32 heads under 4,096 keys run 254-266 us, 1,060
+// TFLOP/s (a library product of 8,192^3: 1,406): matrix cores and lane operations
+// (exponents, sums, masks, packing) are busy about half of the time each and the two
+// wavefronts of a SIMD hardly overlap them.  Weights taken between the products,
+// one by one, came to the same (258 for 260; E4M3FN rows 36 for 39, mixed steps 28
+// for 26), pages looked up a step ahead too; four column blocks a wavefront and one
+// wavefront a SIMD took twice as long.  A launch of few steps mostly waits: 2.5 us
 // to the tile, 3.2 for queries and output, 2.5 for page and first keys, 2.8 for the
 // first step, 1 of them for the first maximum.
 template <int F, int HALVES>

@@ -137,15 +137,17 @@ __device__ __forceinline__ int64_t pool_row(const WinParams& p, const int32_t* t
   return (block * p.block_size + off) * p.hkv + head;
 }
 
-// Four operands of a query, channels 32 kg .. 32 kg + 31 (zeros where not live):
+// Four operands of a query, channels 32 kg .. 32 kg + 31, or with ROWS 8 kg ..
+// 8 kg + 7 of each 32 (zeros where not live):
 // the load, and, once what else is to be loaded is on its way, the sign.
+template <bool ROWS = false>
 __device__ __forceinline__ void load_q(u32x4 (&x)[4], const WinParams& p, int64_t row, int h, int kg, bool live) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) x[i] = u32x4{0, 0, 0, 0};
   if (live) {
-    const uint16_t* from = p.q + row * p.q_stride + h * HD + 32 * kg;
+    const uint16_t* from = p.q + row * p.q_stride + h * HD + (ROWS ? 8 : 32) * kg;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = ld16(from + 8 * i);
+    for (int i = 0; i < 4; ++i) x[i] = ld16(from + (ROWS ? 32 : 8) * i);
   }
 }
 __device__ __forceinline__ void operands(bf16x8 (&q)[4], u32x4 (&x)[4], const WinParams& p) {
@@ -715,10 +717,12 @@ __device__ __forceinline__ void stage(Stage<F>& s, const Quarter<F>& t, int wave
   }
 }
 
-// K's operand i of 16 tokens t, V's operand i of 32 tokens g.
+// K's operand i of 16 tokens t, V's operand i of 32 tokens g.  (bf16 K's channels
+// are 32 i + 8 kg on: with 32 kg + 8 i lanes that are served together meet a bank
+// twice, a third of LDS's time.)
 template <int F>
 __device__ __forceinline__ bf16x8 k_operand(const Stage<F>& s, int t, int i, int lane) {
-  if constexpr (F == KV_BF16) return as_bf16x8(s.k[16 * t + (lane & 15)][(4 * (lane >> 4) + i) ^ (lane & 15)]);
+  if constexpr (F == KV_BF16) return as_bf16x8(s.k[16 * t + (lane & 15)][(4 * i + (lane >> 4)) ^ (lane & 15)]);
   else return as_bf16x8(s.k[t][i][lane]);
 }
 template <int F>
@@ -930,7 +934,7 @@ __device__ void prefill_item(const WinParams& p, PrefillLds<F, HALVES>& lds, int
   for (int n = 0; n < NT; ++n) {
     const int x = 16 * n + c, y = by_group(p, x), tok = w0 + wave * each + y;
     at[n] = g.prefix + min(tok, t1 - 1);
-    load_q(raw[n], p, g.q0 + tok, head * p.group + x - y * p.group, kg, y < each && tok < w1);
+    load_q<F == KV_BF16>(raw[n], p, g.q0 + tok, head * p.group + x - y * p.group, kg, y < each && tok < w1);
 #pragma unroll
     for (int i = 0; i < 8; ++i) a.o[n][i] = f32x4{0, 0, 0, 0};
     a.ncm[n] = INFINITY;

@@ -564,17 +564,25 @@ __device__ __forceinline__ PrefillRow prefill_row(const WinParams& p, int r) {
 // Byte offsets of a lane's pieces (of V, of the first of its four tokens) from
 // its step's first token: the same at every step, so that a load is a uniform
 // base and one of these.
-struct Lanes {
+template <int F> struct Lanes {
   uint32_t k, v;
 };
+template <> struct Lanes<KV_BF16> {
+  int k[4], v[4];  // of tokens kg, kg + 4, .. of 16, whole rows by 16 lanes (see dma16x4_at)
+};
 template <int F>
-__device__ __forceinline__ Lanes lanes_of(const WinParams& p, int wave, int lane) {
+__device__ __forceinline__ Lanes<F> lanes_of(const WinParams& p, int wave, int lane) {
   const uint32_t c = lane & 15, kg = lane >> 4, row = F == KV_BF16 ? 256 : F == KV_FP8_E4M3FN ? 128 : 64;
   const uint32_t stride = F == KV_FP4_E2M1 ? row : p.hkv * row;
-  Lanes l;
-  if constexpr (F == KV_BF16) {  // tokens kg, kg + 4, .. of 16, whole rows by 16 lanes
-    l.k = (16 * wave + kg) * (p.ptables ? stride : (uint32_t)p.rk_stride);
-    l.v = (16 * wave + kg) * (p.ptables ? stride : (uint32_t)p.rv_stride);
+  Lanes<F> l;
+  if constexpr (F == KV_BF16) {
+    const uint32_t ks = p.ptables ? stride : (uint32_t)p.rk_stride, vs = p.ptables ? stride : (uint32_t)p.rv_stride;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // (a row is 256 bytes or more from the next: none is negative)
+      const uint32_t t = 16 * wave + 4 * i + kg, part = 16 * (c ^ (4 * i + kg));
+      l.k[i] = t * ks + part - 1024 * i;
+      l.v[i] = t * vs + part - 1024 * i;
+    }
   } else {
     l.k = (16 * wave + c) * stride + kg * (row / 4);
     l.v = (16 * wave + 4 * kg) * stride + c * (row / 16);
@@ -593,19 +601,15 @@ __device__ __forceinline__ T load(const void* base, uint32_t off, int more = 0) 
 
 // This wavefront's 16 of the 64 tokens from `key` on, bf16, straight to LDS.
 __device__ __forceinline__ void send_quarter(Stage<KV_BF16>& s, const WinParams& p, const PrefillRow& g, const int32_t* table,
-                                             int head, int key, const Lanes& l, int wave, int lane, int& ok) {
-  const uint32_t kg = lane >> 4, part = 16 * ((lane & 15) ^ kg);
+                                             int head, int key, const Lanes<KV_BF16>& l, int wave, int lane, int& ok) {
   const uint32_t tk = lds_addr(&s.k[16 * wave]), tv = lds_addr(&s.v[16 * wave]);
   const uint8_t *k, *v;
-  uint32_t ks = p.hkv * 256, vs = ks;
   ok = true;
   if (p.ptables) {
     const int64_t row = pool_row<KV_BF16>(p, table, head, key, ok);
     k = p.kc + row * 256;
     v = p.vc + row * 256;
   } else {
-    ks = p.rk_stride;
-    vs = p.rv_stride;
     const int64_t row = (int64_t)g.k0 + key;
     k = p.rk + row * p.rk_stride + head * 256;
     v = p.rv + row * p.rv_stride + head * 256;
@@ -613,28 +617,22 @@ __device__ __forceinline__ void send_quarter(Stage<KV_BF16>& s, const WinParams&
     if (last < 63) {  // nothing is read past the rows' end
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t t = min((int)(16 * wave + 4 * i + kg), last);
-        dma16(k + t * ks + (part ^ 64 * i), tk + 1024 * i);
-        dma16(v + t * vs + (part ^ 64 * i), tv + 1024 * i);
+        const int x = 4 * i + (lane >> 4), part = 16 * ((lane & 15) ^ x);
+        const uint32_t t = min(16 * wave + x, last);
+        dma16(k + t * (uint32_t)p.rk_stride + part, tk + 1024 * i);
+        dma16(v + t * (uint32_t)p.rv_stride + part, tv + 1024 * i);
       }
       return;
     }
   }
-  int a[4], b[4];  // (a row is 256 bytes or more from the next: none is negative)
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t x = part ^ 64 * i;
-    a[i] = l.k + x + i * (4 * ks - 1024);
-    b[i] = l.v + x + i * (4 * vs - 1024);
-  }
-  dma16x4_at(k, a, tk);
-  dma16x4_at(v, b, tv);
+  dma16x4_at(k, l.k, tk);
+  dma16x4_at(v, l.v, tv);
 }
 
 // This wavefront's 16 of the 64 tokens from `key` on.
 template <int F>
 __device__ __forceinline__ void load_quarter(Quarter<F>& t, const WinParams& p, const int32_t* table, int head, int key,
-                                             const Lanes& l, int wave, int lane, int& ok) {
+                                             const Lanes<F>& l, int wave, int lane, int& ok) {
   const int c = lane & 15, kg = lane >> 4;
   if constexpr (F == KV_FP8_E4M3FN) {
     const int64_t row = pool_row<F>(p, table, head, key, ok);
@@ -943,7 +941,7 @@ __device__ void prefill_item(const WinParams& p, PrefillLds<F, HALVES>& lds, int
   if (from < to) {
     const int32_t* table = p.ptables ? p.ptables + (int64_t)r * p.pstride : nullptr;
     const int x0 = g.prefix + t0, x1 = g.prefix + t1 - 1;
-    const Lanes lanes = lanes_of<F>(p, wave, lane);
+    const Lanes<F> lanes = lanes_of<F>(p, wave, lane);
     Quarter<F> t;
     int in = 0;
     auto get = [&](int i, int to_buffer) {

@@ -1082,13 +1082,13 @@ window_attention_kernel(WinParams p) {
 }
 
 // Decode rows alone.
-template <int F, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, 2)
+template <int F>
+__global__ void __launch_bounds__(64 * kWaves, 2)
 window_decode_kernel(WinParams p) {
-  __shared__ DecodeLds<F, WAVES> lds;
+  __shared__ DecodeLds<F, kWaves> lds;
   auto div = [](uint32_t x, uint32_t y) { return (int)__builtin_amdgcn_readfirstlane(x / y); };
   const int i = div(blockIdx.x, p.hkv), r = div(i, p.chunks);
-  decode_item<F, WAVES>(p, lds, r, i - r * p.chunks, blockIdx.x - i * p.hkv);
+  decode_item<F, kWaves>(p, lds, r, i - r * p.chunks, blockIdx.x - i * p.hkv);
   if (p.idle) clear_idle(p);
 }
 
@@ -1311,13 +1311,10 @@ int check_args(const slo_paged_attention_args* a, int window, int sinks) {
 }
 
 template <int F>
-constexpr int kDecodeWaves = 4;
-
-template <int F>
 void launch(const WinParams& p, int halves, hipStream_t s) {
   const unsigned blocks = (unsigned)(((int64_t)p.items * p.splits + (int64_t)p.drows * p.chunks) * p.hkv);
   if (!p.items)
-    hipLaunchKernelGGL((window_decode_kernel<F, kDecodeWaves<F>>), dim3(blocks), dim3(64 * kDecodeWaves<F>), 0, s, p);
+    hipLaunchKernelGGL(window_decode_kernel<F>, dim3(blocks), dim3(64 * kWaves), 0, s, p);
   else if (halves == 2)
     hipLaunchKernelGGL((window_attention_kernel<F, 2>), dim3(blocks), dim3(64 * kWaves * 2), 0, s, p);
   else

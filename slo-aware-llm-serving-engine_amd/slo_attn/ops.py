@@ -292,6 +292,12 @@ def _inverse_frequencies(dim: int, base: float, scaling: dict) -> tuple[torch.Te
         return freq, 1.0
     if kind not in ("linear", "yarn"):
         raise ValueError(f"rope scaling {kind!r} is not default, linear or yarn")
+    known = {"rope_type", "type", "factor", "original_max_position_embeddings"}
+    if kind == "yarn":
+        known |= {"attention_factor", "beta_fast", "beta_slow"}
+    if scaling.keys() - known or "factor" not in scaling or (kind == "yarn" and "original_max_position_embeddings" not in scaling):
+        raise ValueError(f"rope scaling {kind!r} needs its factor (yarn: and original_max_position_embeddings) and takes only "
+                         f"{', '.join(sorted(known))}")
     factor = float(scaling["factor"])
     if not factor >= 1.0 or factor == float("inf"):
         raise ValueError("the rope scaling factor must be finite and at least 1")

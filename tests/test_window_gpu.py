@@ -328,6 +328,28 @@ def test_a_conversation_through_the_layer(device, fmt):
         at = m
 
 
+def test_cold_rows_as_far_apart_as_they_may_be(device):
+    # a row every 64 MiB: a step's offsets pass 2^31; keys that no query sees are anything
+    n, keys, hkv, far, window = 40, 134, 2, (1 << 25) - 8, 30
+    g = torch.Generator().manual_seed(4)
+    q, k, v = random_values(g, n, 8, D), random_values(g, keys, hkv, D), random_values(g, keys, hkv, D)
+    k[1:keys - n - window + 1] = v[1:keys - n - window + 1] = float("nan")
+    base = torch.empty((keys - 1) * far + 2 * hkv * D, dtype=torch.bfloat16, device=device)
+    fk, fv = (base.as_strided((keys, hkv, D), (far, D, 1), i * hkv * D) for i in (0, 1))
+    fk.copy_(k)
+    fv.copy_(v)
+    args = dict(num_kv_heads=hkv, num_prefill=1, prefill_cu_q=i32([0, n], device), prefill_cu_k=i32([0, keys], device), max_q=n,
+                max_k=keys, window=window, sinks=1)
+    near = slo_attn.paged_attention(q.to(device), None, None, 0.1, k=k.to(device), v=v.to(device), **args)
+    got = slo_attn.paged_attention(q.to(device), None, None, 0.1, k=fk, v=fv, **args)
+    assert torch.equal(got, near)
+    o, size, logit = owin.attend(q.double(), k.double().nan_to_num(), v.double().nan_to_num(), keys - n, 0.1, window, 1)
+    spread = size + o.abs()
+    check(near, o, (2.0 ** -8 * (spread + o.abs()) + (2 * (D + 4) * 2.0 ** -24 * logit * 0.1)[..., None] * spread) * 1.02)
+    with pytest.raises(RuntimeError, match="elements apart"):
+        slo_attn.paged_attention(q.to(device), None, None, 0.1, k=base.as_strided((keys - 1, hkv, D), (1 << 25, D, 1)), v=fv, **args)
+
+
 def test_refusals(device):
     case = WindowRows("bf16", [40], [(3, 10)], hq=8, hkv=2)
     k = torch.zeros(3, 2, D, dtype=torch.bfloat16, device=device)

@@ -77,6 +77,15 @@ def test_scaled_tables():
             slo_attn.rope_cos_sin(128, 10, base, "cpu", rotary_dim=dim_)
 
 
+def test_scalings_that_the_table_would_not_follow():
+    yarn = dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=2048)
+    slo_attn.rope_cos_sin(64, 10, 1e4, "cpu", scaling=yarn)
+    for bad in ({**yarn, "mscale": 0.7}, {**yarn, "truncate": False}, dict(rope_type="yarn", factor=4.0), dict(rope_type="linear"),
+                dict(rope_type="linear", factor=2.0, beta_fast=8)):
+        with pytest.raises(ValueError, match="takes only"):
+            slo_attn.rope_cos_sin(64, 10, 1e4, "cpu", scaling=bad)
+
+
 def attention_args(**over):
     a = _lib.PagedAttentionArgs()
     a.head_dim, a.num_heads, a.num_kv_heads, a.softmax_scale, a.kv_dtype = 128, 32, 8, 0.1, _lib.KV_FP8_E4M3FN

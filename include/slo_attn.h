@@ -396,7 +396,9 @@ int slo_paged_attention_fp4(const slo_paged_attention_args* args, slo_stream_t s
  * E4M3FN or 4-bit pool (kv_dtype; k_scale / v_scale point to fp32 or E8M0
  * scales) and, without prefill_tables, over the contiguous bf16 rows k and v;
  * store_slot_mapping must be NULL and softmax_scale not zero.  Pages without a
- * visible key are not read: their table entries may be anything.  Entries that
+ * visible key are not read: their table entries may be anything, and so may keys
+ * and values that no query of the row sees.  (An infinity or a NaN that some
+ * queries of a chunk see can reach others of their tile.)  Entries that
  * are not in the pool count as keys that no query sees.  A query without keys
  * gives zeros, and so do query rows past every row's.  max_q and max_k are not
  * read.  At most 32,768 decode and 1,024 prefill rows, tables of up to 2^22
@@ -473,7 +475,7 @@ typedef struct slo_evict_kv_args {
  */
 int slo_evict_kv(const slo_evict_kv_args* args, slo_stream_t stream);
 
-/* Size of slo_evict_kv_args, for binding checks. */
+/* Sizes of slo_rope_store_args and slo_evict_kv_args, for binding checks. */
 size_t slo_rope_store_args_size(void);
 size_t slo_evict_kv_args_size(void);
 

@@ -16,9 +16,10 @@
 // 8), and V's channels 8 c .. 8 c + 7 of tokens 4 kg .. 4 kg + 3, of which two
 // v_perm_b32 per channel pair make the operand that has those tokens side by
 // side; a lane's scores are of tokens 4 kg .. 4 kg + 3 and are, exponentiated,
-// the other operand as they lie.  Pools of all three formats take this one
-// order: codes are converted to bf16 operands exactly (E4M3FN scales multiply
-// scores and weights, E8M0 ones go in with the conversion).
+// the other operand as they lie.  Codes are converted to bf16 operands exactly
+// (E4M3FN scales multiply scores and weights, E8M0 ones go in with the
+// conversion).  Only bf16 prefill rows, which need no conversion, have another
+// order of the channels, that of their way through LDS.
 // Sums, maxima and outputs are fp32 until the one rounding at the end.  Weights
 // are rounded to bf16 for the second product: in two terms, which carry them to
 // 2^-17, for decode rows, whose outputs are then off by the output's rounding alone

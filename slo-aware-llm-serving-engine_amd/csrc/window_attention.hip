@@ -916,7 +916,7 @@ union PrefillLds {
 // step into operands together, a quarter each, and each runs 16 NT columns,
 // (query, head of the group) pairs of consecutive queries, over them; the next
 // step loads meanwhile.  With two halves of four wavefronts each half takes
-// every other step.  4,096 queries of 32 heads under 4,096 keys run 254-266 us, 1,060
+// every other step.  4,096 queries of 32 heads under 4,096 keys run 250-260 us, 1,080
 // TFLOP/s (a library product of 8,192^3: 1,406): matrix cores and lane operations
 // (exponents, sums, masks, packing) are busy about half of the time each and the two
 // wavefronts of a SIMD hardly overlap them.  Weights taken between the products,

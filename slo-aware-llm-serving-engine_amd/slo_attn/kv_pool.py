@@ -69,7 +69,12 @@ def window_blocks(length: int, window: int, sinks: int, block_size: int) -> rang
 
     A token at position t >= ``length`` sees the keys j > t - window and j <
     sinks.  An engine gives these pages back (or to another row) and puts -1 in
-    their places: attention with the window does not read them."""
+    their places: attention with the window does not read them.  ``length``
+    counts the tokens whose K and V are in the pool: neither a sampled token
+    that is not yet there nor the rest of a prompt that comes in chunks; with
+    either, pages that the next tokens see would go, and nothing would say so.
+    Where layers share the table, ``window`` and ``sinks`` are the largest of
+    theirs."""
     if window <= 0 or sinks < 0 or block_size <= 0:
         raise ValueError("window and block_size must be positive and sinks not negative")
     return range(-(-sinks // block_size), max(length - window + 1, 0) // block_size)

@@ -1,7 +1,12 @@
 """Window attention and the rotary layouts on the CPU: the definition by brute
 force, scaled tables, given back pages, and the C-ABI's refusals."""
 import ctypes
+import glob
 import math
+import os
+import re
+import textwrap
+from types import SimpleNamespace
 
 import numpy as np
 import pytest
@@ -37,6 +42,49 @@ def test_blocks_that_no_later_token_sees(window, sinks, block):
     for bad in ((0, 0, 64), (5, -1, 64), (5, 0, 0)):
         with pytest.raises(ValueError):
             window_blocks(10, *bad)
+
+
+class Sequence(SimpleNamespace):
+    def __len__(self):
+        return self.num_tokens
+
+
+@pytest.mark.parametrize("block", [64, 128])
+@pytest.mark.parametrize("spans", [[(64, 0)], [(100, 4), (33, 70)], [(1, 1)], [(256, 0), (300, 2), (7, 130)]])
+def test_documented_give_back_keeps_what_later_tokens_see(spans, block):
+    """The recipe of the documents, run as it stands after every step of a row: its prompt in chunks, then tokens one at a
+    time, each in the sequence before it is in the pool; layers of several widths share the table."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    texts = [open(path).read() for path in sorted(glob.glob(os.path.join(root, "*.md")))]
+    recipes = [x for t in texts for x in re.findall(r"```python\n(.*?)```", t, re.S) if "window_blocks(" in x]
+    assert len(recipes) == 1
+    recipe = compile(textwrap.dedent(recipes[0]), "recipe", "exec")
+    layers = [slo_attn.Attention(8, 128, 0.1, 2, window=w, sinks=s) for w, s in spans]
+    # what a recipe that takes one width and one count of sinks is to be given
+    names = dict(W=max(w for w, _ in spans), S=max(s for _, s in spans))
+    prompt, generated = 700, 200
+    seq = Sequence(num_tokens=prompt, num_cached_tokens=0, num_scheduled_tokens=0, block_table=list(range(-(-(prompt + generated) // block))))
+    freed = []
+
+    def step(first, count, is_prefill):
+        for t in range(first, first + count):
+            assert seq.block_table[t // block] >= 0, f"the page that token {t} is written to is gone"
+            for w, s in spans:
+                seen = owin.visible(1, t + 1, t, w, s)[0].nonzero()[:, 0] // block
+                gone = [b for b in seen.unique().tolist() if seq.block_table[b] < 0]
+                assert not gone, f"token {t} sees keys of pages {gone}"
+        exec(recipe, dict(names, window_blocks=window_blocks, seq=seq, layers=layers, is_prefill=is_prefill,
+                          self=SimpleNamespace(block_size=block), free_page=freed.append))
+
+    for count in (300, 33, 367):
+        seq.num_scheduled_tokens = count
+        step(seq.num_cached_tokens, count, True)
+        seq.num_cached_tokens += count
+    for t in range(prompt, prompt + generated):
+        seq.num_tokens = t + 2  # token t, and the one sampled after it, appended before the recipe runs
+        step(t, 1, False)
+    end = prompt + generated
+    assert len(set(freed)) == len(freed) and sorted(freed) == list(window_blocks(end, names["W"], names["S"], block))
 
 
 def test_scaled_tables():

@@ -283,38 +283,51 @@ def load_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: tor
 
 
 # ------------------------------------------- fused q/k norm + RoPE + KV write
+def _scaling_number(scaling: dict, name: str, default: float | None = None) -> float:
+    """A positive, finite number of a rope scaling (``default`` where it is left out or None)."""
+    given = scaling.get(name)
+    try:
+        x = float(default if given is None else given)
+    except (TypeError, ValueError):
+        x = math.nan
+    if not 0 < x < math.inf:
+        raise ValueError(f"the rope scaling's {name} must be a positive, finite number, not {given!r}")
+    return x
+
+
 def _inverse_frequencies(dim: int, base: float, scaling: dict) -> tuple[torch.Tensor, float]:
     """fp64 frequencies of ``dim / 2`` channel pairs, and the table's factor, after ``scaling``."""
+    kinds = {scaling[name] for name in ("rope_type", "type") if name in scaling} or {"default"}
+    kind = kinds.pop()
+    if kinds or kind not in ("default", "linear", "yarn"):
+        raise ValueError(f"rope scaling {' and '.join(map(repr, {kind, *kinds}))} is not one of default, linear or yarn")
+    needs = {"default": set(), "linear": {"factor"}, "yarn": {"factor", "original_max_position_embeddings"}}[kind]
+    takes = needs | {"rope_type", "type"} | ({"attention_factor", "beta_fast", "beta_slow"} if kind == "yarn" else set())
+    if scaling.keys() - takes or needs - scaling.keys():
+        raise ValueError(f"rope scaling {kind!r} (its rope_type) needs {', '.join(sorted(needs)) or 'no keys'} and takes only "
+                         f"{', '.join(sorted(takes))}")
     i = torch.arange(0, dim, 2, dtype=torch.float64)
     freq = base ** (-i / dim)
-    kind = scaling.get("rope_type", scaling.get("type", "default"))
     if kind == "default":
         return freq, 1.0
-    if kind not in ("linear", "yarn"):
-        raise ValueError(f"rope scaling {kind!r} is not default, linear or yarn")
-    known = {"rope_type", "type", "factor", "original_max_position_embeddings"}
-    if kind == "yarn":
-        known |= {"attention_factor", "beta_fast", "beta_slow"}
-    if scaling.keys() - known or "factor" not in scaling or (kind == "yarn" and "original_max_position_embeddings" not in scaling):
-        raise ValueError(f"rope scaling {kind!r} needs its factor (yarn: and original_max_position_embeddings) and takes only "
-                         f"{', '.join(sorted(known))}")
-    factor = float(scaling["factor"])
-    if not factor >= 1.0 or factor == float("inf"):
-        raise ValueError("the rope scaling factor must be finite and at least 1")
+    factor = _scaling_number(scaling, "factor")
+    if factor < 1.0:
+        raise ValueError("the rope scaling factor must be at least 1")
     if kind == "linear":
         return freq / factor, 1.0
-    trained = scaling["original_max_position_embeddings"]
-    size = scaling.get("attention_factor")
-    if size is None:
-        size = 0.1 * math.log(factor) + 1.0
+    trained = _scaling_number(scaling, "original_max_position_embeddings")
+    size = _scaling_number(scaling, "attention_factor", 0.1 * math.log(factor) + 1.0)
+    fast, slow = _scaling_number(scaling, "beta_fast", 32.0), _scaling_number(scaling, "beta_slow", 1.0)
+    if fast <= slow or base <= 1.0:
+        raise ValueError("rope scaling 'yarn' needs beta_fast above beta_slow and a base above 1")
 
     def channel(turns):  # the pair that turns so many times in the trained positions
         return dim * math.log(trained / (turns * 2 * math.pi)) / (2 * math.log(base))
 
-    low = max(math.floor(channel(scaling.get("beta_fast") or 32.0)), 0)
-    high = min(math.ceil(channel(scaling.get("beta_slow") or 1.0)), dim - 1)
+    low = max(math.floor(channel(fast)), 0)
+    high = min(math.ceil(channel(slow)), dim - 1)
     ramp = ((i / 2 - low) / max(high - low, 0.001)).clamp(0, 1)
-    return freq / factor * ramp + freq * (1 - ramp), float(size)
+    return freq / factor * ramp + freq * (1 - ramp), size
 
 
 def rope_cos_sin(head_dim: int, max_position: int, base: float, device, rotary_dim: int | None = None,
@@ -332,7 +345,8 @@ def rope_cos_sin(head_dim: int, max_position: int, base: float, device, rotary_d
     ``original_max_position_embeddings`` positions, leaves those that turn more
     than ``beta_fast`` (32) times, goes from one to the other linearly over the
     pairs between, and multiplies the table by ``attention_factor`` (0.1
-    ln(factor) + 1).
+    ln(factor) + 1).  Keys that the type does not follow are refused, without a
+    type (or with "default") all of them.
     """
     if rotary_dim is not None or scaling is not None:
         dim = head_dim if rotary_dim is None else rotary_dim

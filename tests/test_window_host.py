@@ -134,6 +134,28 @@ def test_scalings_that_the_table_would_not_follow():
             slo_attn.rope_cos_sin(64, 10, 1e4, "cpu", scaling=bad)
 
 
+def test_scalings_are_followed_or_refused():
+    yarn = dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=2048)
+    table = lambda scaling, base=1e4: slo_attn.rope_cos_sin(64, 10, base, "cpu", scaling=scaling)  # noqa: E731
+    for bad in (dict(factor=4.0), dict(rope_type="default", factor=4.0), {**yarn, "rope_type": "default"},
+                dict(original_max_position_embeddings=2048), {**yarn, "type": "linear"}, dict(rope_type=None, factor=4.0),
+                {**yarn, "factor": None}, {**yarn, "factor": "four"}, {**yarn, "factor": 0.0}, {**yarn, "factor": float("inf")},
+                {**yarn, "attention_factor": 0.0}, {**yarn, "attention_factor": -1.0}, {**yarn, "attention_factor": float("nan")},
+                {**yarn, "original_max_position_embeddings": None}, {**yarn, "original_max_position_embeddings": 0},
+                {**yarn, "original_max_position_embeddings": float("inf")}, {**yarn, "beta_fast": 1.0}, {**yarn, "beta_slow": 32},
+                {**yarn, "beta_fast": 2, "beta_slow": 8}, {**yarn, "beta_fast": 0}, {**yarn, "beta_slow": -1.0}):
+        with pytest.raises(ValueError, match="rope scaling"):
+            table(bad)
+    with pytest.raises(ValueError, match="base"):
+        table(yarn, 1.0)
+    # nothing asked for, and what stands for the defaults
+    plain = slo_attn.rope_cos_sin(64, 10, 1e4, "cpu", rotary_dim=64)
+    for none in ({}, dict(rope_type="default"), dict(type="default", rope_type="default")):
+        assert torch.equal(table(none), plain)
+    assert torch.equal(table({**yarn, "type": "yarn", "attention_factor": None, "beta_fast": None, "beta_slow": 1}), table(yarn))
+    assert not torch.equal(table(yarn), plain)
+
+
 def attention_args(**over):
     a = _lib.PagedAttentionArgs()
     a.head_dim, a.num_heads, a.num_kv_heads, a.softmax_scale, a.kv_dtype = 128, 32, 8, 0.1, _lib.KV_FP8_E4M3FN

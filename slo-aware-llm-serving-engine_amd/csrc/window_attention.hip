@@ -23,8 +23,10 @@
 // Sums, maxima and outputs are fp32 until the one rounding at the end.  Weights
 // are rounded to bf16 for the second product: in two terms, which carry them to
 // 2^-17, for decode rows, whose outputs are then off by the output's rounding alone
-// (0.0016-0.0017 of their size); in one for prefill rows (0.0021-0.0023), where a
-// second term would double that product.
+// (0.0016-0.0017 of their size); in one for prefill rows (0.0020-0.0023), where a
+// second term would double that product.  Prefill rows divide by the sum of the
+// rounded weights (one more row of the second product), so that a weight's rounding
+// cancels where one key dominates.
 #include "capi_internal.h"
 #include "fp4.h"
 #include "tile_io.h"
@@ -36,10 +38,13 @@ namespace {
 
 constexpr int RECORD = HD + 4;   // floats of a decode chunk's partial result: outputs, maximum, sum, 2 unused
 constexpr float kNone = -1e30f;  // running maximum before the first key
-// Largest sum of a prefill lane's weights in a step before its column's
-// reference moves to the step's maximum, so that most steps need no maximum:
-// weights keep their relative rounding up to there, sums far from overflow.
-constexpr float kSumMax = 224.0f;
+// Largest weight of a prefill lane in a step before its column's reference moves to
+// the step's maximum, so that most steps need no maximum over the column: weights
+// keep their relative rounding up to there, sums far from overflow.
+constexpr float kMost = 224.0f;
+// E4M3FN V scales below this count as zero in prefill rows (their reciprocals and the
+// weights that they multiply stay in range): values of less than 448 x 2^-100.
+constexpr float kSmallScale = 0x1p-100f;
 constexpr int NT = 2;            // 16-column blocks of a prefill wavefront
 constexpr int kWaves = 4;        // wavefronts that run a tile
 
@@ -519,7 +524,11 @@ __device__ void decode_item(const WinParams& p, DecodeLds<F, WAVES>& lds, int r,
 template <int F>
 struct Stage {
   u32x4 k[4][4][64], v[2][8][64];
-  float s[F == KV_FP8_E4M3FN ? 2 : 1][64];
+};
+template <> struct Stage<KV_FP8_E4M3FN> {
+  u32x4 k[4][4][64], v[2][8][64];
+  float s[2][64];
+  uint16_t r[3][64];  // 1 / V scale as three bf16 terms
 };
 // bf16 needs no conversion: rows as they are, sent there by the memory system in
 // whole rows, 16-byte part x of token t at part x ^ (t mod 16) so that no read has
@@ -680,7 +689,7 @@ __device__ __forceinline__ void clear_unseen(Quarter<F>& t, int key, int first, 
   }
   if constexpr (F == KV_FP8_E4M3FN) {
     const int k = key + 16 * wave + (lane & 15);
-    if (!((k < end) & ((k >= first) | (k < sinks)))) t.vs = 0.0f;
+    if (!((k < end) & ((k >= first) | (k < sinks)))) t.vs = 1.0f;
   }
 }
 
@@ -694,12 +703,28 @@ __device__ __forceinline__ void stage(Stage<F>& s, const Quarter<F>& t, int wave
       s.k[wave][2 * i][lane] = fp8x8_to_bf16x8(u32x2{t.k[i][0], t.k[i][1]});
       s.k[wave][2 * i + 1][lane] = fp8x8_to_bf16x8(u32x2{t.k[i][2], t.k[i][3]});
     }
+    u32x2 codes[4] = {t.v[0], t.v[1], t.v[2], t.v[3]};
+    float vs = t.vs;
+    const bool small = __builtin_fabsf(vs) < kSmallScale;
+    if (__any(small)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (__shfl((int)small, 4 * (lane >> 4) + i)) codes[i] = u32x2{0, 0};
+      if (small) vs = 1.0f;
+    }
     if (lane < 16) {
       s.s[0][16 * wave + c] = t.ks;
-      s.s[1][16 * wave + c] = t.vs;
+      s.s[1][16 * wave + c] = vs;
+      float rest = __builtin_amdgcn_rcpf(vs);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        const uint32_t term = pack_bf16x2(rest, 0.0f);
+        s.r[i][16 * wave + c] = (uint16_t)term;
+        rest -= __uint_as_float(term << 16);
+      }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = fp8x8_to_bf16x8(t.v[i]);
+    for (int i = 0; i < 4; ++i) v[i] = fp8x8_to_bf16x8(codes[i]);
   } else {
     const float sc = e8m0(t.ks);
 #pragma unroll
@@ -737,10 +762,34 @@ __device__ __forceinline__ bf16x8 v_operand(const Stage<F>& s, int g, int i, int
   }
 }
 
+// The row of the second product that sums 32 tokens' weights, as they were rounded
+// for it: ones, or for E4M3FN, whose weights carry V's scales, the scales'
+// reciprocals, a term in each of the first three rows.  us against lanes' own sums of
+// the unrounded weights: 4,096 queries under 4,096 keys 252.6 / 250.0, cold rows of
+// 7,733 tokens 126.9 / 126.4, three E4M3FN chunks of 1,377 38.0 / 36.8, 24 decode rows
+// and two chunks of 512 24.2 / 24.2 (260.4, 128.4, 37.8 and 24.5 with those sums kept
+// for the test of the reference, which takes the largest weight instead).
+template <int F>
+__device__ __forceinline__ bf16x8 sum_operand(const Stage<F>& s, int g, int lane) {
+  if constexpr (F == KV_FP8_E4M3FN) {
+    const int c = lane & 15, t = 32 * g + 4 * (lane >> 4);
+    const u32x2 x = ld8(&s.r[c < 3 ? c : 0][t]), y = ld8(&s.r[c < 3 ? c : 0][t + 16]);
+    return as_bf16x8(c < 3 ? u32x4{x.x, x.y, y.x, y.y} : u32x4{0, 0, 0, 0});
+  } else {
+    return as_bf16x8(u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
+  }
+}
+
 struct Acc {
   f32x4 o[NT][8];
-  float ncm[NT], l[NT];  // minus the reference in the log2 domain (+inf before the first key), this lane's sum
+  f32x4 l[NT];    // sums of the rounded weights (see sum_operand): four times, or in its first rows
+  float ncm[NT];  // minus the reference in the log2 domain (+inf before the first key)
 };
+// A column's sum, in each of its lanes.
+template <int F>
+__device__ __forceinline__ float column_sum(const f32x4& l) {
+  return F == KV_FP8_E4M3FN ? col_sum(l[0] + l[1] + l[2]) : l[0];
+}
 
 // 64 tokens from `key` on of a wavefront's columns against the staged operands,
 // read four ahead of the products.  A wavefront at its score products goes before
@@ -769,9 +818,9 @@ __device__ __forceinline__ void staged_step(const WinParams& p, const Stage<F>& 
     __builtin_amdgcn_sched_barrier(0);
   }
   __builtin_amdgcn_s_setprio(0);
-  // No maximum is formed: a reference that is too low shows in the sum of a
-  // lane's weights (inf or NaN while it is unset).  Only then are the columns'
-  // maxima found and the weights taken again.
+  // A reference that is too low shows in the largest of a lane's weights (inf or
+  // NaN while it is unset).  Only then are the columns' maxima found and the
+  // weights taken again.
   const float c = p.scale_log2;
   const int few = sink ? 0 : p.sinks - key;  // sinks among the window part's keys
   // Column blocks are taken together (4,096 queries under 4,096 keys 255 us, one after
@@ -807,23 +856,22 @@ __device__ __forceinline__ void staged_step(const WinParams& p, const Stage<F>& 
       }
     }
     f32x4 e[COLS][4];
-    float rs[COLS];
     auto exponents = [&](int n, float ncm) {
-      float& sum = rs[n - n0];
-      sum = 0.0f;
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          e[n - n0][t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][t][i], c, ncm));
-          sum += e[n - n0][t][i];
-        }
+        for (int i = 0; i < 4; ++i) e[n - n0][t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][t][i], c, ncm));
     };
     bool low = false;
 #pragma unroll
     for (int n = n0; n < n0 + COLS; ++n) {
       exponents(n, a.ncm[n]);
-      low |= !(rs[n - n0] <= kSumMax);
+      const f32x4(&x)[4] = e[n - n0];
+      float top = x[0][0];
+#pragma unroll
+      for (int i = 1; i < 15; i += 2) top = fmaxf(fmaxf(top, x[i >> 2][i & 3]), x[(i + 1) >> 2][(i + 1) & 3]);
+      top = fmaxf(top, x[3][3]);
+      low |= !(top <= kMost);
     }
     if (__any(low)) {
 #pragma unroll
@@ -843,7 +891,6 @@ __device__ __forceinline__ void staged_step(const WinParams& p, const Stage<F>& 
 #pragma unroll
     for (int n = n0; n < n0 + COLS; ++n) {
       f32x4(&x)[4] = e[n - n0];
-      a.l[n] += rs[n - n0];
       if constexpr (F == KV_FP8_E4M3FN) {
 #pragma unroll
         for (int t = 0; t < 4; ++t) x[t] *= *reinterpret_cast<const f32x4*>(&st.s[1][16 * t + 4 * kg]);
@@ -862,11 +909,16 @@ __device__ __forceinline__ void staged_step(const WinParams& p, const Stage<F>& 
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[(j + 1) & 1][i] = v_operand<F>(st, (j + 1) >> 1, 4 * ((j + 1) & 1) + i, lane);
     }
+    const bf16x8 ones = sum_operand<F>(st, g, lane);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int n = 0; n < NT; ++n) a.o[n][4 * (j & 1) + i] = mfma16(x[j & 1][i], pr[n][g], a.o[n][4 * (j & 1) + i]);
+    if (j & 1) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) a.l[n] = mfma16(ones, pr[n][g], a.l[n]);
+    }
     __builtin_amdgcn_sched_barrier(0);
   }
 }
@@ -953,7 +1005,7 @@ __device__ void prefill_item(const WinParams& p, PrefillLds<F, HALVES>& lds, int
 #pragma unroll
     for (int i = 0; i < 8; ++i) a.o[n][i] = f32x4{0, 0, 0, 0};
     a.ncm[n] = INFINITY;
-    a.l[n] = 0.0f;
+    a.l[n] = f32x4{0, 0, 0, 0};
   }
   if (from < to) {
     const int32_t* table = p.ptables ? p.ptables + (int64_t)r * p.pstride : nullptr;
@@ -999,6 +1051,9 @@ __device__ void prefill_item(const WinParams& p, PrefillLds<F, HALVES>& lds, int
       }
     }
   }
+  float l[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) l[n] = column_sum<F>(a.l[n]);
   if constexpr (HALVES == 2) {
     Half& h = lds.half;
     __syncthreads();
@@ -1008,7 +1063,7 @@ __device__ void prefill_item(const WinParams& p, PrefillLds<F, HALVES>& lds, int
 #pragma unroll
         for (int e = 0; e < 8; ++e) h.o[wave][n][e][lane] = a.o[n][e];
         h.ncm[wave][n][lane] = a.ncm[n];
-        h.l[wave][n][lane] = a.l[n];
+        h.l[wave][n][lane] = l[n];
       }
     }
     __syncthreads();
@@ -1019,7 +1074,7 @@ __device__ void prefill_item(const WinParams& p, PrefillLds<F, HALVES>& lds, int
       const float mine = a.ncm[n] == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ncm - a.ncm[n]);
       const float w = other == INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ncm - other);
       a.ncm[n] = ncm;
-      a.l[n] = a.l[n] * mine + h.l[wave][n][lane] * w;
+      l[n] = l[n] * mine + h.l[wave][n][lane] * w;
 #pragma unroll
       for (int e = 0; e < 8; ++e) a.o[n][e] = a.o[n][e] * mine + h.o[wave][n][e][lane] * w;
     }
@@ -1028,11 +1083,10 @@ __device__ void prefill_item(const WinParams& p, PrefillLds<F, HALVES>& lds, int
   asm("" : "+v"(col));  // found again here, so that the loop need not hold what follows from it in registers
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const float l = col_sum(a.l[n]);
     if (p.splits == 1) {
       const int x = 16 * n + col, y = by_group(p, x), tok = w0 + wave * each + y, h = head * p.group + x - y * p.group;
       const bool live = y < each && tok < w1;
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const float inv = l[n] == 0.0f ? 0.0f : 1.0f / l[n];
       uint16_t* out = p.out + (int64_t)(g.q0 + tok) * p.out_stride + h * HD;
       if constexpr (F == KV_BF16) {
         // A lane's 4 channels at 64 (kg / 2) + 8 e + 4 (kg mod 2): lanes of
@@ -1068,7 +1122,7 @@ __device__ void prefill_item(const WinParams& p, PrefillLds<F, HALVES>& lds, int
       }
       if (kg == 0) {
         out.m[16 * block + col] = a.ncm[n] == INFINITY ? kNone : -a.ncm[n];
-        out.l[16 * block + col] = l;
+        out.l[16 * block + col] = l[n];
       }
     }
   }

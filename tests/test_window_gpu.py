@@ -75,6 +75,57 @@ def test_cold_rows_under_a_window(device, name):
     check(got, *case.attend())
 
 
+@pytest.mark.parametrize("rows", [1, 11])  # tiles of two halves, and of one
+@pytest.mark.parametrize("fmt", ["bf16", "fp8", "fp4", "cold"])
+def test_rounding_of_a_dominating_weight_cancels(device, fmt, rows):
+    """One late key has nearly all of every query's weight, which is some number between 90 and 190 times the first key's.
+
+    Weights w are rounded to bf16, w' = w (1 + d) with |d| <= 2^-8, and an fp32 logit moves a weight by
+    2 (D + 4) 2^-24 sum|q k| scale = f more.  The outputs sum(w' v) / sum(w') are off by
+    sum(w' (v - o)) / sum(w'), at most (2^-8 + f) sum p|v - o| / (1 - 2^-8 - f) for normalised weights p; sums of 300 products
+    in fp32 by 300 2^-24 of their size, the sum's own (E4M3FN: a reciprocal of three terms) by as much again; the result
+    is rounded once, 2^-8."""
+    n, prefix, late, hq, hkv, scale = 100, 200, 150, 32, 2, 5 / 512
+    case = WindowRows("bf16" if fmt == "cold" else fmt, [], [(n, prefix)] * rows, hq=hq, hkv=hkv, seed=8, window=1000, sinks=0,
+                      scale=scale, give_back=False)
+    g = torch.Generator().manual_seed(12)
+    signs = 2.0 * torch.randint(0, 2, (hkv, D), generator=g) - 1
+    size = torch.full((n + prefix, 1, 1), -8.0)
+    size[0], size[late] = 0.0, 4.0
+    k = (size * signs).to(torch.bfloat16)
+    vs = [random_values(g, n + prefix, hkv, D) for _ in range(rows)]
+    case.q = ((0.9 + 0.15 * torch.rand(rows * n, hq, 1, generator=g)) * signs.repeat_interleave(hq // hkv, 0)).to(torch.bfloat16)
+    for (_, _, _, table), v in zip(case.rows(), vs):
+        case.pool.write(table, k, v)
+    if fmt == "cold":
+        kk, vv = k.repeat(rows, 1, 1).to(device), torch.cat(vs).to(device)
+        got = call(case, device, k=kk, v=vv, prefill_tables=None)
+    else:
+        got = call(case, device)
+    unseen = torch.ones(n, n + prefix, dtype=torch.bool).triu(prefix + 1)
+    for first, _, m, table in case.rows():
+        (k64, _), (v64, _) = (case.pool.values(table, m, side) for side in (0, 1))
+        q64 = case.q[first:first + n].double()
+        for h in range(hq):
+            kh, vh = k64[:, h // (hq // hkv)], v64[:, h // (hq // hkv)]
+            p = torch.softmax((q64[:, h] @ kh.T * scale).masked_fill(unseen, float("-inf")), -1)
+            assert (p[:, late] > 0.98).all() and (p[:, late] < 191 * p[:, 0]).all() and (p[:, late] > 85 * p[:, 0]).all()
+            o = p @ vh
+            apart = torch.stack([(w[:, None] * (vh - x).abs()).sum(0) for w, x in zip(p, o)])
+            moved = 2.0 ** -8 + 2 * (D + 4) * 2.0 ** -24 * (q64[:, h].abs() @ kh.abs().T).max() * scale
+            bound = 2.0 ** -8 * o.abs() + moved * apart / (1 - moved) * (1 + 2.0 ** -8) + 700 * 2.0 ** -24 * (p @ vh.abs() + o.abs())
+            check(got[first:first + n, h], o, bound)
+
+
+def test_scales_that_make_nothing_of_values(device):
+    # E4M3FN V scales of 0, or so small that no bf16 output shows them, leave a key its weight; a negative one turns its values
+    case = WindowRows("fp8", [], [(90, 40)], hq=8, hkv=2, seed=6, window=50, sinks=2, give_back=False)
+    table = case.tables[0]
+    for j, x in ((0, 0.0), (30, 2.0 ** -120), (70, 0.0), (71, 2.0 ** -99), (100, -0.5), (129, 0.0)):
+        case.pool.scale[1][table[j // case.block], j % case.block] = x
+    check(call(case, device), *case.attend())
+
+
 @pytest.mark.parametrize("fmt", ["bf16", "fp8", "fp4"])
 def test_cold_rows_beside_decode_rows_of_a_pool(device, fmt):
     case = WindowRows(fmt, [70, 5], [(33, 0), (150, 0)], hq=16, hkv=4, seed=5, window=40)

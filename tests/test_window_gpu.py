@@ -274,6 +274,27 @@ def test_rows_do_not_depend_on_their_neighbours(device):
     check(call(one, device), *one.attend())
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "fp8", "fp4"])
+def test_a_row_alone_is_what_it_is_among_others(device, fmt):
+    # the same queries, pages and keys in a call of their own, which cuts decode rows and tiles further: within the bound
+    # of the one definition both times, and so within twice that of each other
+    base = WindowRows(fmt, [2200, 700], [(50, 2600), (33, 0)], hq=16, hkv=4, seed=6, window=1500)
+    base.q = torch.randn(311, 16, D, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+    case = base.part([2200, 700] * 31, base.chunks * 3, base.tables[:2] * 31 + base.tables[2:] * 3, slice(0, 311))
+    among = call(case, device)
+    first = len(case.lens)
+    for lens, chunks, row, queries in (([2200], [], 6, slice(6, 7)), ([700], [], 61, slice(61, 62)),
+                                       ([], [(50, 2600)], first + 2, slice(first + 83, first + 133)),
+                                       ([], [(33, 0)], first + 5, slice(first + 216, first + 249)),
+                                       ([2200, 700], [], slice(2, 4), slice(2, 4))):
+        one = case.part(lens, chunks, case.tables[row] if isinstance(row, slice) else [case.tables[row]], queries)
+        want, bound = one.attend()
+        alone = call(one, device)
+        check(alone, want, bound)
+        check(among[queries], want, bound)
+        check(alone, among[queries].double().cpu(), 2 * bound)
+
+
 def test_two_streams_at_once(device):
     cases = [WindowRows("bf16", [2500, 300], [(60, 900)], hq=16, hkv=4, seed=s, window=1400) for s in (21, 22)]
     states = [(c.q.to(device), c.pool.device(device), c.arguments(device)) for c in cases]

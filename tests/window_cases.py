@@ -1,6 +1,8 @@
 """Shared builders of the window attention tests (not collected by pytest)."""
 from __future__ import annotations
 
+import copy
+
 import torch
 
 from fp4_cases import D, Rows
@@ -49,3 +51,10 @@ class WindowRows(Rows):
             fp32 = 2 * (D + 4) * 2.0 ** -24 * logit * abs(self.scale)
             bound[first:first + n] = (2.0 ** -8 * (spread + o.abs()) + fp32[..., None] * spread) * 1.02 + 1e-30
         return out, bound
+
+    def part(self, lens, chunks, tables, queries):
+        """Other rows over the same pool: lengths, (queries, prefix), their tables and their queries' rows of ``q``."""
+        one = copy.copy(self)
+        one.lens, one.chunks, one.tables, one.q = list(lens), list(chunks), list(tables), self.q[queries]
+        one.tokens = len(one.lens) + sum(n for n, _ in one.chunks)
+        return one

@@ -295,6 +295,41 @@ def test_a_row_alone_is_what_it_is_among_others(device, fmt):
         check(alone, among[queries].double().cpu(), 2 * bound)
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "fp8", "fp4"])
+def test_each_replay_is_the_definition_of_its_step(device, fmt):
+    # a captured call with rows shorter than the plan's, empty ones, and fewer queries than its capacity, each replay against
+    # the 64-bit result for the lengths of that replay; query rows past the last row are zeros
+    case = WindowRows(fmt, [1500, 40, 700], [(20, 300)], hq=16, hkv=4, seed=11, window=600, give_back=False)
+    kc, vc, ks, vs = case.pool.device(device)
+    args = case.arguments(device)
+    q = case.q.to(device)
+    out = torch.empty_like(q)
+
+    def step():
+        slo_attn.paged_attention(q, kc, vc, case.scale, num_kv_heads=4, k_scale=ks, v_scale=vs, window=600, sinks=4, out=out, **args)
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for lens, (n, prefix) in (([1500, 40, 700], (20, 300)), ([1, 0, 699], (1, 0)), ([777, 33, 64], (0, 0)), ([0, 0, 0], (19, 301)),
+                              ([1400, 39, 1], (7, 200)), ([1500, 40, 700], (20, 300))):
+        args["decode_lens"].copy_(i32(lens, device))
+        args["prefill_cu_q"].copy_(i32([0, n], device))
+        args["prefill_cu_k"].copy_(i32([0, n + prefix], device))
+        out.fill_(float("nan"))
+        graph.replay()
+        got = out.clone()
+        torch.cuda.synchronize()
+        one = case.part(lens, [(n, prefix)], case.tables, slice(0, 3 + n))
+        check(got[:3 + n], *one.attend())
+        assert not got[3 + n:].any()
+        for row, keys in enumerate(lens):
+            assert keys or not got[row].any()
+        step()
+        assert torch.equal(got, out)
+
+
 def test_two_streams_at_once(device):
     cases = [WindowRows("bf16", [2500, 300], [(60, 900)], hq=16, hkv=4, seed=s, window=1400) for s in (21, 22)]
     states = [(c.q.to(device), c.pool.device(device), c.arguments(device)) for c in cases]

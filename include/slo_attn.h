@@ -400,8 +400,9 @@ int slo_paged_attention_fp4(const slo_paged_attention_args* args, slo_stream_t s
  * and values that no query of the row sees.  (An infinity or a NaN that some
  * queries of a chunk see can reach others of their tile.)  Entries that
  * are not in the pool count as keys that no query sees.  A query without keys
- * gives zeros, and so do query rows past every row's.  E4M3FN V scales below
- * 2^-100 may count as zero.  max_q and max_k are not read.  At most 32,768 decode and 1,024 prefill rows, tables of up to 2^22
+ * gives zeros, and so do query rows past every row's (a call without rows writes
+ * nothing).  E4M3FN V scales below 2^-100 may count as zero.  max_q and max_k are
+ * not read.  At most 32,768 decode and 1,024 prefill rows, tables of up to 2^22
  * tokens, 2^24 rows of k and v.  Workspace as for slo_paged_attention_fp4.
  */
 int slo_paged_attention_window_workspace_bytes(const slo_paged_attention_args* args, int32_t window,

@@ -1,6 +1,8 @@
 // Norms of q and k (or none), rotary embedding in any layout, and the
 // slot-mapped KV write, in one pass over the fused QKV projection's output
-// (gfx950).
+// (gfx950).  For a 4-bit pool q and k only: the store kernel then reads k and V
+// again (4,096 tokens, 32 and 8 heads of 128: 23.7 us in both launches, a bf16 pool
+// 19.7).
 //
 // With the first R channels of a head rotated, h the head after the norm
 // (h = x rsqrt(mean x^2 + eps) w, or x itself) and a pair's channels (a, b)
@@ -23,7 +25,7 @@ namespace {
 // lane keep more loads in flight.  us for 512 x 2 / 128 x 3, 32 and 8 heads of
 // 128: 128 tokens 3.5 / 4.8, 768 6.9 / 8.2, 2,000 12.5 / 11.0, 8,192 (221 MB) 60.6
 // / 44.8 (4.9 TB/s; 256 x 3 45.3, 128 x 6 43.0 but 11.7 for the 2,000); 16 and 1 heads,
-// 8,192 28.0 / 16.6; heads of 64 29.2 / 21.1; E4M3FN, 4,096 29.9 / 28.0.
+// 8,192 28.0 / 16.6; heads of 64 29.2 / 21.1; E4M3FN, 4,096 (103 MB) 26.1 / 21.0.
 constexpr int kFewThreads = 512, kFewHeads = 2, kManyThreads = 128, kManyHeads = 3, kMany = 1024;
 
 struct RopeParams {

@@ -794,7 +794,7 @@ __device__ __forceinline__ float column_sum(const f32x4& l) {
 // 64 tokens from `key` on of a wavefront's columns against the staged operands,
 // read four ahead of the products.  A wavefront at its score products goes before
 // the other one of its SIMD, so that the two do not fall into step (4,096 queries
-// under 4,096 keys 254 us; no priorities, or others, 257-263).  at[n]: position of
+// under 4,096 keys 252 us; without priorities 264).  at[n]: position of
 // column block n's query; keys from `kend` on are not the row's.  A step before the
 // window part (`sink`) shows a query nothing but sinks.
 template <int F>
@@ -823,9 +823,9 @@ __device__ __forceinline__ void staged_step(const WinParams& p, const Stage<F>& 
   // weights taken again.
   const float c = p.scale_log2;
   const int few = sink ? 0 : p.sinks - key;  // sinks among the window part's keys
-  // Column blocks are taken together (4,096 queries under 4,096 keys 255 us, one after
-  // the other 259, 960 on a 4-bit pool 24.7 and 25.1); E4M3FN's scales leave no
-  // registers for it.
+  // Column blocks are taken together (4,096 queries under 4,096 keys 252 us, one after
+  // the other 254, cold rows of 7,733 tokens 124 and 128, 960 queries under 1,024 keys
+  // 29.7 and 30.8, on a 4-bit pool the same); E4M3FN's scales leave no registers for it.
   constexpr int COLS = F == KV_FP8_E4M3FN ? 1 : NT;
   bf16x8 pr[NT][2];
 #pragma unroll
@@ -968,13 +968,13 @@ union PrefillLds {
 // step into operands together, a quarter each, and each runs 16 NT columns,
 // (query, head of the group) pairs of consecutive queries, over them; the next
 // step loads meanwhile.  With two halves of four wavefronts each half takes
-// every other step.  4,096 queries of 32 heads under 4,096 keys run 250-260 us, 1,080
-// TFLOP/s (a library product of 8,192^3: 1,406): matrix cores and lane operations
-// (exponents, sums, masks, packing) are busy about half of the time each and the two
-// wavefronts of a SIMD hardly overlap them.  Weights taken between the products,
-// one by one, came to the same (258 for 260; E4M3FN rows 36 for 39, mixed steps 28
-// for 26), pages looked up a step ahead too; four column blocks a wavefront and one
-// wavefront a SIMD took twice as long.  A launch of few steps mostly waits: 2.5 us
+// every other step.  4,096 queries of 32 heads under 4,096 keys run 250-264 us by the
+// card, 1,050-1,100 TFLOP/s (a library product of 8,192^3: 1,406): matrix cores and lane
+// operations (exponents, masks, packing) are busy about half of the time each and the
+// two wavefronts of a SIMD hardly overlap them.  Weights taken between the products,
+// one by one, came to the same (258 for 260 before the sums' row; E4M3FN rows 36 for
+// 39, mixed steps 28 for 26), pages looked up a step ahead too; four column blocks a
+// wavefront and one wavefront a SIMD took twice as long.  A launch of few steps mostly waits: 2.5 us
 // to the tile, 3.2 for queries and output, 2.5 for page and first keys, 2.8 for the
 // first step, 1 of them for the first maximum.
 template <int F, int HALVES>
@@ -1281,14 +1281,14 @@ int decode_chunks(int64_t pairs, int64_t keys) {
 // Where all tiles fit one to a CU, beside the decode rows' workgroups, a second
 // half of each takes every other step: no records and no join.  us with one
 // half / two, 32 and 8 heads of bf16 behind 6,000 keys: 512 queries under 512 keys
-// 25.3 / 22.9, under 1,024 37.8 / 31.8, 960 under 1,024 38.8 / 34.3, 2,000 (504
-// tiles) 52.3 / 64.3; 24 decode rows and two chunks of 512 32.2 / 38.2.
+// 21.6 / 20.2, under 1,024 32.6 / 28.1, 960 under 1,024 34.1 / 29.7 (4 bits 36.6 /
+// 32.2), 2,000 (504 tiles) 45.6 / 55.6; 24 decode rows and two chunks of 512 24.9 / 30.5.
 // Few tiles are cut into parts besides, as far as CUs are left: of 4 steps or
 // more where there is room for four parts (32 queries, 8 tiles: under 512 keys whole
-// 21.4, so 18.9; under 1,024 30.2, parts of 8, 6, 4 steps 22.9, 20.7, 17.7; under
-// 4,096 parts of 16, 8, 4 steps 32.7, 24.7, 24.2), else of 12 (512 queries, 128
-// tiles: under 512 keys whole 22.8, parts of 4 steps 27.9; under 1,024 31.5, parts
-// of 6 32.5; under 4,096 whole 85.6, in two 55.8).
+// 18.7, so 17.3; under 1,024 26.6, parts of 8, 6, 4 steps 21.4, 18.9, 17.2; under
+// 4,096 76.0, parts of at least 8, 6, 4 steps 24.0, 23.8, 23.6), else of 12 (512
+// queries, 128 tiles: under 512 keys whole 20.0, parts of 4 steps 27.2; under 1,024
+// 28.0, parts of 6 31.5; under 4,096 whole 75.1, in two 54.4).
 int tile_parts(int64_t tiles, int64_t steps) {
   return (int)std::max<int64_t>(1, std::min(kSlots / 2 / tiles, steps / (4 * tiles <= kSlots / 2 ? 4 : 12)));
 }
